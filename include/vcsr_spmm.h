@@ -432,6 +432,189 @@ vcsr_status vcsr_cusparse_create(int M, int N, int nnz, const int *d_row_ptr,
 vcsr_status vcsr_cusparse_run(vcsr_cusparse *h, vcsr_stream_t stream);
 void vcsr_cusparse_destroy(vcsr_cusparse *h);
 
+/* --------------------------------------------------- dense layer operators
+ *
+ * What a layer built on a sparse product needs beside it: the norm that makes
+ * the product's FP32 result the operand of a dense one, the dense product
+ * with its epilogue, their gradients, and the optimizer step.  Matrices are
+ * row-major with a row pitch (ld*, in elements, >= the row's length) and unit
+ * column stride; pointers are device pointers of the current device, aligned
+ * to their element; any size may be odd and any pitch or base unaligned
+ * (vector and TMA forms are taken where 16-byte alignment allows, element or
+ * copying forms elsewhere).  A size of zero is a valid call.  Sums, norms and
+ * states are FP32; a 16-bit output is rounded once, to nearest even, at its
+ * store.  No counterpart in the reference. */
+
+/* Element types. */
+#define VCSR_F32 0
+#define VCSR_BF16 1
+#define VCSR_F16 2
+#define VCSR_E4M3 3 /* 8-bit float, 4 exponent and 3 mantissa bits, largest 448 */
+
+/* Root-mean-square norm with the residual's addition:
+ *   s = x + residual,  rstd = 1 / sqrt(mean(s^2) + eps),  y = s * rstd * weight
+ * per row.  y is computed from the unrounded s.  With y_dtype VCSR_E4M3 a row
+ * is stored as codes and one scale = max|y| / 448 (0 for a row of zeros; a
+ * code stands for code * scale). */
+typedef struct vcsr_rmsnorm_args {
+  int64_t rows, dim;
+  const void *x; /* rows x dim, x_dtype */
+  int64_t ldx;
+  const void *residual; /* rows x dim, x_dtype; NULL = none */
+  int64_t ldr;
+  const void *weight; /* dim, w_dtype */
+  void *y;            /* rows x dim, y_dtype */
+  int64_t ldy;
+  void *sum; /* s, rows x dim, x_dtype; NULL = not stored; may be x or residual itself */
+  int64_t lds;
+  float *rstd;  /* rows; NULL = not stored */
+  float *scale; /* rows; y_dtype VCSR_E4M3 only */
+  float eps;
+  int x_dtype; /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int w_dtype; /* x_dtype or VCSR_F32 */
+  int y_dtype; /* any */
+} vcsr_rmsnorm_args;
+vcsr_status vcsr_rmsnorm(const vcsr_rmsnorm_args *a, vcsr_stream_t stream);
+
+/* Gradient of vcsr_rmsnorm from the stored s and rstd: with h = s * rstd and
+ * g = dy * weight,
+ *   dx = rstd * (g - h * mean(g * h)) + dsum,   dweight = sum over rows of dy * h
+ * (x and residual have the same gradient dx; an 8-bit y passes dy through its
+ * rounding).  dsum is the gradient that reached s by other ways.  dweight is
+ * summed in a fixed order: the result does not depend on the schedule. */
+typedef struct vcsr_rmsnorm_grad_args {
+  int64_t rows, dim;
+  const void *dy; /* rows x dim, dy_dtype */
+  int64_t lddy;
+  const void *s; /* rows x dim, x_dtype */
+  int64_t lds;
+  const void *weight; /* dim, w_dtype */
+  const float *rstd;  /* rows */
+  const void *dsum;   /* rows x dim, x_dtype; NULL = none */
+  int64_t ldds;
+  void *dx; /* rows x dim, x_dtype; may be dsum itself */
+  int64_t lddx;
+  void *dweight;   /* dim, w_dtype; NULL = not wanted */
+  void *workspace; /* vcsr_rmsnorm_grad_workspace bytes, 16-byte aligned; dweight only */
+  size_t workspace_bytes;
+  int x_dtype, w_dtype;
+  int dy_dtype; /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+} vcsr_rmsnorm_grad_args;
+vcsr_status vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args *a, vcsr_stream_t stream);
+size_t vcsr_rmsnorm_grad_workspace(int64_t rows, int64_t dim);
+
+/* out = code * scale (one scale per row), or its square with squared != 0;
+ * codes are VCSR_E4M3, out is VCSR_F32, VCSR_BF16 or VCSR_F16. */
+vcsr_status vcsr_dequantize(const void *codes, int64_t ldc, const float *scale, int64_t rows,
+                            int64_t dim, void *out, int64_t ldo, int out_dtype, int squared,
+                            vcsr_stream_t stream);
+
+/* AdamW over many tensors at once:
+ *   g' = grad_scale * g
+ *   m = beta1 m + (1 - beta1) g',   v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr weight_decay) - lr (m / (1 - beta1^step)) / (sqrt(v / (1 - beta2^step)) + eps)
+ * The handle keeps the tensors' sizes and parameter addresses (so parameters
+ * keep their places while it lives); gradients are given to each step.
+ * States are the caller's: tensor t's state starts at value 256 * b_t, b_t =
+ * the number of 256-value blocks of the tensors before it, in buffers of
+ * vcsr_adamw_state_values values, zero before the first step (padding stays
+ * zero).  state_bits = 32: m and v, FP32.  state_bits = 8: m and u = sqrt(v)
+ * as VCSR_E4M3 codes with one FP32 scale per 256-value block (scale = the
+ * block's largest magnitude / 448); a v above zero is never stored as zero.
+ * Without `dither` codes round to nearest even; with it (256 uniform numbers
+ * in [0, 1) on the device, fresh ones each step) value k of a block rounds
+ * down when its fraction + dither[k] < 1 and up otherwise, so that changes
+ * far below a code's step (1 - beta2 of v) are kept on average instead of
+ * being lost.  A value that is not finite makes its block's scale so too. */
+typedef struct vcsr_adamw vcsr_adamw;
+int64_t vcsr_adamw_state_values(int tensors, const int64_t *numel);
+/* p_dtype: VCSR_F32, VCSR_BF16 or VCSR_F16, of every tensor.  copies (NULL =
+ * none): 16-bit copies of the parameters (copy_dtype), written by each step.
+ * The host arrays are read during the call only. */
+vcsr_status vcsr_adamw_create(int tensors, const int64_t *numel, void *const *params, int p_dtype,
+                              void *const *copies, int copy_dtype, int state_bits,
+                              vcsr_adamw **out, vcsr_stream_t stream);
+typedef struct vcsr_adamw_step_args {
+  const void *const *grads; /* one device pointer per tensor (host array); NULL leaves
+                               the tensor, its copy and its states as they are */
+  int g_dtype;              /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  void *m, *v;              /* states: FP32, or codes of m and of u = sqrt(v) */
+  float *m_scale, *u_scale; /* state_bits = 8: one per block */
+  const float *dither;      /* 256 values, or NULL; state_bits = 8 only */
+  double lr, beta1, beta2, eps, weight_decay;
+  float grad_scale;
+  int64_t step; /* this step's number, from 1 */
+} vcsr_adamw_step_args;
+vcsr_status vcsr_adamw_step(const vcsr_adamw *h, const vcsr_adamw_step_args *a,
+                            vcsr_stream_t stream);
+void vcsr_adamw_destroy(vcsr_adamw *h);
+
+/* Activations of vcsr_linear. */
+#define VCSR_ACT_NONE 0
+#define VCSR_ACT_RELU 1
+#define VCSR_ACT_GELU 2 /* z * Phi(z), Phi by erf */
+#define VCSR_ACT_SILU 3
+
+/* Dense product with its epilogue, in one kernel:
+ *   z = x_scale_i w_scale_j sum_k x[i,k] w[j,k] + bias_j,   y = act(z) + residual
+ * x is M x K, w is N x K (a layer's weights, a row per output).  x and w have
+ * one type; VCSR_E4M3 operands come with their scales (x_scale per row of x,
+ * w_scale per row of w).  The sum of a VCSR_F32 product has FP32 accuracy
+ * (about 1e-6 relative L2); a NaN or infinity in x or w reaches exactly the
+ * outputs whose sums read it. */
+typedef struct vcsr_linear_args {
+  int64_t M, N, K;
+  const void *x; /* M x K, dtype */
+  int64_t ldx;
+  const void *w; /* N x K, dtype */
+  int64_t ldw;
+  const float *x_scale, *w_scale; /* M and N values; VCSR_E4M3 only */
+  const void *bias;               /* N, out_dtype; NULL = none */
+  const void *residual;           /* M x N, out_dtype; NULL = none */
+  int64_t ldr;
+  void *y; /* M x N, out_dtype; may be residual itself */
+  int64_t ldy;
+  void *pre; /* z, M x N, out_dtype; NULL = not stored */
+  int64_t ldp;
+  void *workspace; /* vcsr_linear_workspace bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int dtype;     /* any */
+  int out_dtype; /* dtype; with VCSR_E4M3: VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int act;       /* VCSR_ACT_* */
+} vcsr_linear_args;
+vcsr_status vcsr_linear(const vcsr_linear_args *a, vcsr_stream_t stream);
+/* Bytes of device scratch the call needs (0 for aligned 16- and 8-bit
+ * operands), from the sizes, types, pitches and addresses in *a. */
+size_t vcsr_linear_workspace(const vcsr_linear_args *a);
+
+/* Gradient of vcsr_linear (not for VCSR_E4M3): with dz = dy * act'(pre),
+ *   dx = dz w (M x K),  dw = dz^T x (N x K),  dbias = sum over rows of dz
+ * (the residual's gradient is dy).  16-bit types round dz to their type before
+ * the two products (the tensor cores' operand type); dbias sums the unrounded
+ * dz, in a fixed order. */
+typedef struct vcsr_linear_grad_args {
+  int64_t M, N, K;
+  const void *dy; /* M x N */
+  int64_t lddy;
+  const void *pre; /* z of the forward call, M x N; may be NULL with VCSR_ACT_NONE */
+  int64_t ldp;
+  const void *x; /* M x K; used for dw */
+  int64_t ldx;
+  const void *w; /* N x K; used for dx */
+  int64_t ldw;
+  void *dx; /* M x K; NULL = not wanted */
+  int64_t lddx;
+  void *dw; /* N x K; NULL = not wanted */
+  int64_t lddw;
+  void *dbias;     /* N; NULL = not wanted */
+  void *workspace; /* vcsr_linear_grad_workspace bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int dtype; /* of every matrix: VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int act;
+} vcsr_linear_grad_args;
+vcsr_status vcsr_linear_grad(const vcsr_linear_grad_args *a, vcsr_stream_t stream);
+size_t vcsr_linear_grad_workspace(const vcsr_linear_grad_args *a);
+
 /* -------------------------------------------------------------- multi-GPU */
 
 /* nnz-balanced row panels: cuts[0] = 0, cuts[parts] = M, cut k is the row

@@ -1,0 +1,224 @@
+// layer_linear.cu — vcsr_linear and its gradient: argument checks, the
+// activation's gradient, and which product kernel runs.
+//
+// The gradient takes three steps: dz = dy act'(pre), rounded to the operands'
+// type, with dbias' partial column sums of the unrounded dz in the same pass
+// (one pass over dy and pre; without an activation dz is dy itself and only the
+// sums are made); dx = dz w; dw = dz^T x.
+#include <algorithm>
+
+#include "layer_gemm.cuh"
+
+namespace vcsr {
+namespace layer {
+namespace {
+
+constexpr int kDzWarps = 8;
+
+// Block (c, r): columns [c * 32 V, ...) of a chunk of rows; a lane holds V
+// columns, the warps take every 8th row of the chunk.  partial: one row of N
+// sums per chunk.
+template <class T, int V>
+__global__ void __launch_bounds__(kDzWarps * 32)
+    dz_kernel(const T *dy, int64_t lddy, const T *pre, int64_t ldp, T *dz, int64_t lddz, int64_t M,
+              int64_t N, int64_t chunk, int act, float *partial) {
+  __shared__ float joined[kDzWarps][32 * V + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = ((int64_t)blockIdx.x * 32 + lane) * V;
+  const int64_t r0 = (int64_t)blockIdx.y * chunk, r1 = min(M, r0 + chunk);
+  float sum[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+  if (col < N) {
+#pragma unroll 2
+    for (int64_t r = r0 + warp; r < r1; r += kDzWarps) {
+      const Vec<T, V> d = load_vec<T, V>(dy + r * lddy + col);
+      float o[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = widen(d.v[j]);
+      if (act != VCSR_ACT_NONE) {
+        const Vec<T, V> z = load_vec<T, V>(pre + r * ldp + col);
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] *= activate_slope(act, widen(z.v[j]));
+        if (dz) store_narrow<T, V>(dz + r * lddz + col, o);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += o[j];
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int j = 0; j < V; ++j) joined[warp][lane * V + j] = sum[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * V; c += kDzWarps * 32) {
+    const int64_t at = (int64_t)blockIdx.x * 32 * V + c;
+    if (at < N) {
+      float t = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kDzWarps; ++w) t += joined[w][c];
+      partial[(int64_t)blockIdx.y * N + at] = t;
+    }
+  }
+}
+
+int64_t dz_chunks(int64_t M, int64_t N) {
+  // enough chunks of at least 32 rows for four blocks an SM
+  const int64_t across = ceil_div(N, 256);
+  return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, across)));
+}
+
+template <class T>
+void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *partial, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const T *dy = static_cast<const T *>(a->dy), *pre = static_cast<const T *>(a->pre);
+  const bool vec = a->N % V == 0 && a->lddy % V == 0 && aligned(dy, 16) &&
+                   (a->act == VCSR_ACT_NONE || (a->ldp % V == 0 && aligned(pre, 16)));
+  const int64_t chunks = dz_chunks(a->M, a->N), chunk = ceil_div(a->M, chunks);
+  const dim3 grid((unsigned)ceil_div(a->N, vec ? 32 * V : 32), (unsigned)chunks);
+  if (vec)
+    dz_kernel<T, V><<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N,
+                                                    chunk, a->act, partial);
+  else
+    dz_kernel<T, 1><<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N,
+                                                    chunk, a->act, partial);
+}
+
+constexpr size_t kAlign = 256;
+size_t round_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+vcsr_status check_sizes(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N < 0 || K < 0) return fail(VCSR_ERR_INVALID, "negative size");
+  if (M > 0x7fffffffll || N > 0x7fffffffll || K > 0x7fffffffll)
+    return fail(VCSR_ERR_RANGE, "a size above 2^31 - 1");
+  return VCSR_OK;
+}
+
+vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
+  if (!a) return fail(VCSR_ERR_INVALID, "no arguments");
+  VCSR_TRY(check_sizes(a->M, a->N, a->K));
+  const bool codes = a->dtype == VCSR_E4M3;
+  if (!codes && !is_float16_or_32(a->dtype)) return fail(VCSR_ERR_UNSUPPORTED, "type %d", a->dtype);
+  if (codes ? !is_float16_or_32(a->out_dtype) : a->out_dtype != a->dtype)
+    return fail(VCSR_ERR_UNSUPPORTED, "output type %d for operands of type %d", a->out_dtype, a->dtype);
+  if (a->act < VCSR_ACT_NONE || a->act > VCSR_ACT_SILU)
+    return fail(VCSR_ERR_UNSUPPORTED, "activation %d", a->act);
+  if (a->M == 0 || a->N == 0) return VCSR_OK;
+  if (a->K > 0) {
+    VCSR_TRY(check_matrix("x", a->x, a->ldx, a->K, a->dtype, false));
+    VCSR_TRY(check_matrix("w", a->w, a->ldw, a->K, a->dtype, false));
+  }
+  if (codes && (!a->x_scale || !a->w_scale))
+    return fail(VCSR_ERR_INVALID, "8-bit operands need x_scale and w_scale");
+  if (!codes && (a->x_scale || a->w_scale))
+    return fail(VCSR_ERR_INVALID, "scales are for 8-bit operands");
+  VCSR_TRY(check_matrix("bias", a->bias, a->N, a->N, a->out_dtype, true));
+  VCSR_TRY(check_matrix("residual", a->residual, a->ldr, a->N, a->out_dtype, true));
+  VCSR_TRY(check_matrix("y", a->y, a->ldy, a->N, a->out_dtype, false));
+  VCSR_TRY(check_matrix("pre", a->pre, a->ldp, a->N, a->out_dtype, true));
+  Gemm g{a->M, a->N, a->K, {a->x, a->ldx, false}, {a->w, a->ldw, false}, a->dtype,
+         {a->x_scale, a->w_scale, a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->act,
+          a->out_dtype}};
+  return launch_gemm_simt(g, st);
+}
+
+struct GradPlan {
+  int64_t lddz = 0;
+  size_t dz = 0, partial = 0, total = 0;
+};
+
+GradPlan grad_plan(const vcsr_linear_grad_args *a) {
+  GradPlan p;
+  p.lddz = ceil_div(a->N, 8) * 8;
+  if (a->act != VCSR_ACT_NONE && (a->dx || a->dw))
+    p.dz = round_up((size_t)a->M * p.lddz * type_size(a->dtype));
+  if (a->dbias) p.partial = round_up((size_t)dz_chunks(a->M, a->N) * a->N * sizeof(float));
+  p.total = p.dz + p.partial;
+  return p;
+}
+
+vcsr_status zero_matrix(void *p, int64_t ld, int64_t rows, int64_t cols, int type, cudaStream_t st) {
+  const size_t s = type_size(type);
+  if (rows > 0 && cols > 0)
+    VCSR_CUDA(cudaMemset2DAsync(p, (size_t)ld * s, 0, (size_t)cols * s, (size_t)rows, st));
+  return VCSR_OK;
+}
+
+vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
+  if (!a) return fail(VCSR_ERR_INVALID, "no arguments");
+  VCSR_TRY(check_sizes(a->M, a->N, a->K));
+  if (!is_float16_or_32(a->dtype)) return fail(VCSR_ERR_UNSUPPORTED, "type %d", a->dtype);
+  if (a->act < VCSR_ACT_NONE || a->act > VCSR_ACT_SILU)
+    return fail(VCSR_ERR_UNSUPPORTED, "activation %d", a->act);
+  VCSR_TRY(check_matrix("dx", a->dx, a->lddx, a->K, a->dtype, true));
+  VCSR_TRY(check_matrix("dw", a->dw, a->lddw, a->K, a->dtype, true));
+  VCSR_TRY(check_matrix("dbias", a->dbias, a->N, a->N, a->dtype, true));
+  if (a->M == 0 || a->N == 0) {
+    if (a->dx) VCSR_TRY(zero_matrix(a->dx, a->lddx, a->M, a->K, a->dtype, st));
+    if (a->dw) VCSR_TRY(zero_matrix(a->dw, a->lddw, a->N, a->K, a->dtype, st));
+    if (a->dbias) VCSR_TRY(zero_matrix(a->dbias, a->N, 1, a->N, a->dtype, st));
+    return VCSR_OK;
+  }
+  VCSR_TRY(check_matrix("dy", a->dy, a->lddy, a->N, a->dtype, false));
+  VCSR_TRY(check_matrix("pre", a->pre, a->ldp, a->N, a->dtype, a->act == VCSR_ACT_NONE));
+  if (a->K > 0 && a->dx) VCSR_TRY(check_matrix("w", a->w, a->ldw, a->K, a->dtype, false));
+  if (a->K > 0 && a->dw) VCSR_TRY(check_matrix("x", a->x, a->ldx, a->K, a->dtype, false));
+  const GradPlan p = grad_plan(a);
+  if (p.total > 0 &&
+      (!a->workspace || a->workspace_bytes < p.total || !aligned(a->workspace, kAlign)))
+    return fail(VCSR_ERR_INVALID, "the call needs %zu bytes of 256-byte aligned workspace", p.total);
+  char *ws = static_cast<char *>(a->workspace);
+  void *dz = p.dz ? ws : nullptr;
+  float *partial = p.partial ? reinterpret_cast<float *>(ws + p.dz) : nullptr;
+  if (dz || partial) {
+    if (a->dtype == VCSR_F32)
+      launch_dz<float>(a, static_cast<float *>(dz), p.lddz, partial, st);
+    else if (a->dtype == VCSR_BF16)
+      launch_dz<__nv_bfloat16>(a, static_cast<__nv_bfloat16 *>(dz), p.lddz, partial, st);
+    else
+      launch_dz<__half>(a, static_cast<__half *>(dz), p.lddz, partial, st);
+    VCSR_CUDA(cudaGetLastError());
+    if (a->dbias)
+      VCSR_TRY(column_sum(partial, (int)dz_chunks(a->M, a->N), a->N, a->dbias, a->dtype, st));
+  }
+  if (a->K == 0) return VCSR_OK;
+  const void *d = dz ? dz : a->dy;
+  const int64_t ldd = dz ? p.lddz : a->lddy;
+  Epilogue e{};
+  e.type = a->dtype;
+  if (a->dx) {
+    e.out = a->dx;
+    e.ldo = a->lddx;
+    VCSR_TRY(launch_gemm_simt({a->M, a->K, a->N, {d, ldd, false}, {a->w, a->ldw, true}, a->dtype, e}, st));
+  }
+  if (a->dw) {
+    e.out = a->dw;
+    e.ldo = a->lddw;
+    VCSR_TRY(launch_gemm_simt({a->N, a->K, a->M, {d, ldd, true}, {a->x, a->ldx, true}, a->dtype, e}, st));
+  }
+  return VCSR_OK;
+}
+
+}  // namespace
+}  // namespace layer
+}  // namespace vcsr
+
+extern "C" {
+
+vcsr_status vcsr_linear(const vcsr_linear_args *a, vcsr_stream_t stream) {
+  vcsr::clear_error();
+  return vcsr::no_throw([&] { return vcsr::layer::linear(a, (cudaStream_t)stream); });
+}
+
+size_t vcsr_linear_workspace(const vcsr_linear_args *) { return 0; }
+
+vcsr_status vcsr_linear_grad(const vcsr_linear_grad_args *a, vcsr_stream_t stream) {
+  vcsr::clear_error();
+  return vcsr::no_throw([&] { return vcsr::layer::linear_grad(a, (cudaStream_t)stream); });
+}
+
+size_t vcsr_linear_grad_workspace(const vcsr_linear_grad_args *a) {
+  if (!a || a->M <= 0 || a->N <= 0 || a->K < 0) return 0;
+  return vcsr::layer::grad_plan(a).total;
+}
+
+}  // extern "C"

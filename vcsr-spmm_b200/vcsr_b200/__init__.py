@@ -89,6 +89,50 @@ class _PlanInfo(C.Structure):
                 ("seg_rows", C.c_int64), ("seg_only", C.c_int)]
 
 
+class _RmsnormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("weight", C.c_void_p),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("sum", C.c_void_p), ("lds", C.c_int64),
+                ("rstd", C.c_void_p), ("scale", C.c_void_p), ("eps", C.c_float),
+                ("x_dtype", C.c_int), ("w_dtype", C.c_int), ("y_dtype", C.c_int)]
+
+
+class _RmsnormGradArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int64), ("dy", C.c_void_p), ("lddy", C.c_int64),
+                ("s", C.c_void_p), ("lds", C.c_int64), ("weight", C.c_void_p),
+                ("rstd", C.c_void_p), ("dsum", C.c_void_p), ("ldds", C.c_int64),
+                ("dx", C.c_void_p), ("lddx", C.c_int64), ("dweight", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("x_dtype", C.c_int), ("w_dtype", C.c_int), ("dy_dtype", C.c_int)]
+
+
+class _AdamwStepArgs(C.Structure):
+    _fields_ = [("grads", C.c_void_p), ("g_dtype", C.c_int), ("m", C.c_void_p),
+                ("v", C.c_void_p), ("m_scale", C.c_void_p), ("u_scale", C.c_void_p),
+                ("dither", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double),
+                ("beta2", C.c_double), ("eps", C.c_double), ("weight_decay", C.c_double),
+                ("grad_scale", C.c_float), ("step", C.c_int64)]
+
+
+class _LinearArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("x_scale", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("y", C.c_void_p),
+                ("ldy", C.c_int64), ("pre", C.c_void_p), ("ldp", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("dtype", C.c_int), ("out_dtype", C.c_int), ("act", C.c_int)]
+
+
+class _LinearGradArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("dy", C.c_void_p),
+                ("lddy", C.c_int64), ("pre", C.c_void_p), ("ldp", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64), ("dx", C.c_void_p),
+                ("lddx", C.c_int64), ("dw", C.c_void_p), ("lddw", C.c_int64),
+                ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("dtype", C.c_int), ("act", C.c_int)]
+
+
 _LIB = None
 
 # every function of include/vcsr_spmm.h with its ctypes signature
@@ -154,6 +198,20 @@ _SIGS = {
                                                _i32p]),
     "vcsr_csr_row_panel": (C.c_int, [C.POINTER(_Csr), C.c_int, C.c_int,
                                      C.POINTER(_Csr)]),
+    "vcsr_rmsnorm": (C.c_int, [C.POINTER(_RmsnormArgs), C.c_void_p]),
+    "vcsr_rmsnorm_grad": (C.c_int, [C.POINTER(_RmsnormGradArgs), C.c_void_p]),
+    "vcsr_rmsnorm_grad_workspace": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "vcsr_dequantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                                  C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
+    "vcsr_adamw_state_values": (C.c_int64, [C.c_int, C.c_void_p]),
+    "vcsr_adamw_create": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p,
+                                    C.c_int, C.c_int, C.POINTER(C.c_void_p), C.c_void_p]),
+    "vcsr_adamw_step": (C.c_int, [C.c_void_p, C.POINTER(_AdamwStepArgs), C.c_void_p]),
+    "vcsr_adamw_destroy": (None, [C.c_void_p]),
+    "vcsr_linear": (C.c_int, [C.POINTER(_LinearArgs), C.c_void_p]),
+    "vcsr_linear_workspace": (C.c_size_t, [C.POINTER(_LinearArgs)]),
+    "vcsr_linear_grad": (C.c_int, [C.POINTER(_LinearGradArgs), C.c_void_p]),
+    "vcsr_linear_grad_workspace": (C.c_size_t, [C.POINTER(_LinearGradArgs)]),
     "vcsr_mgpu_create": (C.c_int, [C.POINTER(_Csr), C.c_int, _i32p,
                                    C.POINTER(_PlanParams), C.POINTER(C.c_void_p)]),
     "vcsr_mgpu_set_b": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int,
