@@ -615,6 +615,12 @@ typedef struct vcsr_linear_grad_args {
 vcsr_status vcsr_linear_grad(const vcsr_linear_grad_args *a, vcsr_stream_t stream);
 size_t vcsr_linear_grad_workspace(const vcsr_linear_grad_args *a);
 
+/* Synchronises `stream` and reports (and clears) a bounded wait that ran out
+ * in a kernel of vcsr_linear or vcsr_linear_grad on the current device:
+ * VCSR_ERR_TIMEOUT with the barrier named in vcsr_last_error(), as
+ * vcsr_plan_check does for a plan. */
+vcsr_status vcsr_layers_check(vcsr_stream_t stream);
+
 /* -------------------------------------------------------------- multi-GPU */
 
 /* nnz-balanced row panels: cuts[0] = 0, cuts[parts] = M, cut k is the row

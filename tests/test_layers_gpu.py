@@ -305,6 +305,24 @@ def test_linear_sizes(M, N, K, dtype):
     check_linear(M, N, K, dtype, act="silu", bias=True, residual=True, pre=True)
 
 
+# outputs of many tiles: more than one per pair of SMs, ragged at both edges
+@gpu
+@pytest.mark.parametrize("M,N,K", [(2500, 1300, 200), (5001, 2000, 64), (4096, 4096, 1024), (257, 9000, 72)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32, E4M3])
+def test_linear_many_tiles(M, N, K, dtype):
+    check_linear(M, N, K, dtype, act="gelu", bias=True, residual=True, pre=True)
+    L.check()
+
+
+# k long enough to be split, over and under the number of parts
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 128, 8192), (5, 129, 4097), (16, 1024, 16384), (40, 256, 5000), (130, 300, 9000)])
+@pytest.mark.parametrize("dtype", [BF16, F32, E4M3])
+def test_linear_long_sums(M, N, K, dtype):
+    check_linear(M, N, K, dtype, bias=True, residual=True)
+    L.check()
+
+
 @gpu
 @pytest.mark.parametrize("M", [1, 40, 300])
 @pytest.mark.parametrize("dtype", [BF16, F32, E4M3])
@@ -406,6 +424,14 @@ def check_linear_backward(M, N, K, dtype, act, pads=(0, 0, 0, 0)):
 @pytest.mark.parametrize("dtype,act", [(BF16, "gelu"), (F16, "silu"), (F32, "gelu"), (F32, None), (BF16, None), (F16, "relu")])
 def test_linear_backward(M, N, K, dtype, act):
     check_linear_backward(M, N, K, dtype, act)
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(2600, 1000, 1111), (3000, 2048, 2304), (9000, 40, 2000)])
+@pytest.mark.parametrize("dtype,act", [(BF16, "gelu"), (F16, None), (F32, "silu")])
+def test_linear_backward_many_tiles(M, N, K, dtype, act):
+    check_linear_backward(M, N, K, dtype, act)
+    L.check()
 
 
 @gpu

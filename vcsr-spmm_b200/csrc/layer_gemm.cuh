@@ -52,7 +52,12 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
   return 1.0f;
 }
 
+// On the FP32 units: any operands.
 vcsr_status launch_gemm_simt(const Gemm &g, cudaStream_t st);
+// On the tensor cores: 16-bit operands, and 8-bit ones stored along k, whose
+// bases and pitches are multiples of 16 bytes (tc_aligned); K > 0.
+vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st);
+bool tc_aligned(const void *p, int64_t ld, int dtype);
 
 }  // namespace layer
 }  // namespace vcsr

@@ -1,0 +1,576 @@
+// layer_gemm_tc.cu — the product of 16- and 8-bit operands on the tensor cores
+// (tcgen05, kind::f16 and kind::f8f6f4, FP32 accumulators in tensor memory).
+//
+// out[r, f] = epilogue(sum_k Q(r, k) P(f, k)).  P, the operand of the output's
+// contiguous index f, is the MMA's M side, so a tensor-memory lane is an
+// output column: the epilogue's warps read 32 lanes of one accumulator column
+// at a time and store (and load the residual) 32 neighbouring values of one
+// output row, without a transposition through shared memory.  Operands come by
+// TMA in 128-byte rows (128-byte swizzle): stored along k, 64 16-bit (128 8-bit)
+// values of k per row and stage; stored along f or r, 64 of them per row and a
+// row per k.  Reads past an operand's edge are zeros.
+//
+// Two kernels, by the size of the output:
+//
+// gemm_pair_kernel — many rows: persistent pairs of CTAs (cta_group::2), 256
+// features x 256 rows per pair and tile.  Each CTA stages 128 rows of each
+// operand (32 KB per 64 values of k, half of what a CTA alone with a 128 x 256
+// tile would read from L2 per MMA), two accumulators alternate, so that the
+// epilogue of a tile runs under the next tile's MMAs.  Bound by the tensor cores.
+//
+// gemm_split_kernel — few rows or few tiles: one tile of 128 features x 16 to
+// 128 rows per cluster of 1 to 8 CTAs, which split k between them and join their
+// partial sums through distributed shared memory in rank order (no workspace, no
+// atomics: the same result on every run).  For few rows it is bound by reading
+// the weights once; the split is what puts every SM on that.
+//
+// Every wait is bounded: a role that gives up records where, the CTA drains its
+// own copies and MMAs, frees its tensor memory and returns, and vcsr_layers_check
+// reports it.
+#include <algorithm>
+
+#include "layer_gemm.cuh"
+#include "spmm_tc.h"
+#include "tcgen05.cuh"
+
+namespace vcsr {
+namespace layer {
+namespace {
+
+using namespace tc;
+
+constexpr int kPRows = 128;         // rows of P per CTA
+constexpr int kPBytes = kPRows * 128;
+constexpr int kRing = 192 * 1024;   // stage ring of a CTA, bytes
+
+__device__ int g_wait_error = 0;  // wait site | block << 4 of the first wait that ran out
+
+struct TcArgs {
+  int P, Q;        // extents of f and r
+  int blocks;      // 128-byte blocks of k
+  int block_k;     // values of k in one
+  int p_mn, q_mn;  // operand stored along its own index
+  uint32_t idesc;
+  int tiles_p, tiles_q;
+  Epilogue e;
+};
+
+// Activation of N values, the branch outside the loop.
+template <int N>
+__device__ __forceinline__ void activate_all(int act, float *z) {
+  if (act == VCSR_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_RELU, z[j]);
+  } else if (act == VCSR_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_GELU, z[j]);
+  } else if (act == VCSR_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_SILU, z[j]);
+  }
+}
+
+// The epilogue of output column f, rows r0 + j * step (j < n of N).
+template <int N>
+__device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int step, int n, float *z) {
+  if (e.row_scale) {
+    const float cs = e.col_scale[f];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) z[j] *= e.row_scale[r0 + j * step] * cs;
+  }
+  with_type(e.type, [&](auto type) {
+    using T = decltype(type);
+    if (e.bias) {
+      const float b = widen(static_cast<const T *>(e.bias)[f]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) z[j] += b;
+    }
+    if (e.pre) {
+      T *p = static_cast<T *>(e.pre) + (int64_t)r0 * e.ldp + f;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) p[(int64_t)j * step * e.ldp] = narrow<T>(z[j]);
+    }
+    activate_all<N>(e.act, z);
+    if (e.residual) {
+      const T *p = static_cast<const T *>(e.residual) + (int64_t)r0 * e.ldr + f;
+      T res[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) res[j] = p[(int64_t)j * step * e.ldr];
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n) z[j] += widen(res[j]);
+    }
+    T *p = static_cast<T *>(e.out) + (int64_t)r0 * e.ldo + f;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) p[(int64_t)j * step * e.ldo] = narrow<T>(z[j]);
+  });
+}
+
+// Descriptor of one MMA's slice (32 bytes of k, or 16 rows of k) of a staged
+// operand, and how far it moves from slice to slice.  Along k: 8-row groups of
+// 128-byte rows 1024 bytes apart.  Along the operand's own index: chunks of 64
+// values 8192 bytes apart (a box each), groups of 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int mn, int slice) {
+  return mn ? smem_desc(addr + slice * 2048, 8192, 1024, 2)
+            : smem_desc(addr + slice * 32, 16, 1024, 2);
+}
+
+// Copies of `rows` rows (a multiple of 64 where mn) of an operand, block b of
+// k, to `dst`; LOAD(dst, x, y) issues one.
+template <class LOAD>
+__device__ __forceinline__ void load_operand(unsigned char *dst, int mn, int row0, int rows, int b,
+                                             int block_k, LOAD &&load) {
+  if (mn) {
+    for (int c = 0; c < rows; c += 64) load(dst + c * 128, row0 + c, b * block_k);
+  } else {
+    load(dst, b * block_k, row0);
+  }
+}
+
+// ------------------------------------------------------------ split kernel
+
+constexpr int kSplitThreads = 192;
+
+template <int BN>
+constexpr int kSplitStages = kRing / (kPBytes + BN * 128);
+template <int BN>
+constexpr size_t kSplitSmem = (size_t)kSplitStages<BN> * (kPBytes + BN * 128) + 1024 + 512;
+
+template <int BN, bool CODES>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    gemm_split_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap mp,
+                      const __grid_constant__ CUtensorMap mq, int splits) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char *ring = reinterpret_cast<unsigned char *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int kStages = kSplitStages<BN>, kStage = kPBytes + BN * 128;
+  constexpr uint32_t kColumns = BN < 32 ? 32 : BN;
+  uint64_t *full = reinterpret_cast<uint64_t *>(ring + kStages * kStage), *empty = full + kStages;
+  uint64_t *done = empty + kStages;
+  uint32_t *holder = reinterpret_cast<uint32_t *>(done + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int tile = blockIdx.x / splits;
+  const int f0 = tile % a.tiles_p * kPRows, r0 = tile / a.tiles_p * BN;
+  const int b0 = (int)((int64_t)a.blocks * rank / splits),
+            b1 = (int)((int64_t)a.blocks * (rank + 1) / splits);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) tmem_alloc<1>(holder, kColumns);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *holder;
+  int consumed = b0;  // blocks of k
+
+  if (warp == 4) {
+    if (lane == 0) {
+      for (int b = b0; b < b1; ++b) {
+        const int g = b - b0, s = g % kStages;
+        if (g >= kStages && !mbar_wait(empty + s, (uint32_t)((g / kStages - 1) & 1), abort_flag, kWaitEmpty))
+          break;
+        unsigned char *st = ring + s * kStage;
+        mbar_arrive_tx(full + s, kStage);
+        load_operand(st, a.p_mn, f0, kPRows, b, a.block_k,
+                     [&](void *d, int x, int y) { tma_load_2d(d, &mp, x, y, full + s); });
+        load_operand(st + kPBytes, a.q_mn, r0, BN, b, a.block_k,
+                     [&](void *d, int x, int y) { tma_load_2d(d, &mq, x, y, full + s); });
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      for (int b = b0; b < b1; ++b) {
+        const int g = b - b0, s = g % kStages;
+        if (!mbar_wait(full + s, (uint32_t)((g / kStages) & 1), abort_flag, kWaitFull)) break;
+        fence_after_sync();
+        const uint32_t pa = smem_u32(ring + s * kStage), qa = pa + kPBytes;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma<1, CODES>(tmem, slice_desc(pa, a.p_mn, k), slice_desc(qa, a.q_mn, k), a.idesc,
+                        (b > b0 || k > 0) ? 1u : 0u);
+        mma_commit(empty + s);
+        ++consumed;
+      }
+      mma_commit(done);
+      volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
+      if (!mbar_wait(done, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
+      if (consumed < b1) {  // copies that nobody waited for land before the CTA leaves
+        for (int b = consumed; b < b1; ++b) {
+          const int g = b - b0;
+          if (!mbar_wait(full + g % kStages, (uint32_t)((g / kStages) & 1), &keep, kWaitFull)) break;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const bool ok = *abort_flag == 0;
+  const int nr = min(BN, a.Q - r0);  // output rows of the tile
+  if (splits == 1) {
+    if (warp < 4 && ok) {
+      const int f = f0 + warp * 32 + lane;
+      constexpr int kN = BN < 32 ? BN : 32;
+      for (int c = 0; c < nr; c += kN) {
+        float z[kN];
+        if constexpr (kN == 16)
+          tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
+        else
+          tmem_load32(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
+        tmem_load_wait();
+        if (f < a.P) finish<kN>(a.e, f, r0 + c, 1, nr - c, z);
+        __syncwarp();
+      }
+    }
+  } else {
+    // partial sums, [row][feature], over the ring: its copies have landed and
+    // its MMAs have read it
+    float *part = reinterpret_cast<float *>(ring);
+    if (warp < 4) {
+      constexpr int kN = BN < 32 ? BN : 32;
+      for (int c = 0; c < nr; c += kN) {
+        float z[kN];
+        if constexpr (kN == 16)
+          tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
+        else
+          tmem_load32(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
+        tmem_load_wait();
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          if (c + j < nr) part[(c + j) * kPRows + warp * 32 + lane] = z[j];
+      }
+    }
+    cluster_sync();
+    // rank k finishes rows k, k + splits, ...
+    if (warp < 4 && ok) {
+      const int f = f0 + threadIdx.x;
+      const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
+      constexpr int kN = 8;
+      for (int c = rank; c < nr; c += splits * kN) {
+        float z[kN];
+#pragma unroll
+        for (int j = 0; j < kN; ++j) z[j] = 0.0f;
+        for (int k = 0; k < splits; ++k) {
+          const uint32_t peer = cluster_map(mine, k);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) {
+            const int row = c + j * splits;
+            if (row < nr) {
+              float v;
+              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kPRows * 4));
+              z[j] += v;
+            }
+          }
+        }
+        if (f < a.P) finish<kN>(a.e, f, r0 + c, splits, (nr - c + splits - 1) / splits, z);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // until every peer has read this CTA's partial sums
+  }
+  if (!ok && threadIdx.x == 0) atomicCAS(&g_wait_error, 0, *abort_flag | (int)(blockIdx.x << 4));
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 4) {
+    fence_after_sync();
+    tmem_free<1>(tmem, kColumns);
+  }
+}
+
+// ------------------------------------------------------------- pair kernel
+
+constexpr int kPairEpilogueWarps = 8;
+constexpr int kPairThreads = 32 * (kPairEpilogueWarps + 2);
+
+template <int BN>
+constexpr int kPairStages = kRing / (kPBytes + BN / 2 * 128);
+template <int BN>
+constexpr size_t kPairSmem = (size_t)kPairStages<BN> * (kPBytes + BN / 2 * 128) + 1024 + 512;
+
+// Tile t in an order that keeps the tiles in flight in a block of 8 P tiles by
+// as many Q tiles as it takes: each staged row is then read from L2 by the
+// whole block at about the same time.
+__device__ __forceinline__ void tile_of(int t, int tiles_p, int tiles_q, int *p, int *q) {
+  constexpr int kGroup = 8;
+  const int per = kGroup * tiles_q, g = t / per, first = g * kGroup,
+            width = min(kGroup, tiles_p - first), in = t - g * per;
+  *p = first + in % width;
+  *q = in / width;
+}
+
+template <int BN, bool CODES>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_pair_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap mp,
+                     const __grid_constant__ CUtensorMap mq) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char *ring = reinterpret_cast<unsigned char *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int kStages = kPairStages<BN>, kQRows = BN / 2, kStage = kPBytes + kQRows * 128;
+  constexpr uint32_t kColumns = 2 * BN;
+  uint64_t *full = reinterpret_cast<uint64_t *>(ring + kStages * kStage), *empty = full + kStages;
+  uint64_t *dfull = empty + kStages, *dfree = dfull + 2, *drain = dfree + 2;
+  uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
+  volatile int *consumed = abort_flag + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / 2, stride = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(dfull + b, 1);
+      mbar_init(dfree + b, 2 * kPairEpilogueWarps);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *consumed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kPairEpilogueWarps) tmem_alloc<2>(holder, kColumns);
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers are ready
+  fence_after_sync();
+  const uint32_t tmem = *holder;
+
+  if (warp == kPairEpilogueWarps) {
+    if (lane == 0) {
+      // copies of this CTA's half, complete on the leader's barrier
+      int g = 0;
+      bool go = true;
+      for (int t = first; t < tiles && go; t += stride) {
+        int tp, tq;
+        tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
+        const int f0 = tp * 2 * kPRows + (int)rank * kPRows, r0 = tq * BN + (int)rank * kQRows;
+        for (int b = 0; b < a.blocks; ++b, ++g) {
+          const int s = g % kStages;
+          if (g >= kStages &&
+              !mbar_wait(empty + s, (uint32_t)((g / kStages - 1) & 1), abort_flag, kWaitEmpty)) {
+            go = false;
+            break;
+          }
+          unsigned char *st = ring + s * kStage;
+          const uint32_t bar = cluster_map(smem_u32(full + s), 0);
+          if (rank == 0) mbar_arrive_tx(full + s, 2 * kStage);
+          load_operand(st, a.p_mn, f0, kPRows, b, a.block_k,
+                       [&](void *d, int x, int y) { tma_load_2d_pair(d, &mp, x, y, bar); });
+          load_operand(st + kPBytes, a.q_mn, r0, kQRows, b, a.block_k,
+                       [&](void *d, int x, int y) { tma_load_2d_pair(d, &mq, x, y, bar); });
+        }
+      }
+    }
+  } else if (warp == kPairEpilogueWarps + 1) {
+    if (lane == 0 && rank == 0) {
+      int g = 0, lt = 0;
+      bool go = true;
+      for (int t = first; t < tiles && go; t += stride, ++lt) {
+        const int buf = lt & 1;
+        if (lt >= 2 && !mbar_wait(dfree + buf, (uint32_t)(((lt - 2) >> 1) & 1), abort_flag, kWaitAccFree))
+          break;
+        fence_after_sync();
+        for (int b = 0; b < a.blocks; ++b, ++g) {
+          const int s = g % kStages;
+          if (!mbar_wait(full + s, (uint32_t)((g / kStages) & 1), abort_flag, kWaitFull)) {
+            go = false;
+            break;
+          }
+          fence_after_sync();
+          const uint32_t pa = smem_u32(ring + s * kStage), qa = pa + kPBytes;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma<2, CODES>(tmem + buf * BN, slice_desc(pa, a.p_mn, k), slice_desc(qa, a.q_mn, k),
+                          a.idesc, (b > 0 || k > 0) ? 1u : 0u);
+          mma_commit_pair(empty + s);
+        }
+        if (go) mma_commit_pair(dfull + buf);
+      }
+      *consumed = g;
+      // every MMA issued here has finished before the pair leaves
+      asm volatile(
+          "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+              smem_u32(drain))
+          : "memory");
+      volatile int keep = 0;
+      if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
+    }
+  } else {
+    int lt = 0;
+    for (int t = first; t < tiles; t += stride, ++lt) {
+      int tp, tq;
+      tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
+      const int buf = lt & 1, quarter = warp & 3, half = warp >> 2;
+      if (!mbar_wait(dfull + buf, (uint32_t)((lt >> 1) & 1), abort_flag, kWaitAccFull)) break;
+      __syncwarp();
+      fence_after_sync();
+      const int f = tp * 2 * kPRows + (int)rank * kPRows + quarter * 32 + lane;
+      const int r0 = tq * BN + half * (BN / 2);
+      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + half * (BN / 2);
+#pragma unroll 1
+      for (int c = 0; c < BN / 2; c += 32) {
+        float z[32];
+        tmem_load32(at + c, z);
+        tmem_load_wait();
+        if (c + 32 == BN / 2) {  // the accumulator is read: free it for the tile after next
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(cluster_map(smem_u32(dfree + buf), 0));
+        }
+        if (f < a.P && r0 + c < a.Q) finish<32>(a.e, f, r0 + c, 1, a.Q - r0 - c, z);
+        __syncwarp();
+      }
+    }
+  }
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();
+  cluster_sync();  // no copy, commit or arrival of the peer is still to come
+  fence_after_sync();
+  if (*abort_flag && threadIdx.x == 0) {
+    if (rank == 0) {  // copies that no MMA waited for
+      volatile int keep = 0;
+      for (int g = *consumed, n = 0; n < kStages; ++g, ++n)
+        if (!mbar_wait(full + g % kStages, (uint32_t)((g / kStages) & 1), &keep, kWaitFull, 1 << 16)) break;
+    }
+    atomicCAS(&g_wait_error, 0, *abort_flag | (int)(blockIdx.x << 4));
+  }
+  __syncthreads();
+  cluster_sync();
+  if (warp == kPairEpilogueWarps) tmem_free<2>(tmem, kColumns);
+}
+
+// ------------------------------------------------------------------- host
+
+// A tensor map of an operand (rows x K values): boxes of 128 bytes of k by
+// box_rows rows, or of 64 rows by 64 values of k where it lies along its rows.
+vcsr_status make_map(CUtensorMap *m, const Operand &o, int64_t rows, int64_t K, int dtype, int box_rows) {
+  EncodeTiledFn enc;
+  VCSR_TRY(tensor_map_encoder(&enc));
+  const size_t size = type_size(dtype);
+  const cuuint64_t dims[2] = {(cuuint64_t)(o.transposed ? rows : K), (cuuint64_t)(o.transposed ? K : rows)};
+  const cuuint64_t strides[1] = {(cuuint64_t)o.ld * size};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)(o.transposed ? 64 : box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == VCSR_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                   : dtype == VCSR_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                       : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUresult r = enc(m, type, 2, const_cast<void *>(o.p), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VCSR_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return VCSR_OK;
+}
+
+template <class K, class... A>
+vcsr_status launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
+  VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)grid);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  VCSR_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
+  return VCSR_OK;
+}
+
+template <int BN>
+vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
+  CUtensorMap mp, mq;
+  VCSR_TRY(make_map(&mp, g.b, g.N, g.K, g.dtype, kPRows));
+  VCSR_TRY(make_map(&mq, g.a, g.M, g.K, g.dtype, BN));
+  a.tiles_p = (int)ceil_div(a.P, kPRows);
+  a.tiles_q = (int)ceil_div(a.Q, BN);
+  const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
+  // clusters that fill the GPU, with at least two blocks of k per CTA
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= sm_count() && a.blocks >= 4 * splits) splits *= 2;
+  if (tiles * splits > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
+  const int grid = (int)(tiles * splits);
+  const int format = g.dtype == VCSR_BF16 ? 1 : 0;
+  a.idesc = instr_desc(format, a.p_mn, a.q_mn, 128, BN);
+  return g.dtype == VCSR_E4M3
+             ? launch(gemm_split_kernel<BN, true>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits)
+             : launch(gemm_split_kernel<BN, false>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits);
+}
+
+template <int BN>
+vcsr_status launch_pair(TcArgs &a, const Gemm &g, cudaStream_t st) {
+  CUtensorMap mp, mq;
+  VCSR_TRY(make_map(&mp, g.b, g.N, g.K, g.dtype, kPRows));
+  VCSR_TRY(make_map(&mq, g.a, g.M, g.K, g.dtype, BN / 2));
+  a.tiles_p = (int)ceil_div(a.P, 2 * kPRows);
+  a.tiles_q = (int)ceil_div(a.Q, BN);
+  const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
+  if (tiles > (1 << 30)) return fail(VCSR_ERR_RANGE, "more than 2^30 output tiles");
+  const int grid = 2 * (int)std::min<int64_t>(tiles, sm_count() / 2);
+  const int format = g.dtype == VCSR_BF16 ? 1 : 0;
+  a.idesc = instr_desc(format, a.p_mn, a.q_mn, 256, BN);
+  return g.dtype == VCSR_E4M3
+             ? launch(gemm_pair_kernel<BN, true>, grid, kPairThreads, kPairSmem<BN>, 2, st, a, mp, mq)
+             : launch(gemm_pair_kernel<BN, false>, grid, kPairThreads, kPairSmem<BN>, 2, st, a, mp, mq);
+}
+
+}  // namespace
+
+bool tc_aligned(const void *p, int64_t ld, int dtype) {
+  return aligned(p, 16) && (ld * (int64_t)type_size(dtype)) % 16 == 0;
+}
+
+vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st) {
+  TcArgs a{};
+  a.P = (int)g.N;
+  a.Q = (int)g.M;
+  a.block_k = 128 / (int)type_size(g.dtype);
+  a.blocks = (int)ceil_div(g.K, a.block_k);
+  a.p_mn = g.b.transposed;
+  a.q_mn = g.a.transposed;
+  a.e = g.e;
+  const int64_t pair_tiles = ceil_div(g.N, 256) * ceil_div(g.M, 256);
+  if (pair_tiles >= sm_count() / 4) return launch_pair<256>(a, g, st);
+  if (g.M <= 16 && !a.q_mn) return launch_split<16>(a, g, st);
+  if (g.M <= 32 && !a.q_mn) return launch_split<32>(a, g, st);
+  if (g.M <= 64) return launch_split<64>(a, g, st);
+  return launch_split<128>(a, g, st);
+}
+
+vcsr_status check_waits(cudaStream_t st) {
+  VCSR_CUDA(cudaStreamSynchronize(st));
+  int word = 0, zero = 0;
+  VCSR_CUDA(cudaMemcpyFromSymbol(&word, g_wait_error, sizeof(int)));
+  if (!word) return VCSR_OK;
+  VCSR_CUDA(cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int)));
+  char text[128];
+  describe_tc_error(word, text, sizeof(text));
+  return fail(VCSR_ERR_TIMEOUT, "%s", text);
+}
+
+}  // namespace layer
+}  // namespace vcsr
+
+extern "C" vcsr_status vcsr_layers_check(vcsr_stream_t stream) {
+  vcsr::clear_error();
+  return vcsr::no_throw([&] { return vcsr::layer::check_waits((cudaStream_t)stream); });
+}

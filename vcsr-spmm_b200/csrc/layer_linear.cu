@@ -86,11 +86,80 @@ void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *parti
 constexpr size_t kAlign = 256;
 size_t round_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
+// Copies a matrix whose base or pitch is no multiple of 16 bytes, which TMA
+// cannot read, to one whose pitch is: a thread writes 16 bytes.
+template <class T>
+__global__ void __launch_bounds__(256)
+    pack_kernel(const T *src, int64_t ld, T *dst, int64_t ldd, int64_t rows, int64_t cols) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t per_row = ldd / V, total = rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * V;
+    Vec<T, V> v;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v.v[j] = c + j < cols ? src[r * ld + c + j] : T{};
+    store_vec<T, V>(dst + r * ldd + c, v);
+  }
+}
+
+int64_t packed_pitch(int64_t cols, int dtype) {
+  const int64_t v = 16 / (int64_t)type_size(dtype);
+  return ceil_div(cols, v) * v;
+}
+
+// What the tensor cores read of a matrix: itself, or a copy in the workspace.
+struct Packed {
+  bool copy = false;
+  int64_t ld = 0;
+  size_t bytes = 0;
+};
+Packed packed(const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+  Packed k;
+  k.ld = rows == 1 ? packed_pitch(cols, dtype) : ld;  // the pitch of one row is free
+  if (dtype != VCSR_F32 && !tc_aligned(p, k.ld, dtype)) {
+    k.copy = true;
+    k.ld = packed_pitch(cols, dtype);
+    k.bytes = round_up((size_t)rows * k.ld * type_size(dtype));
+  }
+  return k;
+}
+vcsr_status pack(const Packed &k, const void *&p, int64_t ld, int64_t rows, int64_t cols, int dtype,
+                 char *&ws, cudaStream_t st) {
+  if (!k.copy) return VCSR_OK;
+  const int64_t total = rows * k.ld * (int64_t)type_size(dtype) / 16;
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256), (int64_t)sm_count() * 8);
+  if (dtype == VCSR_E4M3)
+    pack_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t *>(p), ld,
+                                               reinterpret_cast<uint8_t *>(ws), k.ld, rows, cols);
+  else
+    pack_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(p), ld,
+                                                reinterpret_cast<uint16_t *>(ws), k.ld, rows, cols);
+  VCSR_CUDA(cudaGetLastError());
+  p = ws;
+  ws += k.bytes;
+  return VCSR_OK;
+}
+
+vcsr_status launch_gemm(const Gemm &g, cudaStream_t st) {
+  return g.dtype == VCSR_F32 || g.K == 0 ? launch_gemm_simt(g, st) : launch_gemm_tc(g, st);
+}
+
+vcsr_status check_workspace(const void *ws, size_t bytes, size_t need) {
+  if (need > 0 && (!ws || bytes < need || !aligned(ws, kAlign)))
+    return fail(VCSR_ERR_INVALID, "the call needs %zu bytes of 256-byte aligned workspace", need);
+  return VCSR_OK;
+}
+
 vcsr_status check_sizes(int64_t M, int64_t N, int64_t K) {
   if (M < 0 || N < 0 || K < 0) return fail(VCSR_ERR_INVALID, "negative size");
   if (M > 0x7fffffffll || N > 0x7fffffffll || K > 0x7fffffffll)
     return fail(VCSR_ERR_RANGE, "a size above 2^31 - 1");
   return VCSR_OK;
+}
+
+size_t linear_workspace(const vcsr_linear_args *a) {
+  if (a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
+  return packed(a->x, a->ldx, a->M, a->K, a->dtype).bytes + packed(a->w, a->ldw, a->N, a->K, a->dtype).bytes;
 }
 
 vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
@@ -115,24 +184,39 @@ vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
   VCSR_TRY(check_matrix("residual", a->residual, a->ldr, a->N, a->out_dtype, true));
   VCSR_TRY(check_matrix("y", a->y, a->ldy, a->N, a->out_dtype, false));
   VCSR_TRY(check_matrix("pre", a->pre, a->ldp, a->N, a->out_dtype, true));
-  Gemm g{a->M, a->N, a->K, {a->x, a->ldx, false}, {a->w, a->ldw, false}, a->dtype,
-         {a->x_scale, a->w_scale, a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy, a->ldp, a->act,
-          a->out_dtype}};
-  return launch_gemm_simt(g, st);
+  const Packed px = packed(a->x, a->ldx, a->M, a->K, a->dtype), pw = packed(a->w, a->ldw, a->N, a->K, a->dtype);
+  VCSR_TRY(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(a)));
+  const void *x = a->x, *w = a->w;
+  if (a->K > 0) {
+    char *ws = static_cast<char *>(a->workspace);
+    VCSR_TRY(pack(px, x, a->ldx, a->M, a->K, a->dtype, ws, st));
+    VCSR_TRY(pack(pw, w, a->ldw, a->N, a->K, a->dtype, ws, st));
+  }
+  return launch_gemm({a->M, a->N, a->K, {x, px.ld, false}, {w, pw.ld, false}, a->dtype,
+                      {a->x_scale, a->w_scale, a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy,
+                       a->ldp, a->act, a->out_dtype}}, st);
 }
 
+// The parts of the gradient's workspace: dz (or an aligned dy), partial sums
+// of dbias, aligned x and w.
 struct GradPlan {
   int64_t lddz = 0;
   size_t dz = 0, partial = 0, total = 0;
+  Packed dy, x, w;
 };
 
 GradPlan grad_plan(const vcsr_linear_grad_args *a) {
   GradPlan p;
-  p.lddz = ceil_div(a->N, 8) * 8;
+  p.lddz = packed_pitch(a->N, a->dtype);
   if (a->act != VCSR_ACT_NONE && (a->dx || a->dw))
     p.dz = round_up((size_t)a->M * p.lddz * type_size(a->dtype));
   if (a->dbias) p.partial = round_up((size_t)dz_chunks(a->M, a->N) * a->N * sizeof(float));
-  p.total = p.dz + p.partial;
+  if (a->K > 0) {
+    if (!p.dz && (a->dx || a->dw)) p.dy = packed(a->dy, a->lddy, a->M, a->N, a->dtype);
+    if (a->dw) p.x = packed(a->x, a->ldx, a->M, a->K, a->dtype);
+    if (a->dx) p.w = packed(a->w, a->ldw, a->N, a->K, a->dtype);
+  }
+  p.total = p.dz + p.partial + p.dy.bytes + p.x.bytes + p.w.bytes;
   return p;
 }
 
@@ -163,9 +247,7 @@ vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
   if (a->K > 0 && a->dx) VCSR_TRY(check_matrix("w", a->w, a->ldw, a->K, a->dtype, false));
   if (a->K > 0 && a->dw) VCSR_TRY(check_matrix("x", a->x, a->ldx, a->K, a->dtype, false));
   const GradPlan p = grad_plan(a);
-  if (p.total > 0 &&
-      (!a->workspace || a->workspace_bytes < p.total || !aligned(a->workspace, kAlign)))
-    return fail(VCSR_ERR_INVALID, "the call needs %zu bytes of 256-byte aligned workspace", p.total);
+  VCSR_TRY(check_workspace(a->workspace, a->workspace_bytes, p.total));
   char *ws = static_cast<char *>(a->workspace);
   void *dz = p.dz ? ws : nullptr;
   float *partial = p.partial ? reinterpret_cast<float *>(ws + p.dz) : nullptr;
@@ -181,19 +263,23 @@ vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
       VCSR_TRY(column_sum(partial, (int)dz_chunks(a->M, a->N), a->N, a->dbias, a->dtype, st));
   }
   if (a->K == 0) return VCSR_OK;
-  const void *d = dz ? dz : a->dy;
-  const int64_t ldd = dz ? p.lddz : a->lddy;
+  ws += p.dz + p.partial;
+  const void *d = dz ? dz : a->dy, *x = a->x, *w = a->w;
+  if (!dz) VCSR_TRY(pack(p.dy, d, a->lddy, a->M, a->N, a->dtype, ws, st));
+  VCSR_TRY(pack(p.x, x, a->ldx, a->M, a->K, a->dtype, ws, st));
+  VCSR_TRY(pack(p.w, w, a->ldw, a->N, a->K, a->dtype, ws, st));
+  const int64_t ldd = dz ? p.lddz : p.dy.ld;
   Epilogue e{};
   e.type = a->dtype;
   if (a->dx) {
     e.out = a->dx;
     e.ldo = a->lddx;
-    VCSR_TRY(launch_gemm_simt({a->M, a->K, a->N, {d, ldd, false}, {a->w, a->ldw, true}, a->dtype, e}, st));
+    VCSR_TRY(launch_gemm({a->M, a->K, a->N, {d, ldd, false}, {w, p.w.ld, true}, a->dtype, e}, st));
   }
   if (a->dw) {
     e.out = a->dw;
     e.ldo = a->lddw;
-    VCSR_TRY(launch_gemm_simt({a->N, a->K, a->M, {d, ldd, true}, {a->x, a->ldx, true}, a->dtype, e}, st));
+    VCSR_TRY(launch_gemm({a->N, a->K, a->M, {d, ldd, true}, {x, p.x.ld, true}, a->dtype, e}, st));
   }
   return VCSR_OK;
 }
@@ -209,7 +295,9 @@ vcsr_status vcsr_linear(const vcsr_linear_args *a, vcsr_stream_t stream) {
   return vcsr::no_throw([&] { return vcsr::layer::linear(a, (cudaStream_t)stream); });
 }
 
-size_t vcsr_linear_workspace(const vcsr_linear_args *) { return 0; }
+size_t vcsr_linear_workspace(const vcsr_linear_args *a) {
+  return a ? vcsr::layer::linear_workspace(a) : 0;
+}
 
 vcsr_status vcsr_linear_grad(const vcsr_linear_grad_args *a, vcsr_stream_t stream) {
   vcsr::clear_error();

@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 from . import (VcsrError, _AdamwStepArgs, _check, _LinearArgs, _LinearGradArgs, _RmsnormArgs,
-               _RmsnormGradArgs, lib)
+               _RmsnormGradArgs, _stream, lib)
 
 INVALID, UNSUPPORTED = 1, 5
 F32, BF16, F16, E4M3 = range(4)
@@ -303,6 +303,12 @@ def linear_backward(dy, x, w, pre=None, act=None, need_dx=True, need_dw=True,
         a.workspace, a.workspace_bytes = ws.data_ptr(), n
     _check(L.vcsr_linear_grad(a, _current_stream(dy.device.index)))
     return LinearGrad(dx, dw, db)
+
+
+def check(stream=None):
+    """Synchronise and raise VcsrError (status 7) if a bounded wait of linear's or
+    linear_backward's kernels on the current device ran out since the last check."""
+    _check(lib().vcsr_layers_check(_stream(stream)))
 
 
 # -------------------------------------------------------------- the optimizer
