@@ -1,0 +1,456 @@
+// layer_gemm_f32.cu — the product of FP32 operands on the tensor cores at FP32
+// accuracy (tcgen05 kind::f16 on bfloat16 parts).
+//
+// An FP32 value is the exact sum of three bfloat16 values, its leading, middle
+// and last 8 significant bits (cut off, not rounded, so that the leading part
+// never overflows).  Of the nine products of two values' parts the six down to
+// 2^-16 of the largest are summed; the three left out are below 2^-24 of it.  A
+// tensor core may cut its sums off, not round them, so no sum is long: each 32
+// values of k start a new accumulator in tensor memory, smallest products first,
+// and the epilogue's warps add the accumulators in registers, rounded to
+// nearest.  An output that comes out NaN or infinite (a product of an infinity's
+// zero parts is NaN) is summed again in FP32 from the operands themselves.  Values
+// below 2^-110 lose bits under 2^-133, the least bfloat16.
+//
+// Tile: 128 features x 32, 64 or 128 rows per CTA (layer_gemm_tc.cu says why
+// features are the MMA's M side), 32 values of k per stage.  One thread brings the
+// FP32 tiles in by TMA (128-byte rows, 128-byte swizzle); eight warps split them
+// into three planes of bfloat16 in the order the MMAs read (stored along k: 64-byte
+// rows, 64-byte swizzle; along the operand's own index: 128-byte rows of 64 values);
+// one thread issues 12 MMAs per stage; eight warps drain the accumulators, two of
+// which alternate.  All roles run at once.  128 x 128 tiles are bound by shared
+// memory: per stage 32 KB in, 32 KB read and 48 KB written by the split, 96 KB read
+// by the MMAs.  Persistent over tiles; where tiles are too few for the SMs, clusters
+// of 2 to 8 CTAs split k and join their sums in rank order through distributed
+// shared memory.
+#include <algorithm>
+
+#include "layer_gemm_tc.cuh"
+#include "spmm_tc.h"
+
+namespace vcsr {
+namespace layer {
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 128;  // features per tile
+constexpr int kK = 32;      // values of k per stage
+constexpr int kSplitters = 8, kDrainers = 8;  // warps
+constexpr int kLoadWarp = kSplitters + kDrainers, kMmaWarp = kLoadWarp + 1;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kPlane = kRows * kK * 2;  // one part of P's tile, bytes
+
+// Bytes and counts of the FP32 stages and of the split ones.
+template <int BN>
+constexpr int kRaw = (kRows + BN) * kK * 4;
+template <int BN>
+constexpr int kSplit = 3 * (kRows + BN) * kK * 2;
+template <int BN>
+constexpr int kRaws = BN == 128 ? 3 : BN == 64 ? 4 : 5;
+template <int BN>
+constexpr int kSplits = BN == 128 ? 2 : 3;
+template <int BN>
+constexpr size_t kSmem = (size_t)kRaws<BN> * kRaw<BN> + kSplits<BN> * kSplit<BN> + 1024 + 512;
+// Warps that drain: 32 lanes by BN / 2 columns each, or, with 32 columns, by all
+// of them.
+template <int BN>
+constexpr int kDraining = BN == 32 ? 4 : 8;
+
+__device__ int g_wait_error = 0;
+
+struct F32Args {
+  const float *p, *q;
+  int64_t ldp, ldq;
+  int P, Q, K;
+  int p_mn, q_mn;  // operand stored along its own index
+  int tiles_p, tiles_q, splits;
+  Epilogue e;
+};
+
+// Copies of one FP32 tile (`rows` by 32 k) to `dst`: a box of 128-byte rows of k,
+// or boxes of 32 rows by 32 k, a 128-byte row per k, 4 KB each.
+__device__ __forceinline__ void load_raw(unsigned char *dst, const CUtensorMap *m, int mn, int row0, int rows,
+                                         int k0, uint64_t *bar) {
+  if (mn) {
+    for (int c = 0; c < rows; c += 32) tma_load_2d(dst + c * 128, m, row0 + c, k0, bar);
+  } else {
+    tma_load_2d(dst, m, k0, row0, bar);
+  }
+}
+
+// Two values' leading 16 bits as one word.
+__device__ __forceinline__ uint32_t pair(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+__device__ __forceinline__ float leading(float x) {
+  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+
+// Splits one tile: `rows` (a multiple of 64, or 32) by 32 values of k from `raw`
+// to three planes, `plane` bytes apart, from `out` on.  A thread takes 8 values
+// that are neighbours in memory: two 16-byte pieces in, one per plane out.  In both
+// orders 8 neighbouring lanes touch all banks once.
+template <int ROWS>
+__device__ __forceinline__ void split_tile(uint32_t raw, uint32_t out, int mn, int t) {
+  constexpr int kPlaneBytes = ROWS * kK * 2;
+#pragma unroll
+  for (int u = 0; u < (ROWS + 63) / 64; ++u) {
+    uint32_t in0, in1, at;
+    int swap = 0;
+    if (mn) {  // row k of 128 bytes: boxes of 32 values in, chunks of 64 out
+      const int k = t >> 3, c = t & 7;
+      const uint32_t box = raw + (u * 2 + (c >> 2)) * 4096 + k * 128;
+      swap = c >> 2;  // the two boxes of a chunk take their pieces in turn
+      in0 = box + (((2 * (c & 3) + swap) ^ (k & 7)) << 4);
+      in1 = box + (((2 * (c & 3) + 1 - swap) ^ (k & 7)) << 4);
+      at = out + u * 4096 + k * 128 + ((c ^ (k & 7)) << 4);
+    } else {  // rows of 128 bytes in, of 64 bytes out
+      const int r = u * 64 + (t >> 2), c = t & 3;
+      if (ROWS < 64 && r >= ROWS) break;
+      in0 = raw + r * 128 + (((2 * c) ^ (r & 7)) << 4);
+      in1 = raw + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4);
+      at = out + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    }
+    float a[4], b[4], v[8];
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3])
+                 : "r"(in0));
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3])
+                 : "r"(in1));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = swap ? b[j] : a[j];
+      v[4 + j] = swap ? a[j] : b[j];
+    }
+#pragma unroll
+    for (int part = 0; part < 3; ++part) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + part * kPlaneBytes),
+                   "r"(pair(v[0], v[1])), "r"(pair(v[2], v[3])), "r"(pair(v[4], v[5])),
+                   "r"(pair(v[6], v[7]))
+                   : "memory");
+      if (part < 2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] -= leading(v[j]);
+      }
+    }
+  }
+}
+
+// Descriptor of the first 16 values of k of a plane; the second 16 and the other
+// planes are further by their distance in 16-byte units.
+__device__ __forceinline__ uint64_t plane_desc(uint32_t addr, int mn) {
+  return mn ? smem_desc(addr, 4096, 1024, 2) : smem_desc(addr, 16, 512, 4);
+}
+
+__device__ __noinline__ float sum_again(const F32Args &a, int f, int r) {
+  float s = 0.0f;
+  for (int64_t k = 0; k < a.K && s == s; ++k)
+    s = fmaf(a.q_mn ? a.q[k * a.ldq + r] : a.q[r * a.ldq + k],
+             a.p_mn ? a.p[k * a.ldp + f] : a.p[f * a.ldp + k], s);
+  return s;
+}
+
+// The epilogue of N rows of column f, infinite and NaN sums made anew.
+template <int N, class GET>
+__device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int step, int n, GET &&get) {
+  if (f >= a.P) n = 0;
+  finish<N, true>(a.e, f, r0, step, n, [&](float *z) {
+    get(z);
+    float total = 0.0f;  // not finite where a sum is not (or where finite ones add up to that)
+#pragma unroll
+    for (int j = 0; j < N; ++j) total += fabsf(z[j]);
+    if (n > 0 && !(total <= 3.402823466e38f)) {
+      float again[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) again[j] = z[j];
+#pragma unroll 1
+      for (int j = 0; j < min(n, N); ++j)
+        if (!(fabsf(again[j]) <= 3.402823466e38f)) again[j] = sum_again(a, f, r0 + j * step);
+#pragma unroll
+      for (int j = 0; j < N; ++j) z[j] = again[j];
+    }
+  });
+}
+
+template <int BN>
+__global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_constant__ F32Args a,
+                                                             const __grid_constant__ CUtensorMap mp,
+                                                             const __grid_constant__ CUtensorMap mq) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  unsigned char *ring = reinterpret_cast<unsigned char *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  constexpr int R = kRaws<BN>, S = kSplits<BN>;
+  constexpr uint32_t kColumns = 2 * BN;
+  constexpr int kWide = BN == 32 ? 32 : BN / 2;  // columns a draining warp sums
+  unsigned char *raw = ring + S * kSplit<BN>;
+  uint64_t *full = reinterpret_cast<uint64_t *>(raw + R * kRaw<BN>), *empty = full + S;
+  uint64_t *rfull = empty + S, *rempty = rfull + R;
+  uint64_t *dfull = rempty + R, *dfree = dfull + 2, *drain = dfree + 2;
+  uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
+  const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / a.splits, stride = gridDim.x / a.splits;
+  const int all = (a.K + kK - 1) / kK;
+  const int b0 = (int)((int64_t)all * rank / a.splits), b1 = (int)((int64_t)all * (rank + 1) / a.splits);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full + s, kSplitters);
+      mbar_init(empty + s, 1);
+    }
+    for (int s = 0; s < R; ++s) {
+      mbar_init(rfull + s, 1);
+      mbar_init(rempty + s, kSplitters);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(dfull + b, 1);
+      mbar_init(dfree + b, kDraining<BN>);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == kMmaWarp) tmem_alloc<1>(holder, kColumns);
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *holder;
+
+  float acc[kWide];  // draining warps
+#pragma unroll
+  for (int j = 0; j < kWide; ++j) acc[j] = 0.0f;
+  const int drainer = warp - kSplitters, quarter = drainer & 3;
+  const int col0 = BN == 32 ? 0 : (drainer >> 2) * kWide;
+
+  if (warp < kSplitters) {
+    int g = 0;
+    bool go = true;
+    for (int t = first; t < tiles && go; t += stride) {
+      for (int b = b0; b < b1; ++b, ++g) {
+        const int r = g % R, s = g % S;
+        if (!mbar_wait(rfull + r, (uint32_t)((g / R) & 1), abort_flag, kWaitFull) ||
+            (g >= S && !mbar_wait(empty + s, (uint32_t)((g / S - 1) & 1), abort_flag, kWaitEmpty))) {
+          go = false;
+          break;
+        }
+        const uint32_t from = smem_u32(raw + r * kRaw<BN>), to = smem_u32(ring + s * kSplit<BN>);
+        split_tile<kRows>(from, to, a.p_mn, threadIdx.x);
+        split_tile<BN>(from + kRows * kK * 4, to + 3 * kPlane, a.q_mn, threadIdx.x);
+        // the MMAs read what was written by plain stores
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(full + s);
+          mbar_arrive(rempty + r);
+        }
+      }
+    }
+  } else if (warp == kLoadWarp) {
+    if (lane == 0) {
+      int g = 0;
+      bool go = true;
+      for (int t = first; t < tiles && go; t += stride) {
+        int tp, tq;
+        tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
+        for (int b = b0; b < b1; ++b, ++g) {
+          const int r = g % R;
+          if (g >= R && !mbar_wait(rempty + r, (uint32_t)((g / R - 1) & 1), abort_flag, kWaitEmpty)) {
+            go = false;
+            break;
+          }
+          unsigned char *to = raw + r * kRaw<BN>;
+          mbar_arrive_tx(rfull + r, kRaw<BN>);
+          load_raw(to, &mp, a.p_mn, tp * kRows, kRows, b * kK, rfull + r);
+          load_raw(to + kRows * kK * 4, &mq, a.q_mn, tq * BN, BN, b * kK, rfull + r);
+        }
+      }
+      // copies that nobody waited for land before the CTA leaves
+      volatile int keep = 0;
+      for (int n = max(0, g - R); n < g && !go; ++n)
+        mbar_wait(rfull + n % R, (uint32_t)((n / R) & 1), &keep, kWaitFull);
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(1, a.p_mn, a.q_mn, kRows, BN);
+      const uint32_t p_step = a.p_mn ? 2048 / 16 : 32 / 16, q_step = a.q_mn ? 2048 / 16 : 32 / 16;
+      int g = 0;
+      bool go = true;
+      for (int t = first; t < tiles && go; t += stride) {
+        for (int b = b0; b < b1; ++b, ++g) {
+          const int s = g % S, buf = g & 1;
+          if (!mbar_wait(full + s, (uint32_t)((g / S) & 1), abort_flag, kWaitFull) ||
+              (g >= 2 && !mbar_wait(dfree + buf, (uint32_t)(((g - 2) >> 1) & 1), abort_flag, kWaitAccFree))) {
+            go = false;
+            break;
+          }
+          fence_after_sync();
+          const uint32_t pa = smem_u32(ring + s * kSplit<BN>), qa = pa + 3 * kPlane;
+          const uint64_t pd = plane_desc(pa, a.p_mn), qd = plane_desc(qa, a.q_mn);
+          // parts of P and Q, smallest products first
+          constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
+#pragma unroll
+          for (int m = 0; m < 6; ++m)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              mma<1, false>(tmem + buf * BN, pd + kPart[m][0] * (kPlane / 16) + k * p_step,
+                            qd + kPart[m][1] * (BN * kK * 2 / 16) + k * q_step, idesc,
+                            (m > 0 || k > 0) ? 1u : 0u);
+          mma_commit(empty + s);
+          mma_commit(dfull + buf);
+        }
+      }
+      mma_commit(drain);
+      volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
+      if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
+    }
+  } else if (drainer >= 0 && drainer < kDraining<BN>) {
+    int g = 0;
+    bool go = true;
+    for (int t = first; t < tiles && go; t += stride) {
+      int tp, tq;
+      tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
+#pragma unroll
+      for (int j = 0; j < kWide; ++j) acc[j] = 0.0f;
+      for (int b = b0; b < b1; ++b, ++g) {
+        const int buf = g & 1;
+        if (!mbar_wait(dfull + buf, (uint32_t)((g >> 1) & 1), abort_flag, kWaitAccFull)) {
+          go = false;
+          break;
+        }
+        __syncwarp();
+        fence_after_sync();
+#pragma unroll
+        for (int c = 0; c < kWide; c += 16) {
+          float z[16];
+          tmem_load16(tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + col0 + c, z);
+          tmem_load_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c + j] += z[j];
+        }
+        fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dfree + buf);
+      }
+      if (go && a.splits == 1) {
+#pragma unroll
+        for (int c = 0; c < kWide; c += 16)
+          finish_f32<16>(a, tp * kRows + quarter * 32 + lane, tq * BN + col0 + c, 1,
+                         a.Q - (tq * BN + col0 + c), [&](float *z) {
+#pragma unroll
+                           for (int j = 0; j < 16; ++j) z[j] = acc[c + j];
+                         });
+      }
+    }
+  }
+  __syncwarp();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const bool ok = *abort_flag == 0;
+  if (a.splits > 1) {  // one tile per cluster
+    int tp, tq;
+    tile_of(first, a.tiles_p, a.tiles_q, &tp, &tq);
+    const int f0 = tp * kRows, r0 = tq * BN, nr = min(BN, a.Q - r0);
+    // sums of this CTA's k, [row][feature], over the ring, which the MMAs have read
+    float *part = reinterpret_cast<float *>(ring);
+    if (drainer >= 0 && drainer < kDraining<BN>) {
+#pragma unroll
+      for (int j = 0; j < kWide; ++j)
+        if (col0 + j < nr) part[(col0 + j) * kRows + quarter * 32 + lane] = acc[j];
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp < 4 && ok) {  // rank k finishes rows k, k + splits, ...
+      const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
+      constexpr int kN = 8;
+      for (int c = rank; c < nr; c += a.splits * kN) {
+        finish_f32<kN>(a, f0 + threadIdx.x, r0 + c, a.splits, (nr - c + a.splits - 1) / a.splits, [&](float *z) {
+#pragma unroll
+          for (int j = 0; j < kN; ++j) z[j] = 0.0f;
+          for (int k = 0; k < a.splits; ++k) {
+            const uint32_t peer = cluster_map(mine, k);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+              const int row = c + j * a.splits;
+              if (row < nr) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kRows * 4));
+                z[j] += v;
+              }
+            }
+          }
+        });
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // until every peer has read this CTA's sums
+  }
+  if (!ok && threadIdx.x == 0) atomicCAS(&g_wait_error, 0, *abort_flag | (int)(blockIdx.x << 4));
+  fence_before_sync();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    fence_after_sync();
+    tmem_free<1>(tmem, kColumns);
+  }
+}
+
+vcsr_status make_map(CUtensorMap *m, const Operand &o, int64_t rows, int64_t K, int box_rows) {
+  EncodeTiledFn enc;
+  VCSR_TRY(tensor_map_encoder(&enc));
+  const cuuint64_t dims[2] = {(cuuint64_t)(o.transposed ? rows : K), (cuuint64_t)(o.transposed ? K : rows)};
+  const cuuint64_t strides[1] = {(cuuint64_t)o.ld * 4};
+  const cuuint32_t box[2] = {32, (cuuint32_t)(o.transposed ? kK : box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(o.p), dims, strides, box,
+                         estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(VCSR_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return VCSR_OK;
+}
+
+template <int BN>
+vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
+  CUtensorMap mp, mq;
+  VCSR_TRY(make_map(&mp, g.b, g.N, g.K, kRows));
+  VCSR_TRY(make_map(&mq, g.a, g.M, g.K, BN));
+  a.tiles_p = (int)ceil_div(a.P, kRows);
+  a.tiles_q = (int)ceil_div(a.Q, BN);
+  const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
+  if (tiles > (1 << 30)) return fail(VCSR_ERR_RANGE, "more than 2^30 output tiles");
+  a.splits = 1;
+  while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && ceil_div(a.K, kK) >= 4 * a.splits) a.splits *= 2;
+  const int grid = a.splits > 1 ? (int)tiles * a.splits : (int)std::min<int64_t>(tiles, sm_count());
+  return launch(gemm_f32_kernel<BN>, grid, kThreads, kSmem<BN>, a.splits, st, a, mp, mq);
+}
+
+}  // namespace
+
+vcsr_status launch_gemm_f32(const Gemm &g, cudaStream_t st) {
+  F32Args a{};
+  a.p = static_cast<const float *>(g.b.p);
+  a.q = static_cast<const float *>(g.a.p);
+  a.ldp = g.b.ld;
+  a.ldq = g.a.ld;
+  a.P = (int)g.N;
+  a.Q = (int)g.M;
+  a.K = (int)g.K;
+  a.p_mn = g.b.transposed;
+  a.q_mn = g.a.transposed;
+  a.e = g.e;
+  if (g.M <= 32 && !a.q_mn) return launch_tiles<32>(a, g, st);
+  if (g.M <= 64) return launch_tiles<64>(a, g, st);
+  return launch_tiles<128>(a, g, st);
+}
+
+vcsr_status take_wait_error_f32(int *word) {
+  const int zero = 0;
+  VCSR_CUDA(cudaMemcpyFromSymbol(word, g_wait_error, sizeof(int)));
+  if (*word) VCSR_CUDA(cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int)));
+  return VCSR_OK;
+}
+
+}  // namespace layer
+}  // namespace vcsr

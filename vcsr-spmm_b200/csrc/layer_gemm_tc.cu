@@ -29,9 +29,8 @@
 // reports it.
 #include <algorithm>
 
-#include "layer_gemm.cuh"
+#include "layer_gemm_tc.cuh"
 #include "spmm_tc.h"
-#include "tcgen05.cuh"
 
 namespace vcsr {
 namespace layer {
@@ -54,70 +53,6 @@ struct TcArgs {
   int tiles_p, tiles_q;
   Epilogue e;
 };
-
-// Activation of N values, the branch outside the loop.
-template <int N>
-__device__ __forceinline__ void activate_all(int act, float *z) {
-  if (act == VCSR_ACT_RELU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_RELU, z[j]);
-  } else if (act == VCSR_ACT_GELU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_GELU, z[j]);
-  } else if (act == VCSR_ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) z[j] = activate(VCSR_ACT_SILU, z[j]);
-  }
-}
-
-// The epilogue of output column f, rows r0 + j * step (j < n of N).
-template <int N>
-__device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int step, int n, float *z) {
-  if (e.row_scale) {
-    const float cs = e.col_scale[f];
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) z[j] *= e.row_scale[r0 + j * step] * cs;
-  }
-  with_type(e.type, [&](auto type) {
-    using T = decltype(type);
-    if (e.bias) {
-      const float b = widen(static_cast<const T *>(e.bias)[f]);
-#pragma unroll
-      for (int j = 0; j < N; ++j) z[j] += b;
-    }
-    if (e.pre) {
-      T *p = static_cast<T *>(e.pre) + (int64_t)r0 * e.ldp + f;
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < n) p[(int64_t)j * step * e.ldp] = narrow<T>(z[j]);
-    }
-    activate_all<N>(e.act, z);
-    if (e.residual) {
-      const T *p = static_cast<const T *>(e.residual) + (int64_t)r0 * e.ldr + f;
-      T res[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < n) res[j] = p[(int64_t)j * step * e.ldr];
-#pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (j < n) z[j] += widen(res[j]);
-    }
-    T *p = static_cast<T *>(e.out) + (int64_t)r0 * e.ldo + f;
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (j < n) p[(int64_t)j * step * e.ldo] = narrow<T>(z[j]);
-  });
-}
-
-// Descriptor of one MMA's slice (32 bytes of k, or 16 rows of k) of a staged
-// operand, and how far it moves from slice to slice.  Along k: 8-row groups of
-// 128-byte rows 1024 bytes apart.  Along the operand's own index: chunks of 64
-// values 8192 bytes apart (a box each), groups of 8 k 1024 bytes apart.
-__device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int mn, int slice) {
-  return mn ? smem_desc(addr + slice * 2048, 8192, 1024, 2)
-            : smem_desc(addr + slice * 32, 16, 1024, 2);
-}
 
 // Copies of `rows` rows (a multiple of 64 where mn) of an operand, block b of
 // k, to `dst`; LOAD(dst, x, y) issues one.
@@ -226,13 +161,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       const int f = f0 + warp * 32 + lane;
       constexpr int kN = BN < 32 ? BN : 32;
       for (int c = 0; c < nr; c += kN) {
-        float z[kN];
-        if constexpr (kN == 16)
-          tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
-        else
-          tmem_load32(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
-        tmem_load_wait();
-        if (f < a.P) finish<kN>(a.e, f, r0 + c, 1, nr - c, z);
+        finish<kN, false>(a.e, f, r0 + c, 1, f < a.P ? nr - c : 0, [&](float *z) {
+          const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + c;
+          if constexpr (kN == 16)
+            tmem_load16(at, z);
+          else
+            tmem_load32(at, z);
+          tmem_load_wait();
+        });
         __syncwarp();
       }
     }
@@ -261,22 +197,22 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
       constexpr int kN = 8;
       for (int c = rank; c < nr; c += splits * kN) {
-        float z[kN];
+        finish<kN, false>(a.e, f, r0 + c, splits, f < a.P ? (nr - c + splits - 1) / splits : 0, [&](float *z) {
 #pragma unroll
-        for (int j = 0; j < kN; ++j) z[j] = 0.0f;
-        for (int k = 0; k < splits; ++k) {
-          const uint32_t peer = cluster_map(mine, k);
+          for (int j = 0; j < kN; ++j) z[j] = 0.0f;
+          for (int k = 0; k < splits; ++k) {
+            const uint32_t peer = cluster_map(mine, k);
 #pragma unroll
-          for (int j = 0; j < kN; ++j) {
-            const int row = c + j * splits;
-            if (row < nr) {
-              float v;
-              asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kPRows * 4));
-              z[j] += v;
+            for (int j = 0; j < kN; ++j) {
+              const int row = c + j * splits;
+              if (row < nr) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kPRows * 4));
+                z[j] += v;
+              }
             }
           }
-        }
-        if (f < a.P) finish<kN>(a.e, f, r0 + c, splits, (nr - c + splits - 1) / splits, z);
+        });
       }
     }
     __syncwarp();
@@ -300,17 +236,6 @@ template <int BN>
 constexpr int kPairStages = kRing / (kPBytes + BN / 2 * 128);
 template <int BN>
 constexpr size_t kPairSmem = (size_t)kPairStages<BN> * (kPBytes + BN / 2 * 128) + 1024 + 512;
-
-// Tile t in an order that keeps the tiles in flight in a block of 8 P tiles by
-// as many Q tiles as it takes: each staged row is then read from L2 by the
-// whole block at about the same time.
-__device__ __forceinline__ void tile_of(int t, int tiles_p, int tiles_q, int *p, int *q) {
-  constexpr int kGroup = 8;
-  const int per = kGroup * tiles_q, g = t / per, first = g * kGroup,
-            width = min(kGroup, tiles_p - first), in = t - g * per;
-  *p = first + in % width;
-  *q = in / width;
-}
 
 template <int BN, bool CODES>
 __global__ void __launch_bounds__(kPairThreads, 1)
@@ -425,15 +350,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + half * (BN / 2);
 #pragma unroll 1
       for (int c = 0; c < BN / 2; c += 32) {
-        float z[32];
-        tmem_load32(at + c, z);
-        tmem_load_wait();
-        if (c + 32 == BN / 2) {  // the accumulator is read: free it for the tile after next
-          fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_at(cluster_map(smem_u32(dfree + buf), 0));
-        }
-        if (f < a.P && r0 + c < a.Q) finish<32>(a.e, f, r0 + c, 1, a.Q - r0 - c, z);
+        finish<32, false>(a.e, f, r0 + c, 1, f < a.P ? a.Q - r0 - c : 0, [&](float *z) {
+          tmem_load32(at + c, z);
+          tmem_load_wait();
+          if (c + 32 == BN / 2) {  // the accumulator is read: free it for the tile after next
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(cluster_map(smem_u32(dfree + buf), 0));
+          }
+        });
         __syncwarp();
       }
     }
@@ -475,24 +400,6 @@ vcsr_status make_map(CUtensorMap *m, const Operand &o, int64_t rows, int64_t K, 
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(VCSR_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-  return VCSR_OK;
-}
-
-template <class K, class... A>
-vcsr_status launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
-  VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3((unsigned)grid);
-  c.blockDim = dim3((unsigned)threads);
-  c.dynamicSmemBytes = smem;
-  c.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  VCSR_CUDA(cudaLaunchKernelEx(&c, kernel, args...));
   return VCSR_OK;
 }
 
@@ -560,8 +467,9 @@ vcsr_status check_waits(cudaStream_t st) {
   VCSR_CUDA(cudaStreamSynchronize(st));
   int word = 0, zero = 0;
   VCSR_CUDA(cudaMemcpyFromSymbol(&word, g_wait_error, sizeof(int)));
+  if (word) VCSR_CUDA(cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int)));
+  if (!word) VCSR_TRY(take_wait_error_f32(&word));
   if (!word) return VCSR_OK;
-  VCSR_CUDA(cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int)));
   char text[128];
   describe_tc_error(word, text, sizeof(text));
   return fail(VCSR_ERR_TIMEOUT, "%s", text);

@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(kDzWarps * 32)
       if (act != VCSR_ACT_NONE) {
         const Vec<T, V> z = load_vec<T, V>(pre + r * ldp + col);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] *= activate_slope(act, widen(z.v[j]));
+        for (int j = 0; j < V; ++j) o[j] *= activate_slope<sizeof(T) == 2>(act, widen(z.v[j]));
         if (dz) store_narrow<T, V>(dz + r * lddz + col, o);
       }
 #pragma unroll
@@ -116,7 +116,7 @@ struct Packed {
 Packed packed(const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
   Packed k;
   k.ld = rows == 1 ? packed_pitch(cols, dtype) : ld;  // the pitch of one row is free
-  if (dtype != VCSR_F32 && !tc_aligned(p, k.ld, dtype)) {
+  if (!tc_aligned(p, k.ld, dtype)) {
     k.copy = true;
     k.ld = packed_pitch(cols, dtype);
     k.bytes = round_up((size_t)rows * k.ld * type_size(dtype));
@@ -131,6 +131,9 @@ vcsr_status pack(const Packed &k, const void *&p, int64_t ld, int64_t rows, int6
   if (dtype == VCSR_E4M3)
     pack_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t *>(p), ld,
                                                reinterpret_cast<uint8_t *>(ws), k.ld, rows, cols);
+  else if (dtype == VCSR_F32)
+    pack_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float *>(p), ld, reinterpret_cast<float *>(ws),
+                                             k.ld, rows, cols);
   else
     pack_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(p), ld,
                                                 reinterpret_cast<uint16_t *>(ws), k.ld, rows, cols);
@@ -140,8 +143,29 @@ vcsr_status pack(const Packed &k, const void *&p, int64_t ld, int64_t rows, int6
   return VCSR_OK;
 }
 
+// A product over no k: act(bias) + residual.
+__global__ void __launch_bounds__(256) empty_sum_kernel(const __grid_constant__ Gemm g) {
+  const Epilogue &e = g.e;
+  for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < g.M * g.N; n += (int64_t)gridDim.x * 256) {
+    const int64_t i = n / g.N, j = n - i * g.N;
+    float z = 0.0f, t = 0.0f;
+    if (e.bias) load_as_float<1>(e.bias, e.type, j, &z);
+    if (e.pre) store_as<1>(e.pre, e.type, i * e.ldp + j, &z);
+    z = activate<false>(e.act, z);
+    if (e.residual) load_as_float<1>(e.residual, e.type, i * e.ldr + j, &t);
+    z += t;
+    store_as<1>(e.out, e.type, i * e.ldo + j, &z);
+  }
+}
+
 vcsr_status launch_gemm(const Gemm &g, cudaStream_t st) {
-  return g.dtype == VCSR_F32 || g.K == 0 ? launch_gemm_simt(g, st) : launch_gemm_tc(g, st);
+  if (g.K == 0) {
+    const int64_t blocks = std::min<int64_t>(ceil_div(g.M * g.N, 256), (int64_t)sm_count() * 16);
+    empty_sum_kernel<<<(unsigned)blocks, 256, 0, st>>>(g);
+    VCSR_CUDA(cudaGetLastError());
+    return VCSR_OK;
+  }
+  return g.dtype == VCSR_F32 ? launch_gemm_f32(g, st) : launch_gemm_tc(g, st);
 }
 
 vcsr_status check_workspace(const void *ws, size_t bytes, size_t need) {
