@@ -85,6 +85,39 @@ def test_rmsnorm(rows, dim, x_dtype, y_dtype):
             close(out.sum, s, U * s.abs())
 
 
+# rows shorter than a 16-byte access, and enough odd ones to start everywhere in it
+@gpu
+@pytest.mark.parametrize("rows,dim", [(20, 1), (9, 3), (31, 5), (700, 17), (33, 1001), (9, 2051), (17, 6003)])
+@pytest.mark.parametrize("x_dtype,y_dtype", [(F32, BF16), (BF16, F32), (F16, F16), (BF16, E4M3)])
+@pytest.mark.parametrize("pad", [0, 2])
+def test_rmsnorm_odd_rows(rows, dim, x_dtype, y_dtype, pad):
+    x, r = randn(rows, dim, dtype=x_dtype, seed=1, pad=pad), randn(rows, dim, dtype=x_dtype, seed=2, pad=pad)
+    w, y = randn(dim, seed=3, offset=1), randn(rows, dim, dtype=BF16, pad=pad).to(y_dtype)
+    if pad:
+        y = torch.zeros(rows, dim + pad, device="cuda").to(y_dtype)[:, :dim]
+    sums = randn(rows, dim, dtype=x_dtype, pad=pad)
+    out = L.rmsnorm(x, w, residual=r, out=y, sum_out=sums, save_rstd=True)
+    s, rstd, ref = norm_ref(x, w, r, 1e-6)
+    close(sums, s, U * s.abs())
+    rel = (dim / 32 + 48) * U
+    if y_dtype == E4M3:
+        top = ref.abs().amax(1)
+        step = torch.maximum(ref.abs() * 2.0 ** -4, (top / 448 * 2.0 ** -10)[:, None]) * (1 + 2.0 ** -10)
+        assert bool(((d(y.float()) * d(out.scale)[:, None] - ref).abs() <= step + rel * ref.abs()).all())
+    else:
+        close(y, ref, rel * ref.abs())
+        dy, ds = randn(rows, dim, dtype=y_dtype, seed=5, pad=pad), randn(rows, dim, dtype=x_dtype, seed=6, pad=pad)
+        dx, dw = L.rmsnorm_backward(dy, sums, w, out.rstd, dsum=ds)
+        rx, rw, h, g = norm_grad_ref(dy, sums, w, out.rstd, ds)
+        terms = (g * h).abs().mean(1, keepdim=True)
+        mag = d(out.rstd)[:, None] * (g.abs() + h.abs() * terms * (dim / 32 + 40)) + d(ds).abs()
+        close(dx, rx, 8 * U * mag)
+        close(dw, rw, (rows + 4) * U * (d(dy) * h).abs().sum(0))
+    if pad and rows > 1:  # what lies between the rows is untouched
+        gaps = sums.as_strided((rows - 1, pad), (dim + pad, 1), sums.storage_offset() + dim)
+        assert bool((gaps == 77.0).all())
+
+
 @gpu
 @pytest.mark.parametrize("x_dtype", [F32, BF16])
 @pytest.mark.parametrize("pad,offset", [(1, 0), (8, 0), (0, 1), (8, 4), (3, 5)])

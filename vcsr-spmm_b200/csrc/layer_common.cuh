@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 
@@ -128,12 +129,28 @@ __device__ __forceinline__ void load_as_float(const void *p, int type, int64_t a
   }
 }
 
+// N values rounded to T, two per conversion where T has 16 bits.
+template <class T, int N>
+__device__ __forceinline__ Vec<T, N> narrow_vec(const float *x) {
+  Vec<T, N> o;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (std::is_same_v<T, __half>)
+        *reinterpret_cast<__half2 *>(o.v + i) = __floats2half2_rn(x[i], x[i + 1]);
+      else
+        *reinterpret_cast<__nv_bfloat162 *>(o.v + i) = __floats2bfloat162_rn(x[i], x[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o.v[i] = narrow<T>(x[i]);
+  }
+  return o;
+}
+
 template <class T, int N>
 __device__ __forceinline__ void store_narrow(T *p, const float *x) {
-  Vec<T, N> o;
-#pragma unroll
-  for (int i = 0; i < N; ++i) o.v[i] = narrow<T>(x[i]);
-  store_vec<T, N>(p, o);
+  store_vec<T, N>(p, narrow_vec<T, N>(x));
 }
 
 // f(T{}) for the element type named by `type`, which is F32, BF16 or F16.
@@ -194,8 +211,9 @@ __device__ __forceinline__ void store_as(void *p, int type, int64_t at, const fl
 // below 2^-108 are first raised, since their reciprocal overflows FP32.
 struct CodeScale {
   float scale, raise, divisor, inverse;
+  template <bool RAISED = true>
   __device__ __forceinline__ float quotient(float x) const {
-    const float a = x * raise, q = a * inverse;
+    const float a = RAISED ? x * raise : x, q = a * inverse;
     return fmaf(fmaf(-q, divisor, a), inverse, q);
   }
 };

@@ -9,14 +9,22 @@
 // join their warps' sums through shared memory.  Rows past 32,768 values
 // do not fit a block's registers and are walked by one block in passes.
 //
+// Rows that do not start on 16 bytes (odd lengths) are still moved 16 bytes at a
+// time where all matrices share their rows' misalignment, as contiguous ones do:
+// vectors are cut at the memory's boundaries, so the first starts up to V - 1 values
+// before the row.  Loads take it whole (it is the end of the row before; values
+// outside the row are then set to zero), stores write its values one by one.  Other
+// layouts are moved by single values: FP32 20000 x 2001 to bf16 216 us that way.
+//
 // Gradient, per row: with h = s rstd, g = dy weight,
 // dx = rstd (g - h mean(g h)) + dsum, dweight = sum over rows of dy h.  Bound
-// by HBM as well.  Teams take every (team count)-th row and keep their
-// columns' dweight sums in registers over all of them; teams of a block join
-// theirs in shared memory, blocks write one partial row each, and a second
-// kernel adds the partial rows in block order (no atomics: the same result on
-// every run).
+// by HBM as well.  Teams take every (team count)-th row, with the next rows on
+// their way while one is worked on, and keep their columns' dweight sums in
+// registers over all of them; teams of a block join theirs in shared memory, blocks
+// write one partial row each, and a second kernel adds the partial rows in block
+// order (no atomics: the same result on every run).
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "layer_common.cuh"
@@ -78,6 +86,51 @@ constexpr int kMostHeld = V == 1 ? 16 : 32;
 template <int V, int E>
 constexpr int kNormBlock = E == kMostHeld<V> ? 1024 : 512;
 constexpr int kGradBlock = 512;
+// What the gradient's registers are sized for: two blocks of 320 threads an SM
+// (rows of 5,120 16-bit values), or of 512 with single values.
+template <int V, int E>
+constexpr int kGradBound = E == 32 ? 512 : V == 1 ? 512 : 640;
+template <int V, int E>
+constexpr int kGradBlocksPerSm = V == 1 && E == 8 ? 2 : 1;
+
+// V values of a row at `at`, a multiple of V less the row's misalignment when
+// RAGGED: `whole` if they may all be read, then those outside the row become zero.
+template <class X, int V, bool RAGGED>
+__device__ __forceinline__ void row_load(const X *row, int at, int dim, bool whole, float *out) {
+  if (whole) {
+    const Vec<X, V> v = load_vec<X, V>(row + at);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      out[j] = !RAGGED || (unsigned)(at + j) < (unsigned)dim ? widen(v.v[j]) : 0.0f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      out[j] = RAGGED && (unsigned)(at + j) < (unsigned)dim ? widen(row[at + j]) : 0.0f;
+  }
+}
+// V values into a row, those in range.
+template <class X, int V, bool RAGGED>
+__device__ __forceinline__ void row_store(X *row, int at, int dim, const float *x) {
+  if (!RAGGED || (at >= 0 && at + V <= dim)) {
+    store_narrow<X, V>(row + at, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if ((unsigned)(at + j) < (unsigned)dim) row[at + j] = narrow<X>(x[j]);
+  }
+}
+// Weights lie from value 0 on, whatever the rows do.
+template <class X, int V, bool RAGGED>
+__device__ __forceinline__ void weight_load(const X *w, int at, int dim, float *out) {
+  if (!RAGGED) {
+    const Vec<X, V> v = load_vec<X, V>(w + at);
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = widen(v.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) out[j] = (unsigned)(at + j) < (unsigned)dim ? widen(w[at + j]) : 0.0f;
+  }
+}
 
 struct NormArgs {
   int64_t rows, dim;
@@ -90,17 +143,18 @@ struct NormArgs {
 };
 
 // Sum or maximum over a team's threads; every thread gets it.  Teams of up to
-// 32 threads are a power of two of neighbouring lanes.
+// 32 threads are a power of two of neighbouring lanes; a larger team has whole
+// warps, `shared` words of its own and the block's barrier `id`.
 template <bool MAX>
-__device__ __forceinline__ float team_reduce(float v, int team, float *shared) {
+__device__ __forceinline__ float team_reduce(float v, int team, float *shared, int id = 0) {
   for (int o = min(team, 32) >> 1; o > 0; o >>= 1) {
     const float w = __shfl_xor_sync(0xffffffffu, v, o);
     v = MAX ? fmaxf(v, w) : v + w;
   }
   if (team > 32) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = team >> 5;
-    if (lane == 0) shared[warp] = v;
-    __syncthreads();
+    const int lane = threadIdx.x & 31, warps = team >> 5;
+    if (lane == 0) shared[threadIdx.x % team >> 5] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(team) : "memory");
     float t = lane < warps ? shared[lane] : 0.0f;
     for (int o = 16; o > 0; o >>= 1) {
       const float w = __shfl_xor_sync(0xffffffffu, t, o);
@@ -112,41 +166,36 @@ __device__ __forceinline__ float team_reduce(float v, int team, float *shared) {
 }
 
 // One row per team; E values per thread, V at a time (V values from one
-// 16-byte access of x, or single values where a pitch, a base or dim is not
-// aligned).
-template <class T, int V, int E>
-__global__ void __launch_bounds__(kNormBlock<V, E>) rmsnorm_kernel(const NormArgs a, int team) {
-  const int dim = (int)a.dim;
+// 16-byte access of x, or single values).
+template <class T, int V, int E, bool RAGGED>
+__global__ void __launch_bounds__(kNormBlock<V, E>)
+    rmsnorm_kernel(const __grid_constant__ NormArgs a, int team) {
   __shared__ float shared[2][32];
+  const int dim = (int)a.dim;
   const int t = threadIdx.x % team;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + threadIdx.x / team;
   const bool live = row < a.rows;
+  const int shift = RAGGED ? (int)(row * a.ldx & (V - 1)) : 0;
   constexpr int kN = E / V;
   float s[E];
   float ss = 0.0f;
   const T *x = static_cast<const T *>(a.x) + row * a.ldx;
   const T *r = static_cast<const T *>(a.residual) + row * a.ldr;
+  // what lies past a row is the next rows', as far as there are some
+  auto whole = [&](int at) { return live && at < dim && (!RAGGED || at + V <= (a.rows - row) * a.dim); };
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    const int at = (t + i * team) * V;
-    if (live && at < dim) {
-      const Vec<T, V> xv = load_vec<T, V>(x + at);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[i * V + j] = widen(xv.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[i * V + j] = 0.0f;
-    }
+    const int at = (t + i * team) * V - shift;
+    row_load<T, V, RAGGED>(x, at, live ? dim : 0, whole(at), s + i * V);
   }
   if (a.residual) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
-      if (live && at < dim) {
-        const Vec<T, V> rv = load_vec<T, V>(r + at);
+      const int at = (t + i * team) * V - shift;
+      float v[V];
+      row_load<T, V, RAGGED>(r, at, live ? dim : 0, whole(at), v);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[i * V + j] += widen(rv.v[j]);
-      }
+      for (int j = 0; j < V; ++j) s[i * V + j] += v[j];
     }
   }
 #pragma unroll
@@ -155,26 +204,23 @@ __global__ void __launch_bounds__(kNormBlock<V, E>) rmsnorm_kernel(const NormArg
     T *so = static_cast<T *>(a.sum) + row * a.lds;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
-      if (live && at < dim) store_narrow<T, V>(so + at, s + i * V);
+      const int at = (t + i * team) * V - shift;
+      if (live && at < dim) row_store<T, V, RAGGED>(so, at, dim, s + i * V);
     }
   }
   ss = team_reduce<false>(ss, team, shared[0]);
   const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
   if (a.rstd && live && t == 0) a.rstd[row] = rstd;
-  float top = 0.0f;
   auto weigh = [&](auto type) {
     using W = decltype(type);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
+      const int at = (t + i * team) * V - shift;
       if (at < dim) {
-        const Vec<W, V> w = load_vec<W, V>(static_cast<const W *>(a.weight) + at);
+        float w[V];
+        weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          s[i * V + j] *= rstd * widen(w.v[j]);
-          top = fmaxf(top, fabsf(s[i * V + j]));
-        }
+        for (int j = 0; j < V; ++j) s[i * V + j] *= rstd * w[j];
       }
     }
   };
@@ -183,15 +229,31 @@ __global__ void __launch_bounds__(kNormBlock<V, E>) rmsnorm_kernel(const NormArg
   else
     weigh(T{});
   if (a.y_dtype == VCSR_E4M3) {
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(s[e]));
     const CodeScale c = code_scale(team_reduce<true>(top, team, shared[1]));
     if (live && t == 0) a.scale[row] = c.scale;
     uint8_t *y = static_cast<uint8_t *>(a.y) + row * a.ldy;
+    if (c.raise == 1.0f) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) s[e] = c.quotient(s[e]);
+      for (int e = 0; e < E; ++e) s[e] = c.quotient<false>(s[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e] = c.quotient<true>(s[e]);
+    }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
-      if (live && at < dim) store_codes<V>(y + at, s + i * V);
+      const int at = (t + i * team) * V - shift;
+      if (live && at < dim) {
+        if (!RAGGED || (at >= 0 && at + V <= dim)) {
+          store_codes<V>(y + at, s + i * V);
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if ((unsigned)(at + j) < (unsigned)dim) y[at + j] = e4m3_code(s[i * V + j]);
+        }
+      }
     }
   } else {
     with_type(a.y_dtype, [&](auto type) {
@@ -199,8 +261,8 @@ __global__ void __launch_bounds__(kNormBlock<V, E>) rmsnorm_kernel(const NormArg
       Y *y = static_cast<Y *>(a.y) + row * a.ldy;
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int at = (t + i * team) * V;
-        if (live && at < dim) store_narrow<Y, V>(y + at, s + i * V);
+        const int at = (t + i * team) * V - shift;
+        if (live && at < dim) row_store<Y, V, RAGGED>(y, at, dim, s + i * V);
       }
     });
   }
@@ -256,60 +318,143 @@ struct GradArgs {
   float *partial;  // blocks x dim; NULL = no dweight
   int64_t lddy, lds, ldds, lddx;
   int w_dtype, dy_dtype;
+  int depth;  // rows in flight per team (16-byte access)
 };
 
-template <class T, int V, int E>
-__global__ void __launch_bounds__(kGradBlock) rmsnorm_grad_kernel(const GradArgs a, int team) {
-  __shared__ float shared[2][32];
-  extern __shared__ float joined[];  // (teams of the block) x dim
+// An asynchronous copy of `bytes` (8, 16 or 32, 8- or 16-byte aligned) of a
+// row into this thread's own place in shared memory.
+__device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if (bytes == 8) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+  } else {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    if (bytes == 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16),
+                   "l"(static_cast<const char *>(src) + 16)
+                   : "memory");
+  }
+}
+
+// Teams take every (team count)-th row.  With 16-byte access a thread copies its
+// own vectors of this row and the next depth - 1 into shared memory ahead of their use
+// (nobody else reads them: no barrier); single values are loaded as they come, by
+// more teams at a time.
+template <class T, int V, int E, bool RAGGED>
+__global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
+    rmsnorm_grad_kernel(const __grid_constant__ GradArgs a, int team) {
+  __shared__ float words[2][kGradBlock / 32];
+  extern __shared__ __align__(16) unsigned char dynamic[];
   constexpr int kN = E / V;
   const int dim = (int)a.dim;
   const int t = threadIdx.x % team, teams = blockDim.x / team, mine = threadIdx.x / team;
+  const int64_t stride = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + mine;
+  const int id = 1 + mine;
+  // the same for all rows of a team: their distance is a multiple of 8
+  const int shift = RAGGED ? (int)(first * a.lds & (V - 1)) : 0;
+  // what lies past a row is the next rows', as far as there are some
+  auto whole = [&](int64_t row, int at) {
+    return row < a.rows && at < dim && (!RAGGED || at + V <= (a.rows - row) * a.dim);
+  };
+  // what one row takes of shared memory, and of it s, dy, dsum
+  const int dy_size = a.dy_dtype == VCSR_F32 ? 4 : 2, slot = team * E;
+  const int dy_at = slot * (int)sizeof(T), ds_at = dy_at + slot * dy_size,
+            row_bytes = ds_at + (a.dsum ? slot * (int)sizeof(T) : 0);
+  unsigned char *ring = dynamic + (size_t)mine * a.depth * row_bytes;
   float dw[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = 0.0f;
-  int flip = 0;  // two sets of shared words: one barrier per row is enough
-  for (int64_t first = (int64_t)blockIdx.x * teams; first < a.rows;
-       first += (int64_t)gridDim.x * teams, flip ^= 1) {
-    const int64_t row = first + mine;
-    const bool live = row < a.rows;
-    const float rstd = live ? a.rstd[row] : 0.0f;
-    const T *s = static_cast<const T *>(a.s) + row * a.lds;
-    float h[E], g[E];
-    float dot = 0.0f;
-    with_type(a.dy_dtype, [&](auto type) {
-      using D = decltype(type);
-      const D *dy = static_cast<const D *>(a.dy) + row * a.lddy;
+
+  auto fetch = [&](int64_t row, int stage) {
+    if (row < a.rows) {
+      unsigned char *to = ring + (size_t)stage * row_bytes;
+      const T *s = static_cast<const T *>(a.s) + row * a.lds;
+      const char *dy = static_cast<const char *>(a.dy) + row * a.lddy * dy_size;
+      const T *ds = static_cast<const T *>(a.dsum) + row * a.ldds;
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int at = (t + i * team) * V;
-        if (live && at < dim) {
-          const Vec<T, V> sv = load_vec<T, V>(s + at);
-          const Vec<D, V> dv = load_vec<D, V>(dy + at);
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            h[i * V + j] = widen(sv.v[j]);
-            g[i * V + j] = widen(dv.v[j]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) h[i * V + j] = g[i * V + j] = 0.0f;
+        const int place = (t + i * team) * V, at = place - shift;
+        if (whole(row, at)) {
+          copy_async(to + place * sizeof(T), s + at, V * sizeof(T));
+          copy_async(to + dy_at + place * dy_size, dy + (int64_t)at * dy_size, V * dy_size);
+          if (a.dsum) copy_async(to + ds_at + place * sizeof(T), ds + at, V * sizeof(T));
         }
       }
-    });
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (V > 1) {
+    for (int k = 0; k + 1 < a.depth; ++k) fetch(first + k * stride, k);
+  }
+
+  int stage = 0, flip = 0;  // two sets of shared words: one barrier per row is enough
+  // every thread of a warp takes the same number of turns (a warp may hold teams)
+  const int64_t warp_first = (int64_t)blockIdx.x * teams + (threadIdx.x & ~31) / team;
+  for (int64_t turn = team > 32 ? first : warp_first, row = first; turn < a.rows;
+       turn += stride, row += stride, flip ^= 1) {
+    const bool live = row < a.rows;
+    const float rstd = live ? a.rstd[row] : 0.0f;
+    float h[E], g[E];
+    const unsigned char *from = ring + (size_t)stage * row_bytes;
+    if constexpr (V > 1) {
+      int next = stage + a.depth - 1;
+      if (next >= a.depth) next -= a.depth;
+      // the place of the row before this one, read by this thread a turn ago
+      fetch(row + (int64_t)(a.depth - 1) * stride, next);
+      if (a.depth == 4)
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+      else if (a.depth == 3)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else if (a.depth == 2)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (++stage == a.depth) stage = 0;
+      const T *s = static_cast<const T *>(a.s) + row * a.lds;
+      with_type(a.dy_dtype, [&](auto type) {
+        using D = decltype(type);
+        const D *dy = static_cast<const D *>(a.dy) + row * a.lddy;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          const int place = (t + i * team) * V, at = place - shift;
+          if (whole(row, at)) {  // from shared memory, the thread's own place
+            row_load<T, V, RAGGED>(reinterpret_cast<const T *>(from) + shift, at, dim, true, h + i * V);
+            row_load<D, V, RAGGED>(reinterpret_cast<const D *>(from + dy_at) + shift, at, dim, true, g + i * V);
+          } else {  // the last row's end, or nothing
+            row_load<T, V, RAGGED>(s, at, live ? dim : 0, false, h + i * V);
+            row_load<D, V, RAGGED>(dy, at, live ? dim : 0, false, g + i * V);
+          }
+        }
+      });
+    } else {
+      with_type(a.dy_dtype, [&](auto type) {
+        using D = decltype(type);
+        const T *s = static_cast<const T *>(a.s) + row * a.lds;
+        const D *dy = static_cast<const D *>(a.dy) + row * a.lddy;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int at = t + e * team;
+          const bool in = live && at < dim;
+          h[e] = in ? widen(s[at]) : 0.0f;
+          g[e] = in ? widen(dy[at]) : 0.0f;
+        }
+      });
+    }
+    float dot = 0.0f;
     auto weigh = [&](auto type) {
       using W = decltype(type);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int at = (t + i * team) * V;
+        const int at = (t + i * team) * V - shift;
         if (at < dim) {
-          const Vec<W, V> w = load_vec<W, V>(static_cast<const W *>(a.weight) + at);
+          float w[V];
+          weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const int e = i * V + j;
             h[e] *= rstd;
             dw[e] = fmaf(g[e], h[e], dw[e]);
-            g[e] *= widen(w.v[j]);
+            g[e] *= w[j];
             dot = fmaf(g[e], h[e], dot);
           }
         }
@@ -319,50 +464,46 @@ __global__ void __launch_bounds__(kGradBlock) rmsnorm_grad_kernel(const GradArgs
       weigh(float{});
     else
       weigh(T{});
-    const float mean = team_reduce<false>(dot, team, shared[flip]) / (float)a.dim;
-    const T *ds = static_cast<const T *>(a.dsum) + row * a.ldds;
+    const float mean = team_reduce<false>(dot, team, words[flip] + mine * (team >> 5), id) / (float)a.dim;
     T *dx = static_cast<T *>(a.dx) + row * a.lddx;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
+      const int at = (t + i * team) * V - shift;
       if (live && at < dim) {
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = rstd * (g[i * V + j] - h[i * V + j] * mean);
         if (a.dsum) {
-          const Vec<T, V> dv = load_vec<T, V>(ds + at);
+          float d[V];
+          if (V > 1 && whole(row, at))
+            row_load<T, V, RAGGED>(reinterpret_cast<const T *>(from + ds_at) + shift, at, dim, true, d);
+          else
+            row_load<T, V, true>(static_cast<const T *>(a.dsum) + row * a.ldds, at, dim, false, d);
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += widen(dv.v[j]);
+          for (int j = 0; j < V; ++j) o[j] += d[j];
         }
-        store_narrow<T, V>(dx + at, o);
+        row_store<T, V, RAGGED>(dx, at, dim, o);
       }
     }
   }
+  if constexpr (V > 1) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!a.partial) return;
   float *out = a.partial + (int64_t)blockIdx.x * a.dim;
-  if (teams == 1) {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int at = (t + i * team) * V;
-      if (at < dim) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) out[at + j] = dw[i * V + j];
-      }
-    }
-    return;
-  }
+  float *joined = reinterpret_cast<float *>(dynamic);  // teams x dim
+  if (teams > 1) __syncthreads();  // every team is done with its rows in shared memory
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
-    const int at = (t + i * team) * V;
-    if (at < dim) {
+    const int at = (t + i * team) * V - shift;
+    float *to = teams == 1 ? out + at : joined + mine * dim + at;
 #pragma unroll
-      for (int j = 0; j < V; ++j) joined[mine * a.dim + at + j] = dw[i * V + j];
-    }
+    for (int j = 0; j < V; ++j)
+      if ((unsigned)(at + j) < (unsigned)dim) to[j] = dw[i * V + j];
   }
+  if (teams == 1) return;
   __syncthreads();
-  for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+  for (int c = threadIdx.x; c < dim; c += blockDim.x) {
     float sum = 0.0f;
-    for (int k = 0; k < teams; ++k) sum += joined[k * a.dim + c];
+    for (int k = 0; k < teams; ++k) sum += joined[k * dim + c];
     out[c] = sum;
   }
 }
@@ -430,10 +571,27 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------ host
 
-// Values per access for rows of `dim` values: 16 bytes of the widest type
-// where every pitch and base allows it, else one value.
-bool vector_rows(int64_t dim, int v, const void *p, int64_t ld, int type) {
-  return !p || (dim % v == 0 && ld % v == 0 && aligned(p, std::min<size_t>(16, v * type_size(type))));
+// How rows of `dim` values are moved: v values of every matrix at once where all
+// rows start on v values, or all are off them alike (weights are then read one by
+// one), else by single values.
+enum Access { kSingle, kRagged, kVector };
+struct Rows {
+  const void *p;
+  int64_t ld;
+  int type;
+};
+Access access_of(int64_t rows, int64_t dim, int v, const void *weight, std::initializer_list<Rows> all) {
+  bool even = dim % v == 0 && aligned(weight, 16), same = true;
+  int64_t first = -1;
+  for (const Rows &r : all) {
+    if (!r.p) continue;
+    if (!aligned(r.p, std::min<size_t>(16, v * type_size(r.type)))) return kSingle;
+    const int64_t off = rows > 1 ? r.ld % v : 0;
+    even = even && off == 0;
+    same = same && (first < 0 || off == first);
+    first = off;
+  }
+  return even ? kVector : same ? kRagged : kSingle;
 }
 
 struct Shape {
@@ -445,7 +603,8 @@ struct Shape {
 // loads in flight a thread and tensor), 8 where there are too few rows to
 // fill the GPU otherwise, 32 where the row is too long.
 template <int V>
-Shape shape_for(int64_t rows, int64_t dim, bool grad) {
+Shape shape_for(int64_t rows, int64_t dim, bool grad, bool ragged) {
+  if (ragged) dim += V - 1;  // a row may start inside its first vector
   Shape s;
   auto most = [&](int held) {
     return (int64_t)held * (grad ? kGradBlock : held == kMostHeld<V> ? 1024 : 512);
@@ -466,54 +625,75 @@ Shape shape_for(int64_t rows, int64_t dim, bool grad) {
   return s;
 }
 
-template <class T, int V>
+template <class T, int V, bool RAGGED>
 void launch_norm(const NormArgs &a, cudaStream_t st) {
-  const Shape s = shape_for<V>(a.rows, a.dim, false);
+  const Shape s = shape_for<V>(a.rows, a.dim, false, RAGGED);
   if (!s.fits) {
     rmsnorm_long_kernel<T><<<(unsigned)a.rows, kMaxThreads, 0, st>>>(a);
     return;
   }
   const unsigned grid = (unsigned)ceil_div(a.rows, s.threads / s.team);
   if (s.held == 8)
-    rmsnorm_kernel<T, V, 8><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, 8, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
   else if (s.held == 16)
-    rmsnorm_kernel<T, V, 16><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, 16, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
   else
-    rmsnorm_kernel<T, V, kMostHeld<V>><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, kMostHeld<V>, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
 }
 
 // Blocks of the gradient kernel, which are also the partial rows of dweight.
-int grad_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, (int64_t)sm_count() * 4); }
+// A multiple of 8 unless every row has a team of its own (see rmsnorm_grad_kernel).
+int grad_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, (int64_t)sm_count() * 2 / 8 * 8); }
 
-template <class T, int V>
-void launch_grad(const GradArgs &a, int blocks, cudaStream_t st) {
-  const Shape s = shape_for<V>(a.rows, a.dim, true);
+// Shared memory of a block's rows in flight: two blocks an SM.
+constexpr size_t kGradRing = 104 * 1024;
+
+template <class T, int V, bool RAGGED>
+vcsr_status launch_grad(GradArgs a, int blocks, cudaStream_t st) {
+  const Shape s = shape_for<V>(a.rows, a.dim, true, RAGGED);
   if (!s.fits) {
     rmsnorm_long_grad_kernel<T><<<(unsigned)a.rows, kMaxThreads, 0, st>>>(a);
     if (a.partial)
       rmsnorm_long_dweight_kernel<T>
           <<<dim3((unsigned)ceil_div(a.dim, 256), (unsigned)blocks), 256, 0, st>>>(a);
-    return;
+    return VCSR_OK;
   }
-  const int teams = s.threads / s.team;
-  const size_t smem = teams > 1 && a.partial ? (size_t)teams * a.dim * sizeof(float) : 0;
-  if (s.held == 8)
-    rmsnorm_grad_kernel<T, V, 8><<<blocks, s.threads, smem, st>>>(a, s.team);
-  else if (s.held == 16)
-    rmsnorm_grad_kernel<T, V, 16><<<blocks, s.threads, smem, st>>>(a, s.team);
-  else
-    rmsnorm_grad_kernel<T, V, kMostHeld<V>><<<blocks, s.threads, smem, st>>>(a, s.team);
+  // blocks of about 512 threads, two an SM: teams that share one join their dweight
+  const int teams = std::max(1, std::min<int>(kGradBlock / s.team, (int)ceil_div(a.rows, blocks)));
+  const int threads = (int)ceil_div(teams * s.team, 32) * 32, in_block = threads / s.team;
+  size_t smem = in_block > 1 && a.partial ? (size_t)in_block * a.dim * sizeof(float) : 0;
+  if (V > 1) {
+    const size_t row = (size_t)s.team * s.held *
+                       ((a.dsum ? 2 : 1) * sizeof(T) + type_size(a.dy_dtype)) * in_block;
+    a.depth = row * 4 <= kGradRing ? 4 : row * 3 <= kGradRing ? 3 : row * 2 <= 2 * kGradRing ? 2 : 1;
+    smem = std::max(smem, row * a.depth);
+  }
+  auto run = [&](auto kernel) -> vcsr_status {
+    VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    kernel<<<blocks, threads, smem, st>>>(a, s.team);
+    return VCSR_OK;
+  };
+  if (s.held == 8) return run(rmsnorm_grad_kernel<T, V, 8, RAGGED>);
+  if (s.held == 16) return run(rmsnorm_grad_kernel<T, V, 16, RAGGED>);
+  return run(rmsnorm_grad_kernel<T, V, kMostHeld<V>, RAGGED>);
 }
 
 template <class F>
-void by_type(int type, bool vec, F &&f) {
+void by_type(int type, Access how, F &&f) {
+  auto go = [&](auto t, auto v) {
+    if (how == kVector)
+      f(t, v, std::false_type{});
+    else if (how == kRagged)
+      f(t, v, std::true_type{});
+    else
+      f(t, std::integral_constant<int, 1>{}, std::false_type{});
+  };
   if (type == VCSR_F32)
-    vec ? f(float{}, std::integral_constant<int, 4>{}) : f(float{}, std::integral_constant<int, 1>{});
+    go(float{}, std::integral_constant<int, 4>{});
   else if (type == VCSR_BF16)
-    vec ? f(__nv_bfloat16{}, std::integral_constant<int, 8>{})
-        : f(__nv_bfloat16{}, std::integral_constant<int, 1>{});
+    go(__nv_bfloat16{}, std::integral_constant<int, 8>{});
   else
-    vec ? f(__half{}, std::integral_constant<int, 8>{}) : f(__half{}, std::integral_constant<int, 1>{});
+    go(__half{}, std::integral_constant<int, 8>{});
 }
 
 vcsr_status rmsnorm(const vcsr_rmsnorm_args *a, cudaStream_t st) {
@@ -538,12 +718,11 @@ vcsr_status rmsnorm(const vcsr_rmsnorm_args *a, cudaStream_t st) {
              a->rstd, a->scale, a->ldx, a->ldr,      a->ldy,    a->lds,     a->eps,
              a->w_dtype, a->y_dtype};
   const int v = a->x_dtype == VCSR_F32 ? 4 : 8;
-  const bool vec = vector_rows(a->dim, v, a->x, a->ldx, a->x_dtype) &&
-                   vector_rows(a->dim, v, a->residual, a->ldr, a->x_dtype) &&
-                   vector_rows(a->dim, v, a->weight, v, a->w_dtype) &&
-                   vector_rows(a->dim, v, a->y, a->ldy, a->y_dtype) &&
-                   vector_rows(a->dim, v, a->sum, a->lds, a->x_dtype);
-  by_type(a->x_dtype, vec, [&](auto t, auto n) { launch_norm<decltype(t), decltype(n)::value>(k, st); });
+  const Access how = access_of(a->rows, a->dim, v, a->weight, {{a->x, a->ldx, a->x_dtype}, {a->residual, a->ldr, a->x_dtype},
+                                                    {a->y, a->ldy, a->y_dtype}, {a->sum, a->lds, a->x_dtype}});
+  by_type(a->x_dtype, how, [&](auto t, auto n, auto ragged) {
+    launch_norm<decltype(t), decltype(n)::value, decltype(ragged)::value>(k, st);
+  });
   VCSR_CUDA(cudaGetLastError());
   return VCSR_OK;
 }
@@ -578,15 +757,15 @@ vcsr_status rmsnorm_grad(const vcsr_rmsnorm_grad_args *a, cudaStream_t st) {
   }
   GradArgs k{a->rows, a->dim, a->dy, a->s, a->weight, a->dsum, a->rstd, a->dx,
              a->dweight ? static_cast<float *>(a->workspace) : nullptr,
-             a->lddy, a->lds, a->ldds, a->lddx, a->w_dtype, a->dy_dtype};
+             a->lddy, a->lds, a->ldds, a->lddx, a->w_dtype, a->dy_dtype, 0};
   const int v = a->x_dtype == VCSR_F32 ? 4 : 8;
-  const bool vec = vector_rows(a->dim, v, a->dy, a->lddy, a->dy_dtype) &&
-                   vector_rows(a->dim, v, a->s, a->lds, a->x_dtype) &&
-                   vector_rows(a->dim, v, a->weight, v, a->w_dtype) &&
-                   vector_rows(a->dim, v, a->dsum, a->ldds, a->x_dtype) &&
-                   vector_rows(a->dim, v, a->dx, a->lddx, a->x_dtype);
-  by_type(a->x_dtype, vec,
-          [&](auto t, auto n) { launch_grad<decltype(t), decltype(n)::value>(k, blocks, st); });
+  const Access how = access_of(a->rows, a->dim, v, a->weight, {{a->dy, a->lddy, a->dy_dtype}, {a->s, a->lds, a->x_dtype},
+                                                    {a->dsum, a->ldds, a->x_dtype}, {a->dx, a->lddx, a->x_dtype}});
+  vcsr_status done = VCSR_OK;
+  by_type(a->x_dtype, how, [&](auto t, auto n, auto ragged) {
+    done = launch_grad<decltype(t), decltype(n)::value, decltype(ragged)::value>(k, blocks, st);
+  });
+  VCSR_TRY(done);
   VCSR_CUDA(cudaGetLastError());
   return a->dweight ? column_sum(k.partial, blocks, a->dim, a->dweight, a->w_dtype, st) : VCSR_OK;
 }

@@ -426,7 +426,7 @@ class AdamW:
         return m.view(-1), v.view(-1)
 
     def close(self):
-        if getattr(self, "_h", None):
+        if getattr(self, "_h", None) and lib is not None:  # None while Python shuts down
             lib().vcsr_adamw_destroy(self._h)
         self._h = None
 
