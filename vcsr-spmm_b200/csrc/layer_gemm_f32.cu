@@ -17,8 +17,8 @@
 // FP32 tiles in by TMA (128-byte rows, 128-byte swizzle); eight warps split them
 // into three planes of bfloat16 in the order the MMAs read (stored along k: 64-byte
 // rows, 64-byte swizzle; along the operand's own index: 128-byte rows of 64 values);
-// one thread issues 12 MMAs per stage; eight warps drain the accumulators, two of
-// which alternate.  All roles run at once.  128 x 128 tiles are bound by shared
+// one thread issues 12 MMAs per stage; four to sixteen warps drain the accumulators,
+// two of which alternate.  All roles run at once.  128 x 128 tiles are bound by shared
 // memory: per stage 32 KB in, 32 KB read and 48 KB written by the split, 96 KB read
 // by the MMAs.  Persistent over tiles; where tiles are too few for the SMs, clusters
 // of 2 to 8 CTAs split k and join their sums in rank order through distributed
@@ -36,9 +36,13 @@ using namespace tc;
 
 constexpr int kRows = 128;  // features per tile
 constexpr int kK = 32;      // values of k per stage
-constexpr int kSplitters = 8, kDrainers = 8;  // warps
-constexpr int kLoadWarp = kSplitters + kDrainers, kMmaWarp = kLoadWarp + 1;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+// Warps: eight split, BN / 8 drain (32 lanes by 32 columns each), one loads, one
+// issues MMAs.
+constexpr int kSplitters = 8;
+template <int BN>
+constexpr int kDraining = BN / 8;
+template <int BN>
+constexpr int kThreads = 32 * (kSplitters + kDraining<BN> + 2);
 constexpr int kPlane = kRows * kK * 2;  // one part of P's tile, bytes
 
 // Bytes and counts of the FP32 stages and of the split ones.
@@ -52,10 +56,6 @@ template <int BN>
 constexpr int kSplits = BN == 128 ? 2 : 3;
 template <int BN>
 constexpr size_t kSmem = (size_t)kRaws<BN> * kRaw<BN> + kSplits<BN> * kSplit<BN> + 1024 + 512;
-// Warps that drain: 32 lanes by BN / 2 columns each, or, with 32 columns, by all
-// of them.
-template <int BN>
-constexpr int kDraining = BN == 32 ? 4 : 8;
 
 __device__ int g_wait_error = 0;
 
@@ -152,30 +152,35 @@ __device__ __noinline__ float sum_again(const F32Args &a, int f, int r) {
   return s;
 }
 
-// The epilogue of N rows of column f, infinite and NaN sums made anew.
-template <int N, class GET>
-__device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int step, int n, GET &&get) {
-  if (f >= a.P) n = 0;
-  finish<N, true>(a.e, f, r0, step, n, [&](float *z) {
-    get(z);
-    float total = 0.0f;  // not finite where a sum is not (or where finite ones add up to that)
+// Sums that are not finite made anew, those that IN(j) names.
+template <int N, class IN, class AGAIN>
+__device__ __forceinline__ void mend(float *z, IN &&in, AGAIN &&again) {
+  float total = 0.0f;  // not finite where a sum is not (or where finite ones add up to that)
 #pragma unroll
-    for (int j = 0; j < N; ++j) total += fabsf(z[j]);
-    if (n > 0 && !(total <= 3.402823466e38f)) {
-      float again[N];
+  for (int j = 0; j < N; ++j) total += fabsf(z[j]);
+  if (total <= 3.402823466e38f) return;
+  float copy[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) again[j] = z[j];
+  for (int j = 0; j < N; ++j) copy[j] = z[j];
 #pragma unroll 1
-      for (int j = 0; j < min(n, N); ++j)
-        if (!(fabsf(again[j]) <= 3.402823466e38f)) again[j] = sum_again(a, f, r0 + j * step);
+  for (int j = 0; j < N; ++j)
+    if (in(j) && !(fabsf(copy[j]) <= 3.402823466e38f)) copy[j] = again(j);
 #pragma unroll
-      for (int j = 0; j < N; ++j) z[j] = again[j];
-    }
+  for (int j = 0; j < N; ++j) z[j] = copy[j];
+}
+
+// The epilogue of N rows of column f.
+template <int N, class GET>
+__device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int n, GET &&get) {
+  if (f >= a.P) n = 0;
+  finish<N, true>(a.e, f, r0, 1, n, [&](float *z) {
+    get(z);
+    if (n > 0) mend<N>(z, [&](int j) { return j < n; }, [&](int j) { return sum_again(a, f, r0 + j); });
   });
 }
 
 template <int BN>
-__global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_constant__ F32Args a,
+__global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_constant__ F32Args a,
                                                              const __grid_constant__ CUtensorMap mp,
                                                              const __grid_constant__ CUtensorMap mq) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int R = kRaws<BN>, S = kSplits<BN>;
   constexpr uint32_t kColumns = 2 * BN;
-  constexpr int kWide = BN == 32 ? 32 : BN / 2;  // columns a draining warp sums
+  constexpr int kLoadWarp = kSplitters + kDraining<BN>, kMmaWarp = kLoadWarp + 1;
   unsigned char *raw = ring + S * kSplit<BN>;
   uint64_t *full = reinterpret_cast<uint64_t *>(raw + R * kRaw<BN>), *empty = full + S;
   uint64_t *rfull = empty + S, *rempty = rfull + R;
@@ -219,11 +224,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
   fence_after_sync();
   const uint32_t tmem = *holder;
 
-  float acc[kWide];  // draining warps
+  float acc[32];  // draining warps
 #pragma unroll
-  for (int j = 0; j < kWide; ++j) acc[j] = 0.0f;
-  const int drainer = warp - kSplitters, quarter = drainer & 3;
-  const int col0 = BN == 32 ? 0 : (drainer >> 2) * kWide;
+  for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
+  const int drainer = warp - kSplitters, quarter = drainer & 3, col0 = (drainer >> 2) * 32;
 
   if (warp < kSplitters) {
     int g = 0;
@@ -313,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
       int tp, tq;
       tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
 #pragma unroll
-      for (int j = 0; j < kWide; ++j) acc[j] = 0.0f;
+      for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
       for (int b = b0; b < b1; ++b, ++g) {
         const int buf = g & 1;
         if (!mbar_wait(dfull + buf, (uint32_t)((g >> 1) & 1), abort_flag, kWaitAccFull)) {
@@ -323,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
         __syncwarp();
         fence_after_sync();
 #pragma unroll
-        for (int c = 0; c < kWide; c += 16) {
+        for (int c = 0; c < 32; c += 16) {
           float z[16];
           tmem_load16(tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + col0 + c, z);
           tmem_load_wait();
@@ -336,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
       }
       if (go && a.splits == 1) {
 #pragma unroll
-        for (int c = 0; c < kWide; c += 16)
-          finish_f32<16>(a, tp * kRows + quarter * 32 + lane, tq * BN + col0 + c, 1,
+        for (int c = 0; c < 32; c += 16)
+          finish_f32<16>(a, tp * kRows + quarter * 32 + lane, tq * BN + col0 + c,
                          a.Q - (tq * BN + col0 + c), [&](float *z) {
 #pragma unroll
                            for (int j = 0; j < 16; ++j) z[j] = acc[c + j];
@@ -355,36 +359,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_f32_kernel(const __grid_cons
     tile_of(first, a.tiles_p, a.tiles_q, &tp, &tq);
     const int f0 = tp * kRows, r0 = tq * BN, nr = min(BN, a.Q - r0);
     // sums of this CTA's k, [row][feature], over the ring, which the MMAs have read
-    float *part = reinterpret_cast<float *>(ring);
+    float *sums = reinterpret_cast<float *>(ring);
     if (drainer >= 0 && drainer < kDraining<BN>) {
 #pragma unroll
-      for (int j = 0; j < kWide; ++j)
-        if (col0 + j < nr) part[(col0 + j) * kRows + quarter * 32 + lane] = acc[j];
+      for (int j = 0; j < 32; ++j) sums[(col0 + j) * kRows + quarter * 32 + lane] = acc[j];
     }
     __syncwarp();
     cluster_sync();
-    if (warp < 4 && ok) {  // rank k finishes rows k, k + splits, ...
-      const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
-      constexpr int kN = 8;
-      for (int c = rank; c < nr; c += a.splits * kN) {
-        finish_f32<kN>(a, f0 + threadIdx.x, r0 + c, a.splits, (nr - c + a.splits - 1) / a.splits, [&](float *z) {
-#pragma unroll
-          for (int j = 0; j < kN; ++j) z[j] = 0.0f;
-          for (int k = 0; k < a.splits; ++k) {
-            const uint32_t peer = cluster_map(mine, k);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              const int row = c + j * a.splits;
-              if (row < nr) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kRows * 4));
-                z[j] += v;
-              }
-            }
-          }
-        });
-      }
-    }
+    // CTA k finishes rows k, k + splits, ..., shared out among its warps
+    if (ok)
+      finish_rows<true>(a.e, smem_u32(sums), a.splits, f0, a.P, r0, rank + a.splits * warp,
+                        a.splits * (kThreads<BN> / 32), nr, [&](int f, int r, float *z) {
+                          mend<4>(z, [&](int j) { return f + j < a.P; },
+                                  [&](int j) { return sum_again(a, f + j, r); });
+                        });
     __syncwarp();
     cluster_sync();  // until every peer has read this CTA's sums
   }
@@ -423,7 +411,7 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
   a.splits = 1;
   while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && ceil_div(a.K, kK) >= 4 * a.splits) a.splits *= 2;
   const int grid = a.splits > 1 ? (int)tiles * a.splits : (int)std::min<int64_t>(tiles, sm_count());
-  return launch(gemm_f32_kernel<BN>, grid, kThreads, kSmem<BN>, a.splits, st, a, mp, mq);
+  return launch(gemm_f32_kernel<BN>, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
 }
 
 }  // namespace

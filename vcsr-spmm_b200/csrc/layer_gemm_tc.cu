@@ -68,7 +68,7 @@ __device__ __forceinline__ void load_operand(unsigned char *dst, int mn, int row
 
 // ------------------------------------------------------------ split kernel
 
-constexpr int kSplitThreads = 192;
+constexpr int kSplitThreads = 512;  // for the epilogue: two warps do the rest
 
 template <int BN>
 constexpr int kSplitStages = kRing / (kPBytes + BN * 128);
@@ -156,68 +156,32 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   fence_after_sync();
   const bool ok = *abort_flag == 0;
   const int nr = min(BN, a.Q - r0);  // output rows of the tile
-  if (splits == 1) {
-    if (warp < 4 && ok) {
-      const int f = f0 + warp * 32 + lane;
-      constexpr int kN = BN < 32 ? BN : 32;
-      for (int c = 0; c < nr; c += kN) {
-        finish<kN, false>(a.e, f, r0 + c, 1, f < a.P ? nr - c : 0, [&](float *z) {
-          const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + c;
-          if constexpr (kN == 16)
-            tmem_load16(at, z);
-          else
-            tmem_load32(at, z);
-          tmem_load_wait();
-        });
-        __syncwarp();
-      }
-    }
-  } else {
-    // partial sums, [row][feature], over the ring: its copies have landed and
-    // its MMAs have read it
-    float *part = reinterpret_cast<float *>(ring);
-    if (warp < 4) {
-      constexpr int kN = BN < 32 ? BN : 32;
-      for (int c = 0; c < nr; c += kN) {
-        float z[kN];
-        if constexpr (kN == 16)
-          tmem_load16(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
-        else
-          tmem_load32(tmem + ((uint32_t)(warp * 32) << 16) + c, z);
-        tmem_load_wait();
+  // sums, [row][feature], over the ring: its copies have landed and its MMAs have
+  // read it
+  float *sums = reinterpret_cast<float *>(ring);
+  constexpr int kN = BN < 32 ? BN : 32;
+  for (int c = (warp >> 2) * kN; c < nr; c += kSplitThreads / 128 * kN) {
+    const int lanes = (warp & 3) * 32;
+    float z[kN];
+    if constexpr (kN == 16)
+      tmem_load16(tmem + ((uint32_t)lanes << 16) + c, z);
+    else
+      tmem_load32(tmem + ((uint32_t)lanes << 16) + c, z);
+    tmem_load_wait();
 #pragma unroll
-        for (int j = 0; j < kN; ++j)
-          if (c + j < nr) part[(c + j) * kPRows + warp * 32 + lane] = z[j];
-      }
-    }
-    cluster_sync();
-    // rank k finishes rows k, k + splits, ...
-    if (warp < 4 && ok) {
-      const int f = f0 + threadIdx.x;
-      const uint32_t mine = smem_u32(part) + threadIdx.x * 4;
-      constexpr int kN = 8;
-      for (int c = rank; c < nr; c += splits * kN) {
-        finish<kN, false>(a.e, f, r0 + c, splits, f < a.P ? (nr - c + splits - 1) / splits : 0, [&](float *z) {
-#pragma unroll
-          for (int j = 0; j < kN; ++j) z[j] = 0.0f;
-          for (int k = 0; k < splits; ++k) {
-            const uint32_t peer = cluster_map(mine, k);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-              const int row = c + j * splits;
-              if (row < nr) {
-                float v;
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer + row * kPRows * 4));
-                z[j] += v;
-              }
-            }
-          }
-        });
-      }
-    }
-    __syncwarp();
-    cluster_sync();  // until every peer has read this CTA's partial sums
+    for (int j = 0; j < kN; ++j) sums[(c + j) * kPRows + lanes + lane] = z[j];
   }
+  __syncwarp();
+  if (splits > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  // CTA k of a cluster finishes rows k, k + splits, ..., shared out among its warps
+  if (ok)
+    finish_rows<false>(a.e, smem_u32(sums), splits, f0, a.P, r0, rank + splits * warp,
+                       splits * (kSplitThreads / 32), nr, [](int, int, float *) {});
+  __syncwarp();
+  if (splits > 1) cluster_sync();  // until every peer has read this CTA's sums
   if (!ok && threadIdx.x == 0) atomicCAS(&g_wait_error, 0, *abort_flag | (int)(blockIdx.x << 4));
   fence_before_sync();
   __syncthreads();

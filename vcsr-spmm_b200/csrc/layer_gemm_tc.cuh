@@ -87,6 +87,128 @@ __device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int ste
     with_type(e.type, all);
 }
 
+// 4 neighbouring values, or the first n of them.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load_four(const T *p, int n, float *out) {
+  if constexpr (WHOLE) {
+    const Vec<T, 4> v = load_vec<T, 4>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = widen(v.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) out[j] = widen(p[j]);
+  }
+}
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store_four(T *p, int n, const float *x) {
+  if constexpr (WHOLE) {
+    store_narrow<T, 4>(p, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = narrow<T>(x[j]);
+  }
+}
+
+// Whether all of an epilogue's matrices take 4 values at a time from features that
+// are multiples of 4.
+__device__ __forceinline__ bool fours(const Epilogue &e) {
+  const unsigned mask = e.type == VCSR_F32 ? 15 : 7;
+  auto bits = [&](const void *p, int64_t ld) {
+    return p ? ((unsigned)reinterpret_cast<uintptr_t>(p) & mask) | ((unsigned)ld & 3) : 0u;
+  };
+  return (bits(e.out, e.ldo) | bits(e.pre, e.ldp) | bits(e.residual, e.ldr) | bits(e.bias, 0)) == 0;
+}
+
+// The epilogue from sums in shared memory, `sums` [row][128 features] of this CTA
+// and its peers (splits of them, added in rank order): rows first, first + step, ...
+// below n of the tile at (f0, r0).  A warp takes whole rows, a lane 4 features, two
+// rows at a time; a block needs many warps here, since one alone issues an
+// instruction every 7 cycles or so.  FIX(f, r, z) may mend a lane's 4 sums.
+template <bool F32, class FIX>
+__device__ __forceinline__ void finish_rows(const Epilogue &e, uint32_t sums, int splits, int f0, int P, int r0,
+                                            int first, int step, int n, FIX &&fix) {
+  const int lane = threadIdx.x & 31, f = f0 + lane * 4, left = P - f;
+  auto rows = [&](auto type, auto whole) {
+    using T = decltype(type);
+    constexpr bool WHOLE = decltype(whole)::value;
+    constexpr int kAt = 2;
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, cs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (e.bias) load_four<T, WHOLE>(static_cast<const T *>(e.bias) + f, left, bias);
+    if (e.col_scale) load_four<float, false>(e.col_scale + f, left, cs);
+    const int64_t at = (int64_t)(r0 + first);
+    const T *residual = static_cast<const T *>(e.residual) + at * e.ldr + f;
+    T *pre = static_cast<T *>(e.pre) + at * e.ldp + f, *out = static_cast<T *>(e.out) + at * e.ldo + f;
+    const int64_t dr = step * e.ldr, dp = step * e.ldp, dout = step * e.ldo;
+    for (int row = first; row < n; row += step * kAt) {
+      float z[kAt][4], res[kAt][4];
+#pragma unroll
+      for (int q = 0; q < kAt; ++q)
+        if (e.residual && row + q * step < n) load_four<T, WHOLE>(residual + q * dr, left, res[q]);
+#pragma unroll
+      for (int q = 0; q < kAt; ++q) {
+        const uint32_t from = sums + lane * 16 + (row + q * step) * 512;
+        if (row + q * step >= n) break;
+        if (splits == 1) {
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(z[q][0]), "=f"(z[q][1]), "=f"(z[q][2]), "=f"(z[q][3])
+                       : "r"(from));
+        } else {
+          float part[8][4];  // every peer's asked for before the first is used
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < splits)
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(part[k][0]), "=f"(part[k][1]), "=f"(part[k][2]), "=f"(part[k][3])
+                           : "r"(tc::cluster_map(from, k)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[q][j] = part[0][j];
+#pragma unroll
+          for (int k = 1; k < 8; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (k < splits) z[q][j] += part[k][j];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kAt; ++q) {
+        if (row + q * step >= n) break;
+        const int r = r0 + row + q * step;
+        fix(f, r, z[q]);
+        if (e.row_scale) {
+          const float rs = e.row_scale[r];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[q][j] *= rs * cs[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[q][j] += bias[j];
+        if (e.pre) store_four<T, WHOLE>(pre + q * dp, left, z[q]);
+        activate_all<4, sizeof(T) == 2>(e.act, z[q]);
+        if (e.residual) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[q][j] += res[q][j];
+        }
+        store_four<T, WHOLE>(out + q * dout, left, z[q]);
+      }
+      residual += kAt * dr;
+      pre += kAt * dp;
+      out += kAt * dout;
+    }
+  };
+  if (left <= 0) return;
+  auto all = [&](auto type) {
+    if (left >= 4 && fours(e))
+      rows(type, std::true_type{});
+    else
+      rows(type, std::false_type{});
+  };
+  if constexpr (F32)
+    all(float{});
+  else
+    with_type(e.type, all);
+}
+
 // Descriptor of one MMA's slice (32 bytes of k, or 16 rows of k) of a staged
 // operand, and how far it moves from slice to slice.  Along k: 8-row groups of
 // 128-byte rows 1024 bytes apart.  Along the operand's own index: chunks of 64
