@@ -235,12 +235,11 @@ vcsr_status check_matrix(const char *name, const void *p, int64_t ld, int64_t di
 vcsr_status column_sum(const float *partial, int count, int64_t dim, void *out, int dtype,
                        cudaStream_t st);
 
-inline int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess)
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
+// SMs of the current device, and a kernel's dynamic shared memory limit raised to
+// `bytes`: asked of the runtime once per device (and kernel), since each question
+// costs a good part of a microsecond of every call otherwise (layer_norm.cu).
+int sm_count();
+vcsr_status allow_shared(const void *kernel, size_t bytes);
 
 }  // namespace layer
 }  // namespace vcsr

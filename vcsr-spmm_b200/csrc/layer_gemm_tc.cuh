@@ -231,7 +231,7 @@ __device__ __forceinline__ void tile_of(int t, int tiles_p, int tiles_q, int *p,
 
 template <class K, class... A>
 inline vcsr_status launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
-  VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
   cudaLaunchConfig_t c{};
   c.gridDim = dim3((unsigned)grid);
   c.blockDim = dim3((unsigned)threads);

@@ -24,13 +24,54 @@
 // write one partial row each, and a second kernel adds the partial rows in block
 // order (no atomics: the same result on every run).
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
+#include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "layer_common.cuh"
 
 namespace vcsr {
 namespace layer {
+
+namespace {
+constexpr int kDevices = 64;
+}
+
+int sm_count() {
+  static std::atomic<int> known[kDevices];
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return sms;
+  const int have = known[dev].load(std::memory_order_relaxed);
+  if (have) return have;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess)
+    known[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
+vcsr_status allow_shared(const void *kernel, size_t bytes) {
+  struct Known {
+    const void *kernel;
+    int dev;
+    size_t bytes;
+  };
+  static std::mutex mu;
+  static std::vector<Known> known;
+  int dev = 0;
+  VCSR_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  for (Known &k : known)
+    if (k.kernel == kernel && k.dev == dev) {
+      if (bytes <= k.bytes) return VCSR_OK;
+      VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+      k.bytes = bytes;
+      return VCSR_OK;
+    }
+  VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  known.push_back({kernel, dev, bytes});
+  return VCSR_OK;
+}
 
 vcsr_status check_matrix(const char *name, const void *p, int64_t ld, int64_t dim, int type,
                          bool optional) {
@@ -669,7 +710,7 @@ vcsr_status launch_grad(GradArgs a, int blocks, cudaStream_t st) {
     smem = std::max(smem, row * a.depth);
   }
   auto run = [&](auto kernel) -> vcsr_status {
-    VCSR_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
     kernel<<<blocks, threads, smem, st>>>(a, s.team);
     return VCSR_OK;
   };

@@ -47,20 +47,26 @@ def _type(dtype, name):
         raise VcsrError(UNSUPPORTED, f"{name} has type {dtype}") from None
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _operator(fn):
     """Runs fn with the first tensor's device and the given stream current."""
     @functools.wraps(fn)
     def call(first, *args, stream=None, **kw):
-        if not isinstance(first, torch.Tensor) or not first.is_cuda:
+        try:
+            index = first.get_device()
+        except AttributeError:
+            index = -1
+        if index < 0:
             raise VcsrError(INVALID, f"{fn.__name__} takes CUDA tensors")
-        dev = first.device
-        if stream is None and dev.index == torch.cuda.current_device():
+        if stream is None and index == _current_device():
             return fn(first, *args, **kw)
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             if stream is None:
                 return fn(first, *args, **kw)
             if isinstance(stream, int):
-                stream = torch.cuda.ExternalStream(stream, device=dev)
+                stream = torch.cuda.ExternalStream(stream, device=first.device)
             with torch.cuda.stream(stream):
                 return fn(first, *args, **kw)
     return call
@@ -68,23 +74,24 @@ def _operator(fn):
 
 def _matrix(t, name, like, rows, cols, dtype):
     """t as a (rows, cols) input the C entry points read: its tensor and pitch."""
-    if not isinstance(t, torch.Tensor) or t.device != like.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != like.get_device():
         raise VcsrError(INVALID, f"{name} must be a tensor on {like.device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise VcsrError(UNSUPPORTED, f"{name} has type {t.dtype}, expected {dtype}")
-    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+    if t.shape != (rows, cols):
         raise VcsrError(INVALID, f"{name} must be ({rows}, {cols}), got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t, cols
     s0, s1 = t.stride()
     if (s1 != 1 and cols > 1) or (s0 < cols and rows > 1):
-        t = t.contiguous()
-        s0 = cols
+        return t.contiguous(), cols
     return t, max(s0, cols)
 
 
 def _out(t, name, like, rows, cols, dtype):
     """The output t (checked), or a new one."""
     if t is None:
-        return torch.empty((rows, cols), device=like.device, dtype=dtype), cols
+        return like.new_empty((rows, cols), dtype=dtype), cols
     got, ld = _matrix(t, name, like, rows, cols, dtype)
     if got is not t:
         raise VcsrError(INVALID, f"the columns of {name} must be neighbours in memory")
@@ -92,11 +99,11 @@ def _out(t, name, like, rows, cols, dtype):
 
 
 def _vector(t, name, like, n, dtype):
-    if not isinstance(t, torch.Tensor) or t.device != like.device:
+    if not isinstance(t, torch.Tensor) or t.get_device() != like.get_device():
         raise VcsrError(INVALID, f"{name} must be a tensor on {like.device}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise VcsrError(UNSUPPORTED, f"{name} has type {t.dtype}, expected {dtype}")
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise VcsrError(INVALID, f"{name} must be ({n},), got {tuple(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -108,7 +115,7 @@ def _shape(t, name):
 
 
 def _workspace(n, like):
-    return torch.empty(n, device=like.device, dtype=torch.uint8) if n else None
+    return like.new_empty(n, dtype=torch.uint8) if n else None
 
 
 def _p(t):
@@ -149,12 +156,12 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, out=None, sum_ou
     s, lds = (None, 0)
     if residual is not None or sum_out is not None:
         s, lds = _out(sum_out, "sum_out", x, rows, dim, dt)
-    rstd = torch.empty(rows, device=x.device) if save_rstd else None
-    scale = torch.empty(rows, device=x.device) if y_type == E4M3 else None
+    rstd = x.new_empty(rows, dtype=torch.float32) if save_rstd else None
+    scale = x.new_empty(rows, dtype=torch.float32) if y_type == E4M3 else None
     a = _RmsnormArgs(rows, dim, x.data_ptr(), ldx, _p(residual), ldr, weight.data_ptr(),
                      y.data_ptr(), ldy, _p(s), lds, _p(rstd), _p(scale), eps, x_type,
                      _TYPE[weight.dtype], y_type)
-    _check(lib().vcsr_rmsnorm(a, _current_stream(x.device.index)))
+    _check(lib().vcsr_rmsnorm(a, _current_stream(x.get_device())))
     return NormOut(y, x if s is None else s, rstd, scale)
 
 
@@ -177,17 +184,17 @@ def rmsnorm_backward(dy, s, weight, rstd, dsum=None, need_dweight=True):
     ldds = 0
     if dsum is not None:
         dsum, ldds = _matrix(dsum, "dsum", dy, rows, dim, dt)
-    dx = torch.empty((rows, dim), device=dy.device, dtype=dt)
+    dx = s.new_empty((rows, dim))
     dw = ws = None
     n = 0
     if need_dweight:
-        dw = torch.empty(dim, device=dy.device, dtype=weight.dtype)
+        dw = weight.new_empty(dim)
         n = lib().vcsr_rmsnorm_grad_workspace(rows, dim)
         ws = _workspace(n, dy)
     a = _RmsnormGradArgs(rows, dim, dy.data_ptr(), lddy, s.data_ptr(), lds, weight.data_ptr(),
                          rstd.data_ptr(), _p(dsum), ldds, dx.data_ptr(), dim, _p(dw), _p(ws), n,
                          x_type, _TYPE[weight.dtype], dy_type)
-    _check(lib().vcsr_rmsnorm_grad(a, _current_stream(dy.device.index)))
+    _check(lib().vcsr_rmsnorm_grad(a, _current_stream(dy.get_device())))
     return dx, dw
 
 
@@ -198,10 +205,10 @@ def dequantize(codes, scale, out_dtype=torch.float32, squared=False):
     rows, dim = _shape(codes, "codes")
     codes, ldc = _matrix(codes, "codes", codes, rows, dim, torch.float8_e4m3fn)
     scale = _vector(scale, "scale", codes, rows, torch.float32)
-    out = torch.empty((rows, dim), device=codes.device, dtype=out_dtype)
+    out = codes.new_empty((rows, dim), dtype=out_dtype)
     _check(lib().vcsr_dequantize(codes.data_ptr(), ldc, scale.data_ptr(), rows, dim,
                                  out.data_ptr(), dim, _type(out_dtype, "out"), int(squared),
-                                 _current_stream(codes.device.index)))
+                                 _current_stream(codes.get_device())))
     return out
 
 
@@ -255,16 +262,21 @@ def linear(x, w, bias=None, residual=None, act=None, x_scale=None, w_scale=None,
     if residual is not None:
         residual, ldr = _matrix(residual, "residual", x, M, N, out_dtype)
     y, ldy = _out(out, "out", x, M, N, out_dtype)
-    pre = torch.empty((M, N), device=x.device, dtype=out_dtype) if save_pre else None
+    pre = torch.empty_like(y) if save_pre and out is None else None
+    if save_pre and pre is None:
+        pre = x.new_empty((M, N), dtype=out_dtype)
     a = _LinearArgs(M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _p(x_scale), _p(w_scale),
                     _p(bias), _p(residual), ldr, y.data_ptr(), ldy, _p(pre), N, None, 0, code,
                     out_type, _act(act))
     L = lib()
-    n = L.vcsr_linear_workspace(a)
-    if n:
-        ws = _workspace(n, x)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    _check(L.vcsr_linear(a, _current_stream(x.device.index)))
+    # scratch is for operands that are off 16 bytes
+    size = x.element_size()
+    if (x.data_ptr() | w.data_ptr() | ldx * size | ldw * size) & 15:
+        n = L.vcsr_linear_workspace(a)
+        if n:
+            ws = _workspace(n, x)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _check(L.vcsr_linear(a, _current_stream(x.get_device())))
     return LinearOut(y, pre)
 
 
@@ -291,9 +303,9 @@ def linear_backward(dy, x, w, pre=None, act=None, need_dx=True, need_dw=True,
         pre, ldp = _matrix(pre, "pre", dy, M, N, dt)
     else:
         pre = None
-    dx = torch.empty((M, K), device=dy.device, dtype=dt) if need_dx else None
-    dw = torch.empty((N, K), device=dy.device, dtype=dt) if need_dw else None
-    db = torch.empty(N, device=dy.device, dtype=dt) if need_db else None
+    dx = dy.new_empty((M, K)) if need_dx else None
+    dw = dy.new_empty((N, K)) if need_dw else None
+    db = dy.new_empty(N) if need_db else None
     a = _LinearGradArgs(M, N, K, dy.data_ptr(), lddy, _p(pre), ldp, x.data_ptr(), ldx,
                         w.data_ptr(), ldw, _p(dx), K, _p(dw), K, _p(db), None, 0, code, act)
     L = lib()
@@ -301,7 +313,7 @@ def linear_backward(dy, x, w, pre=None, act=None, need_dx=True, need_dw=True,
     if n:
         ws = _workspace(n, dy)
         a.workspace, a.workspace_bytes = ws.data_ptr(), n
-    _check(L.vcsr_linear_grad(a, _current_stream(dy.device.index)))
+    _check(L.vcsr_linear_grad(a, _current_stream(dy.get_device())))
     return LinearGrad(dx, dw, db)
 
 
