@@ -230,13 +230,14 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   const int drainer = warp - kSplitters, quarter = drainer & 3, col0 = (drainer >> 2) * 32;
 
   if (warp < kSplitters) {
-    int g = 0;
+    RingPlace<R> in;
+    RingPlace<S> out;
     bool go = true;
     for (int t = first; t < tiles && go; t += stride) {
-      for (int b = b0; b < b1; ++b, ++g) {
-        const int r = g % R, s = g % S;
-        if (!mbar_wait(rfull + r, (uint32_t)((g / R) & 1), abort_flag, kWaitFull) ||
-            (g >= S && !mbar_wait(empty + s, (uint32_t)((g / S - 1) & 1), abort_flag, kWaitEmpty))) {
+      for (int b = b0; b < b1; ++b, in.next(), out.next()) {
+        const int r = in.stage, s = out.stage;
+        if (!mbar_wait(rfull + r, in.full(), abort_flag, kWaitFull) ||
+            !mbar_wait(empty + s, out.empty(), abort_flag, kWaitEmpty)) {
           go = false;
           break;
         }
@@ -280,13 +281,14 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     if (lane == 0) {
       const uint32_t idesc = instr_desc(1, a.p_mn, a.q_mn, kRows, BN);
       const uint32_t p_step = a.p_mn ? 2048 / 16 : 32 / 16, q_step = a.q_mn ? 2048 / 16 : 32 / 16;
-      int g = 0;
+      RingPlace<S> at;
+      RingPlace<2> sums;
       bool go = true;
       for (int t = first; t < tiles && go; t += stride) {
-        for (int b = b0; b < b1; ++b, ++g) {
-          const int s = g % S, buf = g & 1;
-          if (!mbar_wait(full + s, (uint32_t)((g / S) & 1), abort_flag, kWaitFull) ||
-              (g >= 2 && !mbar_wait(dfree + buf, (uint32_t)(((g - 2) >> 1) & 1), abort_flag, kWaitAccFree))) {
+        for (int b = b0; b < b1; ++b, at.next(), sums.next()) {
+          const int s = at.stage, buf = sums.stage;
+          if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull) ||
+              !mbar_wait(dfree + buf, sums.empty(), abort_flag, kWaitAccFree)) {
             go = false;
             break;
           }

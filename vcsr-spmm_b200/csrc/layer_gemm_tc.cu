@@ -113,10 +113,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 
   if (warp == 4) {
     if (lane == 0) {
-      for (int b = b0; b < b1; ++b) {
-        const int g = b - b0, s = g % kStages;
-        if (g >= kStages && !mbar_wait(empty + s, (uint32_t)((g / kStages - 1) & 1), abort_flag, kWaitEmpty))
-          break;
+      RingPlace<kStages> at;
+      for (int b = b0; b < b1; ++b, at.next()) {
+        const int s = at.stage;
+        if (!mbar_wait(empty + s, at.empty(), abort_flag, kWaitEmpty)) break;
         unsigned char *st = ring + s * kStage;
         mbar_arrive_tx(full + s, kStage);
         load_operand(st, a.p_mn, f0, kPRows, b, a.block_k,
@@ -127,15 +127,18 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   } else if (warp == 5) {
     if (lane == 0) {
-      for (int b = b0; b < b1; ++b) {
-        const int g = b - b0, s = g % kStages;
-        if (!mbar_wait(full + s, (uint32_t)((g / kStages) & 1), abort_flag, kWaitFull)) break;
+      const uint64_t p_first = stage_desc(smem_u32(ring), a.p_mn),
+                     q_first = stage_desc(smem_u32(ring) + kPBytes, a.q_mn);
+      const uint32_t p_step = slice_step(a.p_mn), q_step = slice_step(a.q_mn);
+      RingPlace<kStages> at;
+      for (int b = b0; b < b1; ++b, at.next()) {
+        const int s = at.stage;
+        if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull)) break;
         fence_after_sync();
-        const uint32_t pa = smem_u32(ring + s * kStage), qa = pa + kPBytes;
+        const uint64_t pd = p_first + s * (kStage / 16), qd = q_first + s * (kStage / 16);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma<1, CODES>(tmem, slice_desc(pa, a.p_mn, k), slice_desc(qa, a.q_mn, k), a.idesc,
-                        (b > b0 || k > 0) ? 1u : 0u);
+          mma<1, CODES>(tmem, pd + k * p_step, qd + k * q_step, a.idesc, (b > b0 || k > 0) ? 1u : 0u);
         mma_commit(empty + s);
         ++consumed;
       }
@@ -143,10 +146,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
       if (!mbar_wait(done, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
       if (consumed < b1) {  // copies that nobody waited for land before the CTA leaves
-        for (int b = consumed; b < b1; ++b) {
-          const int g = b - b0;
-          if (!mbar_wait(full + g % kStages, (uint32_t)((g / kStages) & 1), &keep, kWaitFull)) break;
-        }
+        for (int b = consumed; b < b1; ++b, at.next())
+          if (!mbar_wait(full + at.stage, at.full(), &keep, kWaitFull)) break;
       }
     }
   }
@@ -243,16 +244,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == kPairEpilogueWarps) {
     if (lane == 0) {
       // copies of this CTA's half, complete on the leader's barrier
-      int g = 0;
+      RingPlace<kStages> at;
       bool go = true;
       for (int t = first; t < tiles && go; t += stride) {
         int tp, tq;
         tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
         const int f0 = tp * 2 * kPRows + (int)rank * kPRows, r0 = tq * BN + (int)rank * kQRows;
-        for (int b = 0; b < a.blocks; ++b, ++g) {
-          const int s = g % kStages;
-          if (g >= kStages &&
-              !mbar_wait(empty + s, (uint32_t)((g / kStages - 1) & 1), abort_flag, kWaitEmpty)) {
+        for (int b = 0; b < a.blocks; ++b, at.next()) {
+          const int s = at.stage;
+          if (!mbar_wait(empty + s, at.empty(), abort_flag, kWaitEmpty)) {
             go = false;
             break;
           }
@@ -268,25 +268,29 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == kPairEpilogueWarps + 1) {
     if (lane == 0 && rank == 0) {
-      int g = 0, lt = 0;
+      const uint64_t p_first = stage_desc(smem_u32(ring), a.p_mn),
+                     q_first = stage_desc(smem_u32(ring) + kPBytes, a.q_mn);
+      const uint32_t p_step = slice_step(a.p_mn), q_step = slice_step(a.q_mn);
+      RingPlace<kStages> at;
+      RingPlace<2> acc;  // of the accumulators
+      int g = 0;
       bool go = true;
-      for (int t = first; t < tiles && go; t += stride, ++lt) {
-        const int buf = lt & 1;
-        if (lt >= 2 && !mbar_wait(dfree + buf, (uint32_t)(((lt - 2) >> 1) & 1), abort_flag, kWaitAccFree))
-          break;
+      for (int t = first; t < tiles && go; t += stride, acc.next()) {
+        const int buf = acc.stage;
+        if (!mbar_wait(dfree + buf, acc.empty(), abort_flag, kWaitAccFree)) break;
         fence_after_sync();
-        for (int b = 0; b < a.blocks; ++b, ++g) {
-          const int s = g % kStages;
-          if (!mbar_wait(full + s, (uint32_t)((g / kStages) & 1), abort_flag, kWaitFull)) {
+        for (int b = 0; b < a.blocks; ++b, ++g, at.next()) {
+          const int s = at.stage;
+          if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull)) {
             go = false;
             break;
           }
           fence_after_sync();
-          const uint32_t pa = smem_u32(ring + s * kStage), qa = pa + kPBytes;
+          const uint64_t pd = p_first + s * (kStage / 16), qd = q_first + s * (kStage / 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma<2, CODES>(tmem + buf * BN, slice_desc(pa, a.p_mn, k), slice_desc(qa, a.q_mn, k),
-                          a.idesc, (b > 0 || k > 0) ? 1u : 0u);
+            mma<2, CODES>(tmem + buf * BN, pd + k * p_step, qd + k * q_step, a.idesc,
+                          (b > 0 || k > 0) ? 1u : 0u);
           mma_commit_pair(empty + s);
         }
         if (go) mma_commit_pair(dfull + buf);
@@ -301,12 +305,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
     }
   } else {
-    int lt = 0;
-    for (int t = first; t < tiles; t += stride, ++lt) {
+    RingPlace<2> acc;
+    for (int t = first; t < tiles; t += stride, acc.next()) {
       int tp, tq;
       tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
-      const int buf = lt & 1, quarter = warp & 3, half = warp >> 2;
-      if (!mbar_wait(dfull + buf, (uint32_t)((lt >> 1) & 1), abort_flag, kWaitAccFull)) break;
+      const int buf = acc.stage, quarter = warp & 3, half = warp >> 2;
+      if (!mbar_wait(dfull + buf, acc.full(), abort_flag, kWaitAccFull)) break;
       __syncwarp();
       fence_after_sync();
       const int f = tp * 2 * kPRows + (int)rank * kPRows + quarter * 32 + lane;

@@ -209,14 +209,33 @@ __device__ __forceinline__ void finish_rows(const Epilogue &e, uint32_t sums, in
     with_type(e.type, all);
 }
 
-// Descriptor of one MMA's slice (32 bytes of k, or 16 rows of k) of a staged
-// operand, and how far it moves from slice to slice.  Along k: 8-row groups of
-// 128-byte rows 1024 bytes apart.  Along the operand's own index: chunks of 64
-// values 8192 bytes apart (a box each), groups of 8 k 1024 bytes apart.
-__device__ __forceinline__ uint64_t slice_desc(uint32_t addr, int mn, int slice) {
-  return mn ? tc::smem_desc(addr + slice * 2048, 8192, 1024, 2)
-            : tc::smem_desc(addr + slice * 32, 16, 1024, 2);
+// A place in a ring of N stages and the parity of its round.  full() is the parity
+// that a consumer waits for; a producer waits for the other one on the stage's
+// "empty" barrier, which passes at once in the first round.
+template <int N>
+struct RingPlace {
+  int stage = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == N) {
+      stage = 0;
+      round ^= 1;
+    }
+  }
+  __device__ __forceinline__ uint32_t full() const { return round; }
+  __device__ __forceinline__ uint32_t empty() const { return round ^ 1; }
+};
+
+// Descriptor of a staged operand's first MMA slice (32 bytes of k, or 16 rows of
+// k).  Along k: 8-row groups of 128-byte rows 1024 bytes apart.  Along the operand's
+// own index: chunks of 64 values 8192 bytes apart (a box each), groups of 8 k 1024
+// bytes apart.  Later slices and stages are further by their distance in 16-byte
+// units: the issuing thread adds that, a few instructions per MMA (building each
+// descriptor anew took it longer than the tensor core takes for the MMA).
+__device__ __forceinline__ uint64_t stage_desc(uint32_t addr, int mn) {
+  return mn ? tc::smem_desc(addr, 8192, 1024, 2) : tc::smem_desc(addr, 16, 1024, 2);
 }
+__device__ __forceinline__ uint32_t slice_step(int mn) { return (mn ? 2048 : 32) / 16; }
 
 // Tile t in an order that keeps the tiles in flight in a block of 8 P tiles by
 // as many Q tiles as it takes: each staged row is then read from L2 by the
