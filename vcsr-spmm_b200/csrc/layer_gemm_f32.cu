@@ -173,9 +173,10 @@ __device__ __forceinline__ void mend(float *z, IN &&in, AGAIN &&again) {
 template <int N, class GET>
 __device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int n, GET &&get) {
   if (f >= a.P) n = 0;
-  finish<N, true>(a.e, f, r0, 1, n, [&](float *z) {
+  finish<N, true>(a.e, f, r0, n, [&](float *z) {
     get(z);
     if (n > 0) mend<N>(z, [&](int j) { return j < n; }, [&](int j) { return sum_again(a, f, r0 + j); });
+    return true;
   });
 }
 
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
         split_tile<kRows>(from, to, a.p_mn, threadIdx.x);
         split_tile<BN>(from + kRows * kK * 4, to + 3 * kPlane, a.q_mn, threadIdx.x);
         // the MMAs read what was written by plain stores
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_async();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(full + s);
@@ -318,6 +319,8 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     for (int t = first; t < tiles && go; t += stride) {
       int tp, tq;
       tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
+      if (a.splits == 1)  // the residual comes to L2 while the sums are made
+        prefetch_residual(a.e, tp * kRows, a.P, kRows, tq * BN, a.Q, BN, drainer * 32 + lane, 32 * kDraining<BN>);
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
       for (int b = b0; b < b1; ++b, ++g) {

@@ -25,18 +25,19 @@ __device__ __forceinline__ void activate_all(int act, float *z) {
   }
 }
 
-// The epilogue of output column f, rows r0 + j * step (j < n of N).  The warp
-// calls it together; lanes without an output pass n <= 0.  get(z) fills in the
-// sums: it is called after the residual's loads are issued, which so overlap
-// with it and with the activation.  F32: e.type is known to be FP32.
+// The epilogue of output column f, rows r0 .. r0 + N - 1 (the first n of them).  The
+// warp calls it together; lanes without an output pass n <= 0.  get(z) fills in the
+// sums, or returns false: it is called after the residual's loads are issued, which
+// so overlap with the wait for the sums.  F32: e.type is known to be FP32.
 template <int N, bool F32, class GET>
-__device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int step, int n, GET &&get) {
+__device__ __forceinline__ bool finish(const Epilogue &e, int f, int r0, int n, GET &&get) {
+  bool ok = true;
   auto all = [&](auto type) {
     using T = decltype(type);
     T res[N];
     if (e.residual) {
       const T *p = static_cast<const T *>(e.residual) + (int64_t)r0 * e.ldr + f;
-      const int64_t ld = e.ldr * step;
+      const int64_t ld = e.ldr;
       if (n >= N) {
 #pragma unroll
         for (int j = 0; j < N; ++j) res[j] = p[j * ld];
@@ -48,13 +49,13 @@ __device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int ste
       __syncwarp();
     }
     float z[N];
-    get(z);
-    if (n <= 0) return;
+    ok = get(z);
+    if (n <= 0 || !ok) return;
     if (e.row_scale) {
       const float cs = e.col_scale[f];
 #pragma unroll
       for (int j = 0; j < N; ++j)
-        if (j < n) z[j] *= e.row_scale[r0 + j * step] * cs;
+        if (j < n) z[j] *= e.row_scale[r0 + j] * cs;
     }
     if (e.bias) {
       const float b = widen(static_cast<const T *>(e.bias)[f]);
@@ -63,7 +64,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int ste
     }
     auto store = [&](void *to, int64_t pitch) {
       T *p = static_cast<T *>(to) + (int64_t)r0 * pitch + f;
-      const int64_t ld = pitch * step;
+      const int64_t ld = pitch;
       if (n >= N) {
 #pragma unroll
         for (int j = 0; j < N; ++j) p[j * ld] = narrow<T>(z[j]);
@@ -85,6 +86,21 @@ __device__ __forceinline__ void finish(const Epilogue &e, int f, int r0, int ste
     all(float{});
   else
     with_type(e.type, all);
+  return ok;
+}
+
+// Asks L2 for the residual of a tile, `features` by `rows` from (f0, r0): thread t of
+// `threads`, a 128-byte line at a time.
+__device__ __forceinline__ void prefetch_residual(const Epilogue &e, int f0, int P, int features, int r0, int Q,
+                                                  int rows, int t, int threads) {
+  if (!e.residual) return;
+  const int size = e.type == VCSR_F32 ? 4 : 2, lines = features * size / 128;
+  for (int i = t; i < rows * lines; i += threads) {
+    const int r = r0 + i / lines, f = f0 + i % lines * (128 / size);
+    if (r < Q && f < P)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char *>(e.residual) +
+                                                     ((int64_t)r * e.ldr + f) * size));
+  }
 }
 
 // 4 neighbouring values, or the first n of them.

@@ -249,8 +249,10 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+// An arrival that orders nothing of this thread's memory accesses: a releasing one
+// waits until the thread's stores to global memory are through.
+__device__ __forceinline__ void mbar_arrive_relaxed_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
                : "memory");
 }
 // A copy into this CTA that completes on a barrier of either CTA of the pair.
@@ -261,6 +263,11 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *t
       "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
       "l"(tm), "r"(x), "r"(y), "r"(cluster_bar)
       : "memory");
+}
+
+// Orders plain shared-memory accesses before copies and MMAs that follow.
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
 }  // namespace tc
