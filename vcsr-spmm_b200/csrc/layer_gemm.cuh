@@ -39,26 +39,43 @@ struct Gemm {
 // and Phi by Abramowitz and Stegun 7.1.26, erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2)
 // with t = 1 / (1 + 0.3275911 x), |error| <= 1.5e-7, for x = |z| / sqrt(2).
 
-// Phi(-|z|), and exp(-z^2 / 2) on the way.
-__device__ __forceinline__ float lower_tail(float z, float *gauss) {
-  const float t = __fdividef(1.0f, fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.0f));
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  *gauss = __expf(-0.5f * z * z);
-  return 0.5f * p * t * *gauss;
+// Phi(-|z|) of two values, and exp(-z^2 / 2) on the way.
+__device__ __forceinline__ float2 lower_tails(float2 z, float2 *gauss) {
+  auto both = [](float v) { return make_float2(v, v); };
+  const float2 d = __ffma2_rn(make_float2(fabsf(z.x), fabsf(z.y)), both(0.3275911f * 0.70710678f), both(1.0f));
+  float2 t, e;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.x) : "f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t.y) : "f"(d.y));
+  // half of each coefficient
+  float2 p = __ffma2_rn(t, both(0.5f * 1.061405429f), both(-0.5f * 1.453152027f));
+  p = __ffma2_rn(p, t, both(0.5f * 1.421413741f));
+  p = __ffma2_rn(p, t, both(-0.5f * 0.284496736f));
+  p = __ffma2_rn(p, t, both(0.5f * 0.254829592f));
+  const float2 s = __fmul2_rn(__fmul2_rn(z, z), both(-0.5f * 1.44269504f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(s.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(s.y));
+  *gauss = e;
+  return __fmul2_rn(__fmul2_rn(p, t), e);
+}
+// z Phi(z) = max(z, 0) - |z| Phi(-|z|); the second term is long gone at |z| = 64
+__device__ __forceinline__ float2 gelu_pair(float2 z) {
+  float2 g;
+  const float2 q = lower_tails(z, &g);
+  return __ffma2_rn(make_float2(-fminf(fabsf(z.x), 64.0f), -fminf(fabsf(z.y), 64.0f)), q,
+                    make_float2(fmaxf(z.x, 0.0f), fmaxf(z.y, 0.0f)));
+}
+__device__ __forceinline__ float2 gelu_slope_pair(float2 z) {
+  float2 g;
+  const float2 q = lower_tails(z, &g);
+  const float2 phi = make_float2(z.x < 0.0f ? q.x : 1.0f - q.x, z.y < 0.0f ? q.y : 1.0f - q.y);
+  return __ffma2_rn(__fmul2_rn(z, make_float2(0.39894228f, 0.39894228f)), g, phi);
 }
 
 template <bool FAST>
 __device__ __forceinline__ float activate(int act, float z) {
   if (act == VCSR_ACT_RELU) return z < 0.0f ? 0.0f : z;  // a NaN stays
   if (act == VCSR_ACT_GELU) {
-    if constexpr (FAST) {
-      float g;
-      const float q = lower_tail(z, &g);
-      return z * (z < 0.0f ? q : 1.0f - q);
-    }
+    if constexpr (FAST) return gelu_pair(make_float2(z, z)).x;
     return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
   }
   if (act == VCSR_ACT_SILU)
@@ -70,11 +87,7 @@ template <bool FAST>
 __device__ __forceinline__ float activate_slope(int act, float z) {
   if (act == VCSR_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (act == VCSR_ACT_GELU) {
-    if constexpr (FAST) {
-      float g;
-      const float q = lower_tail(z, &g);
-      return fmaf(z * 0.39894228040143268f, g, z < 0.0f ? q : 1.0f - q);
-    }
+    if constexpr (FAST) return gelu_slope_pair(make_float2(z, z)).x;
     return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
            z * 0.39894228040143268f * expf(-0.5f * z * z);
   }
@@ -83,6 +96,28 @@ __device__ __forceinline__ float activate_slope(int act, float z) {
     return s * (1.0f + z * (1.0f - s));
   }
   return 1.0f;
+}
+
+// o[j] *= the slope at z[j], N values, the branch outside the loop.
+template <int N, bool FAST>
+__device__ __forceinline__ void times_slopes(int act, const float *z, float *o) {
+  if (act == VCSR_ACT_GELU && FAST && N % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j + 1 < N; j += 2) {
+      const float2 s = gelu_slope_pair(make_float2(z[j], z[j + 1]));
+      o[j] *= s.x;
+      o[j + 1] *= s.y;
+    }
+  } else if (act == VCSR_ACT_GELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= activate_slope<FAST>(VCSR_ACT_GELU, z[j]);
+  } else if (act == VCSR_ACT_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= activate_slope<FAST>(VCSR_ACT_SILU, z[j]);
+  } else if (act == VCSR_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= activate_slope<FAST>(VCSR_ACT_RELU, z[j]);
+  }
 }
 
 // On the tensor cores: operands whose bases and pitches are multiples of 16 bytes

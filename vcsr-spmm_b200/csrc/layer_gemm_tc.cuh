@@ -16,6 +16,13 @@ __device__ __forceinline__ void activate_all(int act, float *z) {
   if (act == VCSR_ACT_RELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = activate<FAST>(VCSR_ACT_RELU, z[j]);
+  } else if (act == VCSR_ACT_GELU && FAST) {
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+      const float2 y = gelu_pair(make_float2(z[j], z[j + 1]));
+      z[j] = y.x;
+      z[j + 1] = y.y;
+    }
   } else if (act == VCSR_ACT_GELU) {
 #pragma unroll
     for (int j = 0; j < N; ++j) z[j] = activate<FAST>(VCSR_ACT_GELU, z[j]);

@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kDzWarps * 32)
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.0f;
   if (col < N) {
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t r = r0 + warp; r < r1; r += kDzWarps) {
       const Vec<T, V> d = load_vec<T, V>(dy + r * lddy + col);
       float o[V];
@@ -38,8 +38,10 @@ __global__ void __launch_bounds__(kDzWarps * 32)
       for (int j = 0; j < V; ++j) o[j] = widen(d.v[j]);
       if (act != VCSR_ACT_NONE) {
         const Vec<T, V> z = load_vec<T, V>(pre + r * ldp + col);
+        float at[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] *= activate_slope<sizeof(T) == 2>(act, widen(z.v[j]));
+        for (int j = 0; j < V; ++j) at[j] = widen(z.v[j]);
+        times_slopes<V, sizeof(T) == 2>(act, at, o);
         if (dz) store_narrow<T, V>(dz + r * lddz + col, o);
       }
 #pragma unroll
@@ -86,19 +88,37 @@ void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *parti
 constexpr size_t kAlign = 256;
 size_t round_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-// Copies a matrix whose base or pitch is no multiple of 16 bytes, which TMA
-// cannot read, to one whose pitch is: a thread writes 16 bytes.
+// Matrices whose base or pitch is no multiple of 16 bytes, which TMA cannot read,
+// copied to ones whose pitch is.
+struct PackJob {
+  const void *src;
+  void *dst;
+  int64_t ld, ldd, rows, cols;
+};
+struct PackJobs {
+  PackJob job[3];
+};
+
+// Block row y copies job y; a thread writes 16 bytes.
 template <class T>
-__global__ void __launch_bounds__(256)
-    pack_kernel(const T *src, int64_t ld, T *dst, int64_t ldd, int64_t rows, int64_t cols) {
+__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
   constexpr int V = 16 / sizeof(T);
-  const int64_t per_row = ldd / V, total = rows * per_row;
+  const PackJob &p = jobs.job[blockIdx.y];
+  const T *src = static_cast<const T *>(p.src);
+  T *dst = static_cast<T *>(p.dst);
+  const int64_t per_row = p.ldd / V, total = p.rows * per_row;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per_row, c = (i - r * per_row) * V;
+    const T *from = src + r * p.ld + c;
     Vec<T, V> v;
+    if (c + V <= p.cols) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v.v[j] = c + j < cols ? src[r * ld + c + j] : T{};
-    store_vec<T, V>(dst + r * ldd + c, v);
+      for (int j = 0; j < V; ++j) v.v[j] = from[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v.v[j] = c + j < p.cols ? from[j] : T{};
+    }
+    store_vec<T, V>(dst + r * p.ldd + c, v);
   }
 }
 
@@ -123,25 +143,35 @@ Packed packed(const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) 
   }
   return k;
 }
-vcsr_status pack(const Packed &k, const void *&p, int64_t ld, int64_t rows, int64_t cols, int dtype,
-                 char *&ws, cudaStream_t st) {
-  if (!k.copy) return VCSR_OK;
-  const int64_t total = rows * k.ld * (int64_t)type_size(dtype) / 16;
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256), (int64_t)sm_count() * 8);
-  if (dtype == VCSR_E4M3)
-    pack_kernel<uint8_t><<<grid, 256, 0, st>>>(static_cast<const uint8_t *>(p), ld,
-                                               reinterpret_cast<uint8_t *>(ws), k.ld, rows, cols);
-  else if (dtype == VCSR_F32)
-    pack_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float *>(p), ld, reinterpret_cast<float *>(ws),
-                                             k.ld, rows, cols);
-  else
-    pack_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(p), ld,
-                                                reinterpret_cast<uint16_t *>(ws), k.ld, rows, cols);
-  VCSR_CUDA(cudaGetLastError());
-  p = ws;
-  ws += k.bytes;
-  return VCSR_OK;
-}
+// The copies of one call, made by one launch.
+struct Packer {
+  PackJobs jobs{};
+  int count = 0;
+  int64_t most = 0;  // 16-byte pieces of the largest
+  char *ws;
+  explicit Packer(void *workspace) : ws(static_cast<char *>(workspace)) {}
+  // Where the tensor cores read matrix p: the matrix, or its copy to be.
+  const void *add(const Packed &k, const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+    if (!k.copy) return p;
+    jobs.job[count++] = {p, ws, ld, k.ld, rows, cols};
+    most = std::max(most, rows * k.ld * (int64_t)type_size(dtype) / 16);
+    p = ws;
+    ws += k.bytes;
+    return p;
+  }
+  vcsr_status run(int dtype, cudaStream_t st) {
+    if (count == 0) return VCSR_OK;
+    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(most, 256), (int64_t)sm_count() * 8), (unsigned)count);
+    if (dtype == VCSR_E4M3)
+      pack_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
+    else if (dtype == VCSR_F32)
+      pack_kernel<float><<<grid, 256, 0, st>>>(jobs);
+    else
+      pack_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
+    VCSR_CUDA(cudaGetLastError());
+    return VCSR_OK;
+  }
+};
 
 // A product over no k: act(bias) + residual.
 __global__ void __launch_bounds__(256) empty_sum_kernel(const __grid_constant__ Gemm g) {
@@ -212,9 +242,10 @@ vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
   VCSR_TRY(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(a)));
   const void *x = a->x, *w = a->w;
   if (a->K > 0) {
-    char *ws = static_cast<char *>(a->workspace);
-    VCSR_TRY(pack(px, x, a->ldx, a->M, a->K, a->dtype, ws, st));
-    VCSR_TRY(pack(pw, w, a->ldw, a->N, a->K, a->dtype, ws, st));
+    Packer packer(a->workspace);
+    x = packer.add(px, x, a->ldx, a->M, a->K, a->dtype);
+    w = packer.add(pw, w, a->ldw, a->N, a->K, a->dtype);
+    VCSR_TRY(packer.run(a->dtype, st));
   }
   return launch_gemm({a->M, a->N, a->K, {x, px.ld, false}, {w, pw.ld, false}, a->dtype,
                       {a->x_scale, a->w_scale, a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy,
@@ -287,11 +318,11 @@ vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
       VCSR_TRY(column_sum(partial, (int)dz_chunks(a->M, a->N), a->N, a->dbias, a->dtype, st));
   }
   if (a->K == 0) return VCSR_OK;
-  ws += p.dz + p.partial;
-  const void *d = dz ? dz : a->dy, *x = a->x, *w = a->w;
-  if (!dz) VCSR_TRY(pack(p.dy, d, a->lddy, a->M, a->N, a->dtype, ws, st));
-  VCSR_TRY(pack(p.x, x, a->ldx, a->M, a->K, a->dtype, ws, st));
-  VCSR_TRY(pack(p.w, w, a->ldw, a->N, a->K, a->dtype, ws, st));
+  Packer packer(ws + p.dz + p.partial);
+  const void *d = dz ? dz : packer.add(p.dy, a->dy, a->lddy, a->M, a->N, a->dtype);
+  const void *x = packer.add(p.x, a->x, a->ldx, a->M, a->K, a->dtype);
+  const void *w = packer.add(p.w, a->w, a->ldw, a->N, a->K, a->dtype);
+  VCSR_TRY(packer.run(a->dtype, st));
   const int64_t ldd = dz ? p.lddz : p.dy.ld;
   Epilogue e{};
   e.type = a->dtype;
