@@ -183,35 +183,79 @@ struct NormArgs {
   int w_dtype, y_dtype;
 };
 
-// Sum or maximum over a team's threads; every thread gets it.  Teams of up to
-// 32 threads are a power of two of neighbouring lanes; a larger team has whole
-// warps, `shared` words of its own and the block's barrier `id`.
+// A sum, and with MAX a maximum of magnitudes, over a team's threads; every thread
+// gets them.  Teams of up to 32 threads are a power of two of neighbouring lanes; a
+// larger team has whole warps, `words` of its own (two per warp) and the block's
+// barrier `id`.
 template <bool MAX>
-__device__ __forceinline__ float team_reduce(float v, int team, float *shared, int id = 0) {
+__device__ __forceinline__ void team_reduce(float &sum, float &top, int team, float2 *words, int id) {
   for (int o = min(team, 32) >> 1; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, w) : v + w;
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   }
   if (team > 32) {
     const int lane = threadIdx.x & 31, warps = team >> 5;
-    if (lane == 0) shared[threadIdx.x % team >> 5] = v;
+    if (lane == 0) words[threadIdx.x % team >> 5] = make_float2(sum, top);
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(team) : "memory");
-    float t = lane < warps ? shared[lane] : 0.0f;
+    const float2 w = lane < warps ? words[lane] : make_float2(0.0f, 0.0f);
+    sum = w.x;
+    top = w.y;
     for (int o = 16; o > 0; o >>= 1) {
-      const float w = __shfl_xor_sync(0xffffffffu, t, o);
-      t = MAX ? fmaxf(t, w) : t + w;
+      if (o >= warps) continue;  // the lanes from `warps` on hold zeros
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
-    v = t;
+    // the sums now stand in the lanes below the power of two at `warps`
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+    if (MAX) top = __shfl_sync(0xffffffffu, top, 0);
   }
+}
+__device__ __forceinline__ float team_sum(float v, int team, float2 *words, int id) {
+  float none = 0.0f;
+  team_reduce<false>(v, none, team, words, id);
   return v;
 }
 
-// One row per team; E values per thread, V at a time (V values from one
-// 16-byte access of x, or single values).
+// An asynchronous copy of `bytes` (8, 16 or 32, 8- or 16-byte aligned) of a
+// row into this thread's own place in shared memory.
+__device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if (bytes == 8) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
+  } else {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    if (bytes == 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16),
+                   "l"(static_cast<const char *>(src) + 16)
+                   : "memory");
+  }
+}
+
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+// Waits until all but the latest depth - 1 groups of copies have landed.
+__device__ __forceinline__ void copies_wait_oldest(int depth) {
+  if (depth == 4)
+    copies_wait<3>();
+  else if (depth == 3)
+    copies_wait<2>();
+  else if (depth == 2)
+    copies_wait<1>();
+  else
+    copies_wait<0>();
+}
+
+// One row per team; E values per thread, V at a time (V values from one 16-byte
+// access of x, or single values).  16384 x 4096 bf16 with residual to bf16: 94 us, 5.7
+// TB/s.  Blocks that stay and copy rows into shared memory ahead, as the gradient's
+// do, gave 92 us there and 162 instead of 125 for 60000 x 1000 FP32: there are enough
+// blocks to keep loads in flight.
 template <class T, int V, int E, bool RAGGED>
 __global__ void __launch_bounds__(kNormBlock<V, E>)
     rmsnorm_kernel(const __grid_constant__ NormArgs a, int team) {
-  __shared__ float shared[2][32];
+  __shared__ float2 shared[32];
   const int dim = (int)a.dim;
   const int t = threadIdx.x % team;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + threadIdx.x / team;
@@ -249,9 +293,8 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
       if (live && at < dim) row_store<T, V, RAGGED>(so, at, dim, s + i * V);
     }
   }
-  ss = team_reduce<false>(ss, team, shared[0]);
-  const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-  if (a.rstd && live && t == 0) a.rstd[row] = rstd;
+  // s becomes s * weight, which rstd then makes y
+  float top = 0.0f;
   auto weigh = [&](auto type) {
     using W = decltype(type);
 #pragma unroll
@@ -261,7 +304,7 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
         float w[V];
         weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s[i * V + j] *= rstd * w[j];
+        for (int j = 0; j < V; ++j) s[i * V + j] *= w[j];
       }
     }
   };
@@ -270,19 +313,27 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
   else
     weigh(T{});
   if (a.y_dtype == VCSR_E4M3) {
-    float top = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(s[e]));
-    const CodeScale c = code_scale(team_reduce<true>(top, team, shared[1]));
-    if (live && t == 0) a.scale[row] = c.scale;
+    team_reduce<true>(ss, top, team, shared, 1);
+  } else {
+    ss = team_sum(ss, team, shared, 1);
+  }
+  const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+  if (a.rstd && live && t == 0) a.rstd[row] = rstd;
+  if (a.y_dtype == VCSR_E4M3) {
+    // y / scale = s weight * 448 / max|s weight|: rstd, which is alike for the row,
+    // falls out of the codes
+    if (live && t == 0) a.scale[row] = top * rstd * (1.0f / 448.0f);
+    const float raise = top < 1e-30f ? 0x1p64f : 1.0f;  // 448 / top would overflow
+    const float k = rstd != rstd ? rstd : top > 0.0f ? 448.0f / (top * raise) : 0.0f;
     uint8_t *y = static_cast<uint8_t *>(a.y) + row * a.ldy;
-    if (c.raise == 1.0f) {
+    if (raise != 1.0f) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[e] = c.quotient<false>(s[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) s[e] = c.quotient<true>(s[e]);
+      for (int e = 0; e < E; ++e) s[e] *= raise;
     }
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] *= k;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int at = (t + i * team) * V - shift;
@@ -297,6 +348,8 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
       }
     }
   } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] *= rstd;
     with_type(a.y_dtype, [&](auto type) {
       using Y = decltype(type);
       Y *y = static_cast<Y *>(a.y) + row * a.ldy;
@@ -314,7 +367,7 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
 // last pass, so that it may replace x or residual.
 template <class T>
 __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_kernel(const NormArgs a) {
-  __shared__ float shared[2][32];
+  __shared__ float2 shared[2][32];
   const int64_t row = blockIdx.x;
   const T *x = static_cast<const T *>(a.x) + row * a.ldx;
   const T *r = static_cast<const T *>(a.residual) + row * a.ldr;
@@ -327,7 +380,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_kernel(const NormArg
     const float s = value(i);
     ss = fmaf(s, s, ss);
   }
-  ss = team_reduce<false>(ss, blockDim.x, shared[0]);
+  ss = team_sum(ss, blockDim.x, shared[0], 1);
   const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
   if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   CodeScale c = code_scale(448.0f);
@@ -338,7 +391,9 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_kernel(const NormArg
       load_as_float<1>(a.weight, a.w_dtype, i, &w);
       top = fmaxf(top, fabsf(value(i) * (rstd * w)));
     }
-    c = code_scale(team_reduce<true>(top, blockDim.x, shared[1]));
+    float none = 0.0f;
+    team_reduce<true>(none, top, blockDim.x, shared[1], 1);
+    c = code_scale(top);
     if (threadIdx.x == 0) a.scale[row] = c.scale;
   }
   for (int64_t i = threadIdx.x; i < a.dim; i += blockDim.x) {
@@ -362,21 +417,6 @@ struct GradArgs {
   int depth;  // rows in flight per team (16-byte access)
 };
 
-// An asynchronous copy of `bytes` (8, 16 or 32, 8- or 16-byte aligned) of a
-// row into this thread's own place in shared memory.
-__device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes) {
-  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-  if (bytes == 8) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
-  } else {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    if (bytes == 32)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + 16),
-                   "l"(static_cast<const char *>(src) + 16)
-                   : "memory");
-  }
-}
-
 // Teams take every (team count)-th row.  With 16-byte access a thread copies its
 // own vectors of this row and the next depth - 1 into shared memory ahead of their use
 // (nobody else reads them: no barrier); single values are loaded as they come, by
@@ -384,7 +424,7 @@ __device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes
 template <class T, int V, int E, bool RAGGED>
 __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
     rmsnorm_grad_kernel(const __grid_constant__ GradArgs a, int team) {
-  __shared__ float words[2][kGradBlock / 32];
+  __shared__ float2 words[2][kGradBlock / 32];
   extern __shared__ __align__(16) unsigned char dynamic[];
   constexpr int kN = E / V;
   const int dim = (int)a.dim;
@@ -442,14 +482,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
       if (next >= a.depth) next -= a.depth;
       // the place of the row before this one, read by this thread a turn ago
       fetch(row + (int64_t)(a.depth - 1) * stride, next);
-      if (a.depth == 4)
-        asm volatile("cp.async.wait_group 3;" ::: "memory");
-      else if (a.depth == 3)
-        asm volatile("cp.async.wait_group 2;" ::: "memory");
-      else if (a.depth == 2)
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+      copies_wait_oldest(a.depth);
       if (++stage == a.depth) stage = 0;
       const T *s = static_cast<const T *>(a.s) + row * a.lds;
       with_type(a.dy_dtype, [&](auto type) {
@@ -505,7 +538,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
       weigh(float{});
     else
       weigh(T{});
-    const float mean = team_reduce<false>(dot, team, words[flip] + mine * (team >> 5), id) / (float)a.dim;
+    const float mean = team_sum(dot, team, words[flip] + mine * (team >> 5), id) / (float)a.dim;
     T *dx = static_cast<T *>(a.dx) + row * a.lddx;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -553,7 +586,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
 // rmsnorm_long_dweight_kernel.
 template <class T>
 __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_grad_kernel(const GradArgs a) {
-  __shared__ float shared[32];
+  __shared__ float2 shared[32];
   const int64_t row = blockIdx.x;
   const float rstd = a.rstd[row];
   const T *s = static_cast<const T *>(a.s) + row * a.lds;
@@ -564,7 +597,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_grad_kernel(const Gr
     load_as_float<1>(a.weight, a.w_dtype, i, &w);
     dot = fmaf(g * w, widen(s[i]) * rstd, dot);
   }
-  const float mean = team_reduce<false>(dot, blockDim.x, shared) / (float)a.dim;
+  const float mean = team_sum(dot, blockDim.x, shared, 1) / (float)a.dim;
   for (int64_t i = threadIdx.x; i < a.dim; i += blockDim.x) {
     float g, w;
     load_as_float<1>(a.dy, a.dy_dtype, row * a.lddy + i, &g);
