@@ -211,11 +211,13 @@ __device__ __forceinline__ void store_as(void *p, int type, int64_t at, const fl
 // below 2^-108 are first raised, since their reciprocal overflows FP32.
 struct CodeScale {
   float scale, raise, divisor, inverse;
-  template <bool RAISED = true>
-  __device__ __forceinline__ float quotient(float x) const {
-    const float a = RAISED ? x * raise : x, q = a * inverse;
-    return fmaf(fmaf(-q, divisor, a), inverse, q);
+  template <bool RAISED>
+  __device__ __forceinline__ float2 quotients(float2 x) const {
+    auto both = [](float v) { return make_float2(v, v); };
+    const float2 a = RAISED ? __fmul2_rn(x, both(raise)) : x, q = __fmul2_rn(a, both(inverse));
+    return __ffma2_rn(__ffma2_rn(make_float2(-q.x, -q.y), both(divisor), a), both(inverse), q);
   }
+  __device__ __forceinline__ float quotient(float x) const { return quotients<true>(make_float2(x, x)).x; }
 };
 __device__ __forceinline__ CodeScale code_scale(float top) {
   CodeScale s;
