@@ -413,8 +413,8 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
   a.tiles_q = (int)ceil_div(a.Q, BN);
   const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
   if (tiles > (1 << 30)) return fail(VCSR_ERR_RANGE, "more than 2^30 output tiles");
-  a.splits = 1;
-  while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && ceil_div(a.K, kK) >= 4 * a.splits) a.splits *= 2;
+  a.splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>, tiles,
+                           ceil_div(a.K, kK));
   const int grid = a.splits > 1 ? (int)tiles * a.splits : (int)std::min<int64_t>(tiles, sm_count());
   return launch(gemm_f32_kernel<BN>, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
 }

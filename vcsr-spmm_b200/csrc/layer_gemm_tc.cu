@@ -28,6 +28,8 @@
 // own copies and MMAs, frees its tensor memory and returns, and vcsr_layers_check
 // reports it.
 #include <algorithm>
+#include <mutex>
+#include <vector>
 
 #include "layer_gemm_tc.cuh"
 #include "spmm_tc.h"
@@ -380,6 +382,12 @@ vcsr_status make_map(CUtensorMap *m, const Operand &o, int64_t rows, int64_t K, 
 }
 
 template <int BN>
+const void *split_kernel(int dtype) {
+  return dtype == VCSR_E4M3 ? reinterpret_cast<const void *>(gemm_split_kernel<BN, true>)
+                            : reinterpret_cast<const void *>(gemm_split_kernel<BN, false>);
+}
+
+template <int BN>
 vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
   CUtensorMap mp, mq;
   VCSR_TRY(make_map(&mp, g.b, g.N, g.K, g.dtype, kPRows));
@@ -387,9 +395,7 @@ vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
   a.tiles_p = (int)ceil_div(a.P, kPRows);
   a.tiles_q = (int)ceil_div(a.Q, BN);
   const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
-  // clusters that fill the GPU, with at least two blocks of k per CTA
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= sm_count() && a.blocks >= 4 * splits) splits *= 2;
+  const int splits = choose_splits(split_kernel<BN>(g.dtype), kSplitThreads, kSplitSmem<BN>, tiles, a.blocks);
   if (tiles * splits > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
   const int grid = (int)(tiles * splits);
   const int format = g.dtype == VCSR_BF16 ? 1 : 0;
@@ -397,6 +403,28 @@ vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
   return g.dtype == VCSR_E4M3
              ? launch(gemm_split_kernel<BN, true>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits)
              : launch(gemm_split_kernel<BN, false>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits);
+}
+
+// Expected microseconds, to choose between the kernels: a launch, then for every round
+// of tiles on the GPU a fixed part (filling the pipeline, the epilogue) and a part per
+// stage of k.  Fitted to 200 products of 1 to 4096 rows, 128 to 4096 features and k of
+// 128 to 4096 (bf16, bias, silu and residual) in each kernel; within about 10% of them.
+// Some of them, split kernel with 16 / 32 / 64 / 128 rows and pair kernel: 16 x 4096,
+// k = 4096: 10.9 / 10.9 / 11.1 / 11.3 / 27.5; 64 x 2048, k = 512: 7.1 / 6.7 / 6.9 / 7.3 /
+// 11.0; 512 x 1024, k = 1024: - / - / 9.4 / 10.0 / 16.5; 1024 x 4096, k = 1024: - / - /
+// 41.3 / 25.5 / 17.2.
+template <int BN>
+double split_cost(const TcArgs &a, int dtype) {
+  constexpr double kFixed = BN == 16 ? 3.8 : BN == 32 ? 4.2 : BN == 64 ? 5.0 : 7.0;
+  constexpr double kStage = BN == 16 ? 0.29 : BN == 128 ? 0.36 : 0.32;
+  const int64_t tiles = ceil_div(a.P, kPRows) * ceil_div(a.Q, BN);
+  const int splits = choose_splits(split_kernel<BN>(dtype), kSplitThreads, kSplitSmem<BN>, tiles, a.blocks);
+  return 1.2 + (splits > 1 ? 0.7 : 0.0) +
+         (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStage * (double)ceil_div(a.blocks, splits));
+}
+double pair_cost(const TcArgs &a) {
+  const int64_t rounds = ceil_div(ceil_div(a.P, 256) * ceil_div(a.Q, 256), sm_count() / 2);
+  return 11.5 + 0.33 * a.blocks + (double)(rounds - 1) * std::max(8.0, 0.42 * a.blocks);
 }
 
 template <int BN>
@@ -431,12 +459,49 @@ vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st) {
   a.p_mn = g.b.transposed;
   a.q_mn = g.a.transposed;
   a.e = g.e;
-  const int64_t pair_tiles = ceil_div(g.N, 256) * ceil_div(g.M, 256);
-  if (pair_tiles >= sm_count() / 4) return launch_pair<256>(a, g, st);
-  if (g.M <= 16 && !a.q_mn) return launch_split<16>(a, g, st);
-  if (g.M <= 32 && !a.q_mn) return launch_split<32>(a, g, st);
-  if (g.M <= 64) return launch_split<64>(a, g, st);
-  return launch_split<128>(a, g, st);
+  // 16 and 32 rows per tile are for operands stored along k (a box along the
+  // operand's own index is 64 rows)
+  const double costs[5] = {a.q_mn ? 1e30 : split_cost<16>(a, g.dtype), a.q_mn ? 1e30 : split_cost<32>(a, g.dtype),
+                           split_cost<64>(a, g.dtype), split_cost<128>(a, g.dtype), pair_cost(a)};
+  switch (std::min_element(costs, costs + 5) - costs) {
+    case 0: return launch_split<16>(a, g, st);
+    case 1: return launch_split<32>(a, g, st);
+    case 2: return launch_split<64>(a, g, st);
+    case 3: return launch_split<128>(a, g, st);
+    default: return launch_pair<256>(a, g, st);
+  }
+}
+
+int cluster_slots(const void *kernel, int threads, size_t smem, int size) {
+  struct Known {
+    const void *kernel;
+    int dev, size, slots;
+  };
+  static std::mutex mu;
+  static std::vector<Known> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::lock_guard<std::mutex> lk(mu);
+  for (const Known &k : known)
+    if (k.kernel == kernel && k.dev == dev && k.size == size) return k.slots;
+  if (allow_shared(kernel, smem) != VCSR_OK) return 0;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3((unsigned)size);
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)size;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  int slots = 0;
+  if (cudaOccupancyMaxActiveClusters(&slots, kernel, &c) != cudaSuccess) {
+    cudaGetLastError();
+    slots = 0;
+  }
+  known.push_back({kernel, dev, size, slots});
+  return slots;
 }
 
 vcsr_status check_waits(cudaStream_t st) {

@@ -271,6 +271,22 @@ __device__ __forceinline__ void tile_of(int t, int tiles_p, int tiles_q, int *p,
   *q = in / width;
 }
 
+// Clusters of `size` blocks of a kernel that the current device runs at once (asked of
+// the runtime once): with 128 KB of shared memory and more a block has an SM to itself,
+// and an eight-block cluster eight SMs of one of the GPU's unequal parts, so that 16 of
+// them, 128 blocks, are more than fit on 148 SMs.
+int cluster_slots(const void *kernel, int threads, size_t smem, int size);
+
+// How many CTAs share each tile's sum over k: as many as still run at once, up to 8,
+// with at least two stages each.
+inline int choose_splits(const void *kernel, int threads, size_t smem, int64_t tiles, int64_t stages) {
+  int splits = 1;
+  while (splits < 8 && stages >= 4 * splits && tiles * splits * 2 <= sm_count() &&
+         tiles <= cluster_slots(kernel, threads, smem, splits * 2))
+    splits *= 2;
+  return splits;
+}
+
 template <class K, class... A>
 inline vcsr_status launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
   VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
