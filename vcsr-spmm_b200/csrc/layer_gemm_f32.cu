@@ -197,7 +197,9 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be: what the MMA warp computes then stays in
+  // uniform registers, where its instructions want their operands
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
   const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / a.splits, stride = gridDim.x / a.splits;
   const int all = (a.K + kK - 1) / kK;
@@ -279,23 +281,24 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
         mbar_wait(rfull + n % R, (uint32_t)((n / R) & 1), &keep, kWaitFull);
     }
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc(1, a.p_mn, a.q_mn, kRows, BN);
-      const uint32_t p_step = a.p_mn ? 2048 / 16 : 32 / 16, q_step = a.q_mn ? 2048 / 16 : 32 / 16;
-      RingPlace<S> at;
-      RingPlace<2> sums;
-      bool go = true;
-      for (int t = first; t < tiles && go; t += stride) {
-        for (int b = b0; b < b1; ++b, at.next(), sums.next()) {
-          const int s = at.stage, buf = sums.stage;
-          if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull) ||
-              !mbar_wait(dfree + buf, sums.empty(), abort_flag, kWaitAccFree)) {
-            go = false;
-            break;
-          }
-          fence_after_sync();
-          const uint32_t pa = smem_u32(ring + s * kSplit<BN>), qa = pa + 3 * kPlane;
-          const uint64_t pd = plane_desc(pa, a.p_mn), qd = plane_desc(qa, a.q_mn);
+    const uint32_t idesc = instr_desc(1, a.p_mn, a.q_mn, kRows, BN);
+    const uint32_t p_step = a.p_mn ? 2048 / 16 : 32 / 16, q_step = a.q_mn ? 2048 / 16 : 32 / 16;
+    RingPlace<S> at;
+    RingPlace<2> sums;
+    bool go = true;
+    for (int t = first; t < tiles && go; t += stride) {
+      for (int b = b0; b < b1; ++b, at.next(), sums.next()) {
+        const int s = at.stage, buf = sums.stage;
+        const bool ready = mbar_wait(full + s, at.full(), abort_flag, kWaitFull) &&
+                           mbar_wait(dfree + buf, sums.empty(), abort_flag, kWaitAccFree);
+        if (!__all_sync(0xffffffffu, ready)) {
+          go = false;
+          break;
+        }
+        fence_after_sync();
+        const uint32_t pa = smem_u32(ring + s * kSplit<BN>), qa = pa + 3 * kPlane;
+        const uint64_t pd = plane_desc(pa, a.p_mn), qd = plane_desc(qa, a.q_mn);
+        if (elect_one()) {
           // parts of P and Q, smallest products first
           constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
 #pragma unroll
@@ -308,7 +311,10 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
           mma_commit(empty + s);
           mma_commit(dfull + buf);
         }
+        __syncwarp();
       }
+    }
+    if (elect_one()) {
       mma_commit(drain);
       volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
       if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
