@@ -91,7 +91,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   uint32_t *holder = reinterpret_cast<uint32_t *>(done + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be: what the MMA warp computes then stays in
+  // uniform registers, where its instructions want their operands
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0;
   const int tile = blockIdx.x / splits;
   const int f0 = tile % a.tiles_p * kPRows, r0 = tile / a.tiles_p * BN;
@@ -111,7 +113,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *holder;
-  int consumed = b0;  // blocks of k
 
   if (warp == 4) {
     if (lane == 0) {
@@ -128,29 +129,31 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       }
     }
   } else if (warp == 5) {
-    if (lane == 0) {
-      const uint64_t p_first = stage_desc(smem_u32(ring), a.p_mn),
-                     q_first = stage_desc(smem_u32(ring) + kPBytes, a.q_mn);
-      const uint32_t p_step = slice_step(a.p_mn), q_step = slice_step(a.q_mn);
-      RingPlace<kStages> at;
-      for (int b = b0; b < b1; ++b, at.next()) {
-        const int s = at.stage;
-        if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull)) break;
-        fence_after_sync();
-        const uint64_t pd = p_first + s * (kStage / 16), qd = q_first + s * (kStage / 16);
+    const uint64_t p_first = stage_desc(smem_u32(ring), a.p_mn),
+                   q_first = stage_desc(smem_u32(ring) + kPBytes, a.q_mn);
+    const uint32_t p_step = slice_step(a.p_mn), q_step = slice_step(a.q_mn);
+    RingPlace<kStages> at;
+    int b = b0;
+    for (; b < b1; ++b, at.next()) {
+      const int s = at.stage;
+      if (!__all_sync(0xffffffffu, mbar_wait(full + s, at.full(), abort_flag, kWaitFull))) break;
+      fence_after_sync();
+      const uint64_t pd = p_first + s * (kStage / 16), qd = q_first + s * (kStage / 16);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           mma<1, CODES>(tmem, pd + k * p_step, qd + k * q_step, a.idesc, (b > b0 || k > 0) ? 1u : 0u);
         mma_commit(empty + s);
-        ++consumed;
       }
+      __syncwarp();
+    }
+    if (elect_one()) {
       mma_commit(done);
       volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
       if (!mbar_wait(done, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
-      if (consumed < b1) {  // copies that nobody waited for land before the CTA leaves
-        for (int b = consumed; b < b1; ++b, at.next())
-          if (!mbar_wait(full + at.stage, at.full(), &keep, kWaitFull)) break;
-      }
+      // copies that nobody waited for land before the CTA leaves
+      for (; b < b1; ++b, at.next())
+        if (!mbar_wait(full + at.stage, at.full(), &keep, kWaitFull)) break;
     }
   }
   __syncwarp();
@@ -219,7 +222,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
   volatile int *consumed = abort_flag + 1;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the same in all lanes, and known to be: what the MMA warp computes then stays in
+  // uniform registers, where its instructions want their operands
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / 2, stride = gridDim.x / 2;
   if (threadIdx.x == 0) {
@@ -269,7 +274,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else if (warp == kPairEpilogueWarps + 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint64_t p_first = stage_desc(smem_u32(ring), a.p_mn),
                      q_first = stage_desc(smem_u32(ring) + kPBytes, a.q_mn);
       const uint32_t p_step = slice_step(a.p_mn), q_step = slice_step(a.q_mn);
@@ -279,32 +284,38 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       bool go = true;
       for (int t = first; t < tiles && go; t += stride, acc.next()) {
         const int buf = acc.stage;
-        if (!mbar_wait(dfree + buf, acc.empty(), abort_flag, kWaitAccFree)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(dfree + buf, acc.empty(), abort_flag, kWaitAccFree))) break;
         fence_after_sync();
         for (int b = 0; b < a.blocks; ++b, ++g, at.next()) {
           const int s = at.stage;
-          if (!mbar_wait(full + s, at.full(), abort_flag, kWaitFull)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(full + s, at.full(), abort_flag, kWaitFull))) {
             go = false;
             break;
           }
           fence_after_sync();
           const uint64_t pd = p_first + s * (kStage / 16), qd = q_first + s * (kStage / 16);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma<2, CODES>(tmem + buf * BN, pd + k * p_step, qd + k * q_step, a.idesc,
-                          (b > 0 || k > 0) ? 1u : 0u);
-          mma_commit_pair(empty + s);
+            for (int k = 0; k < 4; ++k)
+              mma<2, CODES>(tmem + buf * BN, pd + k * p_step, qd + k * q_step, a.idesc,
+                            (b > 0 || k > 0) ? 1u : 0u);
+            mma_commit_pair(empty + s);
+          }
+          __syncwarp();
         }
-        if (go) mma_commit_pair(dfull + buf);
+        if (go && elect_one()) mma_commit_pair(dfull + buf);
+        __syncwarp();
       }
-      *consumed = g;
-      // every MMA issued here has finished before the pair leaves
-      asm volatile(
-          "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-              smem_u32(drain))
-          : "memory");
-      volatile int keep = 0;
-      if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
+      if (elect_one()) {
+        *consumed = g;
+        // every MMA issued here has finished before the pair leaves
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                smem_u32(drain))
+            : "memory");
+        volatile int keep = 0;
+        if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
+      }
     }
   } else {
     RingPlace<2> acc;
