@@ -425,6 +425,21 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
   return launch(gemm_f32_kernel<BN>, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
 }
 
+// Expected microseconds, to choose the rows of a tile: a launch, then for every round
+// of tiles on the GPU a fixed part (the epilogue) and a part per stage of k.  Fitted to
+// 200 products of 1 to 4096 rows, 128 to 4096 features and k of 128 to 4096 in each
+// tile, with bias, silu and residual.  Tiles of 32 / 64 / 128 rows took, for 32 rows,
+// 4096 features, k = 1024: 12.6 / 14.9 / 19.6 us; 512 x 512, k = 512: 13.5 / 12.5 / 17.3;
+// 4096 x 4096, k = 1024: 740 / 442 / 283.
+template <int BN>
+double tiles_cost(const F32Args &a) {
+  constexpr double kFixed = BN == 32 ? 2.1 : BN == 64 ? 2.6 : 5.4, kStageUs = BN == 32 ? 0.73 : BN == 64 ? 0.82 : 1.13;
+  const int64_t tiles = ceil_div(a.P, kRows) * ceil_div(a.Q, BN), stages = ceil_div(a.K, kK);
+  const int splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>,
+                                   tiles, stages);
+  return 5.2 + (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStageUs * (double)ceil_div(stages, splits));
+}
+
 }  // namespace
 
 vcsr_status launch_gemm_f32(const Gemm &g, cudaStream_t st) {
@@ -439,9 +454,11 @@ vcsr_status launch_gemm_f32(const Gemm &g, cudaStream_t st) {
   a.p_mn = g.b.transposed;
   a.q_mn = g.a.transposed;
   a.e = g.e;
-  if (g.M <= 32 && !a.q_mn) return launch_tiles<32>(a, g, st);
-  if (g.M <= 64) return launch_tiles<64>(a, g, st);
-  return launch_tiles<128>(a, g, st);
+  // 32 rows per tile are for operands stored along k (the planes of one stored along its
+  // own index come in chunks of 64)
+  const double c32 = a.q_mn ? 1e30 : tiles_cost<32>(a), c64 = tiles_cost<64>(a), c128 = tiles_cost<128>(a);
+  if (c32 <= c64 && c32 <= c128) return launch_tiles<32>(a, g, st);
+  return c64 <= c128 ? launch_tiles<64>(a, g, st) : launch_tiles<128>(a, g, st);
 }
 
 vcsr_status take_wait_error_f32(int *word) {

@@ -19,7 +19,7 @@ constexpr int kDzWarps = 8;
 // columns, the warps take every 8th row of the chunk.  partial: one row of N
 // sums per chunk.
 template <class T, int V>
-__global__ void __launch_bounds__(kDzWarps * 32)
+__global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four an SM
     dz_kernel(const T *dy, int64_t lddy, const T *pre, int64_t ldp, T *dz, int64_t lddz, int64_t M,
               int64_t N, int64_t chunk, int act, float *partial) {
   __shared__ float joined[kDzWarps][32 * V + 1];
