@@ -1,0 +1,97 @@
+"""The dense layer operators as torch operators with gradients, and the example that
+trains with them."""
+import os
+import sys
+
+import pytest
+import torch
+
+from vcsr_b200 import layers, torch_ops
+
+gpu = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def leaf(*shape, seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(*shape, generator=g).cuda().to(dtype).requires_grad_()
+
+
+@gpu
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm_autograd(residual):
+    """Against torch's own gradient in 64 bits: a few units of FP32's roundoff of terms
+    of order 1 summed over 20 rows."""
+    x, w, r = leaf(20, 48, seed=1), leaf(48, seed=2), leaf(20, 48, seed=3) if residual else None
+    c, e = torch.randn(20, 48).cuda(), torch.randn(20, 48).cuda()
+    y, s = torch_ops.rmsnorm(x, w, residual=r, eps=1e-5)
+    ((y * c).sum() + (s * e).sum()).backward()
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    rd = r.detach().double().requires_grad_() if residual else None
+    sd = xd + rd if residual else xd
+    yd = sd / torch.sqrt(sd.square().mean(1, keepdim=True) + 1e-5) * wd
+    ((yd * c.double()).sum() + (sd * e.double()).sum()).backward()
+    assert (y.double() - yd).abs().max() < 1e-5
+    for a, b in ((x, xd), (w, wd)) + (((r, rd),) if residual else ()):
+        assert (a.grad.double() - b.grad).abs().max() < 1e-4
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+def test_linear_autograd(act):
+    x, w, b, r = leaf(20, 48, seed=1), leaf(30, 48, seed=2), leaf(30, seed=3), leaf(20, 30, seed=4)
+    c = torch.randn(20, 30).cuda()
+    (torch_ops.linear(x, w, bias=b, residual=r, act=act) * c).sum().backward()
+    d = [t.detach().double().requires_grad_() for t in (x, w, b, r)]
+    z = d[0] @ d[1].t() + d[2]
+    f = {None: lambda v: v, "relu": torch.relu, "gelu": torch.nn.functional.gelu,
+         "silu": torch.nn.functional.silu}[act]
+    ((f(z) + d[3]) * c.double()).sum().backward()
+    for a, q in zip((x, w, b, r), d):
+        # sums of up to 48 FP32 products of terms below 20
+        assert (a.grad.double() - q.grad).abs().max() < 2e-4, act
+
+
+@gpu
+def test_linear_saves_nothing_without_gradients():
+    x, w = leaf(8, 16).detach(), leaf(4, 16)
+    with torch.no_grad():
+        y = torch_ops.linear(x, w, act="gelu")
+    assert not y.requires_grad
+    assert torch.equal(y, layers.linear(x, w.detach(), act="gelu").y)
+
+
+@gpu
+def test_operators_pass_torch_opcheck():
+    x, w, b = leaf(6, 16, seed=1), leaf(5, 16, seed=2), leaf(5, seed=3)
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(torch.ops.vcsr.linear.default, (x, w, b, None, "gelu", True),
+                          test_utils=tests)
+    gain = leaf(16, seed=4)
+    torch.library.opcheck(torch.ops.vcsr.rmsnorm.default, (x, gain, x.detach().clone(), 1e-6, torch.float32),
+                          test_utils=tests)
+
+
+def test_fake_shapes_without_a_gpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = torch.empty(6, 16), torch.empty(5, 16)
+        y, pre = torch.ops.vcsr.linear(x, w, None, None, "gelu", True)
+        assert y.shape == pre.shape == (6, 5)
+        y, s, rstd = torch.ops.vcsr.rmsnorm(x, torch.empty(16), None, 1e-6, torch.bfloat16)
+        assert y.shape == (6, 16) and y.dtype == torch.bfloat16 and s.shape == (0, 16)
+        assert rstd.shape == (6,)
+
+
+@gpu
+def test_example_trains_and_serves():
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    try:
+        import train_layer
+    finally:
+        sys.path.pop(0)
+    losses, off = train_layer.main(rows=3000, width=64, steps=20, verbose=False)
+    assert all(b == b for b in losses) and losses[-1] < 0.7 * losses[0], losses
+    # two 8-bit products: each rounds its operands by up to 2^-4 of them, 3% in the mean
+    # square, on a part of the answer; a wrong scale is off by 1
+    assert off < 0.1, off

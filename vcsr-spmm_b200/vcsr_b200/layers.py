@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -38,6 +39,7 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 BLOCK = 256  # values per scale of an 8-bit AdamW state
 
 _current_stream = torch._C._cuda_getCurrentRawStream
+_dtype = operator.attrgetter("dtype")
 
 
 def _type(dtype, name):
@@ -396,6 +398,22 @@ class AdamW:
             if t.device != dev or t.numel() != n or not t.is_contiguous():
                 raise VcsrError(INVALID, f"{name}[{i}] must be contiguous on {dev} with {n} values")
 
+    def _gradients(self, grads):
+        """The gradients' type and addresses, checked (in whole passes over the list:
+        with hundreds of small tensors the checks are most of a step)."""
+        T = torch.Tensor
+        try:
+            dtypes = set(map(_dtype, grads))
+            if (len(dtypes) == 1 and list(map(T.numel, grads)) == self._numel
+                    and all(map(T.is_contiguous, grads))
+                    and set(map(T.get_device, grads)) == {self.device.index}):
+                return dtypes.pop(), np.fromiter(map(T.data_ptr, grads), np.uint64, len(grads))
+        except (AttributeError, TypeError):
+            pass
+        dtype = next((g.dtype for g in grads if g is not None), torch.float32)
+        self._same(grads, "grads", dtype)
+        return dtype, self._pointers(grads)
+
     @staticmethod
     def _pointers(tensors):
         return np.fromiter((0 if t is None else t.data_ptr() for t in tensors), np.uint64,
@@ -406,10 +424,7 @@ class AdamW:
         or float16), or None for a parameter to leave as it is.  dither: 256 float32
         uniform numbers in [0, 1), fresh ones each step (state_bits=8; without it
         codes round to nearest)."""
-        grads = list(grads)
-        dtype = next((g.dtype for g in grads if g is not None), torch.float32)
-        self._same(grads, "grads", dtype)
-        ptr = self._pointers(grads)
+        dtype, ptr = self._gradients(list(grads))
         if dither is not None:
             dither = _vector(dither, "dither", self.m_flat, BLOCK, torch.float32)
         eight = self.state_bits == 8
