@@ -18,21 +18,6 @@ inline size_t type_size(int t) { return t == VCSR_F32 ? 4 : t == VCSR_E4M3 ? 1 :
 inline bool is_float16_or_32(int t) { return t == VCSR_F32 || t == VCSR_BF16 || t == VCSR_F16; }
 inline bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) % n) == 0; }
 
-template <class T>
-struct TypeOf;
-template <>
-struct TypeOf<float> {
-  static constexpr int id = VCSR_F32;
-};
-template <>
-struct TypeOf<__nv_bfloat16> {
-  static constexpr int id = VCSR_BF16;
-};
-template <>
-struct TypeOf<__half> {
-  static constexpr int id = VCSR_F16;
-};
-
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
@@ -228,14 +213,34 @@ __device__ __forceinline__ CodeScale code_scale(float top) {
   return s;
 }
 
-// Shared host checks and kernels (layer_norm.cu).  check_matrix: a pointer
+// out[c] = the sum of `count` FP32 partial rows of `dim` values, for the 32 columns of
+// `group`, by a block of 256 threads: in order within each of 8 slices of the rows, the
+// slices then added in order.
+__device__ __forceinline__ void column_sum_block(const float *partial, int count, int64_t dim, void *out,
+                                                 int dtype, int64_t group, float (*part)[33]) {
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  const int64_t c = group * 32 + lane;
+  float sum = 0.0f;
+  if (c < dim) {
+    const int per = (count + 7) / 8, lo = slice * per, hi = min(count, lo + per);
+#pragma unroll 8
+    for (int p = lo; p < hi; ++p) sum += partial[(int64_t)p * dim + c];
+  }
+  part[slice][lane] = sum;
+  __syncthreads();
+  if (slice == 0 && c < dim) {
+    float total = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) total += part[k][lane];
+    store_as<1>(out, dtype, c, &total);
+  }
+}
+
+// Shared host checks (layer_norm.cu).  check_matrix: a pointer
 // (NULL only where optional) aligned to its type, and a pitch that holds a
-// row.  column_sum: out[c] = the sum of `count` FP32 partial rows of `dim`
-// values, in a fixed order.
+// row.
 vcsr_status check_matrix(const char *name, const void *p, int64_t ld, int64_t dim, int type,
                          bool optional);
-vcsr_status column_sum(const float *partial, int count, int64_t dim, void *out, int dtype,
-                       cudaStream_t st);
 
 // SMs of the current device, and a kernel's dynamic shared memory limit raised to
 // `bytes`: asked of the runtime once per device (and kernel), since each question

@@ -77,10 +77,15 @@ constexpr int kSplitStages = kRing / (kPBytes + BN * 128);
 template <int BN>
 constexpr size_t kSplitSmem = (size_t)kSplitStages<BN> * (kPBytes + BN * 128) + 1024 + 512;
 
+// One product, or two that share a launch: the clusters from `second` on are the other's.
+struct SplitJobs {
+  TcArgs a[2];
+  CUtensorMap p[2], q[2];
+  int splits, second;
+};
+
 template <int BN, bool CODES>
-__global__ void __launch_bounds__(kSplitThreads, 1)
-    gemm_split_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap mp,
-                      const __grid_constant__ CUtensorMap mq, int splits) {
+__global__ void __launch_bounds__(kSplitThreads, 1) gemm_split_kernel(const __grid_constant__ SplitJobs jobs) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   unsigned char *ring = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -94,8 +99,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // the same in all lanes, and known to be: what the MMA warp computes then stays in
   // uniform registers, where its instructions want their operands
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const int rank = splits > 1 ? (int)cluster_rank() : 0;
-  const int tile = blockIdx.x / splits;
+  const int splits = jobs.splits, rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int cluster = blockIdx.x / splits, which = cluster >= jobs.second ? 1 : 0;
+  const int tile = cluster - which * jobs.second;
+  const TcArgs &a = jobs.a[which];
+  const CUtensorMap *mp = &jobs.p[which], *mq = &jobs.q[which];
   const int f0 = tile % a.tiles_p * kPRows, r0 = tile / a.tiles_p * BN;
   const int b0 = (int)((int64_t)a.blocks * rank / splits),
             b1 = (int)((int64_t)a.blocks * (rank + 1) / splits);
@@ -123,9 +131,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         unsigned char *st = ring + s * kStage;
         mbar_arrive_tx(full + s, kStage);
         load_operand(st, a.p_mn, f0, kPRows, b, a.block_k,
-                     [&](void *d, int x, int y) { tma_load_2d(d, &mp, x, y, full + s); });
+                     [&](void *d, int x, int y) { tma_load_2d(d, mp, x, y, full + s); });
         load_operand(st + kPBytes, a.q_mn, r0, BN, b, a.block_k,
-                     [&](void *d, int x, int y) { tma_load_2d(d, &mq, x, y, full + s); });
+                     [&](void *d, int x, int y) { tma_load_2d(d, mq, x, y, full + s); });
       }
     }
   } else if (warp == 5) {
@@ -398,22 +406,55 @@ const void *split_kernel(int dtype) {
                             : reinterpret_cast<const void *>(gemm_split_kernel<BN, false>);
 }
 
+TcArgs args_of(const Gemm &g) {
+  TcArgs a{};
+  a.P = (int)g.N;
+  a.Q = (int)g.M;
+  a.block_k = 128 / (int)type_size(g.dtype);
+  a.blocks = (int)ceil_div(g.K, a.block_k);
+  a.p_mn = g.b.transposed;
+  a.q_mn = g.a.transposed;
+  a.e = g.e;
+  return a;
+}
+
 template <int BN>
-vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
-  CUtensorMap mp, mq;
-  VCSR_TRY(make_map(&mp, g.b, g.N, g.K, g.dtype, kPRows));
-  VCSR_TRY(make_map(&mq, g.a, g.M, g.K, g.dtype, BN));
-  a.tiles_p = (int)ceil_div(a.P, kPRows);
-  a.tiles_q = (int)ceil_div(a.Q, BN);
-  const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
-  const int splits = choose_splits(split_kernel<BN>(g.dtype), kSplitThreads, kSplitSmem<BN>, tiles, a.blocks);
-  if (tiles * splits > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
-  const int grid = (int)(tiles * splits);
-  const int format = g.dtype == VCSR_BF16 ? 1 : 0;
-  a.idesc = instr_desc(format, a.p_mn, a.q_mn, 128, BN);
+int64_t split_tiles(const Gemm &g) {
+  return ceil_div(g.N, kPRows) * ceil_div(g.M, BN);
+}
+
+// How many CTAs share a tile's k: of one product, or of two of one type in one launch.
+template <int BN>
+int splits_of(const Gemm &g, const Gemm *g1) {
+  const int64_t tiles = split_tiles<BN>(g) + (g1 ? split_tiles<BN>(*g1) : 0);
+  const int b0 = args_of(g).blocks;
+  return choose_splits(split_kernel<BN>(g.dtype), kSplitThreads, kSplitSmem<BN>, tiles,
+                       g1 ? std::min(b0, args_of(*g1).blocks) : b0);
+}
+
+// One product, or two of one type (g1).
+template <int BN>
+vcsr_status launch_split(const Gemm &g, const Gemm *g1, int splits, cudaStream_t st) {
+  SplitJobs jobs{};
+  int64_t tiles = 0;
+  for (int i = 0; i < (g1 ? 2 : 1); ++i) {
+    const Gemm &gi = i ? *g1 : g;
+    TcArgs &a = jobs.a[i];
+    a = args_of(gi);
+    VCSR_TRY(make_map(&jobs.p[i], gi.b, gi.N, gi.K, gi.dtype, kPRows));
+    VCSR_TRY(make_map(&jobs.q[i], gi.a, gi.M, gi.K, gi.dtype, BN));
+    a.tiles_p = (int)ceil_div(a.P, kPRows);
+    a.tiles_q = (int)ceil_div(a.Q, BN);
+    a.idesc = instr_desc(gi.dtype == VCSR_BF16 ? 1 : 0, a.p_mn, a.q_mn, 128, BN);
+    tiles += split_tiles<BN>(gi);
+    if (i == 0) jobs.second = tiles > 0x7fffffffll ? 0x7fffffff : (int)tiles;
+  }
+  jobs.splits = splits;
+  if (tiles * jobs.splits > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
+  const int grid = (int)(tiles * jobs.splits);
   return g.dtype == VCSR_E4M3
-             ? launch(gemm_split_kernel<BN, true>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits)
-             : launch(gemm_split_kernel<BN, false>, grid, kSplitThreads, kSplitSmem<BN>, splits, st, a, mp, mq, splits);
+             ? launch(gemm_split_kernel<BN, true>, grid, kSplitThreads, kSplitSmem<BN>, jobs.splits, st, jobs)
+             : launch(gemm_split_kernel<BN, false>, grid, kSplitThreads, kSplitSmem<BN>, jobs.splits, st, jobs);
 }
 
 // Expected microseconds, to choose between the kernels: a launch, then for every round
@@ -425,21 +466,27 @@ vcsr_status launch_split(TcArgs &a, const Gemm &g, cudaStream_t st) {
 // 11.0; 512 x 1024, k = 1024: - / - / 9.4 / 10.0 / 16.5; 1024 x 4096, k = 1024: - / - /
 // 41.3 / 25.5 / 17.2.
 template <int BN>
-double split_cost(const TcArgs &a, int dtype) {
+double split_cost(const Gemm &g, const Gemm *g1 = nullptr) {
   constexpr double kFixed = BN == 16 ? 3.8 : BN == 32 ? 4.2 : BN == 64 ? 5.0 : 7.0;
   constexpr double kStage = BN == 16 ? 0.29 : BN == 128 ? 0.36 : 0.32;
-  const int64_t tiles = ceil_div(a.P, kPRows) * ceil_div(a.Q, BN);
-  const int splits = choose_splits(split_kernel<BN>(dtype), kSplitThreads, kSplitSmem<BN>, tiles, a.blocks);
+  // boxes along the operand's own index are 64 rows
+  if (BN < 64 && (g.a.transposed || (g1 && g1->a.transposed))) return 1e30;
+  const int64_t tiles = split_tiles<BN>(g) + (g1 ? split_tiles<BN>(*g1) : 0);
+  const int64_t b0 = args_of(g).blocks, b1 = g1 ? args_of(*g1).blocks : b0;
+  const int splits = splits_of<BN>(g, g1);
+  if (g1 && tiles * splits > sm_count()) return 1e30;  // two products share one round or none
   return 1.2 + (splits > 1 ? 0.7 : 0.0) +
-         (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStage * (double)ceil_div(a.blocks, splits));
+         (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStage * (double)ceil_div(std::max(b0, b1), splits));
 }
-double pair_cost(const TcArgs &a) {
-  const int64_t rounds = ceil_div(ceil_div(a.P, 256) * ceil_div(a.Q, 256), sm_count() / 2);
-  return 11.5 + 0.33 * a.blocks + (double)(rounds - 1) * std::max(8.0, 0.42 * a.blocks);
+double pair_cost(const Gemm &g) {
+  const int blocks = args_of(g).blocks;
+  const int64_t rounds = ceil_div(ceil_div(g.N, 256) * ceil_div(g.M, 256), sm_count() / 2);
+  return 11.5 + 0.33 * blocks + (double)(rounds - 1) * std::max(8.0, 0.42 * blocks);
 }
 
 template <int BN>
-vcsr_status launch_pair(TcArgs &a, const Gemm &g, cudaStream_t st) {
+vcsr_status launch_pair(const Gemm &g, cudaStream_t st) {
+  TcArgs a = args_of(g);
   CUtensorMap mp, mq;
   VCSR_TRY(make_map(&mp, g.b, g.N, g.K, g.dtype, kPRows));
   VCSR_TRY(make_map(&mq, g.a, g.M, g.K, g.dtype, BN / 2));
@@ -461,26 +508,46 @@ bool tc_aligned(const void *p, int64_t ld, int dtype) {
   return aligned(p, 16) && (ld * (int64_t)type_size(dtype)) % 16 == 0;
 }
 
-vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st) {
-  TcArgs a{};
-  a.P = (int)g.N;
-  a.Q = (int)g.M;
-  a.block_k = 128 / (int)type_size(g.dtype);
-  a.blocks = (int)ceil_div(g.K, a.block_k);
-  a.p_mn = g.b.transposed;
-  a.q_mn = g.a.transposed;
-  a.e = g.e;
-  // 16 and 32 rows per tile are for operands stored along k (a box along the
-  // operand's own index is 64 rows)
-  const double costs[5] = {a.q_mn ? 1e30 : split_cost<16>(a, g.dtype), a.q_mn ? 1e30 : split_cost<32>(a, g.dtype),
-                           split_cost<64>(a, g.dtype), split_cost<128>(a, g.dtype), pair_cost(a)};
-  switch (std::min_element(costs, costs + 5) - costs) {
-    case 0: return launch_split<16>(a, g, st);
-    case 1: return launch_split<32>(a, g, st);
-    case 2: return launch_split<64>(a, g, st);
-    case 3: return launch_split<128>(a, g, st);
-    default: return launch_pair<256>(a, g, st);
+namespace {
+
+struct Choice {
+  int kernel;  // 0 to 3: split, 16 to 128 rows; 4: pair
+  double cost;
+};
+Choice choose(const Gemm &g) {
+  const double costs[5] = {split_cost<16>(g), split_cost<32>(g), split_cost<64>(g), split_cost<128>(g), pair_cost(g)};
+  const int best = (int)(std::min_element(costs, costs + 5) - costs);
+  return {best, costs[best]};
+}
+vcsr_status launch_chosen(const Choice &c, const Gemm &g, cudaStream_t st) {
+  switch (c.kernel) {
+    case 0: return launch_split<16>(g, nullptr, splits_of<16>(g, nullptr), st);
+    case 1: return launch_split<32>(g, nullptr, splits_of<32>(g, nullptr), st);
+    case 2: return launch_split<64>(g, nullptr, splits_of<64>(g, nullptr), st);
+    case 3: return launch_split<128>(g, nullptr, splits_of<128>(g, nullptr), st);
+    default: return launch_pair<256>(g, st);
   }
+}
+
+}  // namespace
+
+vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st) { return launch_chosen(choose(g), g, st); }
+
+vcsr_status launch_gemms_tc(const Gemm &g0, const Gemm &g1, cudaStream_t st) {
+  const Choice c0 = choose(g0), c1 = choose(g1);
+  const double both64 = split_cost<64>(g0, &g1), both128 = split_cost<128>(g0, &g1);
+  const bool narrow = both64 <= both128;
+  // two microseconds for the launch that one call saves on the host
+  if (std::min(both64, both128) < c0.cost + c1.cost + 2.0) {
+    const int splits = narrow ? splits_of<64>(g0, &g1) : splits_of<128>(g0, &g1);
+    // one of them alone is summed as it is beside the other: the same result
+    const Gemm &first = g0.e.out ? g0 : g1;
+    const Gemm *second = g0.e.out && g1.e.out ? &g1 : nullptr;
+    return narrow ? launch_split<64>(first, second, splits, st) : launch_split<128>(first, second, splits, st);
+  }
+  if (g0.e.out) VCSR_TRY(launch_chosen(c0, g0, st));
+  if (g1.e.out) VCSR_TRY(launch_chosen(c1, g1, st));
+  return VCSR_OK;
 }
 
 int cluster_slots(const void *kernel, int threads, size_t smem, int size) {

@@ -1,10 +1,11 @@
 // layer_linear.cu — vcsr_linear and its gradient: argument checks, the
 // activation's gradient, and which product kernel runs.
 //
-// The gradient takes three steps: dz = dy act'(pre), rounded to the operands'
-// type, with dbias' partial column sums of the unrounded dz in the same pass
-// (one pass over dy and pre; without an activation dz is dy itself and only the
-// sums are made); dx = dz w; dw = dz^T x.
+// The gradient takes up to four launches: dz = dy act'(pre), rounded to the operands'
+// type, with dbias' partial column sums of the unrounded dz in the same pass (one pass
+// over dy and pre; without an activation dz is dy itself and only the sums are made);
+// dbias from the partial sums, with aligned copies of operands that TMA cannot read;
+// dx = dz w and dw = dz^T x, in one launch where both are small.
 #include <algorithm>
 
 #include "layer_gemm.cuh"
@@ -95,13 +96,28 @@ struct PackJob {
   void *dst;
   int64_t ld, ldd, rows, cols;
 };
-struct PackJobs {
+// The copies, and the column sums of dbias' partial rows, that go before the products.
+struct PrepareJobs {
   PackJob job[3];
+  int packs;
+  const float *partial;
+  int partials, dtype;
+  int64_t N;
+  void *dbias;
 };
 
-// Block row y copies job y; a thread writes 16 bytes.
+// Block row y copies job y, a thread 16 bytes at a time; the row after the last sums
+// columns.
 template <class T>
-__global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackJobs jobs) {
+__global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ PrepareJobs jobs) {
+  if (blockIdx.y == jobs.packs) {
+    __shared__ float part[8][33];
+    for (int64_t group = blockIdx.x; group * 32 < jobs.N; group += gridDim.x) {
+      column_sum_block(jobs.partial, jobs.partials, jobs.N, jobs.dbias, jobs.dtype, group, part);
+      __syncthreads();
+    }
+    return;
+  }
   constexpr int V = 16 / sizeof(T);
   const PackJob &p = jobs.job[blockIdx.y];
   const T *src = static_cast<const T *>(p.src);
@@ -143,31 +159,39 @@ Packed packed(const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) 
   }
   return k;
 }
-// The copies of one call, made by one launch.
-struct Packer {
-  PackJobs jobs{};
-  int count = 0;
-  int64_t most = 0;  // 16-byte pieces of the largest
+// What goes before a call's products, made by one launch.
+struct Prepare {
+  PrepareJobs jobs{};
+  int64_t most = 0;  // blocks of the largest job
   char *ws;
-  explicit Packer(void *workspace) : ws(static_cast<char *>(workspace)) {}
+  explicit Prepare(void *workspace) : ws(static_cast<char *>(workspace)) {}
   // Where the tensor cores read matrix p: the matrix, or its copy to be.
-  const void *add(const Packed &k, const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+  const void *matrix(const Packed &k, const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
     if (!k.copy) return p;
-    jobs.job[count++] = {p, ws, ld, k.ld, rows, cols};
-    most = std::max(most, rows * k.ld * (int64_t)type_size(dtype) / 16);
+    jobs.job[jobs.packs++] = {p, ws, ld, k.ld, rows, cols};
+    most = std::max(most, ceil_div(rows * k.ld * (int64_t)type_size(dtype) / 16, 256));
     p = ws;
     ws += k.bytes;
     return p;
   }
+  void column_sums(const float *partial, int count, int64_t N, void *out) {
+    jobs.partial = partial;
+    jobs.partials = count;
+    jobs.N = N;
+    jobs.dbias = out;
+    most = std::max(most, ceil_div(N, 32));
+  }
   vcsr_status run(int dtype, cudaStream_t st) {
-    if (count == 0) return VCSR_OK;
-    const dim3 grid((unsigned)std::min<int64_t>(ceil_div(most, 256), (int64_t)sm_count() * 8), (unsigned)count);
+    const int rows = jobs.packs + (jobs.dbias ? 1 : 0);
+    if (rows == 0) return VCSR_OK;
+    jobs.dtype = dtype;
+    const dim3 grid((unsigned)std::min<int64_t>(most, (int64_t)sm_count() * 8), (unsigned)rows);
     if (dtype == VCSR_E4M3)
-      pack_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
+      prepare_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
     else if (dtype == VCSR_F32)
-      pack_kernel<float><<<grid, 256, 0, st>>>(jobs);
+      prepare_kernel<float><<<grid, 256, 0, st>>>(jobs);
     else
-      pack_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
+      prepare_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
     VCSR_CUDA(cudaGetLastError());
     return VCSR_OK;
   }
@@ -242,10 +266,10 @@ vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
   VCSR_TRY(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(a)));
   const void *x = a->x, *w = a->w;
   if (a->K > 0) {
-    Packer packer(a->workspace);
-    x = packer.add(px, x, a->ldx, a->M, a->K, a->dtype);
-    w = packer.add(pw, w, a->ldw, a->N, a->K, a->dtype);
-    VCSR_TRY(packer.run(a->dtype, st));
+    Prepare before(a->workspace);
+    x = before.matrix(px, x, a->ldx, a->M, a->K, a->dtype);
+    w = before.matrix(pw, w, a->ldw, a->N, a->K, a->dtype);
+    VCSR_TRY(before.run(a->dtype, st));
   }
   return launch_gemm({a->M, a->N, a->K, {x, px.ld, false}, {w, pw.ld, false}, a->dtype,
                       {a->x_scale, a->w_scale, a->bias, a->residual, a->y, a->pre, a->ldr, a->ldy,
@@ -314,28 +338,26 @@ vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
     else
       launch_dz<__half>(a, static_cast<__half *>(dz), p.lddz, partial, st);
     VCSR_CUDA(cudaGetLastError());
-    if (a->dbias)
-      VCSR_TRY(column_sum(partial, (int)dz_chunks(a->M, a->N), a->N, a->dbias, a->dtype, st));
   }
+  Prepare before(ws + p.dz + p.partial);
+  if (a->dbias) before.column_sums(partial, (int)dz_chunks(a->M, a->N), a->N, a->dbias);
+  const void *d = dz ? dz : before.matrix(p.dy, a->dy, a->lddy, a->M, a->N, a->dtype);
+  const void *x = before.matrix(p.x, a->x, a->ldx, a->M, a->K, a->dtype);
+  const void *w = before.matrix(p.w, a->w, a->ldw, a->N, a->K, a->dtype);
+  VCSR_TRY(before.run(a->dtype, st));
   if (a->K == 0) return VCSR_OK;
-  Packer packer(ws + p.dz + p.partial);
-  const void *d = dz ? dz : packer.add(p.dy, a->dy, a->lddy, a->M, a->N, a->dtype);
-  const void *x = packer.add(p.x, a->x, a->ldx, a->M, a->K, a->dtype);
-  const void *w = packer.add(p.w, a->w, a->ldw, a->N, a->K, a->dtype);
-  VCSR_TRY(packer.run(a->dtype, st));
   const int64_t ldd = dz ? p.lddz : p.dy.ld;
   Epilogue e{};
   e.type = a->dtype;
-  if (a->dx) {
-    e.out = a->dx;
-    e.ldo = a->lddx;
-    VCSR_TRY(launch_gemm({a->M, a->K, a->N, {d, ldd, false}, {w, p.w.ld, true}, a->dtype, e}, st));
-  }
-  if (a->dw) {
-    e.out = a->dw;
-    e.ldo = a->lddw;
-    VCSR_TRY(launch_gemm({a->N, a->K, a->M, {d, ldd, true}, {x, p.x.ld, true}, a->dtype, e}, st));
-  }
+  e.out = a->dx;
+  e.ldo = a->lddx;
+  const Gemm dx{a->M, a->K, a->N, {d, ldd, false}, {w, p.w.ld, true}, a->dtype, e};
+  e.out = a->dw;
+  e.ldo = a->lddw;
+  const Gemm dw{a->N, a->K, a->M, {d, ldd, true}, {x, p.x.ld, true}, a->dtype, e};
+  if (a->dtype != VCSR_F32) return launch_gemms_tc(dx, dw, st);
+  if (a->dx) VCSR_TRY(launch_gemm(dx, st));
+  if (a->dw) VCSR_TRY(launch_gemm(dw, st));
   return VCSR_OK;
 }
 

@@ -84,39 +84,12 @@ vcsr_status check_matrix(const char *name, const void *p, int64_t ld, int64_t di
 
 namespace {
 
-// out[c] = sum of `count` partial rows, in order within each of 8 slices of
-// them, the slices then added in order.  A block takes 32 columns.
+// Partial rows to their sums; a block takes 32 columns.
 __global__ void __launch_bounds__(256)
     column_sum_kernel(const float *partial, int count, int64_t dim, void *out, int dtype) {
   __shared__ float part[8][33];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-  float sum = 0.0f;
-  if (c < dim) {
-    const int per = (count + 7) / 8, lo = slice * per, hi = min(count, lo + per);
-#pragma unroll 8
-    for (int p = lo; p < hi; ++p) sum += partial[(int64_t)p * dim + c];
-  }
-  part[slice][lane] = sum;
-  __syncthreads();
-  if (slice == 0 && c < dim) {
-    float total = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) total += part[k][lane];
-    store_as<1>(out, dtype, c, &total);
-  }
+  column_sum_block(partial, count, dim, out, dtype, blockIdx.x, part);
 }
-
-}  // namespace
-
-vcsr_status column_sum(const float *partial, int count, int64_t dim, void *out, int dtype,
-                       cudaStream_t st) {
-  column_sum_kernel<<<(unsigned)ceil_div(dim, 32), 256, 0, st>>>(partial, count, dim, out, dtype);
-  VCSR_CUDA(cudaGetLastError());
-  return VCSR_OK;
-}
-
-namespace {
 
 constexpr int kMaxThreads = 1024;
 // The most values a thread holds, in V-value vectors, and the largest block
@@ -841,7 +814,12 @@ vcsr_status rmsnorm_grad(const vcsr_rmsnorm_grad_args *a, cudaStream_t st) {
   });
   VCSR_TRY(done);
   VCSR_CUDA(cudaGetLastError());
-  return a->dweight ? column_sum(k.partial, blocks, a->dim, a->dweight, a->w_dtype, st) : VCSR_OK;
+  if (a->dweight) {
+    column_sum_kernel<<<(unsigned)ceil_div(a->dim, 32), 256, 0, st>>>(k.partial, blocks, a->dim, a->dweight,
+                                                                    a->w_dtype);
+    VCSR_CUDA(cudaGetLastError());
+  }
+  return VCSR_OK;
 }
 
 vcsr_status dequantize(const void *codes, int64_t ldc, const float *scale, int64_t rows, int64_t dim,

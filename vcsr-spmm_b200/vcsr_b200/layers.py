@@ -93,6 +93,8 @@ def _matrix(t, name, like, rows, cols, dtype):
 def _out(t, name, like, rows, cols, dtype):
     """The output t (checked), or a new one."""
     if t is None:
+        if like.dtype is dtype and like.shape == (rows, cols) and like.is_contiguous():
+            return torch.empty_like(like), cols
         return like.new_empty((rows, cols), dtype=dtype), cols
     got, ld = _matrix(t, name, like, rows, cols, dtype)
     if got is not t:
@@ -186,7 +188,7 @@ def rmsnorm_backward(dy, s, weight, rstd, dsum=None, need_dweight=True):
     ldds = 0
     if dsum is not None:
         dsum, ldds = _matrix(dsum, "dsum", dy, rows, dim, dt)
-    dx = s.new_empty((rows, dim))
+    dx = torch.empty_like(s, memory_format=torch.contiguous_format)
     dw = ws = None
     n = 0
     if need_dweight:
@@ -263,7 +265,7 @@ def linear(x, w, bias=None, residual=None, act=None, x_scale=None, w_scale=None,
     ldr = 0
     if residual is not None:
         residual, ldr = _matrix(residual, "residual", x, M, N, out_dtype)
-    y, ldy = _out(out, "out", x, M, N, out_dtype)
+    y, ldy = _out(out, "out", x if residual is None else residual, M, N, out_dtype)
     pre = torch.empty_like(y) if save_pre and out is None else None
     if save_pre and pre is None:
         pre = x.new_empty((M, N), dtype=out_dtype)
@@ -305,8 +307,8 @@ def linear_backward(dy, x, w, pre=None, act=None, need_dx=True, need_dw=True,
         pre, ldp = _matrix(pre, "pre", dy, M, N, dt)
     else:
         pre = None
-    dx = dy.new_empty((M, K)) if need_dx else None
-    dw = dy.new_empty((N, K)) if need_dw else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_dx else None
+    dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need_dw else None
     db = dy.new_empty(N) if need_db else None
     a = _LinearGradArgs(M, N, K, dy.data_ptr(), lddy, _p(pre), ldp, x.data_ptr(), ldx,
                         w.data_ptr(), ldw, _p(dx), K, _p(dw), K, _p(db), None, 0, code, act)
