@@ -14,15 +14,19 @@
 //
 // Tile: 128 features x 32, 64 or 128 rows per CTA (layer_gemm_tc.cu says why
 // features are the MMA's M side), 32 values of k per stage.  One thread brings the
-// FP32 tiles in by TMA (128-byte rows, 128-byte swizzle); eight warps split them
-// into three planes of bfloat16 in the order the MMAs read (stored along k: 64-byte
-// rows, 64-byte swizzle; along the operand's own index: 128-byte rows of 64 values);
-// one thread issues 12 MMAs per stage; four to sixteen warps drain the accumulators,
-// two of which alternate.  All roles run at once.  128 x 128 tiles are bound by shared
-// memory: per stage 32 KB in, 32 KB read and 48 KB written by the split, 96 KB read
-// by the MMAs.  Persistent over tiles; where tiles are too few for the SMs, clusters
-// of 2 to 8 CTAs split k and join their sums in rank order through distributed
-// shared memory.
+// FP32 tiles in by TMA (128-byte rows, 128-byte swizzle); eight warps split them into
+// three parts, the features' into tensor memory, where the MMAs take their M side from
+// (a third of the shared-memory traffic gone), the rows' into planes of shared memory
+// in the order the MMAs read (stored along k: 64-byte rows, 64-byte swizzle; along the
+// operand's own index: 128-byte rows of 64 values); one thread issues 12 MMAs per stage;
+// four to sixteen warps drain the accumulators, three or four of which take turns.  All
+// roles run at once.  Bound by the splitting warps' instructions: 0.5 to 0.9 us a stage,
+// of which the MMAs take 0.4 (128 x 128).  Two groups of splitting warps that take
+// stages in turn were no faster (255 against 239 us, 4096 x 4096, k = 1024).
+// Persistent over tiles; where tiles are too few for the SMs, clusters of 2 to 8 CTAs
+// split k and join their sums in rank order through distributed shared memory.
+// 4096 x 4096, k = 1024: 208 to 224 us, 153 to 165 TFLOP/s; 16 x 4096, k = 4096: 25 us, 2.7 TB/s;
+// 62451 x 128, k = 128 with every part of the epilogue: 33 us, 3.9 TB/s.
 #include <algorithm>
 
 #include "layer_gemm_tc.cuh"
@@ -43,17 +47,24 @@ template <int BN>
 constexpr int kDraining = BN / 8;
 template <int BN>
 constexpr int kThreads = 32 * (kSplitters + kDraining<BN> + 2);
-constexpr int kPlane = kRows * kK * 2;  // one part of P's tile, bytes
+constexpr int kPart = kK / 2;   // tensor-memory columns of one part of P's tile
 
 // Bytes and counts of the FP32 stages and of the split ones.
 template <int BN>
 constexpr int kRaw = (kRows + BN) * kK * 4;
 template <int BN>
-constexpr int kSplit = 3 * (kRows + BN) * kK * 2;
+constexpr int kSplit = 3 * BN * kK * 2;
 template <int BN>
-constexpr int kRaws = BN == 128 ? 3 : BN == 64 ? 4 : 5;
+constexpr int kRaws = BN == 128 ? 5 : BN == 64 ? 6 : 8;
 template <int BN>
-constexpr int kSplits = BN == 128 ? 2 : 3;
+constexpr int kSplits = BN == 128 ? 2 : 4;
+// Accumulators, as many as tensor memory holds beside P's parts: the next tile's first
+// stages are multiplied while the draining warps are in this one's epilogue.
+template <int BN>
+constexpr int kSums = BN == 128 ? 3 : 4;
+constexpr int kColumns = 512;  // of tensor memory; one CTA an SM
+static_assert(kSums<128> * 128 + kSplits<128> * 3 * kPart <= kColumns, "");
+static_assert(kSums<64> * 64 + kSplits<64> * 3 * kPart <= kColumns, "");
 template <int BN>
 constexpr size_t kSmem = (size_t)kRaws<BN> * kRaw<BN> + kSplits<BN> * kSplit<BN> + 1024 + 512;
 
@@ -83,11 +94,64 @@ __device__ __forceinline__ void load_raw(unsigned char *dst, const CUtensorMap *
 __device__ __forceinline__ uint32_t pair(float lo, float hi) {
   return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
 }
-__device__ __forceinline__ float leading(float x) {
-  return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+// Takes both from the values, exactly.
+__device__ __forceinline__ void take_leading(uint32_t p, float &lo, float &hi) {
+  constexpr unsigned short kMinusOne = 0xbf80;
+  asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; fma.rn.f32.bf16 %0, l, %3, %0; fma.rn.f32.bf16 %1, h, %3, %1; }"
+      : "+f"(lo), "+f"(hi)
+      : "r"(p), "h"(kMinusOne));
+}
+// The leading parts of 2 N values, which are left with the rest.  The 16-bit operands
+// save the masks that would widen them: the split bounds a stage (1.01 us with masks,
+// 0.83 without, tiles of 128 rows).
+template <int N>
+__device__ __forceinline__ void cut(float *v, uint32_t *p) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) p[j] = pair(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) take_leading(p[j], v[2 * j], v[2 * j + 1]);
 }
 
-// Splits one tile: `rows` (a multiple of 64, or 32) by 32 values of k from `raw`
+// The 16 values of v in three parts to `column` (of this warp's 32 lanes) and kPart,
+// 2 kPart further.
+__device__ __forceinline__ void parts_to_tmem(uint32_t column, float *v) {
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    uint32_t p[8];
+    cut<8>(v, p);
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(
+                     column + part * kPart),
+                 "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]), "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
+                 : "memory");
+  }
+}
+
+// Splits P's tile of 128 rows by 32 values of k from `raw` to tensor memory, a row per
+// lane.  Warps w and w + 4 take the rows whose lanes they reach, 16 values of k each.
+__device__ __forceinline__ void split_p(uint32_t raw, uint32_t column, int mn, int warp, int lane) {
+  const int quarter = warp & 3, half = warp >> 2;
+  float v[16];
+  if (mn) {  // boxes of 32 rows: a 128-byte row per k
+    const uint32_t box = raw + quarter * 4096 + (lane & 3) * 4;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int k = half * 16 + j;
+      asm volatile("ld.shared.f32 %0, [%1];"
+                   : "=f"(v[j])
+                   : "r"(box + k * 128 + (((lane >> 2) ^ (k & 7)) << 4)));
+    }
+  } else {
+    const int row = quarter * 32 + lane;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(v[4 * c]), "=f"(v[4 * c + 1]), "=f"(v[4 * c + 2]), "=f"(v[4 * c + 3])
+                   : "r"(raw + row * 128 + (((half * 4 + c) ^ (row & 7)) << 4)));
+  }
+  parts_to_tmem(column + ((uint32_t)(quarter * 32) << 16) + half * 8, v);
+}
+
+// Splits Q's tile, ROWS (a multiple of 64, or 32) by 32 values of k, from `raw`
 // to three planes, `plane` bytes apart, from `out` on.  A thread takes 8 values
 // that are neighbours in memory: two 16-byte pieces in, one per plane out.  In both
 // orders 8 neighbouring lanes touch all banks once.
@@ -112,28 +176,28 @@ __device__ __forceinline__ void split_tile(uint32_t raw, uint32_t out, int mn, i
       in1 = raw + r * 128 + (((2 * c + 1) ^ (r & 7)) << 4);
       at = out + r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
     }
-    float a[4], b[4], v[8];
+    float v[8];
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(a[0]), "=f"(a[1]), "=f"(a[2]), "=f"(a[3])
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
                  : "r"(in0));
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(b[0]), "=f"(b[1]), "=f"(b[2]), "=f"(b[3])
+                 : "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
                  : "r"(in1));
+    if (mn) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = swap ? b[j] : a[j];
-      v[4 + j] = swap ? a[j] : b[j];
+      for (int j = 0; j < 4; ++j) {
+        const float first = v[j];
+        v[j] = swap ? v[4 + j] : first;
+        v[4 + j] = swap ? first : v[4 + j];
+      }
     }
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + part * kPlaneBytes),
-                   "r"(pair(v[0], v[1])), "r"(pair(v[2], v[3])), "r"(pair(v[4], v[5])),
-                   "r"(pair(v[6], v[7]))
+      uint32_t p[4];
+      cut<4>(v, p);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + part * kPlaneBytes), "r"(p[0]),
+                   "r"(p[1]), "r"(p[2]), "r"(p[3])
                    : "memory");
-      if (part < 2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] -= leading(v[j]);
-      }
     }
   }
 }
@@ -188,12 +252,11 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   unsigned char *ring = reinterpret_cast<unsigned char *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   constexpr int R = kRaws<BN>, S = kSplits<BN>;
-  constexpr uint32_t kColumns = 2 * BN;
   constexpr int kLoadWarp = kSplitters + kDraining<BN>, kMmaWarp = kLoadWarp + 1;
   unsigned char *raw = ring + S * kSplit<BN>;
   uint64_t *full = reinterpret_cast<uint64_t *>(raw + R * kRaw<BN>), *empty = full + S;
   uint64_t *rfull = empty + S, *rempty = rfull + R;
-  uint64_t *dfull = rempty + R, *dfree = dfull + 2, *drain = dfree + 2;
+  uint64_t *dfull = rempty + R, *dfree = dfull + kSums<BN>, *drain = dfree + kSums<BN>;
   uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
 
@@ -213,7 +276,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
       mbar_init(rfull + s, 1);
       mbar_init(rempty + s, kSplitters);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kSums<BN>; ++b) {
       mbar_init(dfull + b, 1);
       mbar_init(dfree + b, kDraining<BN>);
     }
@@ -225,7 +288,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  const uint32_t tmem = *holder;
+  const uint32_t tmem = *holder, p_parts = tmem + kSums<BN> * BN;
 
   float acc[32];  // draining warps
 #pragma unroll
@@ -239,16 +302,20 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     for (int t = first; t < tiles && go; t += stride) {
       for (int b = b0; b < b1; ++b, in.next(), out.next()) {
         const int r = in.stage, s = out.stage;
-        if (!mbar_wait(rfull + r, in.full(), abort_flag, kWaitFull) ||
-            !mbar_wait(empty + s, out.empty(), abort_flag, kWaitEmpty)) {
+        const bool ready = mbar_wait(rfull + r, in.full(), abort_flag, kWaitFull) &&
+                           mbar_wait(empty + s, out.empty(), abort_flag, kWaitEmpty);
+        if (!__all_sync(0xffffffffu, ready)) {
           go = false;
           break;
         }
+        fence_after_sync();
         const uint32_t from = smem_u32(raw + r * kRaw<BN>), to = smem_u32(ring + s * kSplit<BN>);
-        split_tile<kRows>(from, to, a.p_mn, threadIdx.x);
-        split_tile<BN>(from + kRows * kK * 4, to + 3 * kPlane, a.q_mn, threadIdx.x);
-        // the MMAs read what was written by plain stores
+        split_p(from, p_parts + s * 3 * kPart, a.p_mn, warp, lane);
+        split_tile<BN>(from + kRows * kK * 4, to, a.q_mn, threadIdx.x);
+        // the MMAs read what was written by plain stores, and to tensor memory
         fence_async();
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        fence_before_sync();
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(full + s);
@@ -275,16 +342,16 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
           load_raw(to + kRows * kK * 4, &mq, a.q_mn, tq * BN, BN, b * kK, rfull + r);
         }
       }
-      // copies that nobody waited for land before the CTA leaves
+      // every copy lands before the CTA leaves, whoever gave up
       volatile int keep = 0;
-      for (int n = max(0, g - R); n < g && !go; ++n)
+      for (int n = max(0, g - R); n < g; ++n)
         mbar_wait(rfull + n % R, (uint32_t)((n / R) & 1), &keep, kWaitFull);
     }
   } else if (warp == kMmaWarp) {
-    const uint32_t idesc = instr_desc(1, a.p_mn, a.q_mn, kRows, BN);
-    const uint32_t p_step = a.p_mn ? 2048 / 16 : 32 / 16, q_step = a.q_mn ? 2048 / 16 : 32 / 16;
+    const uint32_t idesc = instr_desc(1, 0, a.q_mn, kRows, BN);
+    const uint32_t q_step = a.q_mn ? 2048 / 16 : 32 / 16;
     RingPlace<S> at;
-    RingPlace<2> sums;
+    RingPlace<kSums<BN>> sums;
     bool go = true;
     for (int t = first; t < tiles && go; t += stride) {
       for (int b = b0; b < b1; ++b, at.next(), sums.next()) {
@@ -296,18 +363,18 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
           break;
         }
         fence_after_sync();
-        const uint32_t pa = smem_u32(ring + s * kSplit<BN>), qa = pa + 3 * kPlane;
-        const uint64_t pd = plane_desc(pa, a.p_mn), qd = plane_desc(qa, a.q_mn);
+        const uint32_t pa = p_parts + s * 3 * kPart;
+        const uint64_t qd = plane_desc(smem_u32(ring + s * kSplit<BN>), a.q_mn);
         if (elect_one()) {
           // parts of P and Q, smallest products first
-          constexpr int kPart[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
+          constexpr int kParts[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
 #pragma unroll
           for (int m = 0; m < 6; ++m)
 #pragma unroll
             for (int k = 0; k < 2; ++k)
-              mma<1, false>(tmem + buf * BN, pd + kPart[m][0] * (kPlane / 16) + k * p_step,
-                            qd + kPart[m][1] * (BN * kK * 2 / 16) + k * q_step, idesc,
-                            (m > 0 || k > 0) ? 1u : 0u);
+              mma_tmem(tmem + buf * BN, pa + kParts[m][0] * kPart + k * 8,
+                       qd + kParts[m][1] * (BN * kK * 2 / 16) + k * q_step, idesc,
+                       (m > 0 || k > 0) ? 1u : 0u);
           mma_commit(empty + s);
           mma_commit(dfull + buf);
         }
@@ -320,7 +387,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
       if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
     }
   } else if (drainer >= 0 && drainer < kDraining<BN>) {
-    int g = 0;
+    RingPlace<kSums<BN>> sums;
     bool go = true;
     for (int t = first; t < tiles && go; t += stride) {
       int tp, tq;
@@ -329,13 +396,12 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
         prefetch_residual(a.e, tp * kRows, a.P, kRows, tq * BN, a.Q, BN, drainer * 32 + lane, 32 * kDraining<BN>);
 #pragma unroll
       for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
-      for (int b = b0; b < b1; ++b, ++g) {
-        const int buf = g & 1;
-        if (!mbar_wait(dfull + buf, (uint32_t)((g >> 1) & 1), abort_flag, kWaitAccFull)) {
+      for (int b = b0; b < b1; ++b, sums.next()) {
+        const int buf = sums.stage;
+        if (!__all_sync(0xffffffffu, mbar_wait(dfull + buf, sums.full(), abort_flag, kWaitAccFull))) {
           go = false;
           break;
         }
-        __syncwarp();
         fence_after_sync();
 #pragma unroll
         for (int c = 0; c < 32; c += 16) {
@@ -427,17 +493,17 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
 
 // Expected microseconds, to choose the rows of a tile: a launch, then for every round
 // of tiles on the GPU a fixed part (the epilogue) and a part per stage of k.  Fitted to
-// 200 products of 1 to 4096 rows, 128 to 4096 features and k of 128 to 4096 in each
-// tile, with bias, silu and residual.  Tiles of 32 / 64 / 128 rows took, for 32 rows,
-// 4096 features, k = 1024: 12.6 / 14.9 / 19.6 us; 512 x 512, k = 512: 13.5 / 12.5 / 17.3;
-// 4096 x 4096, k = 1024: 740 / 442 / 283.
+// 216 products of 1 to 62451 rows, 128 to 4096 features and k of 128 to 4096 in each
+// tile, with bias, silu and residual (1% over the best tile of each on average).
+// Tiles of 32 / 64 / 128 rows took, for 512 x 512, k = 512: 11.2 / 12.3 / 20.5 us;
+// 62451 x 128, k = 128: 70.5 / 47.9 / 55.3; 4096 x 4096, k = 1024: 504 / 323 / 261.
 template <int BN>
 double tiles_cost(const F32Args &a) {
-  constexpr double kFixed = BN == 32 ? 2.1 : BN == 64 ? 2.6 : 5.4, kStageUs = BN == 32 ? 0.73 : BN == 64 ? 0.82 : 1.13;
+  constexpr double kFixed = BN == 32 ? 2.1 : BN == 64 ? 3.3 : 7.8, kStageUs = BN == 32 ? 0.52 : BN == 64 ? 0.64 : 0.95;
   const int64_t tiles = ceil_div(a.P, kRows) * ceil_div(a.Q, BN), stages = ceil_div(a.K, kK);
   const int splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>,
                                    tiles, stages);
-  return 5.2 + (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStageUs * (double)ceil_div(stages, splits));
+  return 4.8 + (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStageUs * (double)ceil_div(stages, splits));
 }
 
 }  // namespace
