@@ -160,20 +160,18 @@ __device__ __forceinline__ float e4m3_value(uint8_t c) {
 
 template <int N>
 __device__ __forceinline__ void store_codes(uint8_t *p, const float *x) {
-  Vec<uint8_t, N> o;
   if constexpr (N % 2 == 0) {
+    Vec<uint16_t, N / 2> o;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const __nv_fp8x2_storage_t two =
-          __nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3);
-      o.v[i] = (uint8_t)(two & 0xff);
-      o.v[i + 1] = (uint8_t)(two >> 8);
-    }
+    for (int i = 0; i < N; i += 2)
+      o.v[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(x[i], x[i + 1]), __NV_SATFINITE, __NV_E4M3);
+    store_vec<uint16_t, N / 2>(reinterpret_cast<uint16_t *>(p), o);
   } else {
+    Vec<uint8_t, N> o;
 #pragma unroll
     for (int i = 0; i < N; ++i) o.v[i] = e4m3_code(x[i]);
+    store_vec<uint8_t, N>(p, o);
   }
-  store_vec<uint8_t, N>(p, o);
 }
 
 // N values stored in a type chosen at run time.

@@ -159,16 +159,25 @@ struct NormArgs {
 // A sum, and with MAX a maximum of magnitudes, over a team's threads; every thread
 // gets them.  Teams of up to 32 threads are a power of two of neighbouring lanes; a
 // larger team has whole warps, `words` of its own (two per warp) and the block's
-// barrier `id`.
+// barrier `id`.  Blocks are (threads of a team, teams): threadIdx.x is the thread's place
+// in its team without a division.
 template <bool MAX>
 __device__ __forceinline__ void team_reduce(float &sum, float &top, int team, float2 *words, int id) {
-  for (int o = min(team, 32) >> 1; o > 0; o >>= 1) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (team >= 32) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+  } else {
+    for (int o = team >> 1; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
   }
   if (team > 32) {
     const int lane = threadIdx.x & 31, warps = team >> 5;
-    if (lane == 0) words[threadIdx.x % team >> 5] = make_float2(sum, top);
+    if (lane == 0) words[threadIdx.x >> 5] = make_float2(sum, top);
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(team) : "memory");
     const float2 w = lane < warps ? words[lane] : make_float2(0.0f, 0.0f);
     sum = w.x;
@@ -191,8 +200,7 @@ __device__ __forceinline__ float team_sum(float v, int team, float2 *words, int 
 
 // An asynchronous copy of `bytes` (8, 16 or 32, 8- or 16-byte aligned) of a
 // row into this thread's own place in shared memory.
-__device__ __forceinline__ void copy_async(void *dst, const void *src, int bytes) {
-  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+__device__ __forceinline__ void copy_async(uint32_t d, const void *src, int bytes) {
   if (bytes == 8) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
   } else {
@@ -230,8 +238,8 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
     rmsnorm_kernel(const __grid_constant__ NormArgs a, int team) {
   __shared__ float2 shared[32];
   const int dim = (int)a.dim;
-  const int t = threadIdx.x % team;
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / team) + threadIdx.x / team;
+  const int t = threadIdx.x;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const bool live = row < a.rows;
   const int shift = RAGGED ? (int)(row * a.ldx & (V - 1)) : 0;
   constexpr int kN = E / V;
@@ -401,7 +409,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
   extern __shared__ __align__(16) unsigned char dynamic[];
   constexpr int kN = E / V;
   const int dim = (int)a.dim;
-  const int t = threadIdx.x % team, teams = blockDim.x / team, mine = threadIdx.x / team;
+  const int t = threadIdx.x, teams = blockDim.y, mine = threadIdx.y, linear = mine * team + t;
   const int64_t stride = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + mine;
   const int id = 1 + mine;
   // the same for all rows of a team: their distance is a multiple of 8
@@ -419,31 +427,42 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
 #pragma unroll
   for (int e = 0; e < E; ++e) dw[e] = 0.0f;
 
-  auto fetch = [&](int64_t row, int stage) {
-    if (row < a.rows) {
-      unsigned char *to = ring + (size_t)stage * row_bytes;
-      const T *s = static_cast<const T *>(a.s) + row * a.lds;
-      const char *dy = static_cast<const char *>(a.dy) + row * a.lddy * dy_size;
-      const T *ds = static_cast<const T *>(a.dsum) + row * a.ldds;
+  // the row to be copied next, this thread's first vector of it
+  int64_t ahead = first;
+  const int64_t begin = t * V - shift;
+  const char *s_next = static_cast<const char *>(a.s) + (first * a.lds + begin) * (int64_t)sizeof(T),
+             *dy_next = static_cast<const char *>(a.dy) + (first * a.lddy + begin) * dy_size,
+             *ds_next = static_cast<const char *>(a.dsum) + (first * a.ldds + begin) * (int64_t)sizeof(T);
+  const int64_t s_hop = stride * a.lds * (int64_t)sizeof(T), dy_hop = stride * a.lddy * dy_size,
+                ds_hop = stride * a.ldds * (int64_t)sizeof(T);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  auto fetch = [&](int stage) {
+    if (ahead < a.rows) {
+      const uint32_t to = ring_at + (uint32_t)(stage * row_bytes);
 #pragma unroll
       for (int i = 0; i < kN; ++i) {
-        const int place = (t + i * team) * V, at = place - shift;
-        if (whole(row, at)) {
-          copy_async(to + place * sizeof(T), s + at, V * sizeof(T));
-          copy_async(to + dy_at + place * dy_size, dy + (int64_t)at * dy_size, V * dy_size);
-          if (a.dsum) copy_async(to + ds_at + place * sizeof(T), ds + at, V * sizeof(T));
+        const int place = (t + i * team) * V, further = i * team * V;
+        if (whole(ahead, place - shift)) {
+          copy_async(to + place * (int)sizeof(T), s_next + further * (int)sizeof(T), V * sizeof(T));
+          copy_async(to + dy_at + place * dy_size, dy_next + further * dy_size, V * dy_size);
+          if (a.dsum)
+            copy_async(to + ds_at + place * (int)sizeof(T), ds_next + further * (int)sizeof(T), V * sizeof(T));
         }
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    ahead += stride;
+    s_next += s_hop;
+    dy_next += dy_hop;
+    ds_next += ds_hop;
   };
   if constexpr (V > 1) {
-    for (int k = 0; k + 1 < a.depth; ++k) fetch(first + k * stride, k);
+    for (int k = 0; k + 1 < a.depth; ++k) fetch(k);
   }
 
   int stage = 0, flip = 0;  // two sets of shared words: one barrier per row is enough
   // every thread of a warp takes the same number of turns (a warp may hold teams)
-  const int64_t warp_first = (int64_t)blockIdx.x * teams + (threadIdx.x & ~31) / team;
+  const int64_t warp_first = (int64_t)blockIdx.x * teams + (linear & ~31) / team;
   for (int64_t turn = team > 32 ? first : warp_first, row = first; turn < a.rows;
        turn += stride, row += stride, flip ^= 1) {
     const bool live = row < a.rows;
@@ -454,7 +473,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
       int next = stage + a.depth - 1;
       if (next >= a.depth) next -= a.depth;
       // the place of the row before this one, read by this thread a turn ago
-      fetch(row + (int64_t)(a.depth - 1) * stride, next);
+      fetch(next);
       copies_wait_oldest(a.depth);
       if (++stage == a.depth) stage = 0;
       const T *s = static_cast<const T *>(a.s) + row * a.lds;
@@ -548,7 +567,7 @@ __global__ void __launch_bounds__(kGradBound<V, E>, kGradBlocksPerSm<V, E>)
   }
   if (teams == 1) return;
   __syncthreads();
-  for (int c = threadIdx.x; c < dim; c += blockDim.x) {
+  for (int c = linear; c < dim; c += teams * team) {
     float sum = 0.0f;
     for (int k = 0; k < teams; ++k) sum += joined[k * dim + c];
     out[c] = sum;
@@ -680,12 +699,13 @@ void launch_norm(const NormArgs &a, cudaStream_t st) {
     return;
   }
   const unsigned grid = (unsigned)ceil_div(a.rows, s.threads / s.team);
+  const dim3 block((unsigned)s.team, (unsigned)(s.threads / s.team));
   if (s.held == 8)
-    rmsnorm_kernel<T, V, 8, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, 8, RAGGED><<<grid, block, 0, st>>>(a, s.team);
   else if (s.held == 16)
-    rmsnorm_kernel<T, V, 16, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, 16, RAGGED><<<grid, block, 0, st>>>(a, s.team);
   else
-    rmsnorm_kernel<T, V, kMostHeld<V>, RAGGED><<<grid, s.threads, 0, st>>>(a, s.team);
+    rmsnorm_kernel<T, V, kMostHeld<V>, RAGGED><<<grid, block, 0, st>>>(a, s.team);
 }
 
 // Blocks of the gradient kernel, which are also the partial rows of dweight.
@@ -717,7 +737,7 @@ vcsr_status launch_grad(GradArgs a, int blocks, cudaStream_t st) {
   }
   auto run = [&](auto kernel) -> vcsr_status {
     VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
-    kernel<<<blocks, threads, smem, st>>>(a, s.team);
+    kernel<<<blocks, dim3((unsigned)s.team, (unsigned)in_block), smem, st>>>(a, s.team);
     return VCSR_OK;
   };
   if (s.held == 8) return run(rmsnorm_grad_kernel<T, V, 8, RAGGED>);
