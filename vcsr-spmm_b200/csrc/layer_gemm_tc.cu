@@ -16,13 +16,16 @@
 // features x 256 rows per pair and tile.  Each CTA stages 128 rows of each
 // operand (32 KB per 64 values of k, half of what a CTA alone with a 128 x 256
 // tile would read from L2 per MMA), two accumulators alternate, so that the
-// epilogue of a tile runs under the next tile's MMAs.  Bound by the tensor cores.
+// epilogue of a tile runs under the next tile's MMAs.  Bound by the tensor cores and, in
+// a long run, by power: bf16 16384 x 8192, k = 4096 708 us (1,554 TFLOP/s), 800 with every
+// part of the epilogue; e4m3 4096 x 8192, k = 4096 with gelu 104 us (2,650 TFLOP/s).
 //
 // gemm_split_kernel — few rows or few tiles: one tile of 128 features x 16 to
 // 128 rows per cluster of 1 to 8 CTAs, which split k between them and join their
 // partial sums through distributed shared memory in rank order (no workspace, no
 // atomics: the same result on every run).  For few rows it is bound by reading
-// the weights once; the split is what puts every SM on that.
+// the weights once; the split is what puts every SM on that: 1 x 4096, k = 4096 bf16
+// 9.5 us, of which reading 34 MB takes 5.
 //
 // Every wait is bounded: a role that gives up records where, the CTA drains its
 // own copies and MMAs, frees its tensor memory and returns, and vcsr_layers_check

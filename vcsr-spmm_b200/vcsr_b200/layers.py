@@ -4,7 +4,7 @@ the optimizer step over many tensors (AdamW).  The mathematics and the rules of
 types and aliasing stand with the C entry points in include/vcsr_spmm.h.
 
     from vcsr_b200 import layers
-    n = layers.rmsnorm(C, gain, residual=h, out_dtype=torch.bfloat16, save_rstd=True)
+    n = layers.rmsnorm(C, gain, residual=h, save_rstd=True)
     out = layers.linear(n.y, W, bias=b, act="gelu", save_pre=True)
     g = layers.linear_backward(dy, n.y, W, pre=out.pre, act="gelu")
     dx, dgain = layers.rmsnorm_backward(g.dx, n.sum, gain, n.rstd)
@@ -339,7 +339,8 @@ class AdamW:
     states start at value offsets[t] of the flat buffers.  copies: 16-bit copies of
     the parameters (bfloat16 or float16, as many values each), written by every
     step.  `steps` counts the steps done; with the buffers above it is the whole
-    state, to be saved and put back as such."""
+    state, to be saved and put back as such.  Step number, rates and the gradients'
+    addresses go into the launch: a CUDA graph that captured a step repeats them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  state_bits=32, copies=None):
