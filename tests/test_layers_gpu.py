@@ -475,6 +475,39 @@ def test_linear_backward_strided(dtype, act, pads):
     check_linear_backward(130, 72, 96, dtype, act, pads)
 
 
+# small (both products fit one round of the GPU), ragged, and large
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (64, 64, 64), (33, 65, 5), (512, 1024, 1024), (1001, 777, 1501), (3000, 2048, 2304)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_linear_backward_of_chosen_outputs(M, N, K, dtype, act):
+    """Every subset of the three gradients is what the full call gives, bit for bit."""
+    dy, x, w, pre = (randn(*s, dtype=dtype, seed=i) for i, s in enumerate([(M, N), (M, K), (N, K), (M, N)]))
+    full = L.linear_backward(dy, x, w, pre=pre, act=act)
+    for wanted in range(8):
+        need = dict(need_dx=bool(wanted & 1), need_dw=bool(wanted & 2), need_db=bool(wanted & 4))
+        part = L.linear_backward(dy, x, w, pre=pre, act=act, **need)
+        for name, want in need.items():
+            got, ref = getattr(part, name[5:]), getattr(full, name[5:])
+            assert got is None if not want else torch.equal(got, ref), (need, name)
+    L.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_linear_grad_of_the_bias_takes_no_operands(dtype):
+    """dbias alone through the C entry point, with x, w, dx and dw NULL."""
+    dy = randn(40, 24, dtype=dtype, seed=1)
+    db = torch.empty(24, device="cuda", dtype=dtype)
+    a = V._LinearGradArgs(M=40, N=24, K=16, dy=dy.data_ptr(), lddy=24, dbias=db.data_ptr(),
+                          dtype=L._TYPE[dtype])
+    n = V.lib().vcsr_linear_grad_workspace(a)
+    ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    assert V.lib().vcsr_linear_grad(a, torch.cuda.current_stream().cuda_stream) == 0
+    close(db, d(dy).sum(0), 44 * U * d(dy).abs().sum(0))
+
+
 @gpu
 def test_linear_backward_takes_expanded_gradients():
     x, w = randn(30, 40, seed=1), randn(20, 40, seed=2)

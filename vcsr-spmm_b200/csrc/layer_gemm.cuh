@@ -123,8 +123,8 @@ __device__ __forceinline__ void times_slopes(int act, const float *z, float *o) 
 // On the tensor cores: operands whose bases and pitches are multiples of 16 bytes
 // (tc_aligned); K > 0.  16-bit operands, and 8-bit ones stored along k; FP32 ones.
 vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st);
-// Two of them (16-bit), in one launch where that is expected to be faster; one without
-// an output (e.out NULL) is left out.
+// Two of them (16-bit), in one launch where that is expected to be faster; those without
+// an output (e.out NULL) are left out.
 vcsr_status launch_gemms_tc(const Gemm &g0, const Gemm &g1, cudaStream_t st);
 vcsr_status launch_gemm_f32(const Gemm &g, cudaStream_t st);
 bool tc_aligned(const void *p, int64_t ld, int dtype);

@@ -537,6 +537,7 @@ vcsr_status launch_chosen(const Choice &c, const Gemm &g, cudaStream_t st) {
 vcsr_status launch_gemm_tc(const Gemm &g, cudaStream_t st) { return launch_chosen(choose(g), g, st); }
 
 vcsr_status launch_gemms_tc(const Gemm &g0, const Gemm &g1, cudaStream_t st) {
+  if (!g0.e.out && !g1.e.out) return VCSR_OK;
   const Choice c0 = choose(g0), c1 = choose(g1);
   const double both64 = split_cost<64>(g0, &g1), both128 = split_cost<128>(g0, &g1);
   const bool narrow = both64 <= both128;

@@ -348,7 +348,7 @@ vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {
   const void *x = before.matrix(p.x, a->x, a->ldx, a->M, a->K, a->dtype);
   const void *w = before.matrix(p.w, a->w, a->ldw, a->N, a->K, a->dtype);
   VCSR_TRY(before.run(a->dtype, st));
-  if (a->K == 0) return VCSR_OK;
+  if (a->K == 0 || (!a->dx && !a->dw)) return VCSR_OK;
   const int64_t ldd = dz ? p.lddz : p.dy.ld;
   Epilogue e{};
   e.type = a->dtype;
