@@ -713,6 +713,37 @@ def test_operators_run_on_the_given_stream(raw):
     assert torch.equal(got, want)
 
 
+def busy(stream):
+    """Keeps `stream` at work for some milliseconds, so that what is enqueued behind is late."""
+    with torch.cuda.stream(stream):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(20):
+            big = big @ big * 1e-3
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_adamw_state_values_on_the_given_stream(bits, dtype):
+    """The states of a step that is still to come on a side stream, read there into
+    tensors that later steps leave alone."""
+    side = torch.cuda.Stream()
+    p, g = randn(5000, seed=1), randn(5000, seed=2)
+    busy(side)  # warm
+    opt, other = (L.AdamW([p.clone()], state_bits=bits) for _ in range(2))
+    other.step([g])
+    torch.cuda.synchronize()
+    want = [t.clone() for t in other.state_values(dtype)]
+    assert bool((want[0] != 0).any())
+    torch.cuda.synchronize()
+    busy(side)
+    opt.step([g], stream=side)
+    got = opt.state_values(dtype, stream=side)
+    opt.step([g], stream=side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @gpu
 def test_operators_in_a_cuda_graph():
     x, w, b = randn(16, 256, dtype=BF16, seed=1), randn(256, 256, dtype=BF16, seed=2), randn(256, dtype=BF16)

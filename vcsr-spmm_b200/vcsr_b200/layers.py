@@ -329,6 +329,11 @@ def check(stream=None):
 
 # -------------------------------------------------------------- the optimizer
 
+@_operator
+def _values(t, dtype):
+    return t.to(dtype, copy=True)
+
+
 class AdamW:
     """AdamW over many tensors in one launch (vcsr_adamw_*).
 
@@ -447,9 +452,9 @@ class AdamW:
         self.steps += 1
 
     def state_values(self, dtype=torch.float32, stream=None):
-        """(m, v), flat: the states as values of `dtype`."""
+        """(m, v), flat: the states as values of `dtype`, in new tensors."""
         if self.state_bits == 32:
-            return self.m_flat.to(dtype), self.v_flat.to(dtype)
+            return _values(self.m_flat, dtype, stream=stream), _values(self.v_flat, dtype, stream=stream)
         m = dequantize(self.m_flat.view(-1, BLOCK), self.m_scale, dtype, stream=stream)
         v = dequantize(self.u_flat.view(-1, BLOCK), self.u_scale, dtype, squared=True,
                        stream=stream)
