@@ -745,6 +745,29 @@ def test_adamw_state_values_on_the_given_stream(bits, dtype):
 
 
 @gpu
+def test_adamw_dither_of_the_given_stream():
+    """A strided dither that a side stream has still to write is read on that stream."""
+    side = torch.cuda.Stream()
+    p, g, u = randn(5000, seed=1), randn(5000, seed=2), torch.rand(256, device="cuda")
+    late = torch.zeros(256, 2, device="cuda")
+    opt, other = (L.AdamW([p.clone()], state_bits=8) for _ in range(2))
+    # with every kernel loaded, which can wait for the whole device
+    busy(side)
+    late[:, 0].copy_(u)
+    other.step([g], dither=late[:, 0])
+    late.zero_()
+    torch.cuda.synchronize()
+    busy(side)
+    with torch.cuda.stream(side):
+        late[:, 0].copy_(u)
+    opt.step([g], dither=late[:, 0], stream=side)
+    side.synchronize()
+    assert torch.equal(opt.m_flat.view(torch.uint8), other.m_flat.view(torch.uint8))
+    with pytest.raises(V.VcsrError):
+        opt.step([g], dither=torch.rand(256), stream=side)
+
+
+@gpu
 def test_operators_in_a_cuda_graph():
     x, w, b = randn(16, 256, dtype=BF16, seed=1), randn(256, 256, dtype=BF16, seed=2), randn(256, dtype=BF16)
     gain = torch.ones(256, device="cuda", dtype=BF16)

@@ -334,6 +334,11 @@ def _values(t, dtype):
     return t.to(dtype, copy=True)
 
 
+@_operator
+def _dither(t, like):
+    return _vector(t, "dither", like, BLOCK, torch.float32)
+
+
 class AdamW:
     """AdamW over many tensors in one launch (vcsr_adamw_*).
 
@@ -434,7 +439,7 @@ class AdamW:
         codes round to nearest)."""
         dtype, ptr = self._gradients(list(grads))
         if dither is not None:
-            dither = _vector(dither, "dither", self.m_flat, BLOCK, torch.float32)
+            dither = _dither(dither, self.m_flat, stream=stream)
         eight = self.state_bits == 8
         second = self.u_flat if eight else self.v_flat
         a = _AdamwStepArgs(ptr.ctypes.data, _type(dtype, "grads"), self.m_flat.data_ptr(),
