@@ -357,6 +357,19 @@ def test_linear_long_sums(M, N, K, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_linear_longest_sum(dtype):
+    """The longest k there may be, 2^31 - 1 (8.6 GB of FP32): values at its ends and
+    between are all summed."""
+    K = 2 ** 31 - 1
+    x = torch.zeros(1, K, device="cuda", dtype=dtype)
+    x[0, 0], x[0, 2 ** 30 + 5], x[0, K - 40], x[0, K - 1] = 1.0, 2.0, 3.0, 4.0
+    b = torch.full((1,), 0.5, device="cuda", dtype=dtype)
+    assert float(L.linear(x, x, bias=b).y) == 1 + 4 + 9 + 16 + 0.5
+    L.check()
+
+
+@gpu
 @pytest.mark.parametrize("M", [1, 40, 300])
 @pytest.mark.parametrize("dtype", [BF16, F32, E4M3])
 @pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])

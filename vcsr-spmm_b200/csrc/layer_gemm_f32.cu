@@ -74,6 +74,7 @@ struct F32Args {
   const float *p, *q;
   int64_t ldp, ldq;
   int P, Q, K;
+  int stages;      // of 32 values of k
   int p_mn, q_mn;  // operand stored along its own index
   int tiles_p, tiles_q, splits;
   Epilogue e;
@@ -265,8 +266,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
   const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / a.splits, stride = gridDim.x / a.splits;
-  const int all = (a.K + kK - 1) / kK;
-  const int b0 = (int)((int64_t)all * rank / a.splits), b1 = (int)((int64_t)all * (rank + 1) / a.splits);
+  const int b0 = (int)((int64_t)a.stages * rank / a.splits), b1 = (int)((int64_t)a.stages * (rank + 1) / a.splits);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full + s, kSplitters);
@@ -486,7 +486,7 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
   const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
   if (tiles > (1 << 30)) return fail(VCSR_ERR_RANGE, "more than 2^30 output tiles");
   a.splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>, tiles,
-                           ceil_div(a.K, kK));
+                           a.stages);
   const int grid = a.splits > 1 ? (int)tiles * a.splits : (int)std::min<int64_t>(tiles, sm_count());
   return launch(gemm_f32_kernel<BN>, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
 }
@@ -500,7 +500,7 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
 template <int BN>
 double tiles_cost(const F32Args &a) {
   constexpr double kFixed = BN == 32 ? 2.1 : BN == 64 ? 3.3 : 7.8, kStageUs = BN == 32 ? 0.52 : BN == 64 ? 0.64 : 0.95;
-  const int64_t tiles = ceil_div(a.P, kRows) * ceil_div(a.Q, BN), stages = ceil_div(a.K, kK);
+  const int64_t tiles = ceil_div(a.P, kRows) * ceil_div(a.Q, BN), stages = a.stages;
   const int splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>,
                                    tiles, stages);
   return 4.8 + (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStageUs * (double)ceil_div(stages, splits));
@@ -517,6 +517,7 @@ vcsr_status launch_gemm_f32(const Gemm &g, cudaStream_t st) {
   a.P = (int)g.N;
   a.Q = (int)g.M;
   a.K = (int)g.K;
+  a.stages = (int)ceil_div(g.K, kK);
   a.p_mn = g.b.transposed;
   a.q_mn = g.a.transposed;
   a.e = g.e;
