@@ -434,6 +434,26 @@ def test_linear_not_finite(dtype, M, place):
 
 
 @gpu
+def test_linear_not_finite_long_sums():
+    """Infinities in every output of a long FP32 sum, with more tiles than SMs: summing
+    them again outlasts the bounded waits of the tile that follows."""
+    M, N, K = 1280, 2048, 1 << 17
+    x = torch.zeros(M, K, device="cuda")
+    w = torch.full((N, K), 0.5, device="cuda")
+    x[:, 1] = float("inf")
+    x[5, K - 1] = float("-inf")
+    x[:, 77] = 2.0
+    r, b = randn(M, N, seed=1), randn(N, seed=2)
+    y = L.linear(x, w, bias=b, residual=r, act="relu").y
+    L.check()
+    want = torch.full((M, N), float("inf"), device="cuda")
+    want[5] = float("nan")
+    assert torch.equal(y.nan_to_num(7.0, posinf=8.0, neginf=9.0), want.nan_to_num(7.0, posinf=8.0, neginf=9.0))
+    x[:, 1], x[5, K - 1] = 0.0, 0.0
+    assert torch.equal(L.linear(x, w).y, torch.ones(M, N, device="cuda"))
+
+
+@gpu
 def test_linear_float32_extremes():
     """FP32 values from 1e-30 to 1e30: the sums keep FP32 accuracy relative to their
     largest terms."""

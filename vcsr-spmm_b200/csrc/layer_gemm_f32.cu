@@ -1,16 +1,17 @@
 // layer_gemm_f32.cu — the product of FP32 operands on the tensor cores at FP32
 // accuracy (tcgen05 kind::f16 on bfloat16 parts).
 //
-// An FP32 value is the exact sum of three bfloat16 values, its leading, middle
-// and last 8 significant bits (cut off, not rounded, so that the leading part
-// never overflows).  Of the nine products of two values' parts the six down to
-// 2^-16 of the largest are summed; the three left out are below 2^-24 of it.  A
-// tensor core may cut its sums off, not round them, so no sum is long: each 32
-// values of k start a new accumulator in tensor memory, smallest products first,
-// and the epilogue's warps add the accumulators in registers, rounded to
-// nearest.  An output that comes out NaN or infinite (a product of an infinity's
-// zero parts is NaN) is summed again in FP32 from the operands themselves.  Values
-// below 2^-110 lose bits under 2^-133, the least bfloat16.
+// An FP32 value is the exact sum of three bfloat16 values, its leading, middle and last
+// 8 significant bits (cut off, not rounded, so that the leading part never overflows).
+// Of the nine products of two values' parts the six down to 2^-16 of the largest are
+// summed; the three left out are below 2^-24 of it.  A tensor core may cut its sums off,
+// not round them, so no sum is long: each 32 values of k start a new accumulator in
+// tensor memory, smallest products first, and the epilogue's warps add the accumulators
+// in registers, rounded to nearest.  An output that comes out NaN or infinite (a product
+// of an infinity's zero parts is NaN) is summed again in FP32 from the operands
+// themselves, by the warps that drain: where k is long that outlasts the other roles'
+// bounded waits, which therefore start anew while a count of such sums goes on rising.
+// Values below 2^-110 lose bits under 2^-133, the least bfloat16.
 //
 // Tile: 128 features x 32, 64 or 128 rows per CTA (layer_gemm_tc.cu says why
 // features are the MMA's M side), 32 values of k per stage.  One thread brings the
@@ -209,11 +210,15 @@ __device__ __forceinline__ uint64_t plane_desc(uint32_t addr, int mn) {
   return mn ? smem_desc(addr, 4096, 1024, 2) : smem_desc(addr, 16, 512, 4);
 }
 
-__device__ __noinline__ float sum_again(const F32Args &a, int f, int r) {
+// The sum of an output, in order.  `alive` tells the waits of the other roles that it is
+// under way, often enough for loads that all come from memory.
+__device__ __noinline__ float sum_again(const F32Args &a, int f, int r, int *alive) {
   float s = 0.0f;
-  for (int64_t k = 0; k < a.K && s == s; ++k)
+  for (int64_t k = 0; k < a.K && s == s; ++k) {
+    if (k % 4096 == 0) atomicAdd(alive, 1);
     s = fmaf(a.q_mn ? a.q[k * a.ldq + r] : a.q[r * a.ldq + k],
              a.p_mn ? a.p[k * a.ldp + f] : a.p[f * a.ldp + k], s);
+  }
   return s;
 }
 
@@ -236,11 +241,11 @@ __device__ __forceinline__ void mend(float *z, IN &&in, AGAIN &&again) {
 
 // The epilogue of N rows of column f.
 template <int N, class GET>
-__device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int n, GET &&get) {
+__device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int n, int *alive, GET &&get) {
   if (f >= a.P) n = 0;
   finish<N, true>(a.e, f, r0, n, [&](float *z) {
     get(z);
-    if (n > 0) mend<N>(z, [&](int j) { return j < n; }, [&](int j) { return sum_again(a, f, r0 + j); });
+    if (n > 0) mend<N>(z, [&](int j) { return j < n; }, [&](int j) { return sum_again(a, f, r0 + j, alive); });
     return true;
   });
 }
@@ -260,6 +265,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   uint64_t *dfull = rempty + R, *dfree = dfull + kSums<BN>, *drain = dfree + kSums<BN>;
   uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
+  int *alive = reinterpret_cast<int *>(holder + 2);  // rises while sums are made again
 
   // the same in all lanes, and known to be: what the MMA warp computes then stays in
   // uniform registers, where its instructions want their operands
@@ -282,6 +288,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
+    *alive = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) tmem_alloc<1>(holder, kColumns);
@@ -302,8 +309,8 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     for (int t = first; t < tiles && go; t += stride) {
       for (int b = b0; b < b1; ++b, in.next(), out.next()) {
         const int r = in.stage, s = out.stage;
-        const bool ready = mbar_wait(rfull + r, in.full(), abort_flag, kWaitFull) &&
-                           mbar_wait(empty + s, out.empty(), abort_flag, kWaitEmpty);
+        const bool ready = mbar_wait<true>(rfull + r, in.full(), abort_flag, kWaitFull) &&
+                           mbar_wait<true>(empty + s, out.empty(), abort_flag, kWaitEmpty);
         if (!__all_sync(0xffffffffu, ready)) {
           go = false;
           break;
@@ -332,7 +339,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
         tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
         for (int b = b0; b < b1; ++b, ++g) {
           const int r = g % R;
-          if (g >= R && !mbar_wait(rempty + r, (uint32_t)((g / R - 1) & 1), abort_flag, kWaitEmpty)) {
+          if (g >= R && !mbar_wait<true>(rempty + r, (uint32_t)((g / R - 1) & 1), abort_flag, kWaitEmpty)) {
             go = false;
             break;
           }
@@ -356,8 +363,8 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
     for (int t = first; t < tiles && go; t += stride) {
       for (int b = b0; b < b1; ++b, at.next(), sums.next()) {
         const int s = at.stage, buf = sums.stage;
-        const bool ready = mbar_wait(full + s, at.full(), abort_flag, kWaitFull) &&
-                           mbar_wait(dfree + buf, sums.empty(), abort_flag, kWaitAccFree);
+        const bool ready = mbar_wait<true>(full + s, at.full(), abort_flag, kWaitFull) &&
+                           mbar_wait<true>(dfree + buf, sums.empty(), abort_flag, kWaitAccFree);
         if (!__all_sync(0xffffffffu, ready)) {
           go = false;
           break;
@@ -398,7 +405,8 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
       for (int j = 0; j < 32; ++j) acc[j] = 0.0f;
       for (int b = b0; b < b1; ++b, sums.next()) {
         const int buf = sums.stage;
-        if (!__all_sync(0xffffffffu, mbar_wait(dfull + buf, sums.full(), abort_flag, kWaitAccFull))) {
+        const bool ready = mbar_wait<true>(dfull + buf, sums.full(), abort_flag, kWaitAccFull);
+        if (!__all_sync(0xffffffffu, ready)) {
           go = false;
           break;
         }
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
 #pragma unroll
         for (int c = 0; c < 32; c += 16)
           finish_f32<16>(a, tp * kRows + quarter * 32 + lane, tq * BN + col0 + c,
-                         a.Q - (tq * BN + col0 + c), [&](float *z) {
+                         a.Q - (tq * BN + col0 + c), alive, [&](float *z) {
 #pragma unroll
                            for (int j = 0; j < 16; ++j) z[j] = acc[c + j];
                          });
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
       finish_rows<true>(a.e, smem_u32(sums), a.splits, f0, a.P, r0, rank + a.splits * warp,
                         a.splits * (kThreads<BN> / 32), nr, [&](int f, int r, float *z) {
                           mend<4>(z, [&](int j) { return f + j < a.P; },
-                                  [&](int j) { return sum_again(a, f + j, r); });
+                                  [&](int j) { return sum_again(a, f + j, r, alive); });
                         });
     __syncwarp();
     cluster_sync();  // until every peer has read this CTA's sums

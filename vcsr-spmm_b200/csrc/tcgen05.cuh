@@ -42,11 +42,14 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 
 // Bounded wait for the phase with the given parity; false when the poll
 // limit ran out (the site is recorded) or another thread already reported a
-// failure.
+// failure.  ALIVE: the word after *abort_flag is a count that a role at work on
+// something long raises, finitely often; the limit starts anew where it has changed.
+template <bool ALIVE = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
                                           volatile int *abort_flag, int site,
                                           long long limit = kPollLimit) {
   const uint32_t a = smem_u32(bar);
+  int seen = 0;
   for (long long i = 0; i < limit; ++i) {
     uint32_t done;
     asm volatile(
@@ -56,7 +59,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity,
         : "r"(a), "r"(parity)
         : "memory");
     if (done) return true;
-    if ((i & 1023) == 1023 && *abort_flag) return false;
+    if ((i & 1023) == 1023) {
+      if (*abort_flag) return false;
+      if (ALIVE && abort_flag[1] != seen) {
+        seen = abort_flag[1];
+        i = 0;
+      }
+    }
   }
   *abort_flag = site;
   return false;
