@@ -621,6 +621,15 @@ size_t vcsr_linear_grad_workspace(const vcsr_linear_grad_args *a);
  * vcsr_plan_check does for a plan. */
 vcsr_status vcsr_layers_check(vcsr_stream_t stream);
 
+/* Test hook for the failure path above, not for production use: the next tensor-core
+ * product that vcsr_linear or vcsr_linear_grad launches in this process withholds the
+ * first accumulator-ready signal of its first block (or pair of blocks).  The wait for
+ * it runs out after a short bounded poll, the block stops its other roles, waits for its
+ * own copies and MMAs, frees its tensor memory and records the site; its outputs are
+ * incomplete for that call only, and vcsr_layers_check returns VCSR_ERR_TIMEOUT once.
+ * Nothing faults or hangs. */
+vcsr_status vcsr_layers_test_withhold_signal(void);
+
 /* -------------------------------------------------------------- multi-GPU */
 
 /* nnz-balanced row panels: cuts[0] = 0, cuts[parts] = M, cut k is the row

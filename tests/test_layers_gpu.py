@@ -435,9 +435,10 @@ def test_linear_not_finite(dtype, M, place):
 
 @gpu
 def test_linear_not_finite_long_sums():
-    """Infinities in every output of a long FP32 sum, with more tiles than SMs: summing
-    them again outlasts the bounded waits of the tile that follows."""
-    M, N, K = 1280, 2048, 1 << 17
+    """Infinities in every output of a long FP32 sum, with more tiles than SMs: the waits
+    of the tile that follows last while they are summed again (a second here; the waits
+    that knew nothing of it lasted 16 s, and gave up from K of about 2^19 on)."""
+    M, N, K = 1280, 2048, 1 << 15
     x = torch.zeros(M, K, device="cuda")
     w = torch.full((N, K), 0.5, device="cuda")
     x[:, 1] = float("inf")
@@ -719,6 +720,45 @@ def test_adamw_not_finite_gradients_stay_in_their_block():
     assert bool(torch.isfinite(p[:256]).all()) and bool(torch.isfinite(p[512:]).all())
     m, v = opt.state_values()
     assert bool(torch.isfinite(m[:256]).all()) and bool(torch.isfinite(v[512:]).all())
+
+
+# -------------------------------------------- bounded waits, streams, refusals
+
+@gpu
+@pytest.mark.parametrize("dtype,M,N,K", [
+    (BF16, 4, 256, 1024), (E4M3, 33, 200, 4096), (F16, 300, 128, 64),  # clusters that split k, single blocks
+    (BF16, 4096, 4096, 1024), (E4M3, 4096, 2048, 128),                 # pairs of blocks, several tiles and one each
+    (F32, 16, 256, 4096), (F32, 2000, 2000, 512), (F32, 5000, 128, 32)])
+def test_a_wait_that_runs_out_is_reported(dtype, M, N, K):
+    """The first block of each kernel waits for a signal that is not sent: check() names
+    the barrier, once, and the next call is right."""
+    x, w = randn(M, K, seed=1).to(dtype), randn(N, K, seed=2).to(dtype)
+    scales = dict(x_scale=torch.ones(M, device="cuda"), w_scale=torch.ones(N, device="cuda")) if dtype == E4M3 else {}
+    want = L.linear(x, w, **scales).y
+    L.check()
+    L.test_withhold_signal()
+    L.linear(x, w, **scales)
+    with pytest.raises(V.VcsrError) as e:
+        L.check()
+    assert e.value.status == 7 and "accumulator-full" in e.value.msg
+    assert "block 0" in e.value.msg or "block 1" in e.value.msg
+    L.check()
+    assert torch.equal(L.linear(x, w, **scales).y, want)
+    L.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_wait_of_the_gradient_that_runs_out_is_reported(dtype):
+    dy, x, w = randn(64, 96, dtype=dtype, seed=1), randn(64, 80, dtype=dtype, seed=2), randn(96, 80, dtype=dtype, seed=3)
+    want = L.linear_backward(dy, x, w)
+    L.test_withhold_signal()
+    L.linear_backward(dy, x, w)
+    with pytest.raises(V.VcsrError) as e:
+        L.check()
+    assert e.value.status == 7
+    assert all(torch.equal(a, b) for a, b in zip(L.linear_backward(dy, x, w), want))
+    L.check()
 
 
 # ------------------------------------------------------- streams and refusals

@@ -250,7 +250,9 @@ __device__ __forceinline__ void finish_f32(const F32Args &a, int f, int r0, int 
   });
 }
 
-template <int BN>
+// WITHHOLD (a test): the first block waits for a signal that is not sent.  A kernel of its
+// own, since the branches alone cost this one registers (62451 x 128, k = 128 30 -> 34 us).
+template <int BN, bool WITHHOLD>
 __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_constant__ F32Args a,
                                                              const __grid_constant__ CUtensorMap mp,
                                                              const __grid_constant__ CUtensorMap mq) {
@@ -357,6 +359,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   } else if (warp == kMmaWarp) {
     const uint32_t idesc = instr_desc(1, 0, a.q_mn, kRows, BN);
     const uint32_t q_step = a.q_mn ? 2048 / 16 : 32 / 16;
+    const bool withheld = WITHHOLD && blockIdx.x == 0;
     RingPlace<S> at;
     RingPlace<kSums<BN>> sums;
     bool go = true;
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
                        qd + kParts[m][1] * (BN * kK * 2 / 16) + k * q_step, idesc,
                        (m > 0 || k > 0) ? 1u : 0u);
           mma_commit(empty + s);
-          mma_commit(dfull + buf);
+          if (!withheld || b > b0) mma_commit(dfull + buf);
         }
         __syncwarp();
       }
@@ -396,6 +399,8 @@ __global__ void __launch_bounds__(kThreads<BN>, 1) gemm_f32_kernel(const __grid_
   } else if (drainer >= 0 && drainer < kDraining<BN>) {
     RingPlace<kSums<BN>> sums;
     bool go = true;
+    if (WITHHOLD && blockIdx.x == 0)
+      go = __all_sync(0xffffffffu, mbar_wait(dfull, 0, abort_flag, kWaitAccFull, kTestPollLimit));
     for (int t = first; t < tiles && go; t += stride) {
       int tp, tq;
       tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
@@ -493,10 +498,11 @@ vcsr_status launch_tiles(F32Args &a, const Gemm &g, cudaStream_t st) {
   a.tiles_q = (int)ceil_div(a.Q, BN);
   const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
   if (tiles > (1 << 30)) return fail(VCSR_ERR_RANGE, "more than 2^30 output tiles");
-  a.splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>, tiles,
+  a.splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN, false>), kThreads<BN>, kSmem<BN>, tiles,
                            a.stages);
   const int grid = a.splits > 1 ? (int)tiles * a.splits : (int)std::min<int64_t>(tiles, sm_count());
-  return launch(gemm_f32_kernel<BN>, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
+  const auto kernel = take_withhold() ? gemm_f32_kernel<BN, true> : gemm_f32_kernel<BN, false>;
+  return launch(kernel, grid, kThreads<BN>, kSmem<BN>, a.splits, st, a, mp, mq);
 }
 
 // Expected microseconds, to choose the rows of a tile: a launch, then for every round
@@ -509,7 +515,7 @@ template <int BN>
 double tiles_cost(const F32Args &a) {
   constexpr double kFixed = BN == 32 ? 2.1 : BN == 64 ? 3.3 : 7.8, kStageUs = BN == 32 ? 0.52 : BN == 64 ? 0.64 : 0.95;
   const int64_t tiles = ceil_div(a.P, kRows) * ceil_div(a.Q, BN), stages = a.stages;
-  const int splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN>), kThreads<BN>, kSmem<BN>,
+  const int splits = choose_splits(reinterpret_cast<const void *>(gemm_f32_kernel<BN, false>), kThreads<BN>, kSmem<BN>,
                                    tiles, stages);
   return 4.8 + (double)ceil_div(tiles * splits, sm_count()) * (kFixed + kStageUs * (double)ceil_div(stages, splits));
 }

@@ -31,6 +31,7 @@
 // own copies and MMAs, frees its tensor memory and returns, and vcsr_layers_check
 // reports it.
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -87,7 +88,9 @@ struct SplitJobs {
   int splits, second;
 };
 
-template <int BN, bool CODES>
+// WITHHOLD (a test), here and below: the first block (or pair) waits for a signal that is
+// not sent.  Kernels of their own: the branches alone took registers and time from these.
+template <int BN, bool CODES, bool WITHHOLD>
 __global__ void __launch_bounds__(kSplitThreads, 1) gemm_split_kernel(const __grid_constant__ SplitJobs jobs) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   unsigned char *ring = reinterpret_cast<unsigned char *>(
@@ -159,6 +162,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) gemm_split_kernel(const __gr
       __syncwarp();
     }
     if (elect_one()) {
+      if (WITHHOLD && blockIdx.x == 0) mbar_wait(done, 0, abort_flag, kWaitAccFull, kTestPollLimit);
       mma_commit(done);
       volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
       if (!mbar_wait(done, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
@@ -218,7 +222,7 @@ constexpr int kPairStages = kRing / (kPBytes + BN / 2 * 128);
 template <int BN>
 constexpr size_t kPairSmem = (size_t)kPairStages<BN> * (kPBytes + BN / 2 * 128) + 1024 + 512;
 
-template <int BN, bool CODES>
+template <int BN, bool CODES, bool WITHHOLD>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_pair_kernel(const __grid_constant__ TcArgs a, const __grid_constant__ CUtensorMap mp,
                      const __grid_constant__ CUtensorMap mq) {
@@ -238,6 +242,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int tiles = a.tiles_p * a.tiles_q, first = blockIdx.x / 2, stride = gridDim.x / 2;
+  const bool withheld = WITHHOLD && first == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full + s, 1);
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           __syncwarp();
         }
-        if (go && elect_one()) mma_commit_pair(dfull + buf);
+        if (go && !withheld && elect_one()) mma_commit_pair(dfull + buf);
         __syncwarp();
       }
       if (elect_one()) {
@@ -331,6 +336,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   } else {
     RingPlace<2> acc;
     bool go = true;
+    if (withheld) go = __all_sync(0xffffffffu, mbar_wait(dfull, 0, abort_flag, kWaitAccFull, kTestPollLimit));
     for (int t = first; t < tiles && go; t += stride, acc.next()) {
       int tp, tq;
       tile_of(t, a.tiles_p, a.tiles_q, &tp, &tq);
@@ -405,8 +411,8 @@ vcsr_status make_map(CUtensorMap *m, const Operand &o, int64_t rows, int64_t K, 
 
 template <int BN>
 const void *split_kernel(int dtype) {
-  return dtype == VCSR_E4M3 ? reinterpret_cast<const void *>(gemm_split_kernel<BN, true>)
-                            : reinterpret_cast<const void *>(gemm_split_kernel<BN, false>);
+  return dtype == VCSR_E4M3 ? reinterpret_cast<const void *>(gemm_split_kernel<BN, true, false>)
+                            : reinterpret_cast<const void *>(gemm_split_kernel<BN, false, false>);
 }
 
 TcArgs args_of(const Gemm &g) {
@@ -455,9 +461,10 @@ vcsr_status launch_split(const Gemm &g, const Gemm *g1, int splits, cudaStream_t
   jobs.splits = splits;
   if (tiles * jobs.splits > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
   const int grid = (int)(tiles * jobs.splits);
-  return g.dtype == VCSR_E4M3
-             ? launch(gemm_split_kernel<BN, true>, grid, kSplitThreads, kSplitSmem<BN>, jobs.splits, st, jobs)
-             : launch(gemm_split_kernel<BN, false>, grid, kSplitThreads, kSplitSmem<BN>, jobs.splits, st, jobs);
+  const bool withhold = take_withhold(), codes = g.dtype == VCSR_E4M3;
+  const auto kernel = withhold ? (codes ? gemm_split_kernel<BN, true, true> : gemm_split_kernel<BN, false, true>)
+                               : (codes ? gemm_split_kernel<BN, true, false> : gemm_split_kernel<BN, false, false>);
+  return launch(kernel, grid, kSplitThreads, kSplitSmem<BN>, jobs.splits, st, jobs);
 }
 
 // Expected microseconds, to choose between the kernels: a launch, then for every round
@@ -500,12 +507,18 @@ vcsr_status launch_pair(const Gemm &g, cudaStream_t st) {
   const int grid = 2 * (int)std::min<int64_t>(tiles, sm_count() / 2);
   const int format = g.dtype == VCSR_BF16 ? 1 : 0;
   a.idesc = instr_desc(format, a.p_mn, a.q_mn, 256, BN);
-  return g.dtype == VCSR_E4M3
-             ? launch(gemm_pair_kernel<BN, true>, grid, kPairThreads, kPairSmem<BN>, 2, st, a, mp, mq)
-             : launch(gemm_pair_kernel<BN, false>, grid, kPairThreads, kPairSmem<BN>, 2, st, a, mp, mq);
+  const bool withhold = take_withhold(), codes = g.dtype == VCSR_E4M3;
+  const auto kernel = withhold ? (codes ? gemm_pair_kernel<BN, true, true> : gemm_pair_kernel<BN, false, true>)
+                               : (codes ? gemm_pair_kernel<BN, true, false> : gemm_pair_kernel<BN, false, false>);
+  return launch(kernel, grid, kPairThreads, kPairSmem<BN>, 2, st, a, mp, mq);
 }
 
+std::atomic<bool> g_withhold{false};
+
 }  // namespace
+
+bool take_withhold() { return g_withhold.load(std::memory_order_relaxed) && g_withhold.exchange(false); }
+void set_withhold() { g_withhold.store(true); }
 
 bool tc_aligned(const void *p, int64_t ld, int dtype) {
   return aligned(p, 16) && (ld * (int64_t)type_size(dtype)) % 16 == 0;
@@ -600,6 +613,12 @@ vcsr_status check_waits(cudaStream_t st) {
 
 }  // namespace layer
 }  // namespace vcsr
+
+extern "C" vcsr_status vcsr_layers_test_withhold_signal(void) {
+  vcsr::clear_error();
+  vcsr::layer::set_withhold();
+  return VCSR_OK;
+}
 
 extern "C" vcsr_status vcsr_layers_check(vcsr_stream_t stream) {
   vcsr::clear_error();

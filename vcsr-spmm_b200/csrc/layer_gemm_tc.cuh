@@ -287,6 +287,9 @@ inline int choose_splits(const void *kernel, int threads, size_t smem, int64_t t
   return splits;
 }
 
+// Whether this launch is the one that vcsr_layers_test_withhold_signal spoils (asks once).
+bool take_withhold();
+
 template <class K, class... A>
 inline vcsr_status launch(K kernel, int grid, int threads, size_t smem, int cluster, cudaStream_t st, A... args) {
   VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));

@@ -13,7 +13,8 @@ namespace vcsr {
 namespace tc {
 
 constexpr long long kPollLimit = 1ll << 22;
-// The short limit of the one wait a test makes run out (TcView::inject).
+// The short limit of the one wait a test makes run out (TcView::inject, and
+// vcsr_layers_test_withhold_signal).
 constexpr long long kTestPollLimit = 1ll << 12;
 
 // Where a bounded wait gave up (recorded in the plan's error word).

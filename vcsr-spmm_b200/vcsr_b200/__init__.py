@@ -212,6 +212,7 @@ _SIGS = {
     "vcsr_linear_workspace": (C.c_size_t, [C.POINTER(_LinearArgs)]),
     "vcsr_linear_grad": (C.c_int, [C.POINTER(_LinearGradArgs), C.c_void_p]),
     "vcsr_layers_check": (C.c_int, [C.c_void_p]),
+    "vcsr_layers_test_withhold_signal": (C.c_int, []),
     "vcsr_linear_grad_workspace": (C.c_size_t, [C.POINTER(_LinearGradArgs)]),
     "vcsr_mgpu_create": (C.c_int, [C.POINTER(_Csr), C.c_int, _i32p,
                                    C.POINTER(_PlanParams), C.POINTER(C.c_void_p)]),

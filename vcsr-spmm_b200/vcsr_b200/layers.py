@@ -327,6 +327,12 @@ def check(stream=None):
     _check(lib().vcsr_layers_check(_stream(stream)))
 
 
+def test_withhold_signal():
+    """Test hook: one wait of the next product's kernel runs out on purpose
+    (vcsr_layers_test_withhold_signal); check() then reports it."""
+    _check(lib().vcsr_layers_test_withhold_signal())
+
+
 # -------------------------------------------------------------- the optimizer
 
 @_operator
