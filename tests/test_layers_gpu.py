@@ -393,6 +393,45 @@ def test_linear_codes_out(out_dtype, M):
     check_linear(M, 96, 256, E4M3, bias=True, residual=True, pre=True, out_dtype=out_dtype)
 
 
+def every(dtype, limit):
+    """Every value of a 16-bit type up to `limit` in magnitude."""
+    z = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    return z[z.float().abs() <= limit].cuda()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_linear_activations_keep_their_tails(dtype, act):
+    """16-bit activations of every z to 12.5 are off by 2^-13 of themselves before they
+    are rounded (FP32's exp of -z^2 / 2 is off by up to 79 * 1.5 u = 2^-17 of itself)."""
+    z = every(dtype, 12.5)
+    x, w = torch.zeros(len(z), 8, device="cuda", dtype=dtype), torch.zeros(8, 8, device="cuda", dtype=dtype)
+    x[:, 0], w[:, 0] = z, 1.0
+    ref = act_ref(d(z), act)
+    for y in L.linear(x, w, act=act).y.unbind(1):
+        close(y, ref, 2.0 ** -13 * ref.abs())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_linear_slopes_keep_their_tails(dtype, act):
+    """Slopes of the same z, by dbias of one row: their terms (Phi and z phi; s and
+    z s (1 - s)) are off by 2^-13 and 2^-16 of themselves, and sums with 1 by 4 u (1 + |z|)."""
+    z = every(dtype, 12.5)
+    n = len(z)
+    g = L.linear_backward(torch.ones(1, n, device="cuda", dtype=dtype), torch.zeros(1, 8, device="cuda", dtype=dtype),
+                          torch.zeros(n, 8, device="cuda", dtype=dtype), pre=z[None], act=act, need_dx=False, need_dw=False)
+    t = d(z)
+    s = torch.sigmoid(t)
+    slack = {"relu": 0 * t,
+             "gelu": (2.0 ** -13 * 0.5 * torch.special.erfc(t.abs() / math.sqrt(2))
+                      + 2.0 ** -16 * t.abs() * torch.exp(-t * t / 2) * 0.4 + 4 * U * (t > 0)),
+             "silu": 2.0 ** -16 * s * (1 + t.abs() * (1 - s)) + 4 * U * (1 + t.abs()) * s}[act]
+    close(g.db, slope_ref(t, act), slack)
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_linear_empty(dtype):
