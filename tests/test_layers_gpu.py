@@ -761,6 +761,22 @@ def test_adamw_not_finite_gradients_stay_in_their_block():
     assert bool(torch.isfinite(m[:256]).all()) and bool(torch.isfinite(v[512:]).all())
 
 
+@gpu
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dithered", [False, True])
+def test_adamw_8_scales_show_what_is_not_finite(value, dithered):
+    """A gradient that is not finite makes the scales of its block so, and no other's."""
+    p = torch.zeros(1024, device="cuda")
+    opt = L.AdamW([p], state_bits=8)
+    g = torch.ones(1024, device="cuda")
+    g[300] = value
+    opt.step([g], dither=torch.rand(256, device="cuda") if dithered else None)
+    for scale in (opt.m_scale, opt.u_scale):
+        assert scale.isfinite().tolist() == [True, False, True, True]
+    for state in opt.state_values():
+        assert not bool(state[300].isfinite()) and bool(state[:256].isfinite().all()) and bool(state[512:].isfinite().all())
+
+
 # -------------------------------------------- bounded waits, streams, refusals
 
 @gpu

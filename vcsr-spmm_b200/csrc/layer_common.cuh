@@ -174,6 +174,14 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const float *x) {
   }
 }
 
+// The larger of two magnitudes, NaN where one is: a scale made from it shows that its
+// values are not all finite.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // N values stored in a type chosen at run time.
 template <int N>
 __device__ __forceinline__ void store_as(void *p, int type, int64_t at, const float *x) {
