@@ -199,6 +199,22 @@ def test_rmsnorm_not_finite_rows_stay_alone(y_dtype):
         assert torch.equal(got[i], y[i])
 
 
+@gpu
+@pytest.mark.parametrize("dim", [200, 1001, 40000])
+def test_rmsnorm_scales_show_what_is_not_finite(dim):
+    """Rows in registers and rows in passes alike: NaN scales where a y is NaN, by its
+    row or by the weight, and no other row is touched."""
+    x, w = randn(5, dim, seed=1), randn(dim, seed=2)
+    want = L.rmsnorm(x, w, out_dtype=E4M3)
+    x[1, 3], x[3, dim - 1] = float("nan"), float("inf")
+    got = L.rmsnorm(x, w, out_dtype=E4M3)
+    assert got.scale.isnan().tolist() == [False, True, False, True, False]
+    for i in (0, 2, 4):
+        assert torch.equal(got.y[i].float(), want.y[i].float()) and got.scale[i] == want.scale[i]
+    w[5] = float("nan")
+    assert bool(L.rmsnorm(x, w, out_dtype=E4M3).scale.isnan().all())
+
+
 def norm_grad_ref(dy, s, w, rstd, ds):
     h, g = d(s) * d(rstd)[:, None], d(dy) * d(w)
     dx = d(rstd)[:, None] * (g - h * (g * h).mean(1, keepdim=True))

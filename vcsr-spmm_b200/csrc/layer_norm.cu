@@ -168,12 +168,12 @@ __device__ __forceinline__ void team_reduce(float &sum, float &top, int team, fl
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (MAX) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
   } else {
     for (int o = team >> 1; o > 0; o >>= 1) {
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (MAX) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
   }
   if (team > 32) {
@@ -186,7 +186,7 @@ __device__ __forceinline__ void team_reduce(float &sum, float &top, int team, fl
     for (int o = 16; o > 0; o >>= 1) {
       if (o >= warps) continue;  // the lanes from `warps` on hold zeros
       sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (MAX) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (MAX) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     // the sums now stand in the lanes below the power of two at `warps`
     sum = __shfl_sync(0xffffffffu, sum, 0);
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
     weigh(T{});
   if (a.y_dtype == VCSR_E4M3) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) top = fmaxf(top, fabsf(s[e]));
+    for (int e = 0; e < E; ++e) top = max_or_nan(top, fabsf(s[e]));
     team_reduce<true>(ss, top, team, shared, 1);
   } else {
     ss = team_sum(ss, team, shared, 1);
@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_long_kernel(const NormArg
     for (int64_t i = threadIdx.x; i < a.dim; i += blockDim.x) {
       float w;
       load_as_float<1>(a.weight, a.w_dtype, i, &w);
-      top = fmaxf(top, fabsf(value(i) * (rstd * w)));
+      top = max_or_nan(top, fabsf(value(i) * (rstd * w)));
     }
     float none = 0.0f;
     team_reduce<true>(none, top, blockDim.x, shared[1], 1);
