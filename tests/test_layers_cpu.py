@@ -113,3 +113,17 @@ def test_python_operators_refuse_cpu_tensors():
         with pytest.raises(V.VcsrError) as e:
             call(torch.zeros(4, 4))
         assert e.value.status == 1
+
+
+def test_python_operators_take_keywords():
+    """The first tensor by name is refused, or taken, as it is by position."""
+    import torch
+    from vcsr_b200 import layers
+    t = torch.zeros(4, 4)
+    for fn, kw in ((layers.rmsnorm, dict(x=t, weight=t[0])), (layers.linear, dict(x=t, w=t)),
+                   (layers.rmsnorm_backward, dict(dy=t, s=t, weight=t[0], rstd=t[0])),
+                   (layers.linear_backward, dict(dy=t, x=t, w=t)), (layers.dequantize, dict(codes=t, scale=t[0])),
+                   (layers.linear, dict(w=t))):
+        with pytest.raises(V.VcsrError) as e:
+            fn(**kw)
+        assert e.value.status == 1 and fn.__name__ in e.value.msg

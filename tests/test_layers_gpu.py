@@ -912,6 +912,19 @@ def test_adamw_dither_of_the_given_stream():
 
 
 @gpu
+def test_operators_take_keywords():
+    x, w, v = randn(4, 8, seed=1), randn(6, 8, seed=2), randn(8, seed=3)
+    n, o = L.rmsnorm(x, v, save_rstd=True), L.linear(x, w)
+    assert torch.equal(L.rmsnorm(x=x, weight=v).y, n.y) and torch.equal(L.linear(w=w, x=x).y, o.y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = L.rmsnorm_backward(dy=x, s=x, weight=v, rstd=n.rstd, stream=side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, L.rmsnorm_backward(x, x, v, n.rstd)))
+    assert torch.equal(L.linear_backward(dy=o.y, x=x, w=w).dx, L.linear_backward(o.y, x, w).dx)
+
+
+@gpu
 def test_operators_in_a_cuda_graph():
     x, w, b = randn(16, 256, dtype=BF16, seed=1), randn(256, 256, dtype=BF16, seed=2), randn(256, dtype=BF16)
     gain = torch.ones(256, device="cuda", dtype=BF16)

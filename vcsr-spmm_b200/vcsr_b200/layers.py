@@ -54,8 +54,11 @@ _current_device = torch._C._cuda_getDevice
 
 def _operator(fn):
     """Runs fn with the first tensor's device and the given stream current."""
+    name = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(first, *args, stream=None, **kw):
+    def call(*args, stream=None, **kw):
+        first = args[0] if args else kw.get(name)
         try:
             index = first.get_device()
         except AttributeError:
@@ -63,14 +66,14 @@ def _operator(fn):
         if index < 0:
             raise VcsrError(INVALID, f"{fn.__name__} takes CUDA tensors")
         if stream is None and index == _current_device():
-            return fn(first, *args, **kw)
+            return fn(*args, **kw)
         with torch.cuda.device(index):
             if stream is None:
-                return fn(first, *args, **kw)
+                return fn(*args, **kw)
             if isinstance(stream, int):
                 stream = torch.cuda.ExternalStream(stream, device=first.device)
             with torch.cuda.stream(stream):
-                return fn(first, *args, **kw)
+                return fn(*args, **kw)
     return call
 
 
