@@ -83,6 +83,26 @@ def test_fake_shapes_without_a_gpu():
         assert rstd.shape == (6,)
 
 
+def test_fake_results_are_row_major_whatever_the_inputs_are():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w, v = torch.empty(16, 6).t(), torch.empty(16, 5).t(), torch.empty(32)[::2]
+        results = [torch.ops.vcsr.rmsnorm(x, v, x, 1e-6, torch.bfloat16),
+                   torch.ops.vcsr.rmsnorm_backward(x, x, v, torch.empty(6), x),
+                   torch.ops.vcsr.linear(x, w, None, torch.empty(5, 6).t(), "gelu", True),
+                   torch.ops.vcsr.linear_backward(torch.empty(5, 6).t(), x, w, None, "none")]
+        assert all(t.is_contiguous() for ts in results for t in ts)
+
+
+@gpu
+def test_results_are_row_major_whatever_the_inputs_are():
+    x, w, v, r = leaf(16, 6).detach().t(), leaf(16, 5).detach().t(), leaf(32).detach()[::2], leaf(5, 6).detach().t()
+    y, s, rstd = torch.ops.vcsr.rmsnorm(x, v, x, 1e-6, torch.bfloat16)
+    results = [(y, s), torch.ops.vcsr.rmsnorm_backward(y, s, v, rstd, s),
+               torch.ops.vcsr.linear(x, w, None, r, "gelu", True), torch.ops.vcsr.linear_backward(r, x, w, None, "none")]
+    assert all(t.is_contiguous() for ts in results for t in ts)
+
+
 @gpu
 def test_example_trains_and_serves():
     sys.path.insert(0, os.path.join(ROOT, "examples"))

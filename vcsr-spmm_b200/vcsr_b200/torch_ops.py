@@ -88,7 +88,7 @@ def _rmsnorm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
 @_rmsnorm.register_fake
 def _(x, weight, residual, eps, out_dtype):
     rows = x.shape[0] if residual is not None else 0
-    return (torch.empty_like(x, dtype=out_dtype), x.new_empty((rows, x.shape[1])),
+    return (x.new_empty(x.shape, dtype=out_dtype), x.new_empty((rows, x.shape[1])),
             x.new_empty(x.shape[0], dtype=torch.float32))
 
 
@@ -100,7 +100,7 @@ def _rmsnorm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, r
 
 @_rmsnorm_backward.register_fake
 def _(dy, s, weight, rstd, dsum):
-    return s.new_empty(s.shape), torch.empty_like(weight)
+    return s.new_empty(s.shape), weight.new_empty(weight.shape)
 
 
 def _rmsnorm_setup(ctx, inputs, output):
