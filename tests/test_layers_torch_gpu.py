@@ -103,6 +103,81 @@ def test_results_are_row_major_whatever_the_inputs_are():
     assert all(t.is_contiguous() for ts in results for t in ts)
 
 
+class Host:
+    """The layer operators on CPU tensors, in plain operations, that note their calls."""
+
+    def __init__(self, monkeypatch):
+        self.calls = []
+        for name in ("rmsnorm", "rmsnorm_backward", "linear", "linear_backward"):
+            monkeypatch.setattr(layers, name, getattr(self, name))
+
+    def rmsnorm(self, x, weight, residual=None, eps=1e-6, out_dtype=None, save_rstd=False):
+        s = x if residual is None else x + residual
+        rstd = (s.square().mean(1) + eps).rsqrt()
+        return layers.NormOut((s * rstd[:, None] * weight).to(out_dtype), s, rstd, None)
+
+    def rmsnorm_backward(self, dy, s, weight, rstd, dsum=None, need_dweight=True):
+        self.calls.append(("rmsnorm", dict(dsum=dsum is not None, dweight=need_dweight)))
+        h, g = s * rstd[:, None], dy * weight
+        dx = rstd[:, None] * (g - h * (g * h).mean(1, keepdim=True))
+        return dx if dsum is None else dx + dsum, (dy * h).sum(0) if need_dweight else None
+
+    def linear(self, x, w, bias=None, residual=None, act=None, save_pre=False):
+        z = x @ w.t() + (0 if bias is None else bias)
+        y = (torch.nn.functional.silu(z) if act == "silu" else z.clone()) + (0 if residual is None else residual)
+        return layers.LinearOut(y, z if save_pre else None)
+
+    def linear_backward(self, dy, x, w, pre=None, act=None, need_dx=True, need_dw=True, need_db=True):
+        self.calls.append(("linear", dict(dx=need_dx, dw=need_dw, db=need_db)))
+        s = torch.sigmoid(pre) if act == "silu" else None
+        dz = dy * s * (1 + pre * (1 - s)) if act == "silu" else dy
+        return layers.LinearGrad(dz @ w if need_dx else None, dz.t() @ x if need_dw else None,
+                                 dz.sum(0) if need_db else None)
+
+
+class Zeros(torch.utils._python_dispatch.TorchDispatchMode):
+    """Counts the tensors of zeros that are made."""
+    made = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.made += "zero" in func.name()
+        return func(*args, **(kwargs or {}))
+
+
+def host_leaf(*shape):
+    return torch.randn(*shape, dtype=torch.float64).requires_grad_()
+
+
+def test_no_gradient_is_made_of_zeros(monkeypatch):
+    """Results that nothing used have no gradient: no matrix of zeros stands for it."""
+    host = Host(monkeypatch)
+    x, gain, r, w = host_leaf(6, 16), host_leaf(16), host_leaf(6, 16), host_leaf(5, 16)
+    for residual in (None, r):
+        y, _ = torch_ops.rmsnorm(x, gain, residual=residual, out_dtype=torch.float64)
+        z = torch_ops.linear(y, w, act="silu")
+        c = torch.ones_like(z)
+        with Zeros() as zeros:
+            z.backward(c)
+        assert zeros.made == 0
+        assert host.calls[-1] == ("rmsnorm", dict(dsum=False, dweight=True))
+    n = len(host.calls)
+    x.grad = gain.grad = r.grad = None
+    _, s = torch_ops.rmsnorm(x, gain, residual=r, out_dtype=torch.float64)
+    s.backward(torch.full_like(s, 2.0))  # the sum alone: no kernel
+    assert len(host.calls) == n and gain.grad is None
+    assert bool((x.grad == 2.0).all()) and bool((r.grad == 2.0).all())
+
+
+@gpu
+def test_gradient_of_the_sum_alone():
+    x, gain, r = leaf(6, 16, seed=1), leaf(16, seed=2), leaf(6, 16, seed=3)
+    c = torch.randn(6, 16, device="cuda")
+    _, s = torch_ops.rmsnorm(x, gain, residual=r)
+    (s * c).sum().backward()
+    assert torch.equal(x.grad, c) and torch.equal(r.grad, c) and gain.grad is None
+    assert x.grad.data_ptr() != r.grad.data_ptr()
+
+
 @gpu
 def test_example_trains_and_serves():
     sys.path.insert(0, os.path.join(ROOT, "examples"))

@@ -106,10 +106,14 @@ def _(dy, s, weight, rstd, dsum):
 def _rmsnorm_setup(ctx, inputs, output):
     x, weight, residual, _, _ = inputs
     ctx.added = residual is not None
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(*output[2 if ctx.added else 1:])
     ctx.save_for_backward(output[1] if ctx.added else x, weight, output[2])
 
 
 def _rmsnorm_grad(ctx, dy, ds, _):
+    if dy is None:  # only s was used
+        return ds, None, ds, None, None
     s, weight, rstd = ctx.saved_tensors
     dx, dw = _rmsnorm_backward(dy, s, weight, rstd, ds if ctx.added else None)
     return dx, dw, dx if ctx.added else None, None, None
@@ -155,6 +159,8 @@ def _(dy, x, w, pre, act):
 def _linear_setup(ctx, inputs, output):
     x, w, bias, residual, act, save_pre = inputs
     ctx.act, ctx.biased, ctx.added = act, bias is not None, residual is not None
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(x, w, output[1] if save_pre else None)
 
 
