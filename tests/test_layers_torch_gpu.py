@@ -168,6 +168,44 @@ def test_no_gradient_is_made_of_zeros(monkeypatch):
     assert bool((x.grad == 2.0).all()) and bool((r.grad == 2.0).all())
 
 
+def test_only_wanted_gradients_are_asked_for(monkeypatch):
+    """Every choice of inputs that take gradients: the backward call makes theirs and no
+    other's, and they are what they are together."""
+    host = Host(monkeypatch)
+    make = dict(x=(6, 16), w=(5, 16), bias=(5,), residual=(6, 5))
+    values = {k: torch.randn(*s, dtype=torch.float64) for k, s in make.items()}
+    full = None
+    for wanted in range(15, 0, -1):
+        t = {k: v.clone().requires_grad_(bool(wanted >> i & 1)) for i, (k, v) in enumerate(values.items())}
+        host.calls.clear()
+        torch_ops.linear(**t, act="silu").sum().backward()
+        flags = [t[k].requires_grad for k in ("x", "w", "bias")]
+        assert host.calls == ([("linear", dict(zip(("dx", "dw", "db"), flags)))] if any(flags) else [])
+        full = full or {k: v.grad for k, v in t.items()}
+        for k, v in t.items():
+            assert torch.equal(v.grad, full[k]) if v.requires_grad else v.grad is None
+    x, gain, r = (torch.randn(*s, dtype=torch.float64) for s in ((6, 16), (16,), (6, 16)))
+    for wanted in range(7, 0, -1):
+        t = [v.clone().requires_grad_(bool(wanted >> i & 1)) for i, v in enumerate((x, gain, r))]
+        host.calls.clear()
+        y, s = torch_ops.rmsnorm(*t, out_dtype=torch.float64)
+        (y.sum() + s.sum()).backward()
+        assert host.calls[-1][1]["dweight"] == t[1].requires_grad
+        assert [v.grad is not None for v in t] == [v.requires_grad for v in t]
+
+
+@gpu
+@pytest.mark.parametrize("frozen", ["x", "w", "xw"])
+def test_linear_autograd_with_frozen_inputs(frozen):
+    t = dict(x=leaf(20, 48, seed=1), w=leaf(30, 48, seed=2), bias=leaf(30, seed=3), residual=leaf(20, 30, seed=4))
+    c = torch.randn(20, 30).cuda()
+    (torch_ops.linear(**t, act="gelu") * c).sum().backward()
+    some = {k: v.detach().clone().requires_grad_(k not in frozen) for k, v in t.items()}
+    (torch_ops.linear(**some, act="gelu") * c).sum().backward()
+    for k, v in some.items():
+        assert v.grad is None if k in frozen else torch.equal(v.grad, t[k].grad)
+
+
 @gpu
 def test_gradient_of_the_sum_alone():
     x, gain, r = leaf(6, 16, seed=1), leaf(16, seed=2), leaf(6, 16, seed=3)

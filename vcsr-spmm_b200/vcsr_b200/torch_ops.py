@@ -94,13 +94,16 @@ def _(x, weight, residual, eps, out_dtype):
 
 @torch.library.custom_op("vcsr::rmsnorm_backward", mutates_args=())
 def _rmsnorm_backward(dy: torch.Tensor, s: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
-                      dsum: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
-    return layers.rmsnorm_backward(dy, s, weight, rstd, dsum=dsum)
+                      dsum: Optional[torch.Tensor],
+                      need_dweight: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(dx, dweight) of layers.rmsnorm_backward; dweight has no values unless needed."""
+    dx, dw = layers.rmsnorm_backward(dy, s, weight, rstd, dsum=dsum, need_dweight=need_dweight)
+    return dx, weight.new_empty(0) if dw is None else dw
 
 
 @_rmsnorm_backward.register_fake
-def _(dy, s, weight, rstd, dsum):
-    return s.new_empty(s.shape), weight.new_empty(weight.shape)
+def _(dy, s, weight, rstd, dsum, need_dweight=True):
+    return s.new_empty(s.shape), weight.new_empty(weight.shape if need_dweight else 0)
 
 
 def _rmsnorm_setup(ctx, inputs, output):
@@ -115,8 +118,9 @@ def _rmsnorm_grad(ctx, dy, ds, _):
     if dy is None:  # only s was used
         return ds, None, ds, None, None
     s, weight, rstd = ctx.saved_tensors
-    dx, dw = _rmsnorm_backward(dy, s, weight, rstd, ds if ctx.added else None)
-    return dx, dw, dx if ctx.added else None, None, None
+    need = ctx.needs_input_grad
+    dx, dw = _rmsnorm_backward(dy, s, weight, rstd, ds if ctx.added else None, need[1])
+    return dx if need[0] else None, dw if need[1] else None, dx if need[2] else None, None, None
 
 
 _rmsnorm.register_autograd(_rmsnorm_grad, setup_context=_rmsnorm_setup)
@@ -146,19 +150,23 @@ def _(x, w, bias, residual, act, save_pre):
 
 @torch.library.custom_op("vcsr::linear_backward", mutates_args=())
 def _linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor,
-                     pre: Optional[torch.Tensor],
-                     act: str) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return tuple(layers.linear_backward(dy, x, w, pre=pre, act=act))
+                     pre: Optional[torch.Tensor], act: str, need_dx: bool = True, need_dw: bool = True,
+                     need_db: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """layers.linear_backward; what is not needed has no values."""
+    g = layers.linear_backward(dy, x, w, pre=pre, act=act, need_dx=need_dx, need_dw=need_dw,
+                               need_db=need_db)
+    return tuple(x.new_empty(0) if t is None else t for t in g)
 
 
 @_linear_backward.register_fake
-def _(dy, x, w, pre, act):
-    return x.new_empty(x.shape), w.new_empty(w.shape), w.new_empty(w.shape[0])
+def _(dy, x, w, pre, act, need_dx=True, need_dw=True, need_db=True):
+    return (x.new_empty(x.shape if need_dx else 0), w.new_empty(w.shape if need_dw else 0),
+            w.new_empty(w.shape[0] if need_db else 0))
 
 
 def _linear_setup(ctx, inputs, output):
     x, w, bias, residual, act, save_pre = inputs
-    ctx.act, ctx.biased, ctx.added = act, bias is not None, residual is not None
+    ctx.act = act
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(x, w, output[1] if save_pre else None)
@@ -166,8 +174,9 @@ def _linear_setup(ctx, inputs, output):
 
 def _linear_grad(ctx, dy, _):
     x, w, pre = ctx.saved_tensors
-    dx, dw, db = _linear_backward(dy, x, w, pre, ctx.act)
-    return dx, dw, db if ctx.biased else None, dy if ctx.added else None, None, None
+    need = ctx.needs_input_grad
+    made = _linear_backward(dy, x, w, pre, ctx.act, *need[:3]) if any(need[:3]) else (None,) * 3
+    return (*(g if n else None for g, n in zip(made, need)), dy if need[3] else None, None, None)
 
 
 _linear.register_autograd(_linear_grad, setup_context=_linear_setup)
@@ -178,5 +187,5 @@ def linear(x, w, bias=None, residual=None, act=None):
     operands; for 8-bit ones call layers.linear, which has no gradient)."""
     act = act or "none"
     wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                             for t in (x, w, bias, residual))
+                                             for t in (x, w, bias))
     return _linear(x, w, bias, residual, act, wanted and act != "none")[0]
