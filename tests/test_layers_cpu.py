@@ -127,3 +127,15 @@ def test_python_operators_take_keywords():
         with pytest.raises(V.VcsrError) as e:
             fn(**kw)
         assert e.value.status == 1 and fn.__name__ in e.value.msg
+
+
+@pytest.mark.parametrize("name,kw", [("rstd", dict(rstd=P + 2)), ("scale", dict(scale=P + 1, y_dtype=3))])
+def test_rmsnorm_refuses_vectors_off_their_type(name, kw):
+    refused(1, "vcsr_rmsnorm", norm(**kw), f"{name} is not aligned")
+
+
+@pytest.mark.parametrize("name", ["x_scale", "w_scale"])
+def test_linear_refuses_scales_off_their_type(name):
+    a = V._LinearArgs(M=2, N=4, K=16, x=P, ldx=16, w=P, ldw=16, y=P, ldy=4, x_scale=P, w_scale=P, dtype=3)
+    setattr(a, name, P + 2)
+    refused(1, "vcsr_linear", a, f"{name} is not aligned")

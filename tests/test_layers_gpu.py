@@ -944,6 +944,18 @@ def test_operators_in_a_cuda_graph():
 
 
 @gpu
+def test_adamw_refuses_scales_off_their_type():
+    opt = L.AdamW([randn(64)], state_bits=8)
+    for name in ("m_scale", "u_scale"):
+        keep = getattr(opt, name)
+        setattr(opt, name, torch.zeros(8, device="cuda").view(torch.uint8)[2:])
+        with pytest.raises(V.VcsrError, match=f"{name} is not aligned"):
+            opt.step([randn(64)])
+        setattr(opt, name, keep)
+    assert opt.steps == 0
+
+
+@gpu
 def test_refusals():
     x, w, v = randn(4, 8), randn(6, 8), randn(8)
 

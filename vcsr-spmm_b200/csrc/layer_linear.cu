@@ -261,6 +261,8 @@ vcsr_status linear(const vcsr_linear_args *a, cudaStream_t st) {
     return fail(VCSR_ERR_INVALID, "8-bit operands need x_scale and w_scale");
   if (!codes && (a->x_scale || a->w_scale))
     return fail(VCSR_ERR_INVALID, "scales are for 8-bit operands");
+  VCSR_TRY(check_matrix("x_scale", a->x_scale, 1, 1, VCSR_F32, true));
+  VCSR_TRY(check_matrix("w_scale", a->w_scale, 1, 1, VCSR_F32, true));
   VCSR_TRY(check_matrix("bias", a->bias, a->N, a->N, a->out_dtype, true));
   VCSR_TRY(check_matrix("residual", a->residual, a->ldr, a->N, a->out_dtype, true));
   VCSR_TRY(check_matrix("y", a->y, a->ldy, a->N, a->out_dtype, false));

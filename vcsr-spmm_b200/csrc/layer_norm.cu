@@ -783,6 +783,8 @@ vcsr_status rmsnorm(const vcsr_rmsnorm_args *a, cudaStream_t st) {
   VCSR_TRY(check_matrix("sum", a->sum, a->lds, a->dim, a->x_dtype, true));
   if (a->y_dtype == VCSR_E4M3 && !a->scale)
     return fail(VCSR_ERR_INVALID, "an 8-bit y needs scale");
+  VCSR_TRY(check_matrix("rstd", a->rstd, 1, 1, VCSR_F32, true));
+  VCSR_TRY(check_matrix("scale", a->scale, 1, 1, VCSR_F32, true));
   NormArgs k{a->rows, a->dim, a->x,   a->residual, a->weight, a->y,       a->sum,
              a->rstd, a->scale, a->ldx, a->ldr,      a->ldy,    a->lds,     a->eps,
              a->w_dtype, a->y_dtype};
