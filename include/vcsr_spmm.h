@@ -456,7 +456,8 @@ void vcsr_cusparse_destroy(vcsr_cusparse *h);
  * per row.  y is computed from the unrounded s.  With y_dtype VCSR_E4M3 a row
  * is stored as codes and one scale = max|y| / 448 (0 for a row of zeros; a
  * code stands for code * scale; NaN for a row with a NaN among its y, as an
- * infinite s leaves one). */
+ * infinite s leaves one).  With dim 0 rstd is NaN, the mean of nothing, and
+ * scale 0. */
 typedef struct vcsr_rmsnorm_args {
   int64_t rows, dim;
   const void *x; /* rows x dim, x_dtype */

@@ -215,6 +215,17 @@ def test_rmsnorm_scales_show_what_is_not_finite(dim):
     assert bool(L.rmsnorm(x, w, out_dtype=E4M3).scale.isnan().all())
 
 
+@gpu
+def test_rmsnorm_of_rows_without_values():
+    x, w = randn(500, 0), randn(0)
+    for _ in range(2):  # in memory that held something else
+        torch.full((1000,), 5.0, device="cuda")
+        out = L.rmsnorm(x, w, out_dtype=E4M3, save_rstd=True)
+        assert out.y.shape == (500, 0) and bool(out.rstd.isnan().all()) and bool((out.scale == 0).all())
+    dx, dw = L.rmsnorm_backward(x, x, w, out.rstd)
+    assert dx.shape == (500, 0) and dw.shape == (0,)
+
+
 def norm_grad_ref(dy, s, w, rstd, ds):
     h, g = d(s) * d(rstd)[:, None], d(dy) * d(w)
     dx = d(rstd)[:, None] * (g - h * (g * h).mean(1, keepdim=True))

@@ -774,7 +774,13 @@ vcsr_status rmsnorm(const vcsr_rmsnorm_args *a, cudaStream_t st) {
   if (!is_float16_or_32(a->y_dtype) && a->y_dtype != VCSR_E4M3)
     return fail(VCSR_ERR_UNSUPPORTED, "y type %d", a->y_dtype);
   if (!(a->eps >= 0.0f)) return fail(VCSR_ERR_INVALID, "eps must be >= 0");
-  if (a->rows == 0 || a->dim == 0) return VCSR_OK;
+  if (a->rows == 0) return VCSR_OK;
+  if (a->dim == 0) {  // a mean of nothing: NaN (all bits set); a largest value of nothing: 0
+    if (a->rstd) VCSR_CUDA(cudaMemsetAsync(a->rstd, 0xff, (size_t)a->rows * sizeof(float), st));
+    if (a->y_dtype == VCSR_E4M3 && a->scale)
+      VCSR_CUDA(cudaMemsetAsync(a->scale, 0, (size_t)a->rows * sizeof(float), st));
+    return VCSR_OK;
+  }
   if (a->rows > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 rows");
   VCSR_TRY(check_matrix("x", a->x, a->ldx, a->dim, a->x_dtype, false));
   VCSR_TRY(check_matrix("residual", a->residual, a->ldr, a->dim, a->x_dtype, true));
