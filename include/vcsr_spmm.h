@@ -530,7 +530,7 @@ vcsr_status vcsr_dequantize(const void *codes, int64_t ldc, const float *scale, 
  * being lost.  A value that is not finite makes its block's scale so too. */
 typedef struct vcsr_adamw vcsr_adamw;
 int64_t vcsr_adamw_state_values(int tensors, const int64_t *numel);
-/* p_dtype: VCSR_F32, VCSR_BF16 or VCSR_F16, of every tensor.  copies (NULL =
+/* p_dtype: VCSR_F32, VCSR_BF16 or VCSR_F16, of every tensor; no two overlap.  copies (NULL =
  * none): 16-bit copies of the parameters (copy_dtype), written by each step.
  * The host arrays are read during the call only. */
 vcsr_status vcsr_adamw_create(int tensors, const int64_t *numel, void *const *params, int p_dtype,

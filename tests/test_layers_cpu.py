@@ -139,3 +139,20 @@ def test_linear_refuses_scales_off_their_type(name):
     a = V._LinearArgs(M=2, N=4, K=16, x=P, ldx=16, w=P, ldw=16, y=P, ldy=4, x_scale=P, w_scale=P, dtype=3)
     setattr(a, name, P + 2)
     refused(1, "vcsr_linear", a, f"{name} is not aligned")
+
+
+def test_adamw_refuses_overlapping_parameters():
+    L = V.lib()
+    h = ctypes.c_void_p()
+
+    def create(numel, params):
+        numel, params = np.array(numel, np.int64), np.array(params, np.uint64)
+        return L.vcsr_adamw_create(len(numel), numel.ctypes.data, params.ctypes.data, 0, None, 0, 32, ctypes.byref(h), None)
+
+    for numel, params in (([8, 4, 8], [P, P + 64, P]), ([4, 8], [P + 28, P]), ([300, 1], [P, P + 4 * 299])):
+        assert create(numel, params) == 1 and "overlap" in L.vcsr_last_error().decode()
+    # neighbours, and tensors without values wherever they are
+    create([8, 0, 4], [P, P + 16, P + 32])
+    assert "overlap" not in L.vcsr_last_error().decode()
+    if h.value:
+        L.vcsr_adamw_destroy(h)

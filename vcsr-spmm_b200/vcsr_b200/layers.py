@@ -351,8 +351,8 @@ def _dither(t, like):
 class AdamW:
     """AdamW over many tensors in one launch (vcsr_adamw_*).
 
-    params: contiguous CUDA tensors of one type (float32, bfloat16 or float16) that
-    keep their storage while the optimizer lives.  state_bits=32: m and v in
+    params: contiguous CUDA tensors of one type (float32, bfloat16 or float16), no two
+    in the same memory, that keep their storage while the optimizer lives.  state_bits=32: m and v in
     m_flat, v_flat; state_bits=8: codes of m and u = sqrt(v) in m_flat, u_flat
     (float8_e4m3fn), one scale per 256 values in m_scale, u_scale.  Tensor t's
     states start at value offsets[t] of the flat buffers.  copies: 16-bit copies of
