@@ -217,6 +217,22 @@ def test_gradient_of_the_sum_alone():
 
 
 @gpu
+def test_a_step_between_forward_and_backward_is_noticed():
+    """As with torch's optimizers: the weights that the backward pass saved are gone."""
+    x, w, b = leaf(6, 16, seed=1), leaf(5, 16, seed=2), leaf(5, seed=3)
+    half = w.detach().bfloat16().requires_grad_()
+    opt = layers.AdamW([w, b], copies=[half.detach(), b.detach().bfloat16()])
+    for operand, grads in ((w, [w.detach(), None]), (half, [w.detach(), b.detach()])):
+        y = torch_ops.linear(x.to(operand.dtype), operand)
+        opt.step(grads)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    before = b._version
+    opt.step([w.detach(), None])  # what has no gradient is not written
+    assert b._version == before
+
+
+@gpu
 def test_example_trains_and_serves():
     sys.path.insert(0, os.path.join(ROOT, "examples"))
     try:

@@ -40,6 +40,9 @@ BLOCK = 256  # values per scale of an 8-bit AdamW state
 
 _current_stream = torch._C._cuda_getCurrentRawStream
 _dtype = operator.attrgetter("dtype")
+# Tells autograd, as torch's in-place operations do, that tensors hold new values: a
+# backward pass that had saved the old ones raises.
+_new_values = torch.autograd.graph.increment_version
 
 
 def _type(dtype, name):
@@ -379,7 +382,7 @@ class AdamW:
             copies = list(copies)
             self._same(copies, "copies", copies[0].dtype if copies else None)
             copy_type = _type(copies[0].dtype, "copies")
-        self._keep = (params, copies)
+        self._keep = (params, copies or [])
         n = len(params)
         numel = np.asarray(self._numel, np.int64)
         blocks = -(-numel // BLOCK)
@@ -422,19 +425,22 @@ class AdamW:
 
     def _gradients(self, grads):
         """The gradients' type and addresses, checked (in whole passes over the list:
-        with hundreds of small tensors the checks are most of a step)."""
+        with hundreds of small tensors the checks are most of a step), and the tensors
+        that a step with them writes."""
         T = torch.Tensor
         try:
             dtypes = set(map(_dtype, grads))
             if (len(dtypes) == 1 and list(map(T.numel, grads)) == self._numel
                     and all(map(T.is_contiguous, grads))
                     and set(map(T.get_device, grads)) == {self.device.index}):
-                return dtypes.pop(), np.fromiter(map(T.data_ptr, grads), np.uint64, len(grads))
+                return (dtypes.pop(), np.fromiter(map(T.data_ptr, grads), np.uint64, len(grads)),
+                        self._keep[0] + self._keep[1])
         except (AttributeError, TypeError):
             pass
         dtype = next((g.dtype for g in grads if g is not None), torch.float32)
         self._same(grads, "grads", dtype)
-        return dtype, self._pointers(grads)
+        return dtype, self._pointers(grads), [t for ts in self._keep for g, t in zip(grads, ts)
+                                              if g is not None]
 
     @staticmethod
     def _pointers(tensors):
@@ -446,7 +452,7 @@ class AdamW:
         or float16), or None for a parameter to leave as it is.  dither: 256 float32
         uniform numbers in [0, 1), fresh ones each step (state_bits=8; without it
         codes round to nearest)."""
-        dtype, ptr = self._gradients(list(grads))
+        dtype, ptr, written = self._gradients(list(grads))
         if dither is not None:
             dither = _dither(dither, self.m_flat, stream=stream)
         eight = self.state_bits == 8
@@ -464,6 +470,7 @@ class AdamW:
             with torch.cuda.device(self.device):
                 _check(lib().vcsr_adamw_step(self._h, a, raw))
         self.steps += 1
+        _new_values(written)
 
     def state_values(self, dtype=torch.float32, stream=None):
         """(m, v), flat: the states as values of `dtype`, in new tensors."""
