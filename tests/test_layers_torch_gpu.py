@@ -233,6 +233,19 @@ def test_a_step_between_forward_and_backward_is_noticed():
 
 
 @gpu
+def test_results_written_in_place_are_noticed():
+    w, gain = leaf(16, 16, seed=1), leaf(16, seed=2).detach()
+    for write in (lambda t: layers.rmsnorm(t, gain, residual=t.clone(), sum_out=t),
+                  lambda t: layers.rmsnorm(t.clone(), gain, out=t),
+                  lambda t: layers.linear(t.clone(), t.clone(), residual=t, out=t)):
+        x = leaf(16, 16, seed=3).detach()
+        y = torch_ops.linear(x, w)
+        write(x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+@gpu
 def test_example_trains_and_serves():
     sys.path.insert(0, os.path.join(ROOT, "examples"))
     try:

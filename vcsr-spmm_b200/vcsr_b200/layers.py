@@ -172,6 +172,8 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, out=None, sum_ou
                      y.data_ptr(), ldy, _p(s), lds, _p(rstd), _p(scale), eps, x_type,
                      _TYPE[weight.dtype], y_type)
     _check(lib().vcsr_rmsnorm(a, _current_stream(x.get_device())))
+    if out is not None or sum_out is not None:
+        _new_values([t for t in (out, sum_out) if t is not None])
     return NormOut(y, x if s is None else s, rstd, scale)
 
 
@@ -287,6 +289,8 @@ def linear(x, w, bias=None, residual=None, act=None, x_scale=None, w_scale=None,
             ws = _workspace(n, x)
             a.workspace, a.workspace_bytes = ws.data_ptr(), n
     _check(L.vcsr_linear(a, _current_stream(x.get_device())))
+    if out is not None:
+        _new_values(out)
     return LinearOut(y, pre)
 
 
