@@ -967,6 +967,19 @@ def test_adamw_refuses_scales_off_their_type():
 
 
 @gpu
+def test_refuses_what_is_no_tensor():
+    x, v = randn(4, 8), randn(8)
+    opt = L.AdamW([x])
+    for call in (lambda: L.linear(x, [[1.0]]), lambda: L.linear(x, x, bias=1.0), lambda: L.rmsnorm_backward(x, None, v, v),
+                 lambda: L.linear_backward(x, 3, x), lambda: L.AdamW([x], copies=[3]), lambda: L.AdamW([x], copies=[None]),
+                 lambda: opt.step([3]), lambda: L.dequantize(x.to(E4M3), 1.0), lambda: L.rmsnorm(x, v, out=3)):
+        with pytest.raises(V.VcsrError) as e:
+            call()
+        assert e.value.status == 1, e.value
+    assert opt.steps == 0
+
+
+@gpu
 def test_refusals():
     x, w, v = randn(4, 8), randn(6, 8), randn(8)
 

@@ -119,6 +119,8 @@ def _vector(t, name, like, n, dtype):
 
 
 def _shape(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise VcsrError(INVALID, f"{name} must be a tensor")
     if t.dim() != 2:
         raise VcsrError(INVALID, f"{name} must be two-dimensional, got {tuple(t.shape)}")
     return t.shape
@@ -160,7 +162,7 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None, out=None, sum_ou
     ldr = 0
     if residual is not None:
         residual, ldr = _matrix(residual, "residual", x, rows, dim, dt)
-    y_dtype = out_dtype or (out.dtype if out is not None else dt)
+    y_dtype = out_dtype or getattr(out, "dtype", dt)
     y_type = _type(y_dtype, "out")
     y, ldy = _out(out, "out", x, rows, dim, y_dtype)
     s, lds = (None, 0)
@@ -262,7 +264,7 @@ def linear(x, w, bias=None, residual=None, act=None, x_scale=None, w_scale=None,
             raise VcsrError(INVALID, "8-bit operands need x_scale and w_scale")
         x_scale = _vector(x_scale, "x_scale", x, M, torch.float32)
         w_scale = _vector(w_scale, "w_scale", x, N, torch.float32)
-        out_dtype = out_dtype or (out.dtype if out is not None else torch.bfloat16)
+        out_dtype = out_dtype or getattr(out, "dtype", torch.bfloat16)
     else:
         if x_scale is not None or w_scale is not None:
             raise VcsrError(INVALID, "scales are for 8-bit operands")
@@ -379,12 +381,12 @@ class AdamW:
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.state_bits, self.steps = state_bits, 0
         self._numel = [p.numel() for p in params]
-        self._same(params, "params", params[0].dtype)
+        self._same(params, "params")
         p_type = _type(params[0].dtype, "params")
         copy_type = 0
         if copies is not None:
             copies = list(copies)
-            self._same(copies, "copies", copies[0].dtype if copies else None)
+            self._same(copies, "copies")
             copy_type = _type(copies[0].dtype, "copies")
         self._keep = (params, copies or [])
         n = len(params)
@@ -415,17 +417,22 @@ class AdamW:
                 _current_stream(self.device.index)))
         self._h = h
 
-    def _same(self, tensors, name, dtype):
+    def _same(self, tensors, name):
+        """Checks a list against the parameters; its one type."""
         if len(tensors) != len(self._numel):
             raise VcsrError(INVALID, f"{len(tensors)} {name} for {len(self._numel)} parameters")
-        dev = self.device
+        dev, dtype = self.device, None
         for i, (t, n) in enumerate(zip(tensors, self._numel)):
             if t is None and name == "grads":
                 continue
+            if not isinstance(t, torch.Tensor):
+                raise VcsrError(INVALID, f"{name}[{i}] must be a tensor on {dev}")
+            dtype = dtype or t.dtype
             if t.dtype != dtype:
                 raise VcsrError(UNSUPPORTED, f"{name}[{i}] has type {t.dtype}, expected {dtype}")
             if t.device != dev or t.numel() != n or not t.is_contiguous():
                 raise VcsrError(INVALID, f"{name}[{i}] must be contiguous on {dev} with {n} values")
+        return dtype
 
     def _gradients(self, grads):
         """The gradients' type and addresses, checked (in whole passes over the list:
@@ -441,8 +448,7 @@ class AdamW:
                         self._keep[0] + self._keep[1])
         except (AttributeError, TypeError):
             pass
-        dtype = next((g.dtype for g in grads if g is not None), torch.float32)
-        self._same(grads, "grads", dtype)
+        dtype = self._same(grads, "grads") or torch.float32
         return dtype, self._pointers(grads), [t for ts in self._keep for g, t in zip(grads, ts)
                                               if g is not None]
 
@@ -452,8 +458,8 @@ class AdamW:
                            len(tensors))
 
     def step(self, grads, lr=None, grad_scale=1.0, dither=None, stream=None):
-        """One step.  grads: a tensor per parameter, all of one type (float32, bfloat16
-        or float16), or None for a parameter to leave as it is.  dither: 256 float32
+        """One step.  grads: a contiguous tensor per parameter, all of one type (float32,
+        bfloat16 or float16), or None for a parameter to leave as it is.  dither: 256 float32
         uniform numbers in [0, 1), fresh ones each step (state_bits=8; without it
         codes round to nearest)."""
         dtype, ptr, written = self._gradients(list(grads))
