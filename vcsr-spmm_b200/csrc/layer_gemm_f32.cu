@@ -26,8 +26,10 @@
 // stages in turn were no faster (255 against 239 us, 4096 x 4096, k = 1024).
 // Persistent over tiles; where tiles are too few for the SMs, clusters of 2 to 8 CTAs
 // split k and join their sums in rank order through distributed shared memory.
-// 4096 x 4096, k = 1024: 208 to 224 us, 153 to 165 TFLOP/s; 16 x 4096, k = 4096: 25 us, 2.7 TB/s;
-// 62451 x 128, k = 128 with every part of the epilogue: 33 us, 3.9 TB/s.
+// 4096 x 4096, k = 1024: 214 to 219 us, 157 to 160 TFLOP/s; 16 x 4096, k = 4096: 28 us, 2.4 TB/s
+// (22 with w in L2); 62451 x 128, k = 128 with every part of the epilogue: 33 us, 3.9 TB/s.
+// Registers are short at 832 threads a CTA (72 each, 726 bytes spilled a thread; tiles of 64
+// rows 96 and 186, of 32 none).
 #include <algorithm>
 
 #include "layer_gemm_tc.cuh"

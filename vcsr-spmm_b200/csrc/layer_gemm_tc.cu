@@ -17,8 +17,8 @@
 // operand (32 KB per 64 values of k, half of what a CTA alone with a 128 x 256
 // tile would read from L2 per MMA), two accumulators alternate, so that the
 // epilogue of a tile runs under the next tile's MMAs.  Bound by the tensor cores and, in
-// a long run, by power: bf16 16384 x 8192, k = 4096 708 us (1,554 TFLOP/s), 800 with every
-// part of the epilogue; e4m3 4096 x 8192, k = 4096 with gelu 104 us (2,650 TFLOP/s).
+// a long run, by power: bf16 16384 x 8192, k = 4096 708 to 732 us (1,503 to 1,554 TFLOP/s),
+// 805 with every part of the epilogue; e4m3 4096 x 8192, k = 4096 with gelu 105 us (2,630 TFLOP/s).
 //
 // gemm_split_kernel — few rows or few tiles: one tile of 128 features x 16 to
 // 128 rows per cluster of 1 to 8 CTAs, which split k between them and join their

@@ -7,6 +7,10 @@
 // dbias from the partial sums, with aligned copies of operands that TMA cannot read;
 // dx = dz w and dw = dz^T x, in one launch where both are small.
 //
+// The rounding of dz is the price of 16-bit operands: a tensor core takes no wider one
+// beside them, and dz in two parts would double both products.  It is one rounding more
+// than the results' own (error against exact sums 0.0023 instead of 0.0017 in bfloat16).
+//
 // 8192 x 4096, k = 4096 bf16 with gelu: dz 44 us (4.6 TB/s), the products 195 us each
 // (1,410 TFLOP/s); 512 x 1024, k = 1024: 22 us in three launches.
 #include <algorithm>

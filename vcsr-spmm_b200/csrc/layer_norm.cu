@@ -13,8 +13,9 @@
 // time where all matrices share their rows' misalignment, as contiguous ones do:
 // vectors are cut at the memory's boundaries, so the first starts up to V - 1 values
 // before the row.  Loads take it whole (it is the end of the row before; values
-// outside the row are then set to zero), stores write its values one by one.  Other
-// layouts are moved by single values: FP32 20000 x 2001 to bf16 216 us that way.
+// outside the row are then set to zero), stores write its values one by one: FP32
+// 20000 x 2001 to bf16 140 us, where the bytes take 87.  Other layouts are moved by single
+// values (216 us).
 //
 // Gradient, per row: with h = s rstd, g = dy weight,
 // dx = rstd (g - h mean(g h)) + dsum, dweight = sum over rows of dy h.  Its
@@ -93,16 +94,20 @@ __global__ void __launch_bounds__(256)
 }
 
 constexpr int kMaxThreads = 1024;
-// The most values a thread holds, in V-value vectors, and the largest block
-// that leaves it registers for them without spills (the gradient holds three
-// arrays of them).  Single values need an address each and stop at 16.
+// The most values a thread holds, in V-value vectors, and the largest block that
+// leaves it registers for them (the gradient holds three arrays of them).  Single values
+// need an address each and stop at 16.  Up to 16 values there are next to no spills; the
+// forms of 32, for rows past 8,192 values, spill where rows are ragged (220 to 280 bytes
+// stored a thread) and in the gradient (24 to 388).
 template <int V>
 constexpr int kMostHeld = V == 1 ? 16 : 32;
 template <int V, int E>
 constexpr int kNormBlock = E == kMostHeld<V> ? 1024 : 512;
 constexpr int kGradBlock = 512;
-// What the gradient's registers are sized for: two blocks of 320 threads an SM
-// (rows of 5,120 16-bit values), or of 512 with single values.
+// What the gradient's registers are sized for: 640 threads an SM, which is two blocks of
+// teams of up to 320 (16-bit rows of 4,097 to 5,120 values, 8192 x 5120: 72 us; bounds of
+// 512 and 1024 threads took 88 and 100) or one block of 512 made of smaller teams (8192 x
+// 4096: 69 us with the second kernel, against a floor of 42); or two blocks of 512 with 8 single values.
 template <int V, int E>
 constexpr int kGradBound = E == 32 ? 512 : V == 1 ? 512 : 640;
 template <int V, int E>
@@ -306,7 +311,9 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
   if (a.rstd && live && t == 0) a.rstd[row] = rstd;
   if (a.y_dtype == VCSR_E4M3) {
     // y / scale = s weight * 448 / max|s weight|: rstd, which is alike for the row,
-    // falls out of the codes
+    // falls out of the codes.  The factor and the product are rounded, so beside a tie
+    // (within 2^-23 of it) a code may be the neighbouring one; so it may by rstd's own
+    // rounding in the kernel for long rows, which divides.
     if (live && t == 0) a.scale[row] = top * rstd * (1.0f / 448.0f);
     const float raise = top < 1e-30f ? 0x1p64f : 1.0f;  // 448 / top would overflow
     const float k = rstd != rstd ? rstd : top > 0.0f ? 448.0f / (top * raise) : 0.0f;
