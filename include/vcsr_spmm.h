@@ -505,6 +505,59 @@ typedef struct vcsr_rmsnorm_grad_args {
 vcsr_status vcsr_rmsnorm_grad(const vcsr_rmsnorm_grad_args *a, vcsr_stream_t stream);
 size_t vcsr_rmsnorm_grad_workspace(int64_t rows, int64_t dim);
 
+/* Layer norm with the residual's addition:
+ *   s = x + residual,  mean = sum(s) / dim,  rstd = 1 / sqrt(sum((s - mean)^2) / dim + eps),
+ *   y = (s - mean) * rstd * weight + bias
+ * per row.  y is computed from the unrounded s.  An 8-bit y is stored as by
+ * vcsr_rmsnorm: codes and one scale = max|y| / 448 per row, NaN for a row with a
+ * NaN among its y.  With dim 0 mean and rstd are NaN and scale 0. */
+typedef struct vcsr_layernorm_args {
+  int64_t rows, dim;
+  const void *x; /* rows x dim, x_dtype */
+  int64_t ldx;
+  const void *residual; /* rows x dim, x_dtype; NULL = none */
+  int64_t ldr;
+  const void *weight, *bias; /* dim, w_dtype; NULL = ones, zeros */
+  void *y;                   /* rows x dim, y_dtype */
+  int64_t ldy;
+  void *sum; /* s, rows x dim, x_dtype; NULL = not stored; may be x or residual itself */
+  int64_t lds;
+  float *mean, *rstd; /* rows each; NULL = not stored */
+  float *scale;       /* rows; y_dtype VCSR_E4M3 only */
+  float eps;
+  int x_dtype; /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int w_dtype; /* x_dtype or VCSR_F32 */
+  int y_dtype; /* any */
+} vcsr_layernorm_args;
+vcsr_status vcsr_layernorm(const vcsr_layernorm_args *a, vcsr_stream_t stream);
+
+/* Gradient of vcsr_layernorm from the stored s, mean and rstd: with
+ * h = (s - mean) * rstd and g = dy * weight,
+ *   dx = rstd * (g - mean(g) - h * mean(g * h)) + dsum,
+ *   dweight = sum over rows of dy * h,  dbias = sum over rows of dy
+ * (x and residual have the same gradient dx).  dsum is the gradient that reached
+ * s by other ways.  dweight and dbias are summed in a fixed order. */
+typedef struct vcsr_layernorm_grad_args {
+  int64_t rows, dim;
+  const void *dy; /* rows x dim, dy_dtype */
+  int64_t lddy;
+  const void *s; /* rows x dim, x_dtype */
+  int64_t lds;
+  const void *weight;       /* dim, w_dtype; NULL = ones */
+  const float *mean, *rstd; /* rows each */
+  const void *dsum;         /* rows x dim, x_dtype; NULL = none */
+  int64_t ldds;
+  void *dx; /* rows x dim, x_dtype; may be dsum itself */
+  int64_t lddx;
+  void *dweight, *dbias; /* dim, w_dtype; NULL = not wanted */
+  void *workspace;       /* vcsr_layernorm_grad_workspace bytes, 16-byte aligned; dweight, dbias only */
+  size_t workspace_bytes;
+  int x_dtype, w_dtype;
+  int dy_dtype; /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+} vcsr_layernorm_grad_args;
+vcsr_status vcsr_layernorm_grad(const vcsr_layernorm_grad_args *a, vcsr_stream_t stream);
+size_t vcsr_layernorm_grad_workspace(int64_t rows, int64_t dim);
+
 /* out = code * scale (one scale per row), or its square with squared != 0;
  * codes are VCSR_E4M3, out is VCSR_F32, VCSR_BF16 or VCSR_F16. */
 vcsr_status vcsr_dequantize(const void *codes, int64_t ldc, const float *scale, int64_t rows,

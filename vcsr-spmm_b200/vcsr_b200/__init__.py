@@ -106,6 +106,25 @@ class _RmsnormGradArgs(C.Structure):
                 ("x_dtype", C.c_int), ("w_dtype", C.c_int), ("dy_dtype", C.c_int)]
 
 
+class _LayernormArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int64), ("x", C.c_void_p), ("ldx", C.c_int64),
+                ("residual", C.c_void_p), ("ldr", C.c_int64), ("weight", C.c_void_p),
+                ("bias", C.c_void_p), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("sum", C.c_void_p), ("lds", C.c_int64), ("mean", C.c_void_p),
+                ("rstd", C.c_void_p), ("scale", C.c_void_p), ("eps", C.c_float),
+                ("x_dtype", C.c_int), ("w_dtype", C.c_int), ("y_dtype", C.c_int)]
+
+
+class _LayernormGradArgs(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("dim", C.c_int64), ("dy", C.c_void_p), ("lddy", C.c_int64),
+                ("s", C.c_void_p), ("lds", C.c_int64), ("weight", C.c_void_p),
+                ("mean", C.c_void_p), ("rstd", C.c_void_p), ("dsum", C.c_void_p),
+                ("ldds", C.c_int64), ("dx", C.c_void_p), ("lddx", C.c_int64),
+                ("dweight", C.c_void_p), ("dbias", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("x_dtype", C.c_int), ("w_dtype", C.c_int),
+                ("dy_dtype", C.c_int)]
+
+
 class _AdamwStepArgs(C.Structure):
     _fields_ = [("grads", C.c_void_p), ("g_dtype", C.c_int), ("m", C.c_void_p),
                 ("v", C.c_void_p), ("m_scale", C.c_void_p), ("u_scale", C.c_void_p),
@@ -201,6 +220,9 @@ _SIGS = {
     "vcsr_rmsnorm": (C.c_int, [C.POINTER(_RmsnormArgs), C.c_void_p]),
     "vcsr_rmsnorm_grad": (C.c_int, [C.POINTER(_RmsnormGradArgs), C.c_void_p]),
     "vcsr_rmsnorm_grad_workspace": (C.c_size_t, [C.c_int64, C.c_int64]),
+    "vcsr_layernorm": (C.c_int, [C.POINTER(_LayernormArgs), C.c_void_p]),
+    "vcsr_layernorm_grad": (C.c_int, [C.POINTER(_LayernormGradArgs), C.c_void_p]),
+    "vcsr_layernorm_grad_workspace": (C.c_size_t, [C.c_int64, C.c_int64]),
     "vcsr_dequantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
                                   C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p]),
     "vcsr_adamw_state_values": (C.c_int64, [C.c_int, C.c_void_p]),

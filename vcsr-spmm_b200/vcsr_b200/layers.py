@@ -28,8 +28,8 @@ from typing import NamedTuple, Optional
 import numpy as np
 import torch
 
-from . import (VcsrError, _AdamwStepArgs, _check, _LinearArgs, _LinearGradArgs, _RmsnormArgs,
-               _RmsnormGradArgs, _stream, lib)
+from . import (VcsrError, _AdamwStepArgs, _check, _LayernormArgs, _LayernormGradArgs, _LinearArgs,
+               _LinearGradArgs, _RmsnormArgs, _RmsnormGradArgs, _stream, lib)
 
 INVALID, UNSUPPORTED = 1, 5
 F32, BF16, F16, E4M3 = range(4)
@@ -210,6 +210,107 @@ def rmsnorm_backward(dy, s, weight, rstd, dsum=None, need_dweight=True):
                          x_type, _TYPE[weight.dtype], dy_type)
     _check(lib().vcsr_rmsnorm_grad(a, _current_stream(dy.get_device())))
     return dx, dw
+
+
+class LayerNormOut(NamedTuple):
+    y: torch.Tensor                 # the normalised rows (codes with an 8-bit out_dtype)
+    sum: torch.Tensor               # x + residual (x itself without a residual)
+    mean: Optional[torch.Tensor]    # with save_stats
+    rstd: Optional[torch.Tensor]    # with save_stats
+    scale: Optional[torch.Tensor]   # one per row, 8-bit y only
+
+
+def _weights(weight, bias, like, dim, dt):
+    """weight and bias (either may be None), of one type, and that type."""
+    w_dtype = dt
+    for t in (weight, bias):
+        if isinstance(t, torch.Tensor):
+            w_dtype = torch.float32 if t.dtype == torch.float32 else dt
+            break
+    if weight is not None:
+        weight = _vector(weight, "weight", like, dim, w_dtype)
+    if bias is not None:
+        bias = _vector(bias, "bias", like, dim, w_dtype)
+    return weight, bias, w_dtype
+
+
+@_operator
+def layernorm(x, weight=None, bias=None, residual=None, eps=1e-5, out_dtype=None, out=None,
+              sum_out=None, save_stats=False) -> LayerNormOut:
+    """y = (s - mean) * rstd * weight + bias, s = x + residual, mean and
+    rstd = 1/sqrt(var + eps) per row (vcsr_layernorm).  x and residual: (rows, dim)
+    float32, bfloat16 or float16; weight and bias: (dim,) both of x's type or both
+    float32, either may be None; out_dtype: any of the three or float8_e4m3fn (then y
+    holds codes and scale their rows' scales).  sum_out may be x or residual itself."""
+    rows, dim = _shape(x, "x")
+    dt = x.dtype
+    x_type = _type(dt, "x")
+    x, ldx = _matrix(x, "x", x, rows, dim, dt)
+    weight, bias, w_dtype = _weights(weight, bias, x, dim, dt)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _matrix(residual, "residual", x, rows, dim, dt)
+    y_dtype = out_dtype or getattr(out, "dtype", dt)
+    y_type = _type(y_dtype, "out")
+    y, ldy = _out(out, "out", x, rows, dim, y_dtype)
+    s, lds = (None, 0)
+    if residual is not None or sum_out is not None:
+        s, lds = _out(sum_out, "sum_out", x, rows, dim, dt)
+    mean = rstd = None
+    if save_stats:
+        mean, rstd = (x.new_empty(rows, dtype=torch.float32) for _ in range(2))
+    scale = x.new_empty(rows, dtype=torch.float32) if y_type == E4M3 else None
+    a = _LayernormArgs(rows, dim, x.data_ptr(), ldx, _p(residual), ldr, _p(weight), _p(bias),
+                       y.data_ptr(), ldy, _p(s), lds, _p(mean), _p(rstd), _p(scale), eps, x_type,
+                       _TYPE[w_dtype], y_type)
+    _check(lib().vcsr_layernorm(a, _current_stream(x.get_device())))
+    if out is not None or sum_out is not None:
+        _new_values([t for t in (out, sum_out) if t is not None])
+    return LayerNormOut(y, x if s is None else s, mean, rstd, scale)
+
+
+class LayerNormGrad(NamedTuple):
+    dx: torch.Tensor
+    dweight: Optional[torch.Tensor]
+    dbias: Optional[torch.Tensor]
+
+
+@_operator
+def layernorm_backward(dy, s, weight, mean, rstd, dsum=None, need_dweight=True,
+                       need_dbias=True, weight_dtype=None) -> LayerNormGrad:
+    """Gradients of layernorm from its sum, mean and rstd (vcsr_layernorm_grad); dx is
+    the gradient of x and of the residual, dsum (optional) the one that reached s by
+    other ways.  dy: float32, bfloat16 or float16; dsum and dx are of s's type; dweight
+    and dbias of weight's, or of weight_dtype (s's type, the default, or float32) where
+    weight is None."""
+    rows, dim = _shape(s, "s")
+    dy_type = _type(getattr(dy, "dtype", None), "dy")
+    dt = s.dtype
+    x_type = _type(dt, "s")
+    s, lds = _matrix(s, "s", dy, rows, dim, dt)
+    dy, lddy = _matrix(dy, "dy", dy, rows, dim, dy.dtype)
+    weight, _, w_dtype = _weights(weight, None, dy, dim, dt)
+    if weight_dtype is not None:
+        if weight_dtype not in ((dt, torch.float32) if weight is None else (w_dtype,)):
+            raise VcsrError(UNSUPPORTED, f"weight_dtype {weight_dtype}")
+        w_dtype = weight_dtype
+    mean = _vector(mean, "mean", dy, rows, torch.float32)
+    rstd = _vector(rstd, "rstd", dy, rows, torch.float32)
+    ldds = 0
+    if dsum is not None:
+        dsum, ldds = _matrix(dsum, "dsum", dy, rows, dim, dt)
+    dx = torch.empty_like(s, memory_format=torch.contiguous_format)
+    dw = dy.new_empty(dim, dtype=w_dtype) if need_dweight else None
+    db = dy.new_empty(dim, dtype=w_dtype) if need_dbias else None
+    ws, n = None, 0
+    if need_dweight or need_dbias:
+        n = lib().vcsr_layernorm_grad_workspace(rows, dim)
+        ws = _workspace(n, dy)
+    a = _LayernormGradArgs(rows, dim, dy.data_ptr(), lddy, s.data_ptr(), lds, _p(weight),
+                           mean.data_ptr(), rstd.data_ptr(), _p(dsum), ldds, dx.data_ptr(), dim,
+                           _p(dw), _p(db), _p(ws), n, x_type, _TYPE[w_dtype], dy_type)
+    _check(lib().vcsr_layernorm_grad(a, _current_stream(dy.get_device())))
+    return LayerNormGrad(dx, dw, db)
 
 
 @_operator

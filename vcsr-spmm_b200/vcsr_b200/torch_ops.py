@@ -1,5 +1,5 @@
 """PyTorch operators over the C ABI: torch.ops.vcsr.spmm(plan_id, B) -> C, and the
-dense layer operators with their gradients (rmsnorm and linear, below).
+dense layer operators with their gradients (rmsnorm, layernorm and linear, below).
 
 The reference has no Python or PyTorch binding; this one lets PyTorch code
 (and graph capture by tracers, through the fake implementation below) call a
@@ -130,6 +130,72 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None):
     """(y, s) of layers.rmsnorm, s = x + residual, with gradients of x, weight and
     residual (16- and 32-bit y)."""
     y, s, _ = _rmsnorm(x, weight, residual, eps, out_dtype or x.dtype)
+    return y, (x if residual is None else s)
+
+
+@torch.library.custom_op("vcsr::layernorm", mutates_args=())
+def _layernorm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+               residual: Optional[torch.Tensor], eps: float, out_dtype: torch.dtype
+               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, s, mean, rstd) of layers.layernorm; s has no rows without a residual (s is x then)."""
+    out = layers.layernorm(x, weight, bias, residual=residual, eps=eps, out_dtype=out_dtype,
+                           save_stats=True)
+    return (out.y, out.sum if residual is not None else x.new_empty((0, x.shape[1])), out.mean,
+            out.rstd)
+
+
+@_layernorm.register_fake
+def _(x, weight, bias, residual, eps, out_dtype):
+    rows = x.shape[0] if residual is not None else 0
+    return (x.new_empty(x.shape, dtype=out_dtype), x.new_empty((rows, x.shape[1])),
+            x.new_empty(x.shape[0], dtype=torch.float32), x.new_empty(x.shape[0], dtype=torch.float32))
+
+
+@torch.library.custom_op("vcsr::layernorm_backward", mutates_args=())
+def _layernorm_backward(dy: torch.Tensor, s: torch.Tensor, weight: Optional[torch.Tensor],
+                        mean: torch.Tensor, rstd: torch.Tensor, dsum: Optional[torch.Tensor],
+                        weight_dtype: torch.dtype, need_dweight: bool = True, need_dbias: bool = True
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(dx, dweight, dbias) of layers.layernorm_backward; what is not needed has no values."""
+    g = layers.layernorm_backward(dy, s, weight, mean, rstd, dsum=dsum, need_dweight=need_dweight,
+                                  need_dbias=need_dbias, weight_dtype=weight_dtype)
+    none = [s.new_empty(0, dtype=weight_dtype) if t is None else t for t in g[1:]]
+    return g.dx, *none
+
+
+@_layernorm_backward.register_fake
+def _(dy, s, weight, mean, rstd, dsum, weight_dtype, need_dweight=True, need_dbias=True):
+    return (s.new_empty(s.shape), *(s.new_empty(s.shape[1] if need else 0, dtype=weight_dtype)
+                                    for need in (need_dweight, need_dbias)))
+
+
+def _layernorm_setup(ctx, inputs, output):
+    x, weight, bias, residual, _, _ = inputs
+    ctx.added = residual is not None
+    ctx.weight_dtype = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(*output[2 if ctx.added else 1:])
+    ctx.save_for_backward(output[1] if ctx.added else x, weight, output[2], output[3])
+
+
+def _layernorm_grad(ctx, dy, ds, _, __):
+    if dy is None:  # only s was used
+        return ds, None, None, ds, None, None
+    s, weight, mean, rstd = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw, db = _layernorm_backward(dy, s, weight, mean, rstd, ds if ctx.added else None,
+                                     ctx.weight_dtype, need[1], need[2])
+    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None,
+            dx if need[3] else None, None, None)
+
+
+_layernorm.register_autograd(_layernorm_grad, setup_context=_layernorm_setup)
+
+
+def layernorm(x, weight=None, bias=None, residual=None, eps=1e-5, out_dtype=None):
+    """(y, s) of layers.layernorm, s = x + residual, with gradients of x, weight, bias and
+    residual (16- and 32-bit y)."""
+    y, s, _, _ = _layernorm(x, weight, bias, residual, eps, out_dtype or x.dtype)
     return y, (x if residual is None else s)
 
 
