@@ -30,6 +30,8 @@ template <int V>
 constexpr int kMostHeld = V == 1 ? 16 : 32;
 template <int V, int E>
 constexpr int kNormBlock = E == kMostHeld<V> ? 1024 : 512;
+template <int V, int E, bool RAGGED>
+constexpr int kNormBlocksPerSm = V == 8 && E == 16 && !RAGGED ? 3 : V == 8 && E <= 16 ? 2 : 1;
 
 struct NormArgs {
   int64_t rows, dim;
@@ -52,7 +54,7 @@ __device__ __forceinline__ void with_weight_type(int w_dtype, F &&f) {
 
 // One row per team; E values per thread, V at a time.
 template <class T, int V, int E, bool RAGGED>
-__global__ void __launch_bounds__(kNormBlock<V, E>)
+__global__ void __launch_bounds__(kNormBlock<V, E>, (kNormBlocksPerSm<V, E, RAGGED>))
     layernorm_kernel(const __grid_constant__ NormArgs a, int team) {
   __shared__ float2 shared[3][32];
   const int dim = (int)a.dim;
@@ -62,6 +64,20 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
   const int shift = RAGGED ? (int)(row * a.ldx & (V - 1)) : 0;
   constexpr int kN = E / V;
   float s[E];
+  // s[e] = f(s[e], u), two values at a time where there are two
+  auto pairs = [](float *x, int n, auto &&f) {
+    if constexpr (V > 1) {
+#pragma unroll
+      for (int j = 0; j < n; j += 2) {
+        const float2 y = f(make_float2(x[j], x[j + 1]), j);
+        x[j] = y.x;
+        x[j + 1] = y.y;
+      }
+    } else {
+      x[0] = f(make_float2(x[0], 0.0f), 0).x;
+    }
+  };
+  auto both = [](float v) { return make_float2(v, v); };
   const T *x = static_cast<const T *>(a.x) + row * a.ldx;
   const T *r = static_cast<const T *>(a.residual) + row * a.ldr;
   // what lies past a row is the next rows', as far as there are some
@@ -75,15 +91,18 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int at = (t + i * team) * V - shift;
-      float v[V];
+      float v[V + 1];
       row_load<T, V, RAGGED>(r, at, live ? dim : 0, whole(at), v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[i * V + j] += v[j];
+      pairs(s + i * V, V, [&](float2 u, int j) { return __fadd2_rn(u, make_float2(v[j], v[j + 1])); });
     }
   }
-  float total = 0.0f;
+  float2 total = both(0.0f);
 #pragma unroll
-  for (int e = 0; e < E; ++e) total += s[e];
+  for (int i = 0; i < kN; ++i)
+    pairs(s + i * V, V, [&](float2 u, int) {
+      total = __fadd2_rn(total, u);
+      return u;
+    });
   if (a.sum) {
     T *so = static_cast<T *>(a.sum) + row * a.lds;
 #pragma unroll
@@ -92,46 +111,53 @@ __global__ void __launch_bounds__(kNormBlock<V, E>)
       if (live && at < dim) row_store<T, V, RAGGED>(so, at, dim, s + i * V);
     }
   }
-  const float mean = team_sum(total, team, shared[0], 1) / (float)a.dim;
+  const float mean = team_sum(total.x + total.y, team, shared[0], 1) / (float)a.dim;
   // s becomes the distance from the mean, zero outside the row
-  float ss = 0.0f;
+  float2 squares = both(0.0f);
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
     const int at = (t + i * team) * V - shift;
+    if (at < dim) {
+      pairs(s + i * V, V, [&](float2 u, int) { return __fadd2_rn(u, both(-mean)); });
+      if (RAGGED && (at < 0 || at + V > dim)) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float &v = s[i * V + j];
-      v = (RAGGED ? (unsigned)(at + j) < (unsigned)dim : at < dim) ? v - mean : 0.0f;
-      ss = fmaf(v, v, ss);
+        for (int j = 0; j < V; ++j)
+          if ((unsigned)(at + j) >= (unsigned)dim) s[i * V + j] = 0.0f;
+      }
+      pairs(s + i * V, V, [&](float2 u, int) {
+        if (V == 1) u.y = 0.0f;
+        squares = __ffma2_rn(u, u, squares);
+        return u;
+      });
     }
   }
-  ss = team_sum(ss, team, shared[1], 1);
-  const float rstd = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+  const float rstd = 1.0f / sqrtf(team_sum(squares.x + squares.y, team, shared[1], 1) / (float)a.dim + a.eps);
   if (live && t == 0) {
     if (a.mean) a.mean[row] = mean;
     if (a.rstd) a.rstd[row] = rstd;
   }
-  // s becomes y
+  // s becomes y, a vector's weights loaded at a time
   with_weight_type<T>(a.w_dtype, [&](auto type) {
     using W = decltype(type);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int at = (t + i * team) * V - shift;
       if (at >= dim) continue;
-      float w[V], b[V];
-      if (a.weight) weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
-      if (a.bias) weight_load<W, V, RAGGED>(static_cast<const W *>(a.bias), at, dim, b);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float &v = s[i * V + j];
-        v *= rstd;
-        if (a.weight) v *= w[j];
-        if (a.bias) v += b[j];
+      float w[V + 1];
+      float *y = s + i * V;
+      pairs(y, V, [&](float2 u, int) { return __fmul2_rn(u, both(rstd)); });
+      if (a.weight) {
+        weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
+        pairs(y, V, [&](float2 u, int j) { return __fmul2_rn(u, make_float2(w[j], w[j + 1])); });
       }
+      if (a.bias) {
+        weight_load<W, V, RAGGED>(static_cast<const W *>(a.bias), at, dim, w);
+        pairs(y, V, [&](float2 u, int j) { return __fadd2_rn(u, make_float2(w[j], w[j + 1])); });
+      }
+      if (kNormBlocksPerSm<V, E, RAGGED> > 1) asm volatile("" ::: "memory");  // the next vector's loads stay behind
     }
   });
   if (a.y_dtype == VCSR_E4M3) {
-    // outside the row s is zero still, or zero times an rstd that is not finite
     float top = 0.0f, none = 0.0f;
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -236,246 +262,62 @@ struct GradArgs {
   void *dx;
   float *partial;  // blocks x 2 x dim: dweight, dbias; NULL = neither
   int64_t lddy, lds, ldds, lddx;
-  int w_dtype, dy_dtype;
-  int depth;  // groups of R rows in flight per team (16-byte access)
+  int x_dtype, w_dtype, dy_dtype;
+  // 16-byte access: rows in flight per team; bytes that a row takes of shared memory, and
+  // where dy and dsum start in it; bytes from a row of a team to its next
+  int depth, row_bytes, dy_at, ds_at;
+  int64_t s_hop, dy_hop, ds_hop, dx_hop;
 };
 
-// N sums over a team's threads (N = 2, 4 or 8); every thread gets them.  In a warp each
-// step but the last few halves what a lane still adds up: 9 shuffles for 8 values.
-// words: N x 32.
-template <int N>
-__device__ __forceinline__ void team_sums(float (&v)[N], int team, float *words, int id) {
+// The two sums of a row over a team's threads, in two steps with the team's barrier (for
+// teams of more than a warp) between them, so that other work can stand there too.
+// After the first a smaller team has its sums in v; words: 2 x 32.
+__device__ __forceinline__ void team_sums_begin(float2 &v, int team, float *words) {
   constexpr unsigned kAll = 0xffffffffu;
   if (team <= 32) {
     for (int o = team >> 1; o > 0; o >>= 1) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(kAll, v[i], o);
+      v.x += __shfl_xor_sync(kAll, v.x, o);
+      v.y += __shfl_xor_sync(kAll, v.y, o);
     }
     return;
   }
-  constexpr int kLanes = 32 / N;  // that end with the same value
-  const int lane = threadIdx.x & 31, which = lane / kLanes, part = lane % kLanes, warps = team >> 5;
-  int o = 16;
+  const int lane = threadIdx.x & 31;
+  const bool upper = lane & 16;  // the upper lanes go on with v.y
+  float sum = (upper ? v.y : v.x) + __shfl_xor_sync(kAll, upper ? v.x : v.y, 16);
 #pragma unroll
-  for (int half = N / 2; half >= 1; half /= 2, o /= 2) {
-    const bool upper = lane & o;
+  for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(kAll, sum, o);
+  if ((lane & 15) == 0) words[(lane >> 4) * 32 + (threadIdx.x >> 5)] = sum;
+}
+__device__ __forceinline__ void team_barrier(int team, int id) {
+  if (team > 32) asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(team) : "memory");
+}
+__device__ __forceinline__ void team_sums_end(float2 &v, int team, const float *words) {
+  if (team <= 32) return;
+  constexpr unsigned kAll = 0xffffffffu;
+  const int lane = threadIdx.x & 31, part = lane & 15, warps = team >> 5;
+  const float *mine = words + (lane >> 4) * 32;
+  float sum = part < warps ? mine[part] : 0.0f;
+  if (part + 16 < warps) sum += mine[part + 16];
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      if (i >= half) break;
-      const float send = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
-      v[i] = keep + __shfl_xor_sync(kAll, send, o);
-    }
-  }
-  float sum = v[0];
-#pragma unroll
-  for (o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(kAll, sum, o);
-  if (part == 0) words[which * 32 + (threadIdx.x >> 5)] = sum;
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(team) : "memory");
-  sum = 0.0f;
-  for (int w = part; w < warps; w += kLanes) sum += words[which * 32 + w];
-#pragma unroll
-  for (o = kLanes / 2; o > 0; o /= 2) sum += __shfl_xor_sync(kAll, sum, o);
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kAll, sum, i * kLanes);
+  for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(kAll, sum, o);
+  v = make_float2(__shfl_sync(kAll, sum, 0), __shfl_sync(kAll, sum, 16));
 }
 
-constexpr int kGradThreads = 640;  // the most of a block
-// Rows a team takes between two barriers.
-template <int V, int E>
-constexpr int kGradRows = E == 8 ? 2 : 1;
-// What the registers are sized for.
-template <int V, int E>
-constexpr int kGradBound = E == 8 ? 640 : 512;
+constexpr int kGradTeams = 512 / 64;  // of more than a warp, in a block
 
-// With 16-byte access a thread copies its own vectors of R rows, and of the next
-// depth - 1 times R, into shared memory ahead of their use (nobody else reads them: no
-// barrier); single values are loaded as they come.
-template <class T, int V, int E, bool RAGGED>
-__global__ void __launch_bounds__(kGradBound<V, E>, 1)
-    layernorm_grad_kernel(const __grid_constant__ GradArgs a, int team) {
-  constexpr int kN = E / V, R = kGradRows<V, E>;
-  __shared__ float words[2][kGradThreads / 64][2 * R * 32];
-  extern __shared__ __align__(16) unsigned char dynamic[];
-  const int dim = (int)a.dim;
-  const int t = threadIdx.x, teams = blockDim.y, mine = threadIdx.y, linear = mine * team + t;
-  const int64_t stride = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + mine;
-  // the same for all rows of a team: their distance is a multiple of V
-  const int shift = RAGGED ? (int)(first * a.lds & (V - 1)) : 0;
-  auto whole = [&](int64_t row, int at) {
-    return row < a.rows && at < dim && (!RAGGED || at + V <= (a.rows - row) * a.dim);
-  };
-  // what one row takes of shared memory, and of it s, dy, dsum
-  const int dy_size = a.dy_dtype == VCSR_F32 ? 4 : 2, slot = team * E;
-  const int dy_at = slot * (int)sizeof(T), ds_at = dy_at + slot * dy_size,
-            row_bytes = ds_at + (a.dsum ? slot * (int)sizeof(T) : 0);
-  unsigned char *ring = dynamic + (size_t)mine * a.depth * R * row_bytes;
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-  float dw[E], db[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
-
-  // the row to be copied next, this thread's first vector of it
-  int64_t ahead = first;
-  const int64_t begin = t * V - shift;
-  const char *s_next = static_cast<const char *>(a.s) + (first * a.lds + begin) * (int64_t)sizeof(T),
-             *dy_next = static_cast<const char *>(a.dy) + (first * a.lddy + begin) * dy_size,
-             *ds_next = static_cast<const char *>(a.dsum) + (first * a.ldds + begin) * (int64_t)sizeof(T);
-  const int64_t s_hop = stride * a.lds * (int64_t)sizeof(T), dy_hop = stride * a.lddy * dy_size,
-                ds_hop = stride * a.ldds * (int64_t)sizeof(T);
-  auto fetch = [&](int stage) {
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      if (ahead < a.rows) {
-        const uint32_t to = ring_at + (uint32_t)((stage * R + q) * row_bytes);
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          const int place = (t + i * team) * V, further = i * team * V;
-          if (whole(ahead, place - shift)) {
-            copy_async(to + place * (int)sizeof(T), s_next + further * (int)sizeof(T), V * sizeof(T));
-            copy_async(to + dy_at + place * dy_size, dy_next + further * dy_size, V * dy_size);
-            if (a.dsum)
-              copy_async(to + ds_at + place * (int)sizeof(T), ds_next + further * (int)sizeof(T), V * sizeof(T));
-          }
-        }
-      }
-      ahead += stride;
-      s_next += s_hop;
-      dy_next += dy_hop;
-      ds_next += ds_hop;
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  if constexpr (V > 1) {
-    for (int k = 0; k + 1 < a.depth; ++k) fetch(k);
-  }
-
-  // the rows' means and roots, read a turn ahead of their use
-  float mean_next[R], rstd_next[R];
-  auto stats = [&](int64_t row) {
-#pragma unroll
-    for (int q = 0; q < R; ++q, row += stride) {
-      mean_next[q] = row < a.rows ? a.mean[row] : 0.0f;
-      rstd_next[q] = row < a.rows ? a.rstd[row] : 0.0f;
-    }
-  };
-  stats(first);
-
-  int stage = 0, flip = 0;  // two sets of words: one barrier per turn is enough
-  // every thread of a warp takes the same number of turns (a warp may hold teams)
-  const int64_t warp_first = (int64_t)blockIdx.x * teams + (linear & ~31) / team;
-  for (int64_t turn = team > 32 ? first : warp_first, row = first; turn < a.rows;
-       turn += R * stride, row += R * stride, flip ^= 1) {
-    float mean[R], rstd[R], h[R][E], g[R][E], sums[2 * R];
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      mean[q] = mean_next[q];
-      rstd[q] = rstd_next[q];
-    }
-    stats(row + R * stride);
-    const unsigned char *from = ring + (size_t)stage * R * row_bytes;
-    if constexpr (V > 1) {
-      int next = stage + a.depth - 1;
-      if (next >= a.depth) next -= a.depth;
-      // the places of the turn before this one, read by this thread then
-      fetch(next);
-      copies_wait_oldest(a.depth);
-      if (++stage == a.depth) stage = 0;
-    }
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int64_t now = row + q * stride;
-      const bool live = now < a.rows;
-      const T *s = static_cast<const T *>(a.s) + now * a.lds;
-      with_type(a.dy_dtype, [&](auto type) {
-        using D = decltype(type);
-        const D *dy = static_cast<const D *>(a.dy) + now * a.lddy;
-        if constexpr (V > 1) {
-          const unsigned char *at_row = from + q * row_bytes;
-#pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const int place = (t + i * team) * V, at = place - shift;
-            if (whole(now, at)) {  // from shared memory, the thread's own place
-              row_load<T, V, RAGGED>(reinterpret_cast<const T *>(at_row) + shift, at, dim, true, h[q] + i * V);
-              row_load<D, V, RAGGED>(reinterpret_cast<const D *>(at_row + dy_at) + shift, at, dim, true, g[q] + i * V);
-            } else {  // the last row's end, or nothing
-              row_load<T, V, RAGGED>(s, at, live ? dim : 0, false, h[q] + i * V);
-              row_load<D, V, RAGGED>(dy, at, live ? dim : 0, false, g[q] + i * V);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const int at = t + e * team;
-            const bool in = live && at < dim;
-            h[q][e] = in ? widen(s[at]) : 0.0f;
-            g[q][e] = in ? widen(dy[at]) : 0.0f;
-          }
-        }
-      });
-    }
-#pragma unroll
-    for (int q = 0; q < 2 * R; ++q) sums[q] = 0.0f;
-    // outside the row g is zero and nothing is stored, whatever h is
-    with_weight_type<T>(a.w_dtype, [&](auto type) {
-      using W = decltype(type);
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int at = (t + i * team) * V - shift;
-        if (at >= dim) continue;
-        float w[V];
-        if (a.weight) weight_load<W, V, RAGGED>(static_cast<const W *>(a.weight), at, dim, w);
-#pragma unroll
-        for (int q = 0; q < R; ++q)
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int e = i * V + j;
-            float &hv = h[q][e], &gv = g[q][e];
-            hv = (hv - mean[q]) * rstd[q];
-            dw[e] = fmaf(gv, hv, dw[e]);
-            db[e] += gv;
-            if (a.weight) gv *= w[j];
-            sums[2 * q] += gv;
-            sums[2 * q + 1] = fmaf(gv, hv, sums[2 * q + 1]);
-          }
-      }
-    });
-    team_sums<2 * R>(sums, team, words[flip][team > 32 ? mine : 0], 1 + mine);
-#pragma unroll
-    for (int q = 0; q < R; ++q) {
-      const int64_t now = row + q * stride;
-      if (now >= a.rows) continue;
-      const float shift_mean = sums[2 * q] / (float)a.dim, dot_mean = sums[2 * q + 1] / (float)a.dim;
-      T *dx = static_cast<T *>(a.dx) + now * a.lddx;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) {
-        const int at = (t + i * team) * V - shift;
-        if (at >= dim) continue;
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          o[j] = rstd[q] * fmaf(-h[q][i * V + j], dot_mean, g[q][i * V + j] - shift_mean);
-        if (a.dsum) {
-          float d[V];
-          if (V > 1 && whole(now, at))
-            row_load<T, V, RAGGED>(reinterpret_cast<const T *>(from + q * row_bytes + ds_at) + shift, at, dim, true, d);
-          else
-            row_load<T, V, true>(static_cast<const T *>(a.dsum) + now * a.ldds, at, dim, false, d);
-#pragma unroll
-          for (int j = 0; j < V; ++j) o[j] += d[j];
-        }
-        row_store<T, V, RAGGED>(dx, at, dim, o);
-      }
-    }
-  }
-  if constexpr (V > 1) asm volatile("cp.async.wait_all;" ::: "memory");
-  if (!a.partial) return;
+// This block's sums over rows to its partial row: each thread's columns of its team's
+// row (first(i): of vector i), teams added in order through shared memory.
+template <int V, int E, class AT>
+__device__ __forceinline__ void store_partial(const GradArgs &a, const float *dw, const float *db, int team,
+                                              unsigned char *dynamic, AT &&first) {
+  const int dim = (int)a.dim, teams = blockDim.y, linear = threadIdx.y * team + threadIdx.x;
   float *out = a.partial + (int64_t)blockIdx.x * 2 * a.dim;
   float *joined = reinterpret_cast<float *>(dynamic);  // teams x 2 x dim
   if (teams > 1) __syncthreads();  // every team is done with its rows in shared memory
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    const int at = (t + i * team) * V - shift;
-    float *to = teams == 1 ? out + at : joined + mine * 2 * dim + at;
+  for (int i = 0; i < E / V; ++i) {
+    const int at = first(i);
+    float *to = teams == 1 ? out + at : joined + threadIdx.y * 2 * dim + at;
 #pragma unroll
     for (int j = 0; j < V; ++j)
       if ((unsigned)(at + j) < (unsigned)dim) {
@@ -490,6 +332,338 @@ __global__ void __launch_bounds__(kGradBound<V, E>, 1)
     for (int k = 0; k < teams; ++k) sum += joined[k * 2 * dim + c];
     out[c] = sum;
   }
+}
+
+// Waits until all but the latest n groups of copies have landed, n < 8.
+__device__ __forceinline__ void copies_wait_but(int n) {
+  switch (n) {
+    case 0: return copies_wait<0>();
+    case 1: return copies_wait<1>();
+    case 2: return copies_wait<2>();
+    case 3: return copies_wait<3>();
+    case 4: return copies_wait<4>();
+    case 5: return copies_wait<5>();
+    case 6: return copies_wait<6>();
+    default: return copies_wait<7>();
+  }
+}
+
+// Vector access.  A thread copies its own vectors of the next rows into shared memory
+// ahead of their use (nobody else reads them: no barrier).  A row is worked on twice, for
+// its two sums and for dx, and the first half of the next row comes before the second
+// half of this one: the barrier and the shuffles that join a row's sums then have a row's
+// work to stand behind.  RAGGED: vectors are cut at the memory's boundaries, so a row's
+// first and last may hold values of its neighbours.
+template <class T, class W, int V, int E, int BOUND, bool RAGGED>
+__global__ void __launch_bounds__(BOUND, 1) layernorm_grad_kernel(const __grid_constant__ GradArgs a, int team) {
+  constexpr int kN = E / V;
+  // kept in registers where they are enough; BOUND 640 leaves no two vectors' values either
+  constexpr bool kKeepWeight = E <= 16, kOneByOne = BOUND > 512;
+  __shared__ float words[3][kGradTeams][64];
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  const int dim = (int)a.dim, t = threadIdx.x, teams = blockDim.y, mine = threadIdx.y;
+  const unsigned rows = (unsigned)a.rows, block_first = blockIdx.x * teams, stride = gridDim.x * teams;
+  const int64_t first = block_first + mine;
+  const int turns = block_first < rows ? (int)((rows - block_first - 1) / stride) + 1 : 0;
+  const float inverse_dim = 1.0f / (float)dim;
+  const int dy_size = a.dy_dtype == VCSR_F32 ? 4 : 2;
+  // the same for all rows of a team: their distance is a multiple of V
+  const int shift = RAGGED ? (int)(first * a.lds & (V - 1)) : 0;
+  // this thread's place in the first of its team's rows
+  unsigned char *ring = dynamic + mine * a.depth * a.row_bytes;
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int dy_place = a.dy_at + t * V * dy_size, ds_place = a.ds_at + t * V * (int)sizeof(T);
+  auto at_of = [&](int i) { return (t + i * team) * V - shift; };
+  // whether vector i may be read whole: what lies past a row is the next rows', as far as
+  // there are some
+  auto whole = [&](int i, unsigned row) {
+    const int at = at_of(i);
+    return !RAGGED || at + V <= dim || at + V <= (int64_t)(rows - row) * a.dim;
+  };
+  bool in[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) in[i] = at_of(i) < dim;
+
+  // the weights of vector i, as they are stored
+  auto weight_at = [&](int i) {
+    const W *from = static_cast<const W *>(a.weight) + at_of(i);
+    Vec<W, V> w;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w.v[j] = narrow<W>(1.0f);
+    if (a.weight && in[i]) {
+      if constexpr (RAGGED) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if ((unsigned)(at_of(i) + j) < (unsigned)dim) w.v[j] = from[j];
+      } else {
+        w = load_vec<W, V>(from);
+      }
+    }
+    return w;
+  };
+  float2 dw[E / 2], db[E / 2];
+  Vec<W, V> weight[kKeepWeight ? kN : 1];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) dw[e] = db[e] = make_float2(0.0f, 0.0f);
+  if constexpr (kKeepWeight) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) weight[i] = weight_at(i);
+  }
+
+  // the row to be copied next, and its place in the ring
+  unsigned ahead = (unsigned)first;
+  int ahead_stage = 0;
+  const int begin = t * V - shift;
+  const char *s_next = static_cast<const char *>(a.s) + (first * a.lds + begin) * (int64_t)sizeof(T),
+             *dy_next = static_cast<const char *>(a.dy) + (first * a.lddy + begin) * dy_size,
+             *ds_next = static_cast<const char *>(a.dsum) + (first * a.ldds + begin) * (int64_t)sizeof(T);
+  auto fetch = [&] {
+    if (ahead < rows) {
+      const uint32_t to = ring_at + (uint32_t)(ahead_stage * a.row_bytes);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        if (!in[i] || !whole(i, ahead)) continue;
+        const int further = i * team * V;
+        copy_async(to + (t * V + further) * (int)sizeof(T), s_next + further * (int)sizeof(T), V * sizeof(T));
+        copy_async(to + dy_place + further * dy_size, dy_next + further * dy_size, V * dy_size);
+        if (a.dsum)
+          copy_async(to + ds_place + further * (int)sizeof(T), ds_next + further * (int)sizeof(T), V * sizeof(T));
+      }
+      ahead += stride;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    s_next += a.s_hop;
+    dy_next += a.dy_hop;
+    ds_next += a.ds_hop;
+    if (++ahead_stage == a.depth) ahead_stage = 0;
+  };
+  for (int k = 0; k < a.depth; ++k) fetch();
+
+  // what a row keeps between its halves
+  struct Row {
+    float2 sums;
+    float mean, rstd;
+    bool live;
+  };
+  unsigned row_now = (unsigned)first;  // whose first half is next
+  float mean_next = row_now < rows ? a.mean[row_now] : 0.0f, rstd_next = row_now < rows ? a.rstd[row_now] : 0.0f;
+  unsigned row_done = (unsigned)first;  // whose second half is next
+  char *dx_next = static_cast<char *>(a.dx) + (first * a.lddx + begin) * (int64_t)sizeof(T);
+
+  with_type(a.dy_dtype, [&](auto type) {
+    using D = decltype(type);
+    // vector i of the row in a slot as h and g, both zero outside the row
+    auto read = [&](const unsigned char *from, int i, unsigned row, const Row &r, float2 *h, float2 *g) {
+      const int further = i * team * V;
+      Vec<T, V> s;
+      Vec<D, V> dy;
+      if (whole(i, row)) {
+        s = load_vec<T, V>(reinterpret_cast<const T *>(from) + t * V + further);
+        dy = load_vec<D, V>(reinterpret_cast<const D *>(from + dy_place) + further);
+      } else {  // the end of the last rows
+        const T *s_row = static_cast<const T *>(a.s) + row * a.lds + at_of(i);
+        const D *dy_row = static_cast<const D *>(a.dy) + row * a.lddy + at_of(i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const bool is = (unsigned)(at_of(i) + j) < (unsigned)dim;
+          s.v[j] = is ? s_row[j] : T{};
+          dy.v[j] = is ? dy_row[j] : D{};
+        }
+      }
+      const float2 away = make_float2(-r.mean, -r.mean), by = make_float2(r.rstd, r.rstd);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        h[j] = __fmul2_rn(__fadd2_rn(make_float2(widen(s.v[2 * j]), widen(s.v[2 * j + 1])), away), by);
+        g[j] = make_float2(widen(dy.v[2 * j]), widen(dy.v[2 * j + 1]));
+      }
+      if (RAGGED && (at_of(i) < 0 || at_of(i) + V > dim)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if ((unsigned)(at_of(i) + j) >= (unsigned)dim) (&h[j / 2].x)[j % 2] = (&g[j / 2].x)[j % 2] = 0.0f;
+      }
+    };
+    auto weigh = [&](int i, float2 *g) {
+      const Vec<W, V> w = kKeepWeight ? weight[kKeepWeight ? i : 0] : weight_at(i);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) g[j] = __fmul2_rn(g[j], make_float2(widen(w.v[2 * j]), widen(w.v[2 * j + 1])));
+    };
+    int stage = 0;  // of the row whose first half is next
+    auto first_half = [&](Row &r, int k) {
+      r.mean = mean_next;
+      r.rstd = rstd_next;
+      const unsigned row = row_now;
+      r.live = row < rows;
+      if (r.live) row_now += stride;
+      if (row_now < rows) {
+        mean_next = a.mean[row_now];
+        rstd_next = a.rstd[row_now];
+      }
+      float2 sg = make_float2(0.0f, 0.0f), sgh = sg;
+      const unsigned char *from = ring + stage * a.row_bytes;
+      if (++stage == a.depth) stage = 0;
+      if (r.live) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          if (kOneByOne && i > 0) asm volatile("" ::: "memory");
+          if (!in[i]) continue;
+          float2 h[V / 2], g[V / 2];
+          read(from, i, row, r, h, g);
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const int e = i * (V / 2) + j;
+            dw[e] = __ffma2_rn(g[j], h[j], dw[e]);
+            db[e] = __fadd2_rn(db[e], g[j]);
+          }
+          weigh(i, g);
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            sg = __fadd2_rn(sg, g[j]);
+            sgh = __ffma2_rn(g[j], h[j], sgh);
+          }
+        }
+      }
+      __syncwarp();
+      r.sums = make_float2(sg.x + sg.y, sgh.x + sgh.y);
+      team_sums_begin(r.sums, team, words[k % 3][team > 32 ? mine : 0]);
+    };
+    int done_stage = 0;
+    auto second_half = [&](Row &r, int k) {
+      team_sums_end(r.sums, team, words[k % 3][team > 32 ? mine : 0]);
+      const unsigned char *from = ring + done_stage * a.row_bytes;
+      if (++done_stage == a.depth) done_stage = 0;
+      const float m1 = -r.sums.x * inverse_dim, m2 = -r.sums.y * inverse_dim;
+      const float2 away = make_float2(m1, m1), dot = make_float2(m2, m2), by = make_float2(r.rstd, r.rstd);
+      if (r.live) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+          if (!in[i]) continue;
+          if (kOneByOne && i > 0) asm volatile("" ::: "memory");
+          float2 h[V / 2], g[V / 2];
+          read(from, i, row_done, r, h, g);
+          weigh(i, g);
+          float o[V];
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) {
+            const float2 v = __fmul2_rn(by, __ffma2_rn(h[j], dot, __fadd2_rn(g[j], away)));
+            o[2 * j] = v.x;
+            o[2 * j + 1] = v.y;
+          }
+          if (a.dsum) {
+            float d[V];
+            if (whole(i, row_done))
+              row_load<T, V, false>(reinterpret_cast<const T *>(from + ds_place) + i * team * V, 0, V, true, d);
+            else
+              row_load<T, V, RAGGED>(static_cast<const T *>(a.dsum) + row_done * a.ldds, at_of(i), dim, false, d);
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] += d[j];
+          }
+          row_store<T, V, RAGGED>(reinterpret_cast<T *>(dx_next) - begin, at_of(i), dim, o);
+        }
+        row_done += stride;
+      }
+      dx_next += a.dx_hop;
+      fetch();  // into this row's place
+    };
+    // one row ahead in the first half; the rows' sums have three sets of words, since a
+    // warp may be a barrier ahead of one that still reads
+    Row held[2];
+    auto turn = [&](Row &now, Row &next, int k) {
+      if (k + 1 < turns) {
+        copies_wait_but(a.depth - 2);
+        first_half(next, k + 1);
+      }
+      team_barrier(team, 1 + mine);
+      second_half(now, k);
+    };
+    if (turns > 0) {
+      copies_wait_but(a.depth - 1);
+      first_half(held[0], 0);
+    }
+    for (int k = 0; k < turns; k += 2) {
+      turn(held[0], held[1], k);
+      if (k + 1 < turns) turn(held[1], held[0], k + 1);
+    }
+  });
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (!a.partial) return;
+  float dw_out[E], db_out[E];
+#pragma unroll
+  for (int e = 0; e < E / 2; ++e) {
+    dw_out[2 * e] = dw[e].x;
+    dw_out[2 * e + 1] = dw[e].y;
+    db_out[2 * e] = db[e].x;
+    db_out[2 * e + 1] = db[e].y;
+  }
+  store_partial<V, E>(a, dw_out, db_out, team, dynamic, at_of);
+}
+
+// Single values, loaded as they come: for matrices whose rows are off 16 bytes unlike.
+template <class T, int E>
+__global__ void __launch_bounds__(512, 1) layernorm_grad_odd_kernel(const __grid_constant__ GradArgs a, int team) {
+  __shared__ float words[2][kGradTeams][64];
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  const int dim = (int)a.dim;
+  const int t = threadIdx.x, teams = blockDim.y, mine = threadIdx.y, linear = mine * team + t;
+  const int64_t stride = (int64_t)gridDim.x * teams, first = (int64_t)blockIdx.x * teams + mine;
+  float dw[E], db[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) dw[e] = db[e] = 0.0f;
+  int flip = 0;  // two sets of words: one barrier per turn is enough
+  // every thread of a warp takes the same number of turns (a warp may hold teams)
+  const int64_t warp_first = (int64_t)blockIdx.x * teams + (linear & ~31) / team;
+  for (int64_t turn = team > 32 ? first : warp_first, row = first; turn < a.rows;
+       turn += stride, row += stride, flip ^= 1) {
+    const bool live = row < a.rows;
+    const float mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+    float h[E], g[E];
+    const T *s = static_cast<const T *>(a.s) + row * a.lds;
+    with_type(a.dy_dtype, [&](auto type) {
+      using D = decltype(type);
+      const D *dy = static_cast<const D *>(a.dy) + row * a.lddy;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = t + e * team;
+        const bool in = live && at < dim;
+        h[e] = in ? widen(s[at]) : 0.0f;
+        g[e] = in ? widen(dy[at]) : 0.0f;
+      }
+    });
+    // outside the row g is zero and nothing is stored, whatever h is
+    float2 sums = make_float2(0.0f, 0.0f);
+    with_weight_type<T>(a.w_dtype, [&](auto type) {
+      using W = decltype(type);
+      const W *weight = static_cast<const W *>(a.weight);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = t + e * team;
+        if (at >= dim) continue;
+        h[e] = (h[e] - mean) * rstd;
+        dw[e] = fmaf(g[e], h[e], dw[e]);
+        db[e] += g[e];
+        if (weight) g[e] *= widen(weight[at]);
+        sums.x += g[e];
+        sums.y = fmaf(g[e], h[e], sums.y);
+      }
+    });
+    float *const team_words = words[flip][team > 32 ? mine : 0];
+    team_sums_begin(sums, team, team_words);
+    team_barrier(team, 1 + mine);
+    team_sums_end(sums, team, team_words);
+    if (live) {
+      const float away = sums.x / (float)a.dim, dot = sums.y / (float)a.dim;
+      T *dx = static_cast<T *>(a.dx) + row * a.lddx;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int at = t + e * team;
+        if (at >= dim) continue;
+        float o = rstd * fmaf(-h[e], dot, g[e] - away);
+        if (a.dsum) o += widen(static_cast<const T *>(a.dsum)[row * a.ldds + at]);
+        dx[at] = narrow<T>(o);
+      }
+    }
+    __syncwarp();
+  }
+  if (a.partial) store_partial<1, E>(a, dw, db, team, dynamic, [&](int e) { return t + e * team; });
 }
 
 // dx of rows of any length, one block each; their sums over rows come from
@@ -613,38 +787,74 @@ void launch_norm(const NormArgs &a, cudaStream_t st) {
     layernorm_kernel<T, V, kMostHeld<V>, RAGGED><<<grid, block, 0, st>>>(a, s.team);
 }
 
-// The most blocks of the gradient kernel, which are also partial rows: one an SM, and a
-// multiple of 8, so that the rows of a team have one misalignment.
-int grad_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, std::max(8, sm_count() / 8 * 8)); }
+// The most blocks of the gradient kernels, which are also partial rows: one an SM.
+int grad_blocks(int64_t rows) { return (int)std::min<int64_t>(rows, sm_count()); }
 
-// Shared memory of a block's rows in flight.
+// Shared memory of a block's rows in flight, and the most of them per team.
 constexpr size_t kGradRing = 200 * 1024;
+constexpr int kGradDepth = 8;
+
+// Launches kernel(a, team) with teams that hold `held` values a thread, as many as fit
+// into `bound` threads a block; `ring`: with rows in flight.
+template <int V, class K>
+vcsr_status launch_teams(K kernel, GradArgs a, int64_t dim, int held, int bound, int blocks, bool ring,
+                         cudaStream_t st) {
+  const int team = team_of(ceil_div(dim, V), held / V);
+  if (ring) {
+    const int x_size = (int)type_size(a.x_dtype), dy_size = (int)type_size(a.dy_dtype);
+    a.dy_at = team * held * x_size;
+    a.ds_at = a.dy_at + team * held * dy_size;
+    a.row_bytes = a.ds_at + (a.dsum ? team * held * x_size : 0);
+    bound = (int)std::min<size_t>(bound, kGradRing / (2 * a.row_bytes) * team);  // two rows each
+  }
+  // teams that share a block join their sums
+  const int teams = std::max(1, std::min<int>(bound / team, (int)ceil_div(a.rows, blocks)));
+  const int in_block = (int)ceil_div(teams * team, 32) * 32 / team;
+  size_t smem = in_block > 1 && a.partial ? (size_t)in_block * 2 * a.dim * sizeof(float) : 0;
+  if (ring) {
+    const int64_t x_size = (int64_t)type_size(a.x_dtype), dy_size = (int64_t)type_size(a.dy_dtype),
+                  stride = (int64_t)blocks * in_block;
+    a.depth = std::min<int>(kGradDepth, (int)kGradRing / (a.row_bytes * in_block));
+    a.s_hop = stride * a.lds * x_size;
+    a.dy_hop = stride * a.lddy * dy_size;
+    a.ds_hop = stride * a.ldds * x_size;
+    a.dx_hop = stride * a.lddx * x_size;
+    smem = std::max(smem, (size_t)a.row_bytes * in_block * a.depth);
+  }
+  VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
+  kernel<<<blocks, dim3((unsigned)team, (unsigned)in_block), smem, st>>>(a, team);
+  return VCSR_OK;
+}
 
 template <class T, int V, bool RAGGED>
-vcsr_status launch_grad(GradArgs a, int blocks, cudaStream_t st) {
-  const int64_t dim = a.dim + (RAGGED ? V - 1 : 0);
-  auto run = [&](auto kernel, int held, int rows, int bound) -> vcsr_status {
-    const int team = team_of(ceil_div(dim, V), held / V);
-    // teams that share a block join their sums
-    const int teams = std::max(1, std::min<int>(512 / team, (int)ceil_div(a.rows, blocks)));
-    const int threads = (int)ceil_div(teams * team, 32) * 32, in_block = threads / team;
-    if (threads > bound) return fail(VCSR_ERR_RANGE, "block of %d threads", threads);
-    size_t smem = in_block > 1 && a.partial ? (size_t)in_block * 2 * a.dim * sizeof(float) : 0;
-    if (V > 1) {
-      const size_t group = (size_t)team * held * ((a.dsum ? 2 : 1) * sizeof(T) + type_size(a.dy_dtype)) *
-                           in_block * rows;
-      a.depth = (int)std::max<size_t>(1, std::min<size_t>(4, kGradRing / group));
-      smem = std::max(smem, group * a.depth);
+vcsr_status launch_grad(const GradArgs &a, int &blocks, cudaStream_t st) {
+  const int64_t dim = a.dim + (RAGGED ? V - 1 : 0);  // a row may start inside its first vector
+  if constexpr (V > 1) {
+    // a multiple of 8 blocks, so that the rows of a team have one misalignment (or each
+    // team has one row)
+    if (RAGGED && blocks < a.rows) blocks = blocks / 8 * 8;
+    auto run = [&](auto held, auto bound) {
+      constexpr int E = decltype(held)::value, B = decltype(bound)::value;
+      if (a.w_dtype == VCSR_F32)
+        return launch_teams<V>(layernorm_grad_kernel<T, float, V, E, B, RAGGED>, a, dim, E, B, blocks, true, st);
+      return launch_teams<V>(layernorm_grad_kernel<T, T, V, E, B, RAGGED>, a, dim, E, B, blocks, true, st);
+    };
+    using std::integral_constant;
+    const size_t value = (a.dsum ? 2 : 1) * sizeof(T) + type_size(a.dy_dtype);  // bytes in the ring
+    auto two_rows_fit = [&](int held) {
+      return 2 * value * held * team_of(ceil_div(dim, V), held / V) <= kGradRing;
+    };
+    if (dim <= 16 * 512 && two_rows_fit(16)) {
+      // two teams an SM where 512 threads hold only one
+      if constexpr (!RAGGED)
+        if (team_of(ceil_div(dim, V), 16 / V) == 320)
+          return run(integral_constant<int, 16>{}, integral_constant<int, 640>{});
+      return run(integral_constant<int, 16>{}, integral_constant<int, 512>{});
     }
-    VCSR_TRY(allow_shared(reinterpret_cast<const void *>(kernel), smem));
-    kernel<<<blocks, dim3((unsigned)team, (unsigned)in_block), smem, st>>>(a, team);
-    return VCSR_OK;
-  };
-  if (dim <= 8 * kGradBound<V, 8>) return run(layernorm_grad_kernel<T, V, 8, RAGGED>, 8, kGradRows<V, 8>, kGradBound<V, 8>);
-  if (dim <= 16 * 512) return run(layernorm_grad_kernel<T, V, 16, RAGGED>, 16, kGradRows<V, 16>, 512);
-  if (V > 1 && dim <= 32 * 512) {
-    constexpr int kHeld = kMostHeld<V>;
-    return run(layernorm_grad_kernel<T, V, kHeld, RAGGED>, kHeld, kGradRows<V, kHeld>, 512);
+    if (dim <= 32 * 512 && two_rows_fit(32)) return run(integral_constant<int, 32>{}, integral_constant<int, 512>{});
+  } else {
+    if (dim <= 8 * 512) return launch_teams<1>(layernorm_grad_odd_kernel<T, 8>, a, dim, 8, 512, blocks, false, st);
+    if (dim <= 16 * 512) return launch_teams<1>(layernorm_grad_odd_kernel<T, 16>, a, dim, 16, 512, blocks, false, st);
   }
   layernorm_long_grad_kernel<T><<<(unsigned)a.rows, kMaxThreads, 0, st>>>(a);
   if (a.partial)
@@ -732,10 +942,10 @@ vcsr_status layernorm_grad(const vcsr_layernorm_grad_args *a, cudaStream_t st) {
     if (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16))
       return fail(VCSR_ERR_INVALID, "dweight and dbias need %zu bytes of 16-byte aligned workspace", need);
   }
-  const int blocks = grad_blocks(a->rows);
+  int blocks = grad_blocks(a->rows);
   const GradArgs k{a->rows, a->dim,  a->dy,  a->s,    a->weight, a->dsum, a->mean, a->rstd, a->dx,
                    sums ? static_cast<float *>(a->workspace) : nullptr,
-                   a->lddy, a->lds,  a->ldds, a->lddx, a->w_dtype, a->dy_dtype, 0};
+                   a->lddy, a->lds,  a->ldds, a->lddx, a->x_dtype, a->w_dtype, a->dy_dtype};
   const int v = a->x_dtype == VCSR_F32 ? 4 : 8;
   const Access how = access_of(a->rows, a->dim, v, a->weight, {{a->dy, a->lddy, a->dy_dtype}, {a->s, a->lds, a->x_dtype},
                                                     {a->dsum, a->ldds, a->x_dtype}, {a->dx, a->lddx, a->x_dtype}});
