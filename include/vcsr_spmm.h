@@ -670,14 +670,115 @@ typedef struct vcsr_linear_grad_args {
 vcsr_status vcsr_linear_grad(const vcsr_linear_grad_args *a, vcsr_stream_t stream);
 size_t vcsr_linear_grad_workspace(const vcsr_linear_grad_args *a);
 
+/* The first half of a gated feed-forward layer (vcsr_linear is the second):
+ *   z = x_scale_i w_scale_j sum_k x[i,k] w[j,k] + bias_j  (M x 2N),
+ *   y = act(z[:, :N]) * z[:, N:]
+ * x is M x K, w is 2N x K: the N rows of the gate, then the N of the other factor.  Types,
+ * scales and accuracy as in vcsr_linear.  One kernel for 16- and 8-bit operands, two for
+ * VCSR_F32. */
+typedef struct vcsr_gated_linear_args {
+  int64_t M, N, K;
+  const void *x; /* M x K, dtype */
+  int64_t ldx;
+  const void *w; /* 2N x K, dtype */
+  int64_t ldw;
+  const float *x_scale, *w_scale; /* M and 2N values; VCSR_E4M3 only */
+  const void *bias;               /* 2N, out_dtype; NULL = none */
+  void *y;                        /* M x N, out_dtype */
+  int64_t ldy;
+  void *pre; /* z, M x 2N, out_dtype; NULL = not stored */
+  int64_t ldp;
+  void *workspace; /* vcsr_gated_linear_workspace bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int dtype;     /* any */
+  int out_dtype; /* dtype; with VCSR_E4M3: VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int act;       /* VCSR_ACT_* */
+} vcsr_gated_linear_args;
+vcsr_status vcsr_gated_linear(const vcsr_gated_linear_args *a, vcsr_stream_t stream);
+/* Bytes of device scratch the call needs, from *a (0 for aligned 16- and 8-bit operands
+ * with K > 0). */
+size_t vcsr_gated_linear_workspace(const vcsr_gated_linear_args *a);
+
+/* Gradient of vcsr_gated_linear (not for VCSR_E4M3): with g = pre[:, :N], u = pre[:, N:],
+ *   dz = [dy u act'(g) | dy act(g)]  (M x 2N),
+ *   dx = dz w (M x K),  dw = dz^T x (2N x K),  dbias = sum over rows of dz.
+ * dz is rounded to the operands' type before the two products; dbias sums the
+ * unrounded dz, in a fixed order. */
+typedef struct vcsr_gated_linear_grad_args {
+  int64_t M, N, K;
+  const void *dy; /* M x N */
+  int64_t lddy;
+  const void *pre; /* z of the forward call, M x 2N */
+  int64_t ldp;
+  const void *x; /* M x K; used for dw */
+  int64_t ldx;
+  const void *w; /* 2N x K; used for dx */
+  int64_t ldw;
+  void *dx; /* M x K; NULL = not wanted */
+  int64_t lddx;
+  void *dw; /* 2N x K; NULL = not wanted */
+  int64_t lddw;
+  void *dbias;     /* 2N; NULL = not wanted */
+  void *workspace; /* vcsr_gated_linear_grad_workspace bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int dtype; /* of every matrix: VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int act;
+} vcsr_gated_linear_grad_args;
+vcsr_status vcsr_gated_linear_grad(const vcsr_gated_linear_grad_args *a, vcsr_stream_t stream);
+size_t vcsr_gated_linear_grad_workspace(const vcsr_gated_linear_grad_args *a);
+
+/* 8-bit codes with a scale for each block of block_rows x 128 values (block_rows 1, as
+ * for rows of x, or 128, as for weights; blocks at the edges are smaller):
+ *   scale = max|block| * (1 / 448),  code = x / scale rounded to nearest even
+ * (1 / 448, the product and the quotients rounded to FP32; magnitudes past 448, which a
+ * scale that underflows can leave, become 448; a block of zeros has scale 0 and codes 0; one with a NaN
+ * or infinity has that scale).  x is VCSR_F32, VCSR_BF16 or VCSR_F16; scale is
+ * ceil(rows / block_rows) x ceil(dim / 128) with row pitch lds. */
+vcsr_status vcsr_block_quantize(const void *x, int64_t ldx, int64_t rows, int64_t dim, int x_dtype, int block_rows,
+                                void *codes, int64_t ldc, float *scale, int64_t lds, vcsr_stream_t stream);
+/* out = code * scale of its block; out is VCSR_F32, VCSR_BF16 or VCSR_F16. */
+vcsr_status vcsr_block_dequantize(const void *codes, int64_t ldc, const float *scale, int64_t lds, int64_t rows,
+                                  int64_t dim, int block_rows, void *out, int64_t ldo, int out_dtype,
+                                  vcsr_stream_t stream);
+
+/* Product of 8-bit operands whose scales change every 128 values of k:
+ *   z = sum_b x_scale[i,b] w_scale[j/128,b] (sum over k in block b of x[i,k] w[j,k]) + bias_j,
+ *   y = act(z) + residual
+ * (the two scales of a block are multiplied first, in FP32).  A NaN or infinity among the
+ * scales reaches the outputs that they are for. */
+typedef struct vcsr_block_linear_args {
+  int64_t M, N, K;
+  const void *x; /* M x K codes */
+  int64_t ldx;
+  const void *w; /* N x K codes */
+  int64_t ldw;
+  const float *x_scale; /* M x ceil(K / 128) */
+  int64_t ldxs;
+  const float *w_scale; /* ceil(N / 128) x ceil(K / 128) */
+  int64_t ldws;
+  const void *bias;     /* N, out_dtype; NULL = none */
+  const void *residual; /* M x N, out_dtype; NULL = none */
+  int64_t ldr;
+  void *y; /* M x N, out_dtype; may be residual itself */
+  int64_t ldy;
+  void *workspace; /* vcsr_block_linear_workspace bytes, 256-byte aligned */
+  size_t workspace_bytes;
+  int out_dtype; /* VCSR_F32, VCSR_BF16 or VCSR_F16 */
+  int act;       /* VCSR_ACT_* */
+} vcsr_block_linear_args;
+vcsr_status vcsr_block_linear(const vcsr_block_linear_args *a, vcsr_stream_t stream);
+/* Bytes of device scratch the call needs (0 for operands on 16 bytes). */
+size_t vcsr_block_linear_workspace(const vcsr_block_linear_args *a);
+
 /* Synchronises `stream` and reports (and clears) a bounded wait that ran out
- * in a kernel of vcsr_linear or vcsr_linear_grad on the current device:
+ * in a kernel of a dense product (vcsr_linear, vcsr_gated_linear, vcsr_block_linear and
+ * the gradients) on the current device:
  * VCSR_ERR_TIMEOUT with the barrier named in vcsr_last_error(), as
  * vcsr_plan_check does for a plan. */
 vcsr_status vcsr_layers_check(vcsr_stream_t stream);
 
 /* Test hook for the failure path above, not for production use: the next tensor-core
- * product that vcsr_linear or vcsr_linear_grad launches in this process withholds the
+ * product that one of these calls launches in this process withholds the
  * first accumulator-ready signal of its first block (or pair of blocks).  The wait for
  * it runs out after a short bounded poll, the block stops its other roles, waits for its
  * own copies and MMAs, frees its tensor memory and records the site; its outputs are

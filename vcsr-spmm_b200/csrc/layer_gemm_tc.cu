@@ -35,6 +35,7 @@
 #include <mutex>
 #include <vector>
 
+#include "layer_gemm_rows.cuh"
 #include "layer_gemm_tc.cuh"
 #include "spmm_tc.h"
 
@@ -605,6 +606,7 @@ vcsr_status check_waits(cudaStream_t st) {
   VCSR_CUDA(cudaMemcpyFromSymbol(&word, g_wait_error, sizeof(int)));
   if (word) VCSR_CUDA(cudaMemcpyToSymbol(g_wait_error, &zero, sizeof(int)));
   if (!word) VCSR_TRY(take_wait_error_f32(&word));
+  if (!word) VCSR_TRY(take_wait_error_rows(&word));
   if (!word) return VCSR_OK;
   char text[128];
   describe_tc_error(word, text, sizeof(text));

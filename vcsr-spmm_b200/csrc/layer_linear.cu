@@ -15,13 +15,11 @@
 // (1,410 TFLOP/s); 512 x 1024, k = 1024: 22 us in three launches.
 #include <algorithm>
 
-#include "layer_gemm.cuh"
+#include "layer_linear.cuh"
 
 namespace vcsr {
 namespace layer {
 namespace {
-
-constexpr int kDzWarps = 8;
 
 // Block (c, r): columns [c * 32 V, ...) of a chunk of rows; a lane holds V
 // columns, the warps take every 8th row of the chunk.  partial: one row of N
@@ -71,12 +69,6 @@ __global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four
   }
 }
 
-int64_t dz_chunks(int64_t M, int64_t N) {
-  // enough chunks of at least 32 rows for four blocks an SM
-  const int64_t across = ceil_div(N, 256);
-  return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, across)));
-}
-
 template <class T>
 void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *partial, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
@@ -92,26 +84,6 @@ void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *parti
     dz_kernel<T, 1><<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N,
                                                     chunk, a->act, partial);
 }
-
-constexpr size_t kAlign = 256;
-size_t round_up(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
-
-// Matrices whose base or pitch is no multiple of 16 bytes, which TMA cannot read,
-// copied to ones whose pitch is.
-struct PackJob {
-  const void *src;
-  void *dst;
-  int64_t ld, ldd, rows, cols;
-};
-// The copies, and the column sums of dbias' partial rows, that go before the products.
-struct PrepareJobs {
-  PackJob job[3];
-  int packs;
-  const float *partial;
-  int partials, dtype;
-  int64_t N;
-  void *dbias;
-};
 
 // Block row y copies job y, a thread 16 bytes at a time; the row after the last sums
 // columns.
@@ -145,65 +117,6 @@ __global__ void __launch_bounds__(256) prepare_kernel(const __grid_constant__ Pr
   }
 }
 
-int64_t packed_pitch(int64_t cols, int dtype) {
-  const int64_t v = 16 / (int64_t)type_size(dtype);
-  return ceil_div(cols, v) * v;
-}
-
-// What the tensor cores read of a matrix: itself, or a copy in the workspace.
-struct Packed {
-  bool copy = false;
-  int64_t ld = 0;
-  size_t bytes = 0;
-};
-Packed packed(const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
-  Packed k;
-  k.ld = rows == 1 ? packed_pitch(cols, dtype) : ld;  // the pitch of one row is free
-  if (!tc_aligned(p, k.ld, dtype)) {
-    k.copy = true;
-    k.ld = packed_pitch(cols, dtype);
-    k.bytes = round_up((size_t)rows * k.ld * type_size(dtype));
-  }
-  return k;
-}
-// What goes before a call's products, made by one launch.
-struct Prepare {
-  PrepareJobs jobs{};
-  int64_t most = 0;  // blocks of the largest job
-  char *ws;
-  explicit Prepare(void *workspace) : ws(static_cast<char *>(workspace)) {}
-  // Where the tensor cores read matrix p: the matrix, or its copy to be.
-  const void *matrix(const Packed &k, const void *p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
-    if (!k.copy) return p;
-    jobs.job[jobs.packs++] = {p, ws, ld, k.ld, rows, cols};
-    most = std::max(most, ceil_div(rows * k.ld * (int64_t)type_size(dtype) / 16, 256));
-    p = ws;
-    ws += k.bytes;
-    return p;
-  }
-  void column_sums(const float *partial, int count, int64_t N, void *out) {
-    jobs.partial = partial;
-    jobs.partials = count;
-    jobs.N = N;
-    jobs.dbias = out;
-    most = std::max(most, ceil_div(N, 32));
-  }
-  vcsr_status run(int dtype, cudaStream_t st) {
-    const int rows = jobs.packs + (jobs.dbias ? 1 : 0);
-    if (rows == 0) return VCSR_OK;
-    jobs.dtype = dtype;
-    const dim3 grid((unsigned)std::min<int64_t>(most, (int64_t)sm_count() * 8), (unsigned)rows);
-    if (dtype == VCSR_E4M3)
-      prepare_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
-    else if (dtype == VCSR_F32)
-      prepare_kernel<float><<<grid, 256, 0, st>>>(jobs);
-    else
-      prepare_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
-    VCSR_CUDA(cudaGetLastError());
-    return VCSR_OK;
-  }
-};
-
 // A product over no k: act(bias) + residual.
 __global__ void __launch_bounds__(256) empty_sum_kernel(const __grid_constant__ Gemm g) {
   const Epilogue &e = g.e;
@@ -217,6 +130,28 @@ __global__ void __launch_bounds__(256) empty_sum_kernel(const __grid_constant__ 
     z += t;
     store_as<1>(e.out, e.type, i * e.ldo + j, &z);
   }
+}
+
+}  // namespace
+
+int64_t dz_chunks(int64_t M, int64_t N) {
+  const int64_t across = ceil_div(N, 256);
+  return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, across)));
+}
+
+vcsr_status Prepare::run(int dtype, cudaStream_t st) {
+  const int rows = jobs.packs + (jobs.dbias ? 1 : 0);
+  if (rows == 0) return VCSR_OK;
+  jobs.dtype = dtype;
+  const dim3 grid((unsigned)std::min<int64_t>(most, (int64_t)sm_count() * 8), (unsigned)rows);
+  if (dtype == VCSR_E4M3)
+    prepare_kernel<uint8_t><<<grid, 256, 0, st>>>(jobs);
+  else if (dtype == VCSR_F32)
+    prepare_kernel<float><<<grid, 256, 0, st>>>(jobs);
+  else
+    prepare_kernel<uint16_t><<<grid, 256, 0, st>>>(jobs);
+  VCSR_CUDA(cudaGetLastError());
+  return VCSR_OK;
 }
 
 vcsr_status launch_gemm(const Gemm &g, cudaStream_t st) {
@@ -241,6 +176,15 @@ vcsr_status check_sizes(int64_t M, int64_t N, int64_t K) {
     return fail(VCSR_ERR_RANGE, "a size above 2^31 - 1");
   return VCSR_OK;
 }
+
+vcsr_status zero_matrix(void *p, int64_t ld, int64_t rows, int64_t cols, int type, cudaStream_t st) {
+  const size_t s = type_size(type);
+  if (rows > 0 && cols > 0)
+    VCSR_CUDA(cudaMemset2DAsync(p, (size_t)ld * s, 0, (size_t)cols * s, (size_t)rows, st));
+  return VCSR_OK;
+}
+
+namespace {
 
 size_t linear_workspace(const vcsr_linear_args *a) {
   if (a->M <= 0 || a->N <= 0 || a->K <= 0) return 0;
@@ -306,13 +250,6 @@ GradPlan grad_plan(const vcsr_linear_grad_args *a) {
   }
   p.total = p.dz + p.partial + p.dy.bytes + p.x.bytes + p.w.bytes;
   return p;
-}
-
-vcsr_status zero_matrix(void *p, int64_t ld, int64_t rows, int64_t cols, int type, cudaStream_t st) {
-  const size_t s = type_size(type);
-  if (rows > 0 && cols > 0)
-    VCSR_CUDA(cudaMemset2DAsync(p, (size_t)ld * s, 0, (size_t)cols * s, (size_t)rows, st));
-  return VCSR_OK;
 }
 
 vcsr_status linear_grad(const vcsr_linear_grad_args *a, cudaStream_t st) {

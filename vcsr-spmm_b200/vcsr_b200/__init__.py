@@ -152,6 +152,30 @@ class _LinearGradArgs(C.Structure):
                 ("workspace_bytes", C.c_size_t), ("dtype", C.c_int), ("act", C.c_int)]
 
 
+class _GatedLinearArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("x_scale", C.c_void_p), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+                ("y", C.c_void_p), ("ldy", C.c_int64), ("pre", C.c_void_p),
+                ("ldp", C.c_int64), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("dtype", C.c_int), ("out_dtype", C.c_int),
+                ("act", C.c_int)]
+
+
+class _GatedLinearGradArgs(_LinearGradArgs):
+    """The same fields: w, dw, dbias and pre are for both halves."""
+
+
+class _BlockLinearArgs(C.Structure):
+    _fields_ = [("M", C.c_int64), ("N", C.c_int64), ("K", C.c_int64), ("x", C.c_void_p),
+                ("ldx", C.c_int64), ("w", C.c_void_p), ("ldw", C.c_int64),
+                ("x_scale", C.c_void_p), ("ldxs", C.c_int64), ("w_scale", C.c_void_p),
+                ("ldws", C.c_int64), ("bias", C.c_void_p), ("residual", C.c_void_p),
+                ("ldr", C.c_int64), ("y", C.c_void_p), ("ldy", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                ("out_dtype", C.c_int), ("act", C.c_int)]
+
+
 _LIB = None
 
 # every function of include/vcsr_spmm.h with its ctypes signature
@@ -233,6 +257,18 @@ _SIGS = {
     "vcsr_linear": (C.c_int, [C.POINTER(_LinearArgs), C.c_void_p]),
     "vcsr_linear_workspace": (C.c_size_t, [C.POINTER(_LinearArgs)]),
     "vcsr_linear_grad": (C.c_int, [C.POINTER(_LinearGradArgs), C.c_void_p]),
+    "vcsr_gated_linear": (C.c_int, [C.POINTER(_GatedLinearArgs), C.c_void_p]),
+    "vcsr_gated_linear_workspace": (C.c_size_t, [C.POINTER(_GatedLinearArgs)]),
+    "vcsr_gated_linear_grad": (C.c_int, [C.POINTER(_GatedLinearGradArgs), C.c_void_p]),
+    "vcsr_gated_linear_grad_workspace": (C.c_size_t, [C.POINTER(_GatedLinearGradArgs)]),
+    "vcsr_block_quantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int,
+                                      C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                      C.c_void_p]),
+    "vcsr_block_dequantize": (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                                        C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_int,
+                                        C.c_void_p]),
+    "vcsr_block_linear": (C.c_int, [C.POINTER(_BlockLinearArgs), C.c_void_p]),
+    "vcsr_block_linear_workspace": (C.c_size_t, [C.POINTER(_BlockLinearArgs)]),
     "vcsr_layers_check": (C.c_int, [C.c_void_p]),
     "vcsr_layers_test_withhold_signal": (C.c_int, []),
     "vcsr_linear_grad_workspace": (C.c_size_t, [C.POINTER(_LinearGradArgs)]),

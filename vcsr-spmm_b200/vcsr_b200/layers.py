@@ -1,7 +1,9 @@
 """Dense layer operators beside the sparse product, on torch CUDA tensors: the
-norm (rmsnorm), the product with its epilogue (linear), their gradients, and
-the optimizer step over many tensors (AdamW).  The mathematics and the rules of
-types and aliasing stand with the C entry points in include/vcsr_spmm.h.
+norms (rmsnorm, layernorm), the product with its epilogue (linear), the gated one
+(gated_linear), their gradients, 8-bit operands with a scale per block
+(block_quantize, block_linear), and the optimizer step over many tensors (AdamW).
+The mathematics and the rules of types and aliasing stand with the C entry points
+in include/vcsr_spmm.h.
 
     from vcsr_b200 import layers
     n = layers.rmsnorm(C, gain, residual=h, save_rstd=True)
@@ -28,7 +30,8 @@ from typing import NamedTuple, Optional
 import numpy as np
 import torch
 
-from . import (VcsrError, _AdamwStepArgs, _check, _LayernormArgs, _LayernormGradArgs, _LinearArgs,
+from . import (VcsrError, _AdamwStepArgs, _BlockLinearArgs, _check, _GatedLinearArgs,
+               _GatedLinearGradArgs, _LayernormArgs, _LayernormGradArgs, _LinearArgs,
                _LinearGradArgs, _RmsnormArgs, _RmsnormGradArgs, _stream, lib)
 
 INVALID, UNSUPPORTED = 1, 5
@@ -37,6 +40,7 @@ _TYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16,
          torch.float8_e4m3fn: E4M3}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 BLOCK = 256  # values per scale of an 8-bit AdamW state
+SCALE_BLOCK = 128  # values of a row (and rows of weights) per scale of block codes
 
 _current_stream = torch._C._cuda_getCurrentRawStream
 _dtype = operator.attrgetter("dtype")
@@ -434,9 +438,166 @@ def linear_backward(dy, x, w, pre=None, act=None, need_dx=True, need_dw=True,
     return LinearGrad(dx, dw, db)
 
 
+@_operator
+def gated_linear(x, w, bias=None, act="silu", x_scale=None, w_scale=None, out_dtype=None,
+                 save_pre=False, out=None) -> LinearOut:
+    """y = act(g) * u, [g | u] = x w^T + bias (vcsr_gated_linear): the first half of a gated
+    feed-forward layer.  x: (M, K), w: (2 N, K), the gate's N rows first, both float32,
+    bfloat16, float16, or float8_e4m3fn with x_scale (M,) and w_scale (2 N,); bias: (2 N,); y
+    (M, N) and bias are of x's type, or of out_dtype (bfloat16 by default) with 8-bit
+    operands.  save_pre keeps [g | u], (M, 2 N), for the gradient."""
+    M, K = _shape(x, "x")
+    N2, _ = _shape(w, "w")
+    if N2 % 2:
+        raise VcsrError(INVALID, f"w must have the rows of both factors, got {N2}")
+    N = N2 // 2
+    dt = x.dtype
+    code = _type(dt, "x")
+    x, ldx = _matrix(x, "x", x, M, K, dt)
+    w, ldw = _matrix(w, "w", x, N2, K, dt)
+    if code == E4M3:
+        if x_scale is None or w_scale is None:
+            raise VcsrError(INVALID, "8-bit operands need x_scale and w_scale")
+        x_scale = _vector(x_scale, "x_scale", x, M, torch.float32)
+        w_scale = _vector(w_scale, "w_scale", x, N2, torch.float32)
+        out_dtype = out_dtype or getattr(out, "dtype", torch.bfloat16)
+    else:
+        if x_scale is not None or w_scale is not None:
+            raise VcsrError(INVALID, "scales are for 8-bit operands")
+        out_dtype = out_dtype or dt
+    out_type = _type(out_dtype, "out")
+    if bias is not None:
+        bias = _vector(bias, "bias", x, N2, out_dtype)
+    y, ldy = _out(out, "out", x, M, N, out_dtype)
+    pre = x.new_empty((M, N2), dtype=out_dtype) if save_pre else None
+    a = _GatedLinearArgs(M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, _p(x_scale), _p(w_scale),
+                         _p(bias), y.data_ptr(), ldy, _p(pre), N2, None, 0, code, out_type,
+                         _act(act))
+    L = lib()
+    n = L.vcsr_gated_linear_workspace(a)
+    if n:
+        ws = _workspace(n, x)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _check(L.vcsr_gated_linear(a, _current_stream(x.get_device())))
+    if out is not None:
+        _new_values(out)
+    return LinearOut(y, pre)
+
+
+@_operator
+def gated_linear_backward(dy, x, w, pre, act="silu", need_dx=True, need_dw=True,
+                          need_db=True) -> LinearGrad:
+    """Gradients of gated_linear (vcsr_gated_linear_grad): dy (M, N), x (M, K), w (2 N, K)
+    and pre (M, 2 N) of one type, float32, bfloat16 or float16."""
+    M, N = _shape(dy, "dy")
+    K = _shape(x, "x")[1]
+    dt = dy.dtype
+    code = _type(dt, "dy")
+    if code == E4M3:
+        raise VcsrError(UNSUPPORTED, "8-bit operands have no gradient")
+    act = _act(act)
+    dy, lddy = _matrix(dy, "dy", dy, M, N, dt)
+    x, ldx = _matrix(x, "x", dy, M, K, dt)
+    w, ldw = _matrix(w, "w", dy, 2 * N, K, dt)
+    pre, ldp = _matrix(pre, "pre", dy, M, 2 * N, dt)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_dx else None
+    dw = torch.empty_like(w, memory_format=torch.contiguous_format) if need_dw else None
+    db = dy.new_empty(2 * N) if need_db else None
+    a = _GatedLinearGradArgs(M, N, K, dy.data_ptr(), lddy, pre.data_ptr(), ldp, x.data_ptr(), ldx,
+                             w.data_ptr(), ldw, _p(dx), K, _p(dw), K, _p(db), None, 0, code, act)
+    L = lib()
+    n = L.vcsr_gated_linear_grad_workspace(a)
+    if n:
+        ws = _workspace(n, dy)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _check(L.vcsr_gated_linear_grad(a, _current_stream(dy.get_device())))
+    return LinearGrad(dx, dw, db)
+
+
+# ------------------------------------- 8-bit operands with a scale per block
+
+class BlockCodes(NamedTuple):
+    codes: torch.Tensor  # (rows, dim) float8_e4m3fn
+    scale: torch.Tensor  # (ceil(rows / block_rows), ceil(dim / 128)) float32
+
+
+def _block_shape(rows, dim, block_rows):
+    if block_rows not in (1, SCALE_BLOCK):
+        raise VcsrError(UNSUPPORTED, f"block_rows {block_rows!r} (1 or {SCALE_BLOCK})")
+    return -(-rows // block_rows), -(-dim // SCALE_BLOCK)
+
+
+@_operator
+def block_quantize(x, block_rows=1) -> BlockCodes:
+    """8-bit codes of x, (rows, dim) float32, bfloat16 or float16, with a scale for each
+    block of block_rows x 128 values, scale = max|block| / 448 (vcsr_block_quantize):
+    block_rows=1 for a product's x, 128 for its w."""
+    rows, dim = _shape(x, "x")
+    dt = x.dtype
+    x, ldx = _matrix(x, "x", x, rows, dim, dt)
+    down, across = _block_shape(rows, dim, block_rows)
+    codes = x.new_empty((rows, dim), dtype=torch.float8_e4m3fn)
+    scale = x.new_empty((down, across), dtype=torch.float32)
+    _check(lib().vcsr_block_quantize(x.data_ptr(), ldx, rows, dim, _type(dt, "x"), block_rows,
+                                     codes.data_ptr(), dim, scale.data_ptr(), across,
+                                     _current_stream(x.get_device())))
+    return BlockCodes(codes, scale)
+
+
+@_operator
+def block_dequantize(codes, scale, block_rows=1, out_dtype=torch.float32):
+    """codes * scale of their block, as out_dtype (vcsr_block_dequantize)."""
+    rows, dim = _shape(codes, "codes")
+    codes, ldc = _matrix(codes, "codes", codes, rows, dim, torch.float8_e4m3fn)
+    scale, lds = _matrix(scale, "scale", codes, *_block_shape(rows, dim, block_rows), torch.float32)
+    out = codes.new_empty((rows, dim), dtype=out_dtype)
+    _check(lib().vcsr_block_dequantize(codes.data_ptr(), ldc, scale.data_ptr(), lds, rows, dim,
+                                       block_rows, out.data_ptr(), dim, _type(out_dtype, "out"),
+                                       _current_stream(codes.get_device())))
+    return out
+
+
+@_operator
+def block_linear(x, w, x_scale, w_scale, bias=None, residual=None, act=None, out_dtype=None,
+                 out=None):
+    """y = act(x w^T + bias) + residual on float8_e4m3fn codes with a scale for each block
+    (vcsr_block_linear): x (M, K) with x_scale (M, ceil(K / 128)), w (N, K) with w_scale
+    (ceil(N / 128), ceil(K / 128)), as block_quantize makes them with block_rows 1 and 128.
+    y, bias and residual are of out_dtype (bfloat16 by default).  out may be residual
+    itself."""
+    M, K = _shape(x, "x")
+    N, _ = _shape(w, "w")
+    x, ldx = _matrix(x, "x", x, M, K, torch.float8_e4m3fn)
+    w, ldw = _matrix(w, "w", x, N, K, torch.float8_e4m3fn)
+    x_scale, ldxs = _matrix(x_scale, "x_scale", x, *_block_shape(M, K, 1), torch.float32)
+    w_scale, ldws = _matrix(w_scale, "w_scale", x, *_block_shape(N, K, SCALE_BLOCK), torch.float32)
+    out_dtype = out_dtype or getattr(out, "dtype", torch.bfloat16)
+    out_type = _type(out_dtype, "out")
+    if bias is not None:
+        bias = _vector(bias, "bias", x, N, out_dtype)
+    ldr = 0
+    if residual is not None:
+        residual, ldr = _matrix(residual, "residual", x, M, N, out_dtype)
+    y, ldy = _out(out, "out", x, M, N, out_dtype)
+    a = _BlockLinearArgs(M, N, K, x.data_ptr(), ldx, w.data_ptr(), ldw, x_scale.data_ptr(), ldxs,
+                         w_scale.data_ptr(), ldws, _p(bias), _p(residual), ldr, y.data_ptr(), ldy,
+                         None, 0, out_type, _act(act))
+    L = lib()
+    # scratch is for operands that are off 16 bytes
+    if (x.data_ptr() | w.data_ptr() | ldx | ldw) & 15:
+        n = L.vcsr_block_linear_workspace(a)
+        if n:
+            ws = _workspace(n, x)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    _check(L.vcsr_block_linear(a, _current_stream(x.get_device())))
+    if out is not None:
+        _new_values(out)
+    return y
+
+
 def check(stream=None):
-    """Synchronise and raise VcsrError (status 7) if a bounded wait of linear's or
-    linear_backward's kernels on the current device ran out since the last check."""
+    """Synchronise and raise VcsrError (status 7) if a bounded wait of the dense products'
+    kernels on the current device ran out since the last check."""
     _check(lib().vcsr_layers_check(_stream(stream)))
 
 

@@ -1,5 +1,6 @@
 """PyTorch operators over the C ABI: torch.ops.vcsr.spmm(plan_id, B) -> C, and the
-dense layer operators with their gradients (rmsnorm, layernorm and linear, below).
+dense layer operators with their gradients (rmsnorm, layernorm, linear and
+gated_linear, below).
 
 The reference has no Python or PyTorch binding; this one lets PyTorch code
 (and graph capture by tracers, through the fake implementation below) call a
@@ -255,3 +256,60 @@ def linear(x, w, bias=None, residual=None, act=None):
     wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad
                                              for t in (x, w, bias))
     return _linear(x, w, bias, residual, act, wanted and act != "none")[0]
+
+
+@torch.library.custom_op("vcsr::gated_linear", mutates_args=())
+def _gated_linear(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], act: str,
+                  save_pre: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, pre) of layers.gated_linear; pre has no rows unless saved."""
+    out = layers.gated_linear(x, w, bias=bias, act=act, save_pre=save_pre)
+    return out.y, out.pre if save_pre else out.y.new_empty((0, w.shape[0]))
+
+
+@_gated_linear.register_fake
+def _(x, w, bias, act, save_pre):
+    return (x.new_empty((x.shape[0], w.shape[0] // 2)),
+            x.new_empty((x.shape[0] if save_pre else 0, w.shape[0])))
+
+
+@torch.library.custom_op("vcsr::gated_linear_backward", mutates_args=())
+def _gated_linear_backward(dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor, pre: torch.Tensor, act: str,
+                           need_dx: bool = True, need_dw: bool = True, need_db: bool = True
+                           ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """layers.gated_linear_backward; what is not needed has no values."""
+    g = layers.gated_linear_backward(dy, x, w, pre, act=act, need_dx=need_dx, need_dw=need_dw,
+                                     need_db=need_db)
+    return tuple(x.new_empty(0) if t is None else t for t in g)
+
+
+@_gated_linear_backward.register_fake
+def _(dy, x, w, pre, act, need_dx=True, need_dw=True, need_db=True):
+    return (x.new_empty(x.shape if need_dx else 0), w.new_empty(w.shape if need_dw else 0),
+            w.new_empty(w.shape[0] if need_db else 0))
+
+
+def _gated_linear_setup(ctx, inputs, output):
+    x, w, _, act, save_pre = inputs
+    ctx.act = act
+    ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(x, w, output[1])
+
+
+def _gated_linear_grad(ctx, dy, _):
+    x, w, pre = ctx.saved_tensors
+    need = ctx.needs_input_grad[:3]
+    if dy is None or not any(need):
+        return (None,) * 5
+    made = _gated_linear_backward(dy, x, w, pre, ctx.act, *need)
+    return (*(g if n else None for g, n in zip(made, need)), None, None)
+
+
+_gated_linear.register_autograd(_gated_linear_grad, setup_context=_gated_linear_setup)
+
+
+def gated_linear(x, w, bias=None, act="silu"):
+    """y of layers.gated_linear with gradients of x, w and bias (16- and 32-bit operands; for
+    8-bit ones call layers.gated_linear, which has no gradient)."""
+    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
+    return _gated_linear(x, w, bias, act or "none", wanted)[0]
