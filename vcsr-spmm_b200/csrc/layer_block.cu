@@ -15,114 +15,192 @@ namespace vcsr {
 namespace layer {
 namespace {
 
-constexpr int kLanes = 16, kPer = kScaleBlock / kLanes;  // that hold 128 values, and how many each
+constexpr int kLanes = 8, kPer = kScaleBlock / kLanes;  // that hold 128 values, and how many each
 
-// A lane's 8 values of a block of columns of a row (n of them in the row), zeros beyond.
-template <class T, bool VEC>
-__device__ __forceinline__ void block_load(const T *p, int n, float *out) {
-  if (VEC && n >= kPer) {
-    const Vec<T, kPer> v = load_vec<T, kPer>(p);
+// kPer values at p, the first n of them (zeros beyond), moved `bytes` at a time: a power of
+// two from the element's size to 16 that p is a multiple of.
+template <int BYTES, class T>
+__device__ __forceinline__ void load_by(const T *p, Vec<T, kPer> &v) {
+  constexpr int W = BYTES / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) out[j] = widen(v.v[j]);
+  for (int i = 0; i < kPer; i += W) *reinterpret_cast<Vec<T, W> *>(v.v + i) = load_vec<T, W>(p + i);
+}
+template <class T>
+__device__ __forceinline__ Vec<T, kPer> load_some(const T *p, int n, int bytes) {
+  Vec<T, kPer> v;
+  if (n >= kPer && bytes == 16) {
+    load_by<16>(p, v);
+  } else if (n >= kPer && bytes == 8) {
+    load_by<8>(p, v);
+  } else if (n >= kPer && bytes == 4) {
+    load_by<4>(p, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) out[j] = j < n ? widen(p[j]) : 0.0f;
+    for (int j = 0; j < kPer; ++j) v.v[j] = j < n ? p[j] : T{};
   }
+  return v;
 }
-template <bool VEC>
-__device__ __forceinline__ void block_store(uint8_t *p, int n, const CodeScale &c, const float *x) {
-  float q[kPer];
+template <int BYTES, class T>
+__device__ __forceinline__ void store_by(T *p, const Vec<T, kPer> &v) {
+  constexpr int W = BYTES / sizeof(T);
 #pragma unroll
-  for (int j = 0; j < kPer; j += 2) {
-    const float2 y = c.quotients<true>(make_float2(x[j], x[j + 1]));
-    q[j] = y.x;
-    q[j + 1] = y.y;
-  }
-  if (VEC && n >= kPer) {
-    store_codes<kPer>(p, q);
+  for (int i = 0; i < kPer; i += W) store_vec<T, W>(p + i, *reinterpret_cast<const Vec<T, W> *>(v.v + i));
+}
+template <class T>
+__device__ __forceinline__ void store_some(T *p, int n, int bytes, const Vec<T, kPer> &v) {
+  if (n >= kPer && bytes == 16) {
+    store_by<16>(p, v);
+  } else if (n >= kPer && bytes == 8) {
+    store_by<8>(p, v);
+  } else if (n >= kPer && bytes == 4) {
+    store_by<4>(p, v);
   } else {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
-      if (j < n) p[j] = e4m3_code(q[j]);
+      if (j < n) p[j] = v.v[j];
   }
 }
-__device__ __forceinline__ float block_top(const float *x) {
-  float top = 0.0f;
+
+// The largest magnitude, NaN where a value is one: 16-bit values two at a time.
+template <class T>
+__device__ __forceinline__ float top_of(const Vec<T, kPer> &v) {
+  if constexpr (sizeof(T) == 2) {
+    using P = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const P *pairs = reinterpret_cast<const P *>(v.v);
+    P top = __habs2(pairs[0]);
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) top = max_or_nan(top, fabsf(x[j]));
-  return top;
+    for (int j = 1; j < kPer / 2; ++j) top = __hmax2_nan(top, __habs2(pairs[j]));
+    return max_or_nan(widen(top.x), widen(top.y));
+  } else {
+    float top = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) top = max_or_nan(top, fabsf(widen(v.v[j])));
+    return top;
+  }
+}
+// Codes of a lane's values.
+template <class T>
+__device__ __forceinline__ Vec<uint8_t, kPer> codes_of(const CodeScale &c, const Vec<T, kPer> &v) {
+  float2 q[kPer / 2];
+  if (c.raise == 1.0f) {
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) q[j] = c.quotients<false>(make_float2(widen(v.v[2 * j]), widen(v.v[2 * j + 1])));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer / 2; ++j) q[j] = c.quotients<true>(make_float2(widen(v.v[2 * j]), widen(v.v[2 * j + 1])));
+  }
+  Vec<uint8_t, kPer> o;
+#pragma unroll
+  for (int j = 0; j < kPer / 2; ++j)
+    reinterpret_cast<uint16_t *>(o.v)[j] = __nv_cvt_float2_to_fp8x2(q[j], __NV_SATFINITE, __NV_E4M3);
+  return o;
 }
 
-// Blocks of 1 x 128: 16 lanes each.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(256)
-    quantize_rows_kernel(const T *x, int64_t ldx, uint8_t *codes, int64_t ldc, float *scale, int64_t lds, int64_t rows,
-                         int64_t dim) {
-  const int64_t across = (dim + kScaleBlock - 1) / kScaleBlock, total = rows * across;
-  const int lane = threadIdx.x % kLanes;
-  // both halves of a warp take the same number of turns
-  for (int64_t i = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes; i - (threadIdx.x / kLanes & 1) < total;
-       i += (int64_t)gridDim.x * (256 / kLanes)) {
-    const bool live = i < total;
-    const int64_t r = live ? i / across : 0, b = live ? i - r * across : 0, c = b * kScaleBlock + lane * kPer;
-    const int n = live ? (int)max((int64_t)0, min((int64_t)kPer, dim - c)) : 0;
-    float v[kPer];
-    block_load<T, VEC>(x + r * ldx + c, n, v);
-    float top = block_top(v);
+constexpr int kBlocksPerSm = 6;
+
+struct BlockArgs {
+  const void *x;  // values, or codes to be turned back
+  void *out;      // codes, or values
+  float *scale;
+  int64_t ldx, ldo, lds, rows;
+  int dim, across;     // values and blocks of a row
+  int x_bytes, o_bytes;  // that neighbouring values can be moved by
+  int block_rows, dtype;
+};
+
+// A thread's place: groups of 8 lanes take neighbouring blocks of columns, and rows where
+// the blocks are fewer than a thread block's 32 groups; no division.
+struct Place {
+  int block, lane, n;  // n: values of the lane's that are in the row
+  int64_t row, step;
+  __device__ __forceinline__ Place(const BlockArgs &a, int wide) {  // log2 of groups side by side
+    const int group = threadIdx.x / kLanes;
+    lane = threadIdx.x % kLanes;
+    block = (blockIdx.x << wide) + (group & ((1 << wide) - 1));
+    const int down = (blockDim.x / kLanes) >> wide;
+    row = (int64_t)blockIdx.y * down + (group >> wide);
+    step = (int64_t)gridDim.y * down;
+    n = max(0, min(kPer, a.dim - block * kScaleBlock - lane * kPer));
+  }
+};
+
+// Blocks of 1 x 128, 8 lanes each.
+template <class T>
+__global__ void __launch_bounds__(256, kBlocksPerSm) quantize_rows_kernel(const __grid_constant__ BlockArgs a, int wide) {
+  const Place at(a, wide);
+  const int64_t column = (int64_t)at.block * kScaleBlock + at.lane * kPer;
+  const T *x = static_cast<const T *>(a.x) + column;
+  uint8_t *codes = static_cast<uint8_t *>(a.out) + column;
+  // the rows of a warp's groups may differ: all take the turns of the first
+  const int64_t warp_row = __shfl_sync(0xffffffffu, at.row, 0);
+  for (int64_t r = at.row, w = warp_row; w < a.rows; r += at.step, w += at.step) {
+    const Vec<T, kPer> v = load_some<T>(x + r * a.ldx, r < a.rows ? at.n : 0, a.x_bytes);
+    float top = top_of(v);
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o /= 2) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (r >= a.rows || at.n == 0) continue;
     const CodeScale s = code_scale(top);
-    block_store<VEC>(codes + r * ldc + c, n, s, v);
-    if (live && lane == 0) scale[r * lds + b] = s.scale;
+    store_some<uint8_t>(codes + r * a.ldo, at.n, a.o_bytes, codes_of(s, v));
+    if (at.lane == 0) a.scale[r * a.lds + at.block] = s.scale;
   }
 }
 
-// Blocks of 128 x 128: 256 threads each, 16 rows at a time.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(256)
-    quantize_tiles_kernel(const T *x, int64_t ldx, uint8_t *codes, int64_t ldc, float *scale, int64_t lds, int64_t rows,
-                          int64_t dim) {
-  __shared__ float tops[8];
+// Blocks of 128 x 128: 512 threads each, 64 rows at a time.
+template <class T>
+__global__ void __launch_bounds__(512, sizeof(T) == 2 ? 3 : 2) quantize_tiles_kernel(const __grid_constant__ BlockArgs a) {
+  __shared__ float tops[16];
   const int lane = threadIdx.x % kLanes, sub = threadIdx.x / kLanes;
-  constexpr int kAtOnce = 256 / kLanes, kTurns = kScaleBlock / kAtOnce;
-  const int64_t c = (int64_t)blockIdx.x * kScaleBlock + lane * kPer, r0 = (int64_t)blockIdx.y * kScaleBlock + sub;
-  const int n = (int)max((int64_t)0, min((int64_t)kPer, dim - c));
-  float v[kTurns][kPer], top = 0.0f;
+  constexpr int kAtOnce = 512 / kLanes, kTurns = kScaleBlock / kAtOnce;
+  const int64_t column = (int64_t)blockIdx.x * kScaleBlock + lane * kPer, r0 = (int64_t)blockIdx.y * kScaleBlock + sub;
+  const int n = (int)max((int64_t)0, min((int64_t)kPer, a.dim - column));
+  const T *x = static_cast<const T *>(a.x) + column;
+  uint8_t *codes = static_cast<uint8_t *>(a.out) + column;
+  Vec<T, kPer> v[kTurns];
 #pragma unroll
   for (int k = 0; k < kTurns; ++k) {
     const int64_t r = r0 + k * kAtOnce;
-    block_load<T, VEC>(x + r * ldx + c, r < rows ? n : 0, v[k]);
-    top = max_or_nan(top, block_top(v[k]));
+    v[k] = load_some<T>(x + r * a.ldx, r < a.rows ? n : 0, a.x_bytes);
   }
+  float top = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) top = max_or_nan(top, top_of(v[k]));
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
   __syncthreads();
+  top = tops[threadIdx.x & 15];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = max_or_nan(top, tops[k]);
+  for (int o = 8; o > 0; o /= 2) top = max_or_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
   const CodeScale s = code_scale(top);
 #pragma unroll
   for (int k = 0; k < kTurns; ++k) {
     const int64_t r = r0 + k * kAtOnce;
-    block_store<VEC>(codes + r * ldc + c, r < rows ? n : 0, s, v[k]);
+    if (r < a.rows) store_some<uint8_t>(codes + r * a.ldo, n, a.o_bytes, codes_of(s, v[k]));
   }
-  if (threadIdx.x == 0) scale[blockIdx.y * lds + blockIdx.x] = s.scale;
+  if (threadIdx.x == 0) a.scale[blockIdx.y * a.lds + blockIdx.x] = s.scale;
 }
 
-// V values from codes, a divisor of 128.
-template <int V>
-__global__ void __launch_bounds__(256)
-    dequantize_blocks_kernel(const uint8_t *codes, int64_t ldc, const float *scale, int64_t lds, int64_t rows,
-                             int64_t dim, int block_rows, void *out, int64_t ldo, int dtype) {
-  const int64_t per_row = dim / V, total = rows * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * V;
-    const Vec<uint8_t, V> q = load_vec<uint8_t, V>(codes + r * ldc + c);
-    const float s = scale[(block_rows == 1 ? r : r / kScaleBlock) * lds + c / kScaleBlock];
-    float o[V];
+// Values of codes.
+template <class T>
+__global__ void __launch_bounds__(256, kBlocksPerSm)
+    dequantize_blocks_kernel(const __grid_constant__ BlockArgs a, int wide) {
+  const Place at(a, wide);
+  const int64_t column = (int64_t)at.block * kScaleBlock + at.lane * kPer;
+  const uint8_t *codes = static_cast<const uint8_t *>(a.x) + column;
+  T *out = static_cast<T *>(a.out) + column;
+  if (at.n == 0) return;
+  for (int64_t r = at.row; r < a.rows; r += at.step) {
+    const Vec<uint8_t, kPer> q = load_some<uint8_t>(codes + r * a.ldx, at.n, a.x_bytes);
+    const float s = a.scale[(a.block_rows == 1 ? r : r / kScaleBlock) * a.lds + at.block];
+    float o[kPer];
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = e4m3_value(q.v[j]) * s;
-    store_as<V>(out, dtype, r * ldo + c, o);
+    for (int j = 0; j < kPer; j += 2) {
+      const __nv_fp8x2_storage_t two = *reinterpret_cast<const __nv_fp8x2_storage_t *>(q.v + j);
+      const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+      o[j] = y.x * s;
+      o[j + 1] = y.y * s;
+    }
+    store_some<T>(out + r * a.ldo, at.n, a.o_bytes, narrow_vec<T, kPer>(o));
   }
 }
 
@@ -136,28 +214,32 @@ vcsr_status check_blocks(int64_t rows, int64_t dim, int block_rows) {
   return VCSR_OK;
 }
 
-template <class T>
-vcsr_status launch_quantize(const void *from, int64_t ldx, int64_t rows, int64_t dim, int block_rows, void *to,
-                            int64_t ldc, float *scale, int64_t lds, cudaStream_t st) {
-  const T *x = static_cast<const T *>(from);
-  uint8_t *codes = static_cast<uint8_t *>(to);
-  const bool vec = aligned(x, 16) && ldx * (int64_t)sizeof(T) % 16 == 0 && aligned(codes, kPer) && ldc % kPer == 0;
-  if (block_rows == 1) {
-    const int64_t total = rows * ceil_div(dim, kScaleBlock);
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256 / kLanes), (int64_t)sm_count() * 32);
-    if (vec)
-      quantize_rows_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, codes, ldc, scale, lds, rows, dim);
-    else
-      quantize_rows_kernel<T, false><<<grid, 256, 0, st>>>(x, ldx, codes, ldc, scale, lds, rows, dim);
-    return VCSR_OK;
-  }
-  if (ceil_div(rows, kScaleBlock) > 65535) return fail(VCSR_ERR_RANGE, "more than 65535 blocks of rows");
-  const dim3 grid((unsigned)ceil_div(dim, kScaleBlock), (unsigned)ceil_div(rows, kScaleBlock));
-  if (vec)
-    quantize_tiles_kernel<T, true><<<grid, 256, 0, st>>>(x, ldx, codes, ldc, scale, lds, rows, dim);
+// The most bytes, up to 16, that neighbouring values of a matrix can be moved by.
+int access_bytes(const void *p, int64_t ld, int type) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (uint64_t)(ld * (int64_t)type_size(type)) | 16;
+  return (int)(bits & (~bits + 1));
+}
+
+// kernel(a, log2 of groups side by side) on blocks of 256 threads, 32 groups of 8 lanes.
+template <class K>
+void launch_blocks(K kernel, const BlockArgs &a, cudaStream_t st) {
+  int wide = 0;
+  while (wide < 5 && (1 << wide) < a.across) ++wide;
+  const int64_t down = 32 >> wide, columns = ceil_div(a.across, 1 << wide);
+  // some rows each, where there are many
+  const int64_t rows = std::min<int64_t>(ceil_div(a.rows, down), std::max<int64_t>(1, ceil_div(sm_count() * 4 * kBlocksPerSm, columns)));
+  kernel<<<dim3((unsigned)columns, (unsigned)std::min<int64_t>(rows, 65535)), 256, 0, st>>>(a, wide);
+}
+
+// f(T{}) for the element type named by `type`, which is F32, BF16 or F16.
+template <class F>
+void for_type(int type, F &&f) {
+  if (type == VCSR_F32)
+    f(float{});
+  else if (type == VCSR_BF16)
+    f(__nv_bfloat16{});
   else
-    quantize_tiles_kernel<T, false><<<grid, 256, 0, st>>>(x, ldx, codes, ldc, scale, lds, rows, dim);
-  return VCSR_OK;
+    f(__half{});
 }
 
 vcsr_status quantize(const void *x, int64_t ldx, int64_t rows, int64_t dim, int x_dtype, int block_rows, void *codes,
@@ -168,14 +250,17 @@ vcsr_status quantize(const void *x, int64_t ldx, int64_t rows, int64_t dim, int 
   VCSR_TRY(check_matrix("x", x, ldx, dim, x_dtype, false));
   VCSR_TRY(check_matrix("codes", codes, ldc, dim, VCSR_E4M3, false));
   VCSR_TRY(check_matrix("scale", scale, lds, ceil_div(dim, kScaleBlock), VCSR_F32, false));
-  vcsr_status done;
-  if (x_dtype == VCSR_F32)
-    done = launch_quantize<float>(x, ldx, rows, dim, block_rows, codes, ldc, scale, lds, st);
-  else if (x_dtype == VCSR_BF16)
-    done = launch_quantize<__nv_bfloat16>(x, ldx, rows, dim, block_rows, codes, ldc, scale, lds, st);
-  else
-    done = launch_quantize<__half>(x, ldx, rows, dim, block_rows, codes, ldc, scale, lds, st);
-  VCSR_TRY(done);
+  const BlockArgs a{x, codes, scale, ldx, ldc, lds, rows, (int)dim, (int)ceil_div(dim, kScaleBlock),
+                    access_bytes(x, ldx, x_dtype), access_bytes(codes, ldc, VCSR_E4M3), block_rows, x_dtype};
+  if (block_rows != 1 && ceil_div(rows, kScaleBlock) > 65535)
+    return fail(VCSR_ERR_RANGE, "more than 65535 blocks of rows");
+  for_type(x_dtype, [&](auto t) {
+    using T = decltype(t);
+    if (block_rows == 1)
+      launch_blocks(quantize_rows_kernel<T>, a, st);
+    else
+      quantize_tiles_kernel<T><<<dim3((unsigned)a.across, (unsigned)ceil_div(rows, kScaleBlock)), 512, 0, st>>>(a);
+  });
   VCSR_CUDA(cudaGetLastError());
   return VCSR_OK;
 }
@@ -188,18 +273,9 @@ vcsr_status dequantize(const void *codes, int64_t ldc, const float *scale, int64
   VCSR_TRY(check_matrix("codes", codes, ldc, dim, VCSR_E4M3, false));
   VCSR_TRY(check_matrix("scale", scale, lds, ceil_div(dim, kScaleBlock), VCSR_F32, false));
   VCSR_TRY(check_matrix("out", out, ldo, dim, out_dtype, false));
-  const uint8_t *c = static_cast<const uint8_t *>(codes);
-  auto fits = [&](int v) {
-    return dim % v == 0 && ldc % v == 0 && aligned(c, v) && aligned(out, 16) && ldo * (int64_t)type_size(out_dtype) % 16 == 0;
-  };
-  const int v = fits(16) ? 16 : fits(4) ? 4 : 1;
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows * (dim / v), 256), (int64_t)sm_count() * 16);
-  if (v == 16)
-    dequantize_blocks_kernel<16><<<grid, 256, 0, st>>>(c, ldc, scale, lds, rows, dim, block_rows, out, ldo, out_dtype);
-  else if (v == 4)
-    dequantize_blocks_kernel<4><<<grid, 256, 0, st>>>(c, ldc, scale, lds, rows, dim, block_rows, out, ldo, out_dtype);
-  else
-    dequantize_blocks_kernel<1><<<grid, 256, 0, st>>>(c, ldc, scale, lds, rows, dim, block_rows, out, ldo, out_dtype);
+  const BlockArgs a{codes, out, const_cast<float *>(scale), ldc, ldo, lds, rows, (int)dim, (int)ceil_div(dim, kScaleBlock),
+                    access_bytes(codes, ldc, VCSR_E4M3), access_bytes(out, ldo, out_dtype), block_rows, out_dtype};
+  for_type(out_dtype, [&](auto t) { launch_blocks(dequantize_blocks_kernel<decltype(t)>, a, st); });
   VCSR_CUDA(cudaGetLastError());
   return VCSR_OK;
 }

@@ -84,8 +84,8 @@ void launch_combine(const void *z, int64_t ldz, void *y, int64_t ldy, int64_t M,
 // Block (c, r): columns [c * 32 V, ...) of both halves, a chunk of rows; a lane holds V
 // columns of each, the warps take every 8th row of the chunk.  partial: one row of 2N sums
 // per chunk.
-template <class T, int V>
-__global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four an SM
+template <class T, int V, bool SUMS>
+__global__ void __launch_bounds__(kDzWarps * 32, 3)
     gated_dz_kernel(const T *dy, int64_t lddy, const T *pre, int64_t ldp, T *dz, int64_t lddz, int64_t M, int64_t N,
                     int64_t chunk, int act, float *partial) {
   __shared__ float joined[kDzWarps][32 * V + 1];
@@ -109,8 +109,10 @@ __global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four
         // rounded products, stored or not: dbias is then the same with and without dz
         dg[j] = __fmul_rn(__fmul_rn(widen(d.v[j]), widen(u.v[j])), slope[j]);
         du[j] = __fmul_rn(widen(d.v[j]), value[j]);
-        sum[0][j] += dg[j];
-        sum[1][j] += du[j];
+        if (SUMS) {
+          sum[0][j] += dg[j];
+          sum[1][j] += du[j];
+        }
       }
       if (dz) {
         store_narrow<T, V>(dz + r * lddz + col, dg);
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four
       }
     }
   }
-  if (!partial) return;
+  if (!SUMS) return;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     __syncthreads();
@@ -144,12 +146,13 @@ void launch_dz(const vcsr_gated_linear_grad_args *a, void *to, int64_t lddz, flo
   const bool vec = a->N % V == 0 && a->lddy % V == 0 && a->ldp % V == 0 && aligned(dy, 16) && aligned(pre, 16);
   const int64_t chunks = dz_chunks(a->M, a->N), chunk = ceil_div(a->M, chunks);
   const dim3 grid((unsigned)ceil_div(a->N, vec ? 32 * V : 32), (unsigned)chunks);
+  auto run = [&](auto kernel) {
+    kernel<<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N, chunk, a->act, partial);
+  };
   if (vec)
-    gated_dz_kernel<T, V><<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N, chunk, a->act,
-                                                          partial);
+    run(partial ? gated_dz_kernel<T, V, true> : gated_dz_kernel<T, V, false>);
   else
-    gated_dz_kernel<T, 1><<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N, chunk, a->act,
-                                                          partial);
+    run(partial ? gated_dz_kernel<T, 1, true> : gated_dz_kernel<T, 1, false>);
 }
 
 // f(T{}) for the element type named by `type`, which is F32, BF16 or F16.

@@ -54,10 +54,79 @@ struct RowsArgs {
   Epilogue e;
 };
 
-// 16 neighbouring values, or the first n of them: by 16 bytes where `vec`.
-template <class T>
-__device__ __forceinline__ void load_some(const T *p, int n, bool vec, float *out) {
-  if (vec && n >= 16) {
+// What the epilogue of four columns f .. f + 3 (n of them) needs of vectors along the row.
+struct Columns {
+  float scale[2][4], bias[2][4];  // of g and u; a product without pairs has the first only
+};
+template <class T, bool PAIRS>
+__device__ __forceinline__ Columns columns_at(const Epilogue &e, int64_t N, int f, int n) {
+  Columns c;
+#pragma unroll
+  for (int h = 0; h < (PAIRS ? 2 : 1); ++h)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      c.scale[h][j] = PAIRS && e.col_scale && j < n ? e.col_scale[h * N + f + j] : 1.0f;
+      c.bias[h][j] = e.bias && j < n ? widen(static_cast<const T *>(e.bias)[h * N + f + j]) : 0.0f;
+    }
+  return c;
+}
+
+// The outputs of four columns of row r from the sums of g and u.  WHOLE, here and below: all
+// four are there, and their matrices are moved four values at a time.
+template <class T, bool CODES, bool WHOLE>
+__device__ __forceinline__ void finish_pairs(const Epilogue &e, int64_t N, int64_t r, int f, int n, float row_scale,
+                                             const Columns &c, float *g, float *u) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (CODES) {
+      g[j] *= row_scale * c.scale[0][j];
+      u[j] *= row_scale * c.scale[1][j];
+    }
+    g[j] += c.bias[0][j];
+    u[j] += c.bias[1][j];
+  }
+  if (e.pre) {
+    T *pre = static_cast<T *>(e.pre) + r * e.ldp + f;
+    store_four<T, WHOLE>(pre, n, g);
+    store_four<T, WHOLE>(pre + N, n, u);
+  }
+  activate_all<4, sizeof(T) == 2>(e.act, g);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) g[j] *= u[j];
+  store_four<T, WHOLE>(static_cast<T *>(e.out) + r * e.ldo + f, n, g);
+}
+
+// The outputs of four columns of row r of a product of block-scaled operands.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void finish_four(const Epilogue &e, int64_t r, int f, int n, const Columns &c,
+                                            const float *residual, float *z) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) z[j] += c.bias[0][j];
+  activate_all<4, sizeof(T) == 2>(e.act, z);
+  if (e.residual) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) z[j] += residual[j];
+  }
+  store_four<T, WHOLE>(static_cast<T *>(e.out) + r * e.ldo + f, n, z);
+}
+
+// f(T{}, WHOLE) for the type of the outputs and whether `n` columns and their matrices
+// (pairs: u's part of pre too) take four values at a time.
+template <bool PAIRS, class F>
+__device__ __forceinline__ void with_outputs(const Epilogue &e, int64_t N, int n, F &&f) {
+  const bool whole = n >= 4 && fours(e) && (!PAIRS || !e.pre || N % 4 == 0);
+  with_type(e.type, [&](auto type) {
+    if (whole)
+      f(type, std::true_type{});
+    else
+      f(type, std::false_type{});
+  });
+}
+
+// 16 neighbouring values, or the first n of them; VEC: 16 bytes at a time.
+template <class T, bool VEC>
+__device__ __forceinline__ void load_sixteen(const T *p, int n, float *out) {
+  if constexpr (VEC) {
     constexpr int V = 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < 16; i += V) {
@@ -70,9 +139,9 @@ __device__ __forceinline__ void load_some(const T *p, int n, bool vec, float *ou
     for (int j = 0; j < 16; ++j) out[j] = j < n ? widen(p[j]) : 0.0f;
   }
 }
-template <class T>
-__device__ __forceinline__ void store_some(T *p, int n, bool vec, const float *x) {
-  if (vec && n >= 16) {
+template <class T, bool VEC>
+__device__ __forceinline__ void store_sixteen(T *p, int n, const float *x) {
+  if constexpr (VEC) {
     constexpr int V = 16 / sizeof(T);
 #pragma unroll
     for (int i = 0; i < 16; i += V) store_narrow<T, V>(p + i, x + i);
@@ -82,62 +151,69 @@ __device__ __forceinline__ void store_some(T *p, int n, bool vec, const float *x
       if (j < n) p[j] = narrow<T>(x[j]);
   }
 }
-// Whether a matrix (a vector: ld 0) takes 16 bytes at a time from columns that are
-// multiples of 16.
-__device__ __forceinline__ bool sixteens(const void *p, int64_t ld, int size) {
-  return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size)) & 15) == 0;
+// Whether all of an epilogue's matrices take 16 bytes at a time from columns that are
+// multiples of 16 (pairs: u's part of pre and of the vectors too).
+template <bool PAIRS>
+__device__ __forceinline__ bool sixteens(const Epilogue &e, int64_t N) {
+  const int size = e.type == VCSR_F32 ? 4 : 2;
+  auto bits = [&](const void *p, int64_t ld) { return p ? reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * size) : 0; };
+  const uintptr_t all = bits(e.out, e.ldo) | bits(e.pre, e.ldp) | bits(e.residual, e.ldr) | bits(e.bias, 0) |
+                        bits(e.col_scale, 0) | (PAIRS ? (uintptr_t)N * size : 0);
+  return (all & 15) == 0;
+}
+// f(T{}, VEC) for 16 columns, n of them there.
+template <bool PAIRS, class F>
+__device__ __forceinline__ void with_sixteen(const Epilogue &e, int64_t N, int n, F &&f) {
+  const bool vec = n >= 16 && sixteens<PAIRS>(e, N);
+  with_type(e.type, [&](auto type) {
+    if (vec)
+      f(type, std::true_type{});
+    else
+      f(type, std::false_type{});
+  });
 }
 
-// The epilogue of 16 columns f .. f + 15 (n of them) of row r, from the sums of g and u.
-template <class T>
-__device__ __forceinline__ void finish_gated(const Epilogue &e, int64_t N, int64_t r, int f, int n, float row_scale,
-                                             float *g, float *u) {
+// The outputs of columns f .. f + 15 (n of them) of row r from the sums of g and u.
+template <class T, bool CODES, bool VEC>
+__device__ __forceinline__ void finish_row_pairs(const Epilogue &e, int64_t N, int64_t r, int f, int n, float row_scale,
+                                                 float *g, float *u) {
   auto scaled = [&](float *z, int64_t column) {
     float c[16];
-    if (e.col_scale) {
-      load_some<float>(e.col_scale + column, n, sixteens(e.col_scale + column, 0, 4), c);
+    if (CODES) {
+      load_sixteen<float, VEC>(e.col_scale + column, n, c);
 #pragma unroll
       for (int j = 0; j < 16; ++j) z[j] *= row_scale * c[j];
     }
     if (e.bias) {
-      const T *bias = static_cast<const T *>(e.bias) + column;
-      load_some<T>(bias, n, sixteens(bias, 0, sizeof(T)), c);
+      load_sixteen<T, VEC>(static_cast<const T *>(e.bias) + column, n, c);
 #pragma unroll
       for (int j = 0; j < 16; ++j) z[j] += c[j];
     }
-    if (e.pre) {
-      T *pre = static_cast<T *>(e.pre) + r * e.ldp + column;
-      store_some<T>(pre, n, sixteens(pre, 0, sizeof(T)), z);
-    }
+    if (e.pre) store_sixteen<T, VEC>(static_cast<T *>(e.pre) + r * e.ldp + column, n, z);
   };
   scaled(u, N + f);
   scaled(g, f);
   activate_all<16, sizeof(T) == 2>(e.act, g);
 #pragma unroll
   for (int j = 0; j < 16; ++j) g[j] *= u[j];
-  T *out = static_cast<T *>(e.out) + r * e.ldo + f;
-  store_some<T>(out, n, sixteens(out, 0, sizeof(T)), g);
+  store_sixteen<T, VEC>(static_cast<T *>(e.out) + r * e.ldo + f, n, g);
 }
 
-// The epilogue of 16 columns of row r of a product of block-scaled operands.
-template <class T>
-__device__ __forceinline__ void finish_blocks(const Epilogue &e, int64_t r, int f, int n, float *z) {
-  float c[16];
+// The outputs of 16 columns of row r of a product of block-scaled operands.
+template <class T, bool VEC>
+__device__ __forceinline__ void finish_row(const Epilogue &e, int64_t r, int f, int n, const float *residual, float *z) {
   if (e.bias) {
-    const T *bias = static_cast<const T *>(e.bias) + f;
-    load_some<T>(bias, n, sixteens(bias, 0, sizeof(T)), c);
+    float c[16];
+    load_sixteen<T, VEC>(static_cast<const T *>(e.bias) + f, n, c);
 #pragma unroll
     for (int j = 0; j < 16; ++j) z[j] += c[j];
   }
   activate_all<16, sizeof(T) == 2>(e.act, z);
   if (e.residual) {
-    const T *residual = static_cast<const T *>(e.residual) + r * e.ldr + f;
-    load_some<T>(residual, n, sixteens(residual, 0, sizeof(T)), c);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) z[j] += c[j];
+    for (int j = 0; j < 16; ++j) z[j] += residual[j];
   }
-  T *out = static_cast<T *>(e.out) + r * e.ldo + f;
-  store_some<T>(out, n, sixteens(out, 0, sizeof(T)), z);
+  store_sixteen<T, VEC>(static_cast<T *>(e.out) + r * e.ldo + f, n, z);
 }
 
 // Waits for this warp's loads from tensor memory, among them the 16 values at z: naming
@@ -170,10 +246,28 @@ __device__ __forceinline__ void add_scaled(uint32_t from, float scale, float2 *s
   }
 }
 
+// Four neighbouring scales of a row from block b on, those below `blocks`.  (A row per lane
+// is a line of L1 per lane: by fours they take a quarter of its time.)
+__device__ __forceinline__ float4 four_scales(const float *p, int b, int blocks, bool aligned) {
+  if (aligned && b + 4 <= blocks) return *reinterpret_cast<const float4 *>(p + b);
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (b < blocks) v.x = p[b];
+  if (b + 1 < blocks) v.y = p[b + 1];
+  if (b + 2 < blocks) v.z = p[b + 2];
+  if (b + 3 < blocks) v.w = p[b + 3];
+  return v;
+}
+
 // ------------------------------------------------------------- pair kernel
 
 constexpr int kPairWarps = 8;  // of the epilogue
-constexpr int kPairThreads = 32 * (kPairWarps + 2);
+// Two of the four that follow do nothing, but a register split is by fours.
+template <bool BLOCKS>
+constexpr int kPairThreads = 32 * (kPairWarps + (BLOCKS ? 4 : 2));
+// Registers of a thread after the split (block-scaled sums take 128 of them): the
+// launch's 168 x 384 in all.
+constexpr int kPairFew = 40, kPairMany = 232;
+static_assert(kPairFew * 128 + kPairMany * 256 <= 168 * 384, "");
 constexpr int kPairStage = 2 * kTileBytes, kPairStages = kRing / kPairStage;
 constexpr size_t kPairSmem = (size_t)kRing + 1024 + 512;
 constexpr int kColumns = 256;  // of an accumulator
@@ -181,7 +275,7 @@ constexpr int kColumns = 256;  // of an accumulator
 // WITHHOLD (a test), here and below: the first block (or pair) waits for a signal that is
 // not sent.
 template <bool BLOCKS, bool CODES, bool WITHHOLD>
-__global__ void __launch_bounds__(kPairThreads, 1)
+__global__ void __launch_bounds__(kPairThreads<BLOCKS>, 1)
     rows_pair_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ CUtensorMap mx,
                      const __grid_constant__ CUtensorMap mw) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -221,7 +315,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   fence_after_sync();
   const uint32_t tmem = *holder;
 
-  if (warp == kPairWarps) {
+  if (warp >= kPairWarps) {
+   if (BLOCKS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFew));
+   if (warp == kPairWarps) {
     if (lane == 0) {
       // copies of this CTA's halves, complete on the leader's barrier
       RingPlace<kPairStages> at;
@@ -288,9 +384,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
       }
     }
+   }
   } else {
+    if (BLOCKS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairMany));
     RingPlace<2> acc;
-    const int quarter = warp & 3, half = warp >> 2;
+    const int quarter = warp & 3, half = warp >> 2;  // of the lanes, and of the columns
     bool go = true;
     if (withheld) go = __all_sync(0xffffffffu, mbar_wait(dfull, 0, abort_flag, kWaitAccFull, kTestPollLimit));
     auto ready = [&] {
@@ -309,7 +407,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int t = first; t < tiles && go; t += stride) {
       int tn, tm;
       tile_of(t, a.tiles_n, a.tiles_m, &tn, &tm);
-      const int r = tm * 2 * kRows + (int)rank * kRows + quarter * 32 + lane;
+      const int r0 = tm * 2 * kRows + (int)rank * kRows + quarter * 32, r = r0 + lane;
       const bool live = r < a.M;
       if constexpr (!BLOCKS) {
         if (!(go = ready())) break;
@@ -325,8 +423,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (c + 16 == 64) release();
           const int f = tn * kOut + half * 64 + c, n = a.N - f;
           if (live && n > 0)
-            with_type(a.e.type, [&](auto type) {
-              finish_gated<decltype(type)>(a.e, a.N, r, f, n, row_scale, g, u);
+            with_sixteen<true>(a.e, a.N, n, [&](auto type, auto vec) {
+              finish_row_pairs<decltype(type), CODES, decltype(vec)::value>(a.e, a.N, r, f, n, row_scale, g, u);
             });
           __syncwarp();
         }
@@ -335,30 +433,51 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         float2 sums[64];
 #pragma unroll
         for (int j = 0; j < 64; ++j) sums[j] = make_float2(0.0f, 0.0f);
-        // a block's scales are read while the one before is added up
+        // four blocks' scales are read while the four before are added up
         const float *xs = a.x_scale + (live ? r : 0) * a.ldxs;
         const float *ws = a.w_scale + (int64_t)min(tn * 2 + half, (a.N - 1) / kScaleBlock) * a.ldws;
-        float scale = xs[0] * ws[0];
-        for (int b = 0; b < a.blocks; ++b) {
-          const int ahead = min(b + 1, a.blocks - 1);
-          const float xs_next = xs[ahead], ws_next = ws[ahead];
-          if (!(go = ready())) break;
-          add_scaled<128>(lanes + acc.stage * kColumns + half * 128, scale, sums, release);
-          acc.next();
-          scale = xs_next * ws_next;
+        const bool by_four = ((reinterpret_cast<uintptr_t>(a.x_scale) | reinterpret_cast<uintptr_t>(a.w_scale)) & 15) == 0 &&
+                             ((a.ldxs | a.ldws) & 3) == 0;
+        float4 xs_next = four_scales(xs, 0, a.blocks, by_four), ws_next = four_scales(ws, 0, a.blocks, by_four);
+        // the tile's sums are under way: its residual comes to L2 meanwhile
+        prefetch_residual(a.e, tn * kOut + half * 128, a.N, 128, r0, a.M, 32, lane, 32);
+#pragma unroll 1
+        for (int b0 = 0; b0 < a.blocks && go; b0 += 4) {
+          float scale[4] = {xs_next.x * ws_next.x, xs_next.y * ws_next.y, xs_next.z * ws_next.z, xs_next.w * ws_next.w};
+          xs_next = four_scales(xs, b0 + 4, a.blocks, by_four);
+          ws_next = four_scales(ws, b0 + 4, a.blocks, by_four);
+#pragma unroll 1
+          for (int b = b0; b < min(b0 + 4, a.blocks); ++b) {
+            if (!(go = ready())) break;
+            add_scaled<128>(lanes + acc.stage * kColumns + half * 128, scale[0], sums, release);
+            acc.next();
+            scale[0] = scale[1];
+            scale[1] = scale[2];
+            scale[2] = scale[3];
+          }
         }
         if (!go) break;
         with_type(a.e.type, [&](auto type) {
+          using T = decltype(type);
+          const bool vec = sixteens<false>(a.e, a.N);
 #pragma unroll
           for (int c = 0; c < 128; c += 16) {
             const int f = tn * kOut + half * 128 + c, n = a.N - f;
-            float z[16];
+            float z[16], residual[16];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               z[2 * j] = sums[c / 2 + j].x;
               z[2 * j + 1] = sums[c / 2 + j].y;
             }
-            if (live && n > 0) finish_blocks<decltype(type)>(a.e, r, f, n, z);
+            if (!live || n <= 0) continue;
+            const T *from = static_cast<const T *>(a.e.residual) + (int64_t)r * a.e.ldr + f;
+            if (vec && n >= 16) {
+              if (a.e.residual) load_sixteen<T, true>(from, n, residual);
+              finish_row<T, true>(a.e, r, f, n, residual, z);
+            } else {
+              if (a.e.residual) load_sixteen<T, false>(from, n, residual);
+              finish_row<T, false>(a.e, r, f, n, residual, z);
+            }
           }
         });
         __syncwarp();
@@ -420,24 +539,6 @@ __device__ __forceinline__ void gather_four(uint32_t from, int splits, float *z)
       if (k < splits) z[j] += part[k][j];
 }
 
-// Four neighbouring values of a matrix's row, the first n of them.
-template <class T>
-__device__ __forceinline__ void get_four(const T *p, int n, float *out) {
-  const bool whole = n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
-  if (whole)
-    load_four<T, true>(p, n, out);
-  else
-    load_four<T, false>(p, n, out);
-}
-template <class T>
-__device__ __forceinline__ void put_four(T *p, int n, const float *x) {
-  const bool whole = n >= 4 && (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
-  if (whole)
-    store_four<T, true>(p, n, x);
-  else
-    store_four<T, false>(p, n, x);
-}
-
 template <bool BLOCKS, bool CODES, bool WITHHOLD>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     rows_split_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ CUtensorMap mx,
@@ -459,6 +560,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // x's staged rows, then w's: the MMA's 128 lanes read on from the former into the latter
   const int x_bytes = a.box_rows * 128, stage_bytes = x_bytes + kTileBytes, stages = min(kMaxStages, kRing / stage_bytes);
   const bool withheld = WITHHOLD && blockIdx.x == 0;
+  const int quarter = warp & 3, column = (warp >> 2) * 32;  // of an adding warp
+  const int nr = min(kRows, a.M - r0);                      // output rows of the tile
+  const bool mine = quarter * 32 < nr;                      // any of them in this warp's lanes
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(full + s, 1);
@@ -466,7 +570,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
     for (int b = 0; b < kSplitSums; ++b) {
       mbar_init(dfull + b, 1);
-      mbar_init(dfree + b, kSplitWarps);
+      mbar_init(dfree + b, 4 * min(4, (nr + 31) / 32));  // the warps with rows
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -477,9 +581,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *holder;
-  const int quarter = warp & 3, column = (warp >> 2) * 32;  // of an adding warp
-  const int nr = min(kRows, a.M - r0);                      // output rows of the tile
-  const bool mine = quarter * 32 < nr;                      // any of them in this warp's lanes
   float2 sums[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) sums[j] = make_float2(0.0f, 0.0f);
@@ -541,7 +642,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       volatile int keep = 0;  // wait for the issued MMAs even when another role gave up
       if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
     }
-  } else if (BLOCKS) {
+  } else if (BLOCKS && mine) {
     RingPlace<kSplitSums> acc;
     const int r = r0 + quarter * 32 + lane;
     const float *xs = a.x_scale + (r < a.M ? r : 0) * a.ldxs;
@@ -559,10 +660,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(dfree + acc.stage);
       };
-      if (mine)
-        add_scaled<32>(tmem + ((uint32_t)(quarter * 32) << 16) + acc.stage * kSplitColumns + column, scale, sums, release);
-      else
-        release();
+      add_scaled<32>(tmem + ((uint32_t)(quarter * 32) << 16) + acc.stage * kSplitColumns + column, scale, sums, release);
       scale = xs_next * ws_next;
     }
   }
@@ -608,46 +706,20 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       const int local = rank + i * splits;
       const int64_t r = r0 + local;
       const uint32_t from = to + (local * kSumPitch + c) * 4;
-      float z[4], u[4], v[4];
+      float z[4], u[4];
       gather_four(from, splits, z);
       if (!BLOCKS) gather_four(from + kOut * 4, splits, u);
-      with_type(a.e.type, [&](auto type) {
+      with_outputs<!BLOCKS>(a.e, a.N, n, [&](auto type, auto whole) {
         using T = decltype(type);
-        const Epilogue &e = a.e;
+        constexpr bool WHOLE = decltype(whole)::value;
+        const Columns columns = columns_at<T, !BLOCKS>(a.e, a.N, f, n);
         if constexpr (!BLOCKS) {
-          auto scaled = [&](float *x, int64_t at) {
-            if (CODES) {
-              const float rs = e.row_scale[r];
-              get_four<float>(e.col_scale + at, n, v);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[j] *= rs * v[j];
-            }
-            if (e.bias) {
-              get_four<T>(static_cast<const T *>(e.bias) + at, n, v);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) x[j] += v[j];
-            }
-            if (e.pre) put_four<T>(static_cast<T *>(e.pre) + r * e.ldp + at, n, x);
-          };
-          scaled(u, (int64_t)a.N + f);
-          scaled(z, f);
-          activate_all<4, sizeof(T) == 2>(e.act, z);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[j] *= u[j];
+          finish_pairs<T, CODES, WHOLE>(a.e, a.N, r, f, n, CODES ? a.e.row_scale[r] : 1.0f, columns, z, u);
         } else {
-          if (e.bias) {
-            get_four<T>(static_cast<const T *>(e.bias) + f, n, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) z[j] += v[j];
-          }
-          activate_all<4, sizeof(T) == 2>(e.act, z);
-          if (e.residual) {
-            get_four<T>(static_cast<const T *>(e.residual) + r * e.ldr + f, n, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) z[j] += v[j];
-          }
+          float residual[4];
+          if (a.e.residual) load_four<T, WHOLE>(static_cast<const T *>(a.e.residual) + r * a.e.ldr + f, n, residual);
+          finish_four<T, WHOLE>(a.e, r, f, n, columns, residual, z);
         }
-        put_four<T>(static_cast<T *>(e.out) + r * e.ldo + f, n, z);
       });
     }
   }
@@ -715,7 +787,7 @@ vcsr_status launch_pair(const RowsGemm &g, cudaStream_t st) {
   a.idesc = instr_desc(g.dtype == VCSR_BF16 ? 1 : 0, 0, 0, 256, kColumns);
   const int grid = 2 * (int)std::min<int64_t>(tiles, sm_count() / 2);
   const auto kernel = take_withhold() ? rows_pair_kernel<BLOCKS, CODES, true> : rows_pair_kernel<BLOCKS, CODES, false>;
-  return launch(kernel, grid, kPairThreads, kPairSmem, 2, st, a, mx, mw);
+  return launch(kernel, grid, kPairThreads<BLOCKS>, kPairSmem, 2, st, a, mx, mw);
 }
 
 template <bool BLOCKS>
