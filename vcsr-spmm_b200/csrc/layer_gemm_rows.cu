@@ -509,6 +509,7 @@ constexpr int kSplitThreads = 32 * (kSplitWarps + 2);
 constexpr int kMaxStages = 10;
 constexpr size_t kSplitSmem = (size_t)kRing + 1024 + 512;
 constexpr int kSplitColumns = 128;  // of an accumulator
+constexpr int kFew = 16;
 constexpr int kSplitSums = 4;       // accumulators of blocks of k
 // Floats from a row of sums to the next: 16-byte accesses of 8 neighbouring rows then
 // touch all banks once.
@@ -539,7 +540,10 @@ __device__ __forceinline__ void gather_four(uint32_t from, int splits, float *z)
       if (k < splits) z[j] += part[k][j];
 }
 
-template <bool BLOCKS, bool CODES, bool WITHHOLD>
+// FEW: up to 16 rows of x, which are the MMA's N side here: a lane is a column of the
+// output, and the MMA costs as much as 16 rows do, not 128 (1 x 8192, k = 4096: 11.0 us in
+// 8 bits with block scales, against 12.2).
+template <bool BLOCKS, bool CODES, bool FEW, bool WITHHOLD>
 __global__ void __launch_bounds__(kSplitThreads, 1)
     rows_split_kernel(const __grid_constant__ RowsArgs a, const __grid_constant__ CUtensorMap mx,
                       const __grid_constant__ CUtensorMap mw, int splits) {
@@ -551,18 +555,21 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   uint32_t *holder = reinterpret_cast<uint32_t *>(drain + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(holder + 1);
   constexpr int kOut = BLOCKS ? 128 : 64;  // output columns of a tile
-  constexpr uint32_t kTmem = BLOCKS ? kSplitSums * kSplitColumns : kSplitColumns;
+  constexpr int kTile = FEW ? kFew : kRows;                // rows of x
+  constexpr int kWidth = FEW ? kFew : kSplitColumns;       // tensor-memory columns of an accumulator
+  constexpr int kColumn = FEW ? kFew : 32;                 // of them, an adding warp's
+  constexpr uint32_t kTmem = BLOCKS ? kSplitSums * kWidth : FEW ? 32 : kWidth;
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = splits > 1 ? (int)cluster_rank() : 0, tile = blockIdx.x / splits;
-  const int f0 = tile % a.tiles_n * kOut, r0 = tile / a.tiles_n * kRows;
+  const int f0 = tile % a.tiles_n * kOut, r0 = tile / a.tiles_n * kTile;
   const int b0 = (int)((int64_t)a.blocks * rank / splits), b1 = (int)((int64_t)a.blocks * (rank + 1) / splits);
   // x's staged rows, then w's: the MMA's 128 lanes read on from the former into the latter
   const int x_bytes = a.box_rows * 128, stage_bytes = x_bytes + kTileBytes, stages = min(kMaxStages, kRing / stage_bytes);
   const bool withheld = WITHHOLD && blockIdx.x == 0;
-  const int quarter = warp & 3, column = (warp >> 2) * 32;  // of an adding warp
-  const int nr = min(kRows, a.M - r0);                      // output rows of the tile
-  const bool mine = quarter * 32 < nr;                      // any of them in this warp's lanes
+  const int quarter = warp & 3, column = (warp >> 2) * kColumn;  // of an adding warp
+  const int nr = min(kTile, a.M - r0);                           // output rows of the tile
+  const bool mine = FEW ? column == 0 : quarter * 32 < nr;       // any of them in this warp
   if (threadIdx.x == 0) {
     for (int s = 0; s < kMaxStages; ++s) {
       mbar_init(full + s, 1);
@@ -570,7 +577,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
     for (int b = 0; b < kSplitSums; ++b) {
       mbar_init(dfull + b, 1);
-      mbar_init(dfree + b, 4 * min(4, (nr + 31) / 32));  // the warps with rows
+      mbar_init(dfree + b, FEW ? 4 : 4 * ((nr + 31) / 32));  // the warps with rows
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -581,9 +588,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   __syncthreads();
   fence_after_sync();
   const uint32_t tmem = *holder;
-  float2 sums[16];
+  float2 sums[kColumn / 2];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) sums[j] = make_float2(0.0f, 0.0f);
+  for (int j = 0; j < kColumn / 2; ++j) sums[j] = make_float2(0.0f, 0.0f);
 
   if (warp == kSplitWarps) {
     if (lane == 0) {
@@ -624,7 +631,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma<1, CODES>(tmem + acc.stage * kSplitColumns, xd + k * 2, wd + k * 2, a.idesc,
+          mma<1, CODES>(tmem + acc.stage * kWidth, (FEW ? wd : xd) + k * 2, (FEW ? xd : wd) + k * 2, a.idesc,
                         ((!BLOCKS && b > b0) || k > 0) ? 1u : 0u);
         mma_commit(empty + s);
         if (BLOCKS && !withheld) mma_commit(dfull + acc.stage);
@@ -644,24 +651,48 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     }
   } else if (BLOCKS && mine) {
     RingPlace<kSplitSums> acc;
-    const int r = r0 + quarter * 32 + lane;
+    // the scales of this lane's row; FEW: of row `lane % 16`, for the lanes to share out
+    const int r = r0 + (FEW ? lane % kFew : quarter * 32 + lane);
     const float *xs = a.x_scale + (r < a.M ? r : 0) * a.ldxs;
     const float *ws = a.w_scale + (int64_t)(f0 / kScaleBlock) * a.ldws;
-    float scale = b0 < b1 ? xs[b0] * ws[b0] : 0.0f;
-    for (int b = b0; b < b1; ++b, acc.next()) {
-      const int ahead = min(b + 1, b1 - 1);
-      const float xs_next = xs[ahead], ws_next = ws[ahead];
-      const bool now = mbar_wait(dfull + acc.stage, acc.full(), abort_flag, kWaitAccFull,
-                                 withheld ? kTestPollLimit : kPollLimit);
-      if (!__all_sync(0xffffffffu, now)) break;
-      fence_after_sync();
-      auto release = [&] {
-        fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dfree + acc.stage);
-      };
-      add_scaled<32>(tmem + ((uint32_t)(quarter * 32) << 16) + acc.stage * kSplitColumns + column, scale, sums, release);
-      scale = xs_next * ws_next;
+    const bool by_four = ((reinterpret_cast<uintptr_t>(a.x_scale) | reinterpret_cast<uintptr_t>(a.w_scale)) & 15) == 0 &&
+                         ((a.ldxs | a.ldws | b0) & 3) == 0;
+    float4 xs_next = four_scales(xs, b0, b1, by_four), ws_next = four_scales(ws, b0, b1, by_four);
+    bool go = true;
+#pragma unroll 1
+    for (int g = b0; g < b1 && go; g += 4) {
+      float scale[4] = {xs_next.x * ws_next.x, xs_next.y * ws_next.y, xs_next.z * ws_next.z, xs_next.w * ws_next.w};
+      xs_next = four_scales(xs, g + 4, b1, by_four);
+      ws_next = four_scales(ws, g + 4, b1, by_four);
+#pragma unroll 1
+      for (int b = g; b < min(g + 4, b1); ++b, acc.next()) {
+        const bool now = mbar_wait(dfull + acc.stage, acc.full(), abort_flag, kWaitAccFull,
+                                   withheld ? kTestPollLimit : kPollLimit);
+        if (!(go = __all_sync(0xffffffffu, now))) break;
+        fence_after_sync();
+        auto release = [&] {
+          fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(dfree + acc.stage);
+        };
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + acc.stage * kWidth + column;
+        if constexpr (FEW) {
+          float z[kFew];
+          tmem_load16(from, z);
+          loaded16(z);
+          release();
+#pragma unroll
+          for (int j = 0; j < kFew; j += 2) {
+            const float2 s = make_float2(__shfl_sync(0xffffffffu, scale[0], j), __shfl_sync(0xffffffffu, scale[0], j + 1));
+            sums[j / 2] = __ffma2_rn(make_float2(z[j], z[j + 1]), s, sums[j / 2]);
+          }
+        } else {
+          add_scaled<32>(from, scale[0], sums, release);
+        }
+        scale[0] = scale[1];
+        scale[1] = scale[2];
+        scale[2] = scale[3];
+      }
     }
   }
   __syncwarp();
@@ -672,24 +703,35 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   // sums over the ring: its copies have landed and its MMAs have read it
   const uint32_t to = smem_u32(ring);
   if (warp < kSplitWarps && mine) {
-    float z[32];
+    float z[kColumn];
     if constexpr (BLOCKS) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
+      for (int j = 0; j < kColumn / 2; ++j) {
         z[2 * j] = sums[j].x;
         z[2 * j + 1] = sums[j].y;
       }
     } else {
-      tmem_load32(tmem + ((uint32_t)(quarter * 32) << 16) + column, z);
+      const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + column;
+      if constexpr (FEW)
+        tmem_load16(from, z);
+      else
+        tmem_load32(from, z);
       loaded16(z);
-      loaded16(z + 16);
+      if (!FEW) loaded16(z + kColumn - 16);
     }
-    const uint32_t row = to + ((quarter * 32 + lane) * kSumPitch + column) * 4;
+    if constexpr (FEW) {
+      const uint32_t at = to + (quarter * 32 + lane) * 4;
 #pragma unroll
-    for (int j = 0; j < 32; j += 4)
-      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(row + j * 4), "f"(z[j]), "f"(z[j + 1]),
-                   "f"(z[j + 2]), "f"(z[j + 3])
-                   : "memory");
+      for (int j = 0; j < kColumn; ++j)
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + j * kSumPitch * 4), "f"(z[j]) : "memory");
+    } else {
+      const uint32_t at = to + ((quarter * 32 + lane) * kSumPitch + column) * 4;
+#pragma unroll
+      for (int j = 0; j < kColumn; j += 4)
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + j * 4), "f"(z[j]), "f"(z[j + 1]),
+                     "f"(z[j + 2]), "f"(z[j + 3])
+                     : "memory");
+    }
   }
   __syncwarp();
   if (splits > 1)
@@ -790,40 +832,40 @@ vcsr_status launch_pair(const RowsGemm &g, cudaStream_t st) {
   return launch(kernel, grid, kPairThreads<BLOCKS>, kPairSmem, 2, st, a, mx, mw);
 }
 
-template <bool BLOCKS>
+template <bool BLOCKS, bool FEW>
 int64_t split_tiles(const RowsGemm &g) {
-  return ceil_div(g.N, BLOCKS ? 128 : 64) * ceil_div(g.M, kRows);
+  return ceil_div(g.N, BLOCKS ? 128 : 64) * ceil_div(g.M, FEW ? kFew : kRows);
 }
-template <bool BLOCKS, bool CODES>
+template <bool BLOCKS, bool CODES, bool FEW>
 int splits_of(const RowsGemm &g) {
-  return choose_splits(reinterpret_cast<const void *>(rows_split_kernel<BLOCKS, CODES, false>), kSplitThreads, kSplitSmem,
-                       split_tiles<BLOCKS>(g), args_of(g).blocks);
+  return choose_splits(reinterpret_cast<const void *>(rows_split_kernel<BLOCKS, CODES, FEW, false>), kSplitThreads,
+                       kSplitSmem, split_tiles<BLOCKS, FEW>(g), args_of(g).blocks);
 }
 
-template <bool BLOCKS, bool CODES>
+template <bool BLOCKS, bool CODES, bool FEW>
 vcsr_status launch_split(const RowsGemm &g, cudaStream_t st) {
   RowsArgs a = args_of(g);
   CUtensorMap mx, mw;
-  a.box_rows = kRows;
-  while (a.box_rows > 16 && a.box_rows / 2 >= g.M) a.box_rows /= 2;
+  a.box_rows = FEW ? kFew : kRows;
+  while (!FEW && a.box_rows / 2 >= g.M) a.box_rows /= 2;
   VCSR_TRY(make_map(&mx, g.x, g.ldx, g.M, g.K, g.dtype, a.box_rows));
   VCSR_TRY(make_map(&mw, g.w, g.ldw, w_rows<BLOCKS>(g), g.K, g.dtype, BLOCKS ? 128 : 64));
   a.tiles_n = (int)ceil_div(a.N, BLOCKS ? 128 : 64);
-  a.tiles_m = (int)ceil_div(a.M, kRows);
-  a.idesc = instr_desc(g.dtype == VCSR_BF16 ? 1 : 0, 0, 0, kRows, kSplitColumns);
-  const int splits = splits_of<BLOCKS, CODES>(g);
-  const int64_t grid = split_tiles<BLOCKS>(g) * splits;
+  a.tiles_m = (int)ceil_div(a.M, FEW ? kFew : kRows);
+  a.idesc = instr_desc(g.dtype == VCSR_BF16 ? 1 : 0, 0, 0, 128, FEW ? kFew : kSplitColumns);
+  const int splits = splits_of<BLOCKS, CODES, FEW>(g);
+  const int64_t grid = split_tiles<BLOCKS, FEW>(g) * splits;
   if (grid > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 thread blocks");
-  const auto kernel = take_withhold() ? rows_split_kernel<BLOCKS, CODES, true> : rows_split_kernel<BLOCKS, CODES, false>;
+  const auto kernel = take_withhold() ? rows_split_kernel<BLOCKS, CODES, FEW, true> : rows_split_kernel<BLOCKS, CODES, FEW, false>;
   return launch(kernel, (int)grid, kSplitThreads, kSplitSmem, splits, st, a, mx, mw, splits);
 }
 
 // Expected microseconds, as in layer_gemm_tc.cu.
 template <bool BLOCKS, bool CODES>
 double split_cost(const RowsGemm &g) {
-  const int splits = splits_of<BLOCKS, CODES>(g);
+  const int splits = splits_of<BLOCKS, CODES, false>(g);
   return 1.2 + (splits > 1 ? 0.7 : 0.0) +
-         (double)ceil_div(split_tiles<BLOCKS>(g) * splits, sm_count()) *
+         (double)ceil_div(split_tiles<BLOCKS, false>(g) * splits, sm_count()) *
              (7.0 + 0.36 * (double)ceil_div(args_of(g).blocks, splits));
 }
 template <bool BLOCKS>
@@ -835,7 +877,8 @@ double pair_cost(const RowsGemm &g) {
 
 template <bool BLOCKS, bool CODES>
 vcsr_status launch_rows(const RowsGemm &g, cudaStream_t st) {
-  return split_cost<BLOCKS, CODES>(g) <= pair_cost<BLOCKS>(g) ? launch_split<BLOCKS, CODES>(g, st)
+  if (g.M <= kFew) return launch_split<BLOCKS, CODES, true>(g, st);
+  return split_cost<BLOCKS, CODES>(g) <= pair_cost<BLOCKS>(g) ? launch_split<BLOCKS, CODES, false>(g, st)
                                                                : launch_pair<BLOCKS, CODES>(g, st);
 }
 
