@@ -355,9 +355,11 @@ __global__ void __launch_bounds__(kPairThreads<BLOCKS>, 1)
   fence_after_sync();
   const uint32_t tmem = *holder;
 
+  // (each part with its own register count, which a common one would limit both to)
   if (warp >= kPairWarps) {
-   if (BLOCKS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFew));
-   if (warp == kPairWarps) {
+    if (BLOCKS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPairFew));
+  }
+  if (warp == kPairWarps) {
     if (lane == 0) {
       // copies of this CTA's halves, complete on the leader's barrier
       RingPlace<kPairStages> at;
@@ -424,8 +426,7 @@ __global__ void __launch_bounds__(kPairThreads<BLOCKS>, 1)
         if (!mbar_wait(drain, 0, &keep, kWaitDrain)) *abort_flag = kWaitDrain;
       }
     }
-   }
-  } else {
+  } else if (warp < kPairWarps) {
     if (BLOCKS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPairMany));
     RingPlace<2> acc;
     const int quarter = warp & 3, half = warp >> 2;  // of the lanes, and of the columns
@@ -900,13 +901,19 @@ vcsr_status launch_split(const RowsGemm &g, cudaStream_t st) {
   return launch(kernel, (int)grid, kSplitThreads, kSplitSmem, splits, st, a, mx, mw, splits);
 }
 
-// Expected microseconds, as in layer_gemm_tc.cu.
-template <bool BLOCKS, bool CODES>
+// Expected microseconds, as in layer_gemm_tc.cu: a launch, then for every round of tiles a
+// fixed part and a part per stage of k.  The best of the three kernels, or within 8% of it,
+// for 132 products of 1 to 2048 rows, 256 to 8192 columns and k of 256 to 4096, gated bf16
+// and block-scaled.  Some of them, up to 16 rows a tile / up to 128 / pairs: gated 17 x 8192,
+// k = 4096 47.8 / 26.6 / 29.8; 128 x 256, k = 1024 7.4 / 9.3 / 11.4; 512 x 8192, k = 1024 - / 41.1 /
+// 17.9; block-scaled 64 x 1024, k = 1024 6.1 / 7.3 / 12.0; 1024 x 4096, k = 4096 - / 37.3 / 25.4.
+template <bool BLOCKS, bool CODES, bool FEW>
 double split_cost(const RowsGemm &g) {
-  const int splits = splits_of<BLOCKS, CODES, false>(g);
+  const int splits = splits_of<BLOCKS, CODES, FEW>(g);
+  const double fixed = FEW ? 4.6 : 5.0 + (double)std::min<int64_t>(g.M, kRows) / 64;
   return 1.2 + (splits > 1 ? 0.7 : 0.0) +
-         (double)ceil_div(split_tiles<BLOCKS, false>(g) * splits, sm_count()) *
-             (7.0 + 0.36 * (double)ceil_div(args_of(g).blocks, splits));
+         (double)ceil_div(split_tiles<BLOCKS, FEW>(g) * splits, sm_count()) *
+             (fixed + 0.36 * (double)ceil_div(args_of(g).blocks, splits));
 }
 template <bool BLOCKS>
 double pair_cost(const RowsGemm &g) {
@@ -917,9 +924,10 @@ double pair_cost(const RowsGemm &g) {
 
 template <bool BLOCKS, bool CODES>
 vcsr_status launch_rows(const RowsGemm &g, cudaStream_t st) {
-  if (g.M <= kFew) return launch_split<BLOCKS, CODES, true>(g, st);
-  return split_cost<BLOCKS, CODES>(g) <= pair_cost<BLOCKS>(g) ? launch_split<BLOCKS, CODES, false>(g, st)
-                                                               : launch_pair<BLOCKS, CODES>(g, st);
+  const double few = split_cost<BLOCKS, CODES, true>(g), split = split_cost<BLOCKS, CODES, false>(g),
+               pair = pair_cost<BLOCKS>(g);
+  if (g.M <= kFew || (few <= split && few <= pair)) return launch_split<BLOCKS, CODES, true>(g, st);
+  return split <= pair ? launch_split<BLOCKS, CODES, false>(g, st) : launch_pair<BLOCKS, CODES>(g, st);
 }
 
 }  // namespace
