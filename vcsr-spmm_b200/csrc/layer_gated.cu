@@ -138,18 +138,33 @@ __global__ void __launch_bounds__(kDzWarps * 32, 3)
   }
 }
 
+// How the gradient's pass covers its matrices: columns of a block, and chunks of rows (the
+// partial rows of dbias), which fill three blocks an SM once.
+struct DzShape {
+  bool vec;
+  int64_t across, chunks;
+};
+DzShape dz_shape(const vcsr_gated_linear_grad_args *a) {
+  const int64_t v = 16 / (int64_t)type_size(a->dtype);
+  DzShape s;
+  s.vec = a->N % v == 0 && a->lddy % v == 0 && a->ldp % v == 0 && aligned(a->dy, 16) && aligned(a->pre, 16);
+  s.across = ceil_div(a->N, s.vec ? 32 * v : 32);
+  s.chunks = std::max<int64_t>(1, std::min(ceil_div(a->M, 32), sm_count() * 3 / s.across));
+  return s;
+}
+
 template <class T>
 void launch_dz(const vcsr_gated_linear_grad_args *a, void *to, int64_t lddz, float *partial, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const T *dy = static_cast<const T *>(a->dy), *pre = static_cast<const T *>(a->pre);
   T *dz = static_cast<T *>(to);
-  const bool vec = a->N % V == 0 && a->lddy % V == 0 && a->ldp % V == 0 && aligned(dy, 16) && aligned(pre, 16);
-  const int64_t chunks = dz_chunks(a->M, a->N), chunk = ceil_div(a->M, chunks);
-  const dim3 grid((unsigned)ceil_div(a->N, vec ? 32 * V : 32), (unsigned)chunks);
+  const DzShape s = dz_shape(a);
+  const int64_t chunk = ceil_div(a->M, s.chunks);
+  const dim3 grid((unsigned)s.across, (unsigned)s.chunks);
   auto run = [&](auto kernel) {
     kernel<<<grid, kDzWarps * 32, 0, st>>>(dy, a->lddy, pre, a->ldp, dz, lddz, a->M, a->N, chunk, a->act, partial);
   };
-  if (vec)
+  if (s.vec)
     run(partial ? gated_dz_kernel<T, V, true> : gated_dz_kernel<T, V, false>);
   else
     run(partial ? gated_dz_kernel<T, 1, true> : gated_dz_kernel<T, 1, false>);
@@ -256,7 +271,7 @@ GradPlan grad_plan(const vcsr_gated_linear_grad_args *a) {
   GradPlan p;
   p.lddz = packed_pitch(2 * a->N, a->dtype);
   if (a->dx || a->dw) p.dz = round_up((size_t)a->M * p.lddz * type_size(a->dtype));
-  if (a->dbias) p.partial = round_up((size_t)dz_chunks(a->M, a->N) * 2 * a->N * sizeof(float));
+  if (a->dbias) p.partial = round_up((size_t)dz_shape(a).chunks * 2 * a->N * sizeof(float));
   if (a->K > 0) {
     if (a->dw) p.x = packed(a->x, a->ldx, a->M, a->K, a->dtype);
     if (a->dx) p.w = packed(a->w, a->ldw, 2 * a->N, a->K, a->dtype);
@@ -294,7 +309,7 @@ vcsr_status gated_linear_grad(const vcsr_gated_linear_grad_args *a, cudaStream_t
   for_type(a->dtype, [&](auto t) { launch_dz<decltype(t)>(a, dz, p.lddz, partial, st); });
   VCSR_CUDA(cudaGetLastError());
   Prepare before(ws + p.dz + p.partial);
-  if (a->dbias) before.column_sums(partial, (int)dz_chunks(a->M, a->N), N2, a->dbias);
+  if (a->dbias) before.column_sums(partial, (int)dz_shape(a).chunks, N2, a->dbias);
   const void *x = before.matrix(p.x, a->x, a->ldx, a->M, a->K, a->dtype);
   const void *w = before.matrix(p.w, a->w, a->ldw, N2, a->K, a->dtype);
   VCSR_TRY(before.run(a->dtype, st));
