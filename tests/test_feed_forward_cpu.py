@@ -75,7 +75,8 @@ def gated(**kw):
     (1, "scales", dict(x_scale=P)), (1, "need x_scale", dict(dtype=3)), (1, "pitch of pre", dict(pre=P, ldp=7)),
     (1, "bias is not aligned", dict(bias=P + 1)), (1, "x_scale is not aligned", dict(dtype=3, x_scale=P + 2, w_scale=P)),
     (1, "workspace", dict(x=P + 2)), (1, "workspace", dict(dtype=0, out_dtype=0)),
-    (1, "workspace", dict(dtype=0, out_dtype=0, workspace=P + 16, workspace_bytes=1 << 20))])
+    (1, "workspace", dict(dtype=0, out_dtype=0, workspace=P + 16, workspace_bytes=1 << 20)),
+    (8, "2^31 - 513", dict(M=(1 << 31) - 512))])
 def test_gated_linear_refuses(status, text, kw):
     refused(status, "vcsr_gated_linear", gated(**kw), text)
 
@@ -114,7 +115,8 @@ def block(**kw):
     (1, "pitch of w ", dict(ldw=0)), (1, "x_scale is NULL", dict(x_scale=None)), (1, "pitch of x_scale", dict(ldxs=1)),
     (1, "pitch of w_scale", dict(ldws=1)), (1, "w_scale is not aligned", dict(w_scale=P + 1)),
     (1, "pitch of residual", dict(residual=P, ldr=3)), (1, "bias is not aligned", dict(bias=P + 2)),
-    (1, "y is NULL", dict(y=None)), (1, "workspace", dict(x=P + 1)), (1, "workspace", dict(ldw=257))])
+    (1, "y is NULL", dict(y=None)), (1, "workspace", dict(x=P + 1)), (1, "workspace", dict(ldw=257)),
+    (8, "2^31 - 513", dict(M=(1 << 31) - 512)), (8, "2^31 - 513", dict(N=(1 << 31) - 1, ldy=1 << 31))])
 def test_block_linear_refuses(status, text, kw):
     refused(status, "vcsr_block_linear", block(**kw), text)
 
