@@ -36,7 +36,7 @@ constexpr int kMostHeld = V == 1 ? 16 : 32;
 template <int V, int E>
 constexpr int kNormBlock = E == kMostHeld<V> ? 1024 : 512;
 template <int V, int E, bool RAGGED>
-constexpr int kNormBlocksPerSm = V == 8 && E == 16 && !RAGGED ? 3 : V == 8 && E <= 16 ? 2 : 1;
+constexpr int kNormBlocksPerSm = V == 8 && E == 16 && !RAGGED ? 3 : E <= 16 && (V == 8 || (V > 1 && RAGGED)) ? 2 : 1;
 
 struct NormArgs {
   int64_t rows, dim;
@@ -55,6 +55,15 @@ __device__ __forceinline__ void with_weight_type(int w_dtype, F &&f) {
     f(float{});
   else
     f(T{});
+}
+
+// row_load that looks at single values only in a row's first and last vector.
+template <class X, int V, bool RAGGED>
+__device__ __forceinline__ void row_load_ends(const X *row, int at, int dim, bool whole, float *out) {
+  if (RAGGED && whole && at >= 0 && at + V <= dim)
+    row_load<X, V, false>(row, at, dim, true, out);
+  else
+    row_load<X, V, RAGGED>(row, at, dim, whole, out);
 }
 
 // One row per team; E values per thread, V at a time.
@@ -90,14 +99,14 @@ __global__ void __launch_bounds__(kNormBlock<V, E>, (kNormBlocksPerSm<V, E, RAGG
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
     const int at = (t + i * team) * V - shift;
-    row_load<T, V, RAGGED>(x, at, live ? dim : 0, whole(at), s + i * V);
+    row_load_ends<T, V, RAGGED>(x, at, live ? dim : 0, whole(at), s + i * V);
   }
   if (a.residual) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int at = (t + i * team) * V - shift;
       float v[V + 1];
-      row_load<T, V, RAGGED>(r, at, live ? dim : 0, whole(at), v);
+      row_load_ends<T, V, RAGGED>(r, at, live ? dim : 0, whole(at), v);
       pairs(s + i * V, V, [&](float2 u, int j) { return __fadd2_rn(u, make_float2(v[j], v[j + 1])); });
     }
   }
