@@ -341,3 +341,31 @@ def test_layernorm_refusals():
     refused(1, L.layernorm_backward, x, None, v, out.mean, out.rstd)
     refused(5, L.layernorm_backward, x, x, None, out.mean, out.rstd, weight_dtype=BF16)
     refused(5, L.layernorm_backward, x, x, v, out.mean, out.rstd, weight_dtype=BF16)
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", [(700, 1000), (333, 1001), (300, 5120), (5, 40000)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layernorm_gradient_over_dsum(rows, dim, dtype):
+    """dx in dsum's own memory, as the C entry point allows."""
+    s, dy, ds = (randn(rows, dim, dtype=dtype, seed=i) for i in range(3))
+    w = randn(dim, dtype=dtype, seed=3)
+    n = L.layernorm(s, w, save_stats=True)
+    want = L.layernorm_backward(dy, s, w, n.mean, n.rstd, dsum=ds).dx
+    a = V._LayernormGradArgs(rows, dim, dy.data_ptr(), dim, s.data_ptr(), dim, w.data_ptr(), n.mean.data_ptr(),
+                             n.rstd.data_ptr(), ds.data_ptr(), dim, ds.data_ptr(), dim, None, None, None, 0,
+                             L._TYPE[dtype], L._TYPE[dtype], L._TYPE[dtype])
+    assert V.lib().vcsr_layernorm_grad(a, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(ds, want)
+
+
+@gpu
+def test_layernorm_of_some_rows():
+    """A row's results are those it has among others (within one rounding: the sums of few
+    rows are made by more threads), and the same bits whole and in a view."""
+    x, w, b = randn(4000, 1024, dtype=BF16, seed=1), randn(1024, seed=2), randn(1024, seed=3)
+    for rows in (slice(0, 1), slice(17, 20), slice(3999, 4000)):
+        part = L.layernorm(x[rows], w, b, save_stats=True)
+        close(part.y, d(L.layernorm(x, w, b).y[rows]), 2.0 ** -8 * d(part.y).abs())
+        again = L.layernorm(x[rows].clone(), w, b, save_stats=True)
+        assert torch.equal(again.y, part.y) and torch.equal(again.mean, part.mean) and torch.equal(again.rstd, part.rstd)

@@ -10,6 +10,8 @@
 // Gradient: dg = dy u act'(g) and du = dy act(g) are the two halves of dz's rows, rounded to
 // the operands' type, made in one pass with dbias' partial sums of the unrounded ones; then
 // dx = dz w and dw = dz^T x are single products over 2N values of k and for 2N rows.
+// 4096 x 8192, k = 4096 bf16: dz 52 us (335 MB, 6.4 TB/s), the products 392 each (1,402 TFLOP/s);
+// FP32 1024 x 2048, k = 1024 with pre 84 us, of which the pass over pre takes 15.
 #include <algorithm>
 
 #include "layer_gemm_rows.cuh"
@@ -84,6 +86,8 @@ void launch_combine(const void *z, int64_t ldz, void *y, int64_t ldy, int64_t M,
 // Block (c, r): columns [c * 32 V, ...) of both halves, a chunk of rows; a lane holds V
 // columns of each, the warps take every 8th row of the chunk.  partial: one row of 2N sums
 // per chunk.
+// Three blocks an SM in one round: with two 79 us (4096 x 8192 bf16, dbias alone), three 66, and
+// 50 with chunks for just that many.
 template <class T, int V, bool SUMS>
 __global__ void __launch_bounds__(kDzWarps * 32, 3)
     gated_dz_kernel(const T *dy, int64_t lddy, const T *pre, int64_t ldp, T *dz, int64_t lddz, int64_t M, int64_t N,
