@@ -369,3 +369,23 @@ def test_layernorm_of_some_rows():
         close(part.y, d(L.layernorm(x, w, b).y[rows]), 2.0 ** -8 * d(part.y).abs())
         again = L.layernorm(x[rows].clone(), w, b, save_stats=True)
         assert torch.equal(again.y, part.y) and torch.equal(again.mean, part.mean) and torch.equal(again.rstd, part.rstd)
+
+
+def stats(s):
+    mean = s.float().mean(1)
+    return mean, 1 / torch.sqrt((s.float() - mean[:, None]).square().mean(1) + 1e-5)
+
+
+@gpu
+@pytest.mark.parametrize("dim", [4104, 4608, 5120, 5632])
+@pytest.mark.parametrize("x_dtype,dy_dtype", [(BF16, BF16), (F16, F32), (F32, F32)])
+def test_layernorm_backward_by_width(dim, x_dtype, dy_dtype):
+    """Widths whose teams take 264 to 352 threads, two or one of them a block, for several rows each."""
+    s, ds = randn(700, dim, dtype=x_dtype, seed=1), randn(700, dim, dtype=x_dtype, seed=4)
+    dy, w = randn(700, dim, dtype=dy_dtype, seed=2), randn(dim, seed=3)
+    mean, rstd = stats(s)
+    for dsum in (None, ds):
+        g = L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum)
+        check_grad(dy, s, w, mean, rstd, dsum, g)
+        again = L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum)
+        assert all(torch.equal(a, b) for a, b in zip(g, again))

@@ -20,8 +20,9 @@
 // their sums in shared memory, blocks write one partial row of each, and a second kernel
 // adds the partial rows in block order (no atomics: the same result on every run).
 // 8191 x 5120 bf16 with dsum 77 us (4.4 TB/s), 16384 x 4096 109 (4.9), 60000 x 1000 FP32 157
-// (6.1): bound by instructions (60% of issue slots) at 16 to 20 warps an SM, whose registers
-// hold the sums.
+// (6.1): bound by instructions (60% of issue slots) at few warps an SM, whose registers
+// hold the sums: 20 at 5,120 16-bit values, 16 at 4,096 and at 8,192, 11 just past 5,120 and 9
+// just past 8,192.
 #include <algorithm>
 
 #include "layer_rows.cuh"
@@ -863,9 +864,12 @@ vcsr_status launch_grad(const GradArgs &a, int &blocks, cudaStream_t st) {
       return 2 * value * held * team_of(ceil_div(dim, V), held / V) <= kGradRing;
     };
     if (dim <= 16 * 512 && two_rows_fit(16)) {
-      // two teams an SM where 512 threads hold only one
-      if constexpr (!RAGGED)
-        if (team_of(ceil_div(dim, V), 16 / V) == 320)
+      // 16-bit rows: 640 threads a block where they hold two teams and 512 only one (8191 x
+      // 4608 bf16 with dsum 74 us against 99, 8191 x 5120 77 against 100, with FP32 dy 93 against 99
+      // and 96 against 102).  Not FP32 rows, whose one team keeps HBM busier with its 128 registers
+      // a thread (8191 x 4608 107 us against 123 in two teams, 8191 x 5120 111 against 125).
+      if constexpr (V == 8 && !RAGGED)
+        if (const int team = team_of(ceil_div(dim, V), 16 / V); 2 * team > 512 && 2 * team <= 640)
           return run(integral_constant<int, 16>{}, integral_constant<int, 640>{});
       return run(integral_constant<int, 16>{}, integral_constant<int, 512>{});
     }
