@@ -299,3 +299,23 @@ def test_gated_refusals():
     refused(5, L.gated_linear_backward, x.to(E4M3), x, w, pre)
     refused(1, L.gated_linear_backward, randn(4, 5), x, w, pre)
     refused(5, L.gated_linear_backward, randn(4, 6), x, w, pre, act="tanh")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("M,N", [(4, 8), (300, 77)])
+def test_gated_bias_gradient_over_no_k(dtype, act, M, N):
+    """K = 0: dx and dw have no values, dbias sums dz as ever (bound as in check_backward)."""
+    dy, pre = randn(M, N, dtype=dtype, seed=1), randn(M, 2 * N, dtype=dtype, seed=2)
+    x, w = torch.empty(M, 0, device="cuda", dtype=dtype), torch.empty(2 * N, 0, device="cuda", dtype=dtype)
+    for need in (True, False):
+        torch.full((4096,), 5.0, device="cuda")  # in memory that held something else
+        got = L.gated_linear_backward(dy, x, w, pre, act=act, need_dx=need, need_dw=need)
+        g, u = d(pre)[:, :N], d(pre)[:, N:]
+        dz = torch.cat([d(dy) * u * slope_ref(g, act), d(dy) * act_ref(g, act)], 1)
+        unit = 16 * U + (2.0 ** -12 if dtype != F32 else 0)
+        off = unit * torch.cat([(d(dy) * u).abs() * (1 + g.abs()), d(dy).abs() * g.abs()], 1)
+        close(got.db, dz.sum(0), (off + (M + 4) * U * dz.abs()).sum(0))
+        if need:
+            assert got.dx.shape == (M, 0) and got.dw.shape == (2 * N, 0)

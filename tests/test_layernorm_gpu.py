@@ -389,3 +389,51 @@ def test_layernorm_backward_by_width(dim, x_dtype, dy_dtype):
         check_grad(dy, s, w, mean, rstd, dsum, g)
         again = L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum)
         assert all(torch.equal(a, b) for a, b in zip(g, again))
+
+
+# rows for several turns of every team: vectors cut at memory boundaries ((6001, 333) in teams of
+# less than a warp, (700, 9001) with 32 values a thread), and short rows
+MANY_TURNS = [(2001, 1501), (6001, 333), (9001, 17), (700, 9001), (1201, 5121)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", MANY_TURNS)
+@pytest.mark.parametrize("x_dtype,dy_dtype", [(F32, F32), (BF16, BF16), (F32, BF16), (F16, F32)])
+def test_layernorm_backward_odd_rows_in_many_turns(rows, dim, x_dtype, dy_dtype):
+    s, ds = randn(rows, dim, dtype=x_dtype, seed=1), randn(rows, dim, dtype=x_dtype, seed=4)
+    dy, w = randn(rows, dim, dtype=dy_dtype, seed=2), randn(dim, dtype=x_dtype, seed=3)
+    mean, rstd = stats(s)
+    for dsum in (None, ds):
+        g = L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum)
+        check_grad(dy, s, w, mean, rstd, dsum, g)
+        again = L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum)
+        assert all(torch.equal(a, b) for a, b in zip(g, again))
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", [(3001, 1001), (1200, 200), (700, 5000), (9001, 17)])
+@pytest.mark.parametrize("x_dtype,dy_dtype", [(F32, F32), (BF16, BF16), (F16, F32)])
+def test_layernorm_backward_single_values_in_many_turns(rows, dim, x_dtype, dy_dtype):
+    """s a value further apart than dy and dx: rows that are off 16 bytes unlike, for teams of one
+    warp and more."""
+    s = randn(rows, dim, dtype=x_dtype, seed=1, pad=1)
+    dy, w = randn(rows, dim, dtype=dy_dtype, seed=2), randn(dim, seed=3)
+    ds = randn(rows, dim, dtype=x_dtype, seed=4)
+    mean, rstd = stats(s)
+    for dsum in (None, ds):
+        check_grad(dy, s, w, mean, rstd, dsum, L.layernorm_backward(dy, s, w, mean, rstd, dsum=dsum))
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", [(700, 4096), (700, 5121), (2600, 1000), (2500, 1001)])
+@pytest.mark.parametrize("x_dtype,y_dtype", [(BF16, BF16), (F16, F32), (BF16, E4M3), (F32, BF16)])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_layernorm_of_rows_that_fill_the_gpu(rows, dim, x_dtype, y_dtype, pad):
+    """16 and 32 values a thread, which few rows do not get: whole, ragged, and single values (a
+    residual further apart than x)."""
+    x, r = randn(rows, dim, dtype=x_dtype, seed=1), randn(rows, dim, dtype=x_dtype, seed=2, pad=pad)
+    w, b = randn(dim, dtype=x_dtype, seed=3), randn(dim, dtype=x_dtype, seed=4)
+    if y_dtype == E4M3:
+        check_codes(L.layernorm(x, w, b, residual=r, out_dtype=E4M3), *ref(x, w, b, r, 1e-5)[3::3])
+    else:
+        check(x, w, b, r, 1e-5, y_dtype)
