@@ -220,3 +220,19 @@ def test_fake_shapes():
         assert torch.ops.vcsr.gated_linear(x, w, None, "silu", False)[1].shape == (0, 10)
         dx, dw, db = torch.ops.vcsr.gated_linear_backward(y, x, w, pre, "silu", True, True, False)
         assert dx.shape == (6, 16) and dw.shape == (10, 16) and db.shape == (0,) and dw.is_contiguous()
+
+
+@pytest.mark.parametrize("fake", [False, True])
+def test_layernorm_refuses_codes_without_scales(fake):
+    """The operator returns no scales: 8-bit rows from it could not be read."""
+    from contextlib import nullcontext
+
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from vcsr_b200 import VcsrError
+    with FakeTensorMode() if fake else nullcontext():
+        x, v = torch.ones(4, 16), torch.ones(16)
+        for call in (lambda t: torch_ops.layernorm(x, v, v, out_dtype=t),
+                     lambda t: torch.ops.vcsr.layernorm(x, v, None, x.clone(), 1e-6, t)):
+            with pytest.raises(VcsrError) as e:
+                call(torch.float8_e4m3fn)
+            assert e.value.status == 5

@@ -25,7 +25,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import Plan, layers
+from . import Plan, VcsrError, layers
 
 _plans: dict[int, Plan] = {}
 _ids = itertools.count(1)
@@ -134,11 +134,18 @@ def rmsnorm(x, weight, residual=None, eps=1e-6, out_dtype=None):
     return y, (x if residual is None else s)
 
 
+def _floats(out_dtype):
+    """Refuses 8-bit codes, whose scales these operators do not return."""
+    if out_dtype == torch.float8_e4m3fn:
+        raise VcsrError(layers.UNSUPPORTED, "8-bit rows need their scales: call layers.layernorm")
+
+
 @torch.library.custom_op("vcsr::layernorm", mutates_args=())
 def _layernorm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
                residual: Optional[torch.Tensor], eps: float, out_dtype: torch.dtype
                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, s, mean, rstd) of layers.layernorm; s has no rows without a residual (s is x then)."""
+    _floats(out_dtype)
     out = layers.layernorm(x, weight, bias, residual=residual, eps=eps, out_dtype=out_dtype,
                            save_stats=True)
     return (out.y, out.sum if residual is not None else x.new_empty((0, x.shape[1])), out.mean,
@@ -147,6 +154,7 @@ def _layernorm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[t
 
 @_layernorm.register_fake
 def _(x, weight, bias, residual, eps, out_dtype):
+    _floats(out_dtype)
     rows = x.shape[0] if residual is not None else 0
     return (x.new_empty(x.shape, dtype=out_dtype), x.new_empty((rows, x.shape[1])),
             x.new_empty(x.shape[0], dtype=torch.float32), x.new_empty(x.shape[0], dtype=torch.float32))
@@ -195,7 +203,7 @@ _layernorm.register_autograd(_layernorm_grad, setup_context=_layernorm_setup)
 
 def layernorm(x, weight=None, bias=None, residual=None, eps=1e-5, out_dtype=None):
     """(y, s) of layers.layernorm, s = x + residual, with gradients of x, weight, bias and
-    residual (16- and 32-bit y)."""
+    residual (16- and 32-bit y; an 8-bit one is refused, call layers.layernorm)."""
     y, s, _, _ = _layernorm(x, weight, bias, residual, eps, out_dtype or x.dtype)
     return y, (x if residual is None else s)
 
