@@ -108,7 +108,7 @@ struct BlockArgs {
   int64_t ldx, ldo, lds, rows;
   int dim, across;     // values and blocks of a row
   int x_bytes, o_bytes;  // that neighbouring values can be moved by
-  int block_rows, dtype;
+  int block_rows;
 };
 
 // A thread's place: groups of 8 lanes take neighbouring blocks of columns, and rows where
@@ -235,17 +235,6 @@ void launch_blocks(K kernel, const BlockArgs &a, cudaStream_t st) {
   kernel<<<dim3((unsigned)columns, (unsigned)std::min<int64_t>(rows, 65535)), 256, 0, st>>>(a, wide);
 }
 
-// f(T{}) for the element type named by `type`, which is F32, BF16 or F16.
-template <class F>
-void for_type(int type, F &&f) {
-  if (type == VCSR_F32)
-    f(float{});
-  else if (type == VCSR_BF16)
-    f(__nv_bfloat16{});
-  else
-    f(__half{});
-}
-
 vcsr_status quantize(const void *x, int64_t ldx, int64_t rows, int64_t dim, int x_dtype, int block_rows, void *codes,
                      int64_t ldc, float *scale, int64_t lds, cudaStream_t st) {
   VCSR_TRY(check_blocks(rows, dim, block_rows));
@@ -255,7 +244,7 @@ vcsr_status quantize(const void *x, int64_t ldx, int64_t rows, int64_t dim, int 
   VCSR_TRY(check_matrix("codes", codes, ldc, dim, VCSR_E4M3, false));
   VCSR_TRY(check_matrix("scale", scale, lds, ceil_div(dim, kScaleBlock), VCSR_F32, false));
   const BlockArgs a{x, codes, scale, ldx, ldc, lds, rows, (int)dim, (int)ceil_div(dim, kScaleBlock),
-                    access_bytes(x, ldx, x_dtype), access_bytes(codes, ldc, VCSR_E4M3), block_rows, x_dtype};
+                    access_bytes(x, ldx, x_dtype), access_bytes(codes, ldc, VCSR_E4M3), block_rows};
   const int64_t tiles = a.across * ceil_div(rows, kScaleBlock);
   if (block_rows != 1 && tiles > 0x7fffffffll) return fail(VCSR_ERR_RANGE, "more than 2^31 - 1 blocks");
   for_type(x_dtype, [&](auto t) {
@@ -278,7 +267,7 @@ vcsr_status dequantize(const void *codes, int64_t ldc, const float *scale, int64
   VCSR_TRY(check_matrix("scale", scale, lds, ceil_div(dim, kScaleBlock), VCSR_F32, false));
   VCSR_TRY(check_matrix("out", out, ldo, dim, out_dtype, false));
   const BlockArgs a{codes, out, const_cast<float *>(scale), ldc, ldo, lds, rows, (int)dim, (int)ceil_div(dim, kScaleBlock),
-                    access_bytes(codes, ldc, VCSR_E4M3), access_bytes(out, ldo, out_dtype), block_rows, out_dtype};
+                    access_bytes(codes, ldc, VCSR_E4M3), access_bytes(out, ldo, out_dtype), block_rows};
   for_type(out_dtype, [&](auto t) { launch_blocks(dequantize_blocks_kernel<decltype(t)>, a, st); });
   VCSR_CUDA(cudaGetLastError());
   return VCSR_OK;

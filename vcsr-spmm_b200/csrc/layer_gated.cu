@@ -174,17 +174,6 @@ void launch_dz(const vcsr_gated_linear_grad_args *a, void *to, int64_t lddz, flo
     run(partial ? gated_dz_kernel<T, 1, true> : gated_dz_kernel<T, 1, false>);
 }
 
-// f(T{}) for the element type named by `type`, which is F32, BF16 or F16.
-template <class F>
-void for_type(int type, F &&f) {
-  if (type == VCSR_F32)
-    f(float{});
-  else if (type == VCSR_BF16)
-    f(__nv_bfloat16{});
-  else
-    f(__half{});
-}
-
 vcsr_status check_gated_sizes(int64_t M, int64_t N, int64_t K) {
   VCSR_TRY(check_sizes(M, N, K));
   if (N > 0x3fffffffll) return fail(VCSR_ERR_RANGE, "2 N above 2^31 - 1");

@@ -46,7 +46,7 @@ struct NormArgs {
   float *mean, *rstd, *scale;
   int64_t ldx, ldr, ldy, lds;
   float eps;
-  int x_dtype, w_dtype, y_dtype;
+  int w_dtype, y_dtype;
 };
 
 // f(W{}) for the type of weight and bias, T or float.
@@ -916,7 +916,7 @@ vcsr_status layernorm(const vcsr_layernorm_args *a, cudaStream_t st) {
   VCSR_TRY(check_matrix("rstd", a->rstd, 1, 1, VCSR_F32, true));
   VCSR_TRY(check_matrix("scale", a->scale, 1, 1, VCSR_F32, true));
   const NormArgs k{a->rows, a->dim,  a->x,     a->residual, a->weight, a->bias, a->y,   a->sum,     a->mean,    a->rstd,
-                   a->scale, a->ldx, a->ldr,   a->ldy,      a->lds,    a->eps,  a->x_dtype, a->w_dtype, a->y_dtype};
+                   a->scale, a->ldx, a->ldr,   a->ldy,      a->lds,    a->eps,  a->w_dtype, a->y_dtype};
   const int v = a->x_dtype == VCSR_F32 ? 4 : 8;
   const Access how = with_vectors(
       access_of(a->rows, a->dim, v, a->weight, {{a->x, a->ldx, a->x_dtype}, {a->residual, a->ldr, a->x_dtype},

@@ -69,6 +69,13 @@ __global__ void __launch_bounds__(kDzWarps * 32, 4)  // dz_chunks counts on four
   }
 }
 
+// Enough chunks of at least 32 rows for four blocks an SM that take 256 columns each: the
+// partial rows of dbias.
+int64_t dz_chunks(int64_t M, int64_t N) {
+  const int64_t across = ceil_div(N, 256);
+  return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, across)));
+}
+
 template <class T>
 void launch_dz(const vcsr_linear_grad_args *a, T *dz, int64_t lddz, float *partial, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
@@ -133,11 +140,6 @@ __global__ void __launch_bounds__(256) empty_sum_kernel(const __grid_constant__ 
 }
 
 }  // namespace
-
-int64_t dz_chunks(int64_t M, int64_t N) {
-  const int64_t across = ceil_div(N, 256);
-  return std::max<int64_t>(1, std::min(ceil_div(M, 32), ceil_div((int64_t)sm_count() * 4, across)));
-}
 
 vcsr_status Prepare::run(int dtype, cudaStream_t st) {
   const int rows = jobs.packs + (jobs.dbias ? 1 : 0);

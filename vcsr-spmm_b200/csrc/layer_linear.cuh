@@ -75,10 +75,18 @@ struct Prepare {
   vcsr_status run(int dtype, cudaStream_t st);
 };
 
-// Enough chunks of at least 32 rows for four blocks an SM that take 256 columns each: the
-// partial rows of dbias.
-int64_t dz_chunks(int64_t M, int64_t N);
-constexpr int kDzWarps = 8;
+constexpr int kDzWarps = 8;  // of the blocks that make dz
+
+// f(T{}) for the element type named by `type`, which is F32, BF16 or F16.
+template <class F>
+inline void for_type(int type, F &&f) {
+  if (type == VCSR_F32)
+    f(float{});
+  else if (type == VCSR_BF16)
+    f(__nv_bfloat16{});
+  else
+    f(__half{});
+}
 
 // The product by the kernel for its type; over no k, the epilogue of zeros.
 vcsr_status launch_gemm(const Gemm &g, cudaStream_t st);
