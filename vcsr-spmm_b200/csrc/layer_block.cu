@@ -4,11 +4,13 @@
 //
 // Making codes is bound by HBM and by instructions: a block's values stay in registers
 // between its largest magnitude and their codes, so x is read once.  16384 x 4096 bf16 by rows
-// 40 us (5.0 TB/s; 73% of issue slots), FP32 51 (6.6 TB/s), 16384 x 8192 FP32 by 128 x 128 103 (6.5);
-// values of 16384 x 4096 codes as bf16 40 (5.1).  Eight lanes take a block: with sixteen, whose
-// exchanges and scales serve half as many values, rows took 63 us and values 60.  scale is the largest magnitude times 1/448
-// and a code x / scale, each rounded once to nearest (CodeScale gives correctly rounded
-// quotients), so codes are those of the same formula in any IEEE arithmetic.
+// 42 us (4.8 TB/s; 72% of issue slots), FP32 52 (6.5 TB/s), 16384 x 8192 by 128 x 128 FP32 107
+// (6.3), bf16 112 (3.6); values of 16384 x 4096 codes as bf16 43 (4.7).  Rows off 16 bytes are
+// moved by their elements: 16384 x 4097 bf16 180 us, its values 374.  Eight lanes take a block:
+// with sixteen, whose exchanges and scales serve half as many values, rows took 63 us and values
+// 60.  scale is the largest magnitude times 1/448 and a code x / scale, each rounded once to
+// nearest (CodeScale gives correctly rounded quotients), so codes are those of the same formula
+// in any IEEE arithmetic.
 #include <algorithm>
 
 #include "layer_gemm_rows.cuh"

@@ -17,9 +17,9 @@
 // CTA of the pair, or 256 columns.  Two accumulators alternate: from tile to tile (gated),
 // or from one block of k to the next, while eight warps add up the one before in 128
 // registers a thread (the loading and issuing warps give theirs up for that).
-// Gated bf16 8192 x 8192, k = 4096: 690 us (1,593 TFLOP/s), 711 with both factors kept; the tensor
-// pipe is 89% busy.  Block-scaled 8192 x 8192, k = 4096: 292 us (1,885 TFLOP/s), 372 to 385 with a
-// residual from memory.  There a block of k takes 0.51 us: two accumulators' way from the
+// Gated bf16 8192 x 8192, k = 4096: 665 to 690 us (1,593 TFLOP/s and more, by the power cap), 707
+// to 734 with both factors kept; the tensor pipe is 88% busy.  Block-scaled 8192 x 8192, k = 4096:
+// 292 us (1,885 TFLOP/s), 335 to 385 with a residual from memory.  There a block of k takes 0.51 us: two accumulators' way from the
 // MMAs to the adding warps and back alone takes 0.39, reading them 0.07, adding 0.06 (in scratch
 // copies without these parts); a tile's epilogue, which no other tile's sums can run under for
 // want of registers, 3.4 us of 21.  Not kept, all the same or slower: 32 columns at a time,

@@ -8,9 +8,9 @@
 // their mean (one sum of squares less the mean's square would cancel where the mean is
 // large against the spread).  Teams, vector access and ragged rows are those of
 // layer_norm.cu; rows past a block's registers are walked by one block in passes.
-// 16384 x 4096 bf16 with residual 90 us (6.0 TB/s), 62451 x 128 FP32 to bf16 19.7 (5.7 TB/s);
-// for 16-bit rows the instructions come close to the bandwidth (70% of issue slots), so
-// two values are worked on at a time.
+// 16384 x 4096 bf16 with residual 92 us (5.9 TB/s), to 8 bits 100 (4.7), 62451 x 128 FP32 to
+// bf16 19.7 (5.7 TB/s); for 16-bit rows the instructions come close to the bandwidth (60% of
+// issue slots), so two values are worked on at a time.
 //
 // Gradient, per row: with h = (s - mean) rstd, g = dy weight,
 //   dx = rstd (g - mean(g) - h mean(g h)) + dsum,
