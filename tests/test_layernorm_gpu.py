@@ -437,3 +437,15 @@ def test_layernorm_of_rows_that_fill_the_gpu(rows, dim, x_dtype, y_dtype, pad):
         check_codes(L.layernorm(x, w, b, residual=r, out_dtype=E4M3), *ref(x, w, b, r, 1e-5)[3::3])
     else:
         check(x, w, b, r, 1e-5, y_dtype)
+
+
+@gpu
+@pytest.mark.parametrize("rows,dim", [(100001, 20), (20000, 200), (1000, 4000), (700, 4096), (700, 4097)])
+@pytest.mark.parametrize("x_dtype", [F32, BF16])
+def test_layernorm_single_values_of_many_rows(rows, dim, x_dtype):
+    """x a value further apart than residual and y, in matrices that fill the GPU: 8 values a thread
+    to 4,096 a row, 16 beyond."""
+    x, r = randn(rows, dim, dtype=x_dtype, seed=1, pad=1), randn(rows, dim, dtype=x_dtype, seed=2)
+    w, b = randn(dim, dtype=x_dtype, seed=3), randn(dim, dtype=x_dtype, seed=4)
+    check(x, w, b, r, 1e-5, x_dtype)
+    check_codes(L.layernorm(x, w, b, residual=r, out_dtype=E4M3), *ref(x, w, b, r, 1e-5)[3::3])

@@ -774,7 +774,9 @@ int team_of(int64_t vectors, int per_thread) {
 // fill the GPU otherwise, 32 where the row is too long, and for 16-bit rows from 4,096
 // values on, where what a thread does once a row counts (8191 x 5120 66.6 -> 61.4 us, 16384 x
 // 4096 94.1 -> 89.9, 8191 x 5121 157 -> 129; 20000 x 1024 30.1 against 30.4, FP32 8192 x 4096 77.4
-// against 80.6).
+// against 80.6).  Single values stay at 8 while 512 threads hold the row so: 16 addresses and
+// values spill (20000 x 200 bf16 with residual 22 us against 31, 9000 x 4000 186 against 208; FP32
+// 22 against 34, 176 against 219).
 template <int V>
 Shape norm_shape(int64_t rows, int64_t dim, bool ragged) {
   if (ragged) dim += V - 1;  // a row may start inside its first vector
@@ -782,6 +784,7 @@ Shape norm_shape(int64_t rows, int64_t dim, bool ragged) {
   auto most = [&](int held) { return (int64_t)held * (held == kMostHeld<V> ? 1024 : 512); };
   s.held = rows * dim < (int64_t)sm_count() * 2048 * 8 ? 8 : 16;
   if (V == 8 && dim >= 4096 && s.held == 16) s.held = 32;
+  if (V == 1) s.held = 8;
   while (s.held < kMostHeld<V> && dim > most(s.held)) s.held *= 2;
   s.fits = dim <= most(s.held);
   s.team = team_of(ceil_div(dim, V), s.held / V);
